@@ -233,6 +233,132 @@ int sb_layernorm(const float *x, const float *w, const float *b, float *y, int n
                  void *stream);
 int sb_gelu(const float *x, float *y, int n, void *stream);
 
+/* ---- a batch of requests that share a prompt ---------------------------------
+ * Operators of a serving or scoring step over several requests, beside the
+ * single-sequence engines: sb_kv_plan -> sb_rotary_kv -> sb_attn_prefix ->
+ * (the LM head) -> sb_logprobs.  None has a counterpart in the reference.
+ * All lengths, tables and positions are device arrays, so a captured graph
+ * replays with new contents; the host values are sizes and upper bounds.
+ * Nothing is allocated: scratch comes from the caller, one per call that may
+ * overlap another (two streams, two captured graphs that run side by side).
+ * Element types: */
+#define SB_F32 0
+#define SB_F16 1
+#define SB_BF16 2
+
+/* Keys and values in pages: position i of page p and key head h starts at
+ * element p page_stride + i pos_stride + h head_stride of k and of v, its HD
+ * values next to each other.  One layer of an engine's cache
+ * (sb_engine_kv_cache) is a pool of max_ctx / page pages. */
+typedef struct sb_kv_pages {
+    void *k, *v;
+    int64_t page_stride, pos_stride, head_stride;
+    int type, n_pages, page, NKV, HD;
+} sb_kv_pages;
+
+/* Page plan of a step: request b (B <= SB_PLAN_MAX_B) has cache_len[b]
+ * positions and gets new_len[b] tokens (negative lengths count as 0; the
+ * sums stay below 2^31).  Pages it lacks are taken from free_pages in request
+ * order and written into its table row (table + b table_stride, `width`
+ * entries), whose first ceil(cache_len / page) entries are its pages so far;
+ * entries past what it needs are left as they are.  The new tokens are
+ * numbered request by request: cu_q[B + 1] receives the first token of each
+ * request, kv_len[B] = cache_len + new_len, and for token t < T slots[t]
+ * (page x page size + place, -1 without a page), pos[t] and req[t]; rows
+ * behind the last token get -1 in all three, tokens past T are not listed.
+ * used[0] = pages taken, used[1] = pages lacking (free list or table width
+ * too short: their table entries inside the width become -1).  A negative
+ * entry of free_pages or of a table is a page that is not there.  Outputs
+ * must not overlap inputs, except that the table is both. */
+#define SB_PLAN_MAX_B 16384
+int sb_kv_plan(const int *cache_len, const int *new_len, int B, int page, const int *free_pages, int n_free, int *table,
+               int table_stride, int width, int64_t *slots, int *pos, int *req, int T, int *cu_q, int *kv_len, int *used,
+               void *stream);
+
+/* Rotary positions: pair i of the first `dim` values of a head turns by pos x
+ * f_i, f_i = theta^(-2 i / dim), scaled for contexts longer than the trained
+ * one.  Layouts: HALF pairs (i, i + dim / 2), PAIRS (2 i, 2 i + 1).
+ * Scalings: LINEAR f / factor; NTK theta x factor^(dim / (dim - 2)); YARN
+ * keeps pairs that turn 32 times and more over orig_ctx, divides those that
+ * turn once and less by factor, blends between, and multiplies cosine and
+ * sine by 0.1 ln factor + 1; BANDS keeps pairs of 4 turns and more, divides
+ * those of 1 turn and less, blends by turns between.  The plan is plain host
+ * memory (copied into each launch), exact for any position below 2^31. */
+#define SB_ROTARY_MAX_DIM 256
+#define SB_ROPE_HALF 0
+#define SB_ROPE_PAIRS 1
+#define SB_ROPE_PLAIN 0
+#define SB_ROPE_LINEAR 1
+#define SB_ROPE_NTK 2
+#define SB_ROPE_YARN 3
+#define SB_ROPE_BANDS 4
+typedef struct sb_rotary_plan {
+    uint64_t turn[SB_ROTARY_MAX_DIM / 2]; /* turns per position x 2^64 */
+    float mscale;
+    int dim, layout;
+} sb_rotary_plan;
+int sb_rotary_plan_init(sb_rotary_plan *r, int dim, int layout, double theta, int scaling, double factor, int orig_ctx);
+/* y = x [T][H][HD] turned by pos[t] (strides in elements; y may be x with
+ * the same strides); inverse != 0 turns back, the gradient of the rotation.
+ * Rows with pos < 0 are left as they were. */
+int sb_rotary(const void *x, int64_t x_tok, int64_t x_head, void *y, int64_t y_tok, int64_t y_head, int type, int T, int H,
+              int HD, const int *pos, const sb_rotary_plan *r, int inverse, void *stream);
+/* One launch for a step's new tokens: q_out = q turned, k turned and v copied
+ * into slot slots[t] of kv (slots of different tokens must differ; a slot
+ * outside the pages, as -1, writes nothing).  Rows with pos < 0 are left. */
+int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int64_t qo_tok, int64_t qo_head, const void *k,
+                 int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, int T, int NH, const int *pos,
+                 const int64_t *slots, const sb_rotary_plan *r, const sb_kv_pages *kv, void *stream);
+
+/* Attention of a batch over a prefix that all requests share, read once for
+ * all of them, and each request's own positions.  q, out [T][NH][HD] (HD % 8
+ * == 0, <= 128; 16-byte aligned rows) of the pages' type; NH / NKV query
+ * heads share a key head.  Rows cu_q[b] .. cu_q[b + 1] belong to request b
+ * (cu_q nondecreasing from 0; NULL: row b is request b); row i of n sees all
+ * prefix_len positions of the prefix and the first kv_len[b] - n + i + 1 of
+ * the request's own (its new tokens are in the pages already).  prefix_table
+ * and table rows hold page numbers (prefix_table NULL: 0, 1, 2, ...); a
+ * position whose page number is outside the pool is skipped, never read, and
+ * so is everything past a length.  Values that some row of a tile sees must
+ * be finite (a weight of 0 times an infinity is NaN).  prefix and kv may be
+ * different pools; with prefix_len == 0 or max_kv == 0 the other one's
+ * arguments may be NULL.  max_q (rows of a request) sizes the launch, larger
+ * requests are still right; kv_len is cut to max_kv.  A row that sees nothing
+ * gives zeros and lse = -inf; rows from cu_q[B] on are left as they were.
+ * lse [T][NH] (natural log of the softmax denominator) may be NULL.
+ * ws: sb_attn_prefix_ws bytes for the same sizes (16-byte aligned).  FP32
+ * runs on CUDA cores in FP32 throughout; 16-bit types use the tensor cores
+ * with FP32 scores, sums and outputs and 16-bit softmax weights. */
+int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes);
+int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
+                   int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
+                   int prefix_len, const sb_kv_pages *kv, const int *table, int table_stride, const int *kv_len, int max_kv,
+                   float scale, void *ws, size_t ws_bytes, void *stream);
+
+/* Log probabilities from logits [R][V] (any row stride and alignment) in one
+ * pass, x = logits / temperature: lse[r] = ln sum e^x, entropy[r] of the
+ * softmax, logp[r] = x[tokens[r]] - lse, rank[r] = how many ids come before
+ * the token (larger logit, or equal and a lower id), and the top_k (0..64)
+ * best ids with their log probabilities, best first, equal logits by id.
+ * Any output may be NULL.  A token outside [0, V) gives logp 0 and rank -1.
+ * Masked choices (-inf) have probability 0 and are not listed (id -1,
+ * -inf fill up); a row of them gives lse = logp = -inf and entropy 0.  A row
+ * with a NaN or +inf gives NaN sums, its ids and rank mean nothing.
+ * ws: sb_logprobs_ws bytes (16-byte aligned). */
+int sb_logprobs_ws(int type, int R, int V, int top_k, size_t *bytes);
+int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
+                float *logp, float *entropy, float *lse, int *rank, int top_k, int *top_ids, float *top_logp, void *ws,
+                size_t ws_bytes, void *stream);
+/* The gradient of logp and entropy with respect to the logits:
+ * grad[r][v] = (g_logp[r] ([v == token] - p) - g_entropy[r] p (ln p + H)) / temperature
+ * with lse and entropy from sb_logprobs at the same temperature.  g_logp or
+ * g_entropy may be NULL (0); entropy may be NULL without g_entropy.  A row
+ * without a token takes no g_logp, a row of masked choices gives zeros.
+ * grad has the logits' type and may be the logits (same strides). */
+int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
+                     const float *lse, const float *entropy, const float *g_logp, const float *g_entropy, void *grad,
+                     int64_t grad_stride, void *stream);
+
 /* ---- engines ---------------------------------------------------------------
  * One process, one model, one GPU.  Weight files use the reference's exact
  * flat layouts (qwen_engine.c:8-16,60-75 / conv_qwen.py; gpt2_engine.c:10-13,

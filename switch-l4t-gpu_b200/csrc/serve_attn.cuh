@@ -1,0 +1,635 @@
+// serve_attn.cuh -- attention of a batch over a shared prefix and each
+// request's own pages (attn_prefix).
+//
+// Row r of request b sees every position of the prefix and the first
+// len - n + i + 1 of the request's own (row i of its n).  With s_j = scale
+// q.k_j the result is sum_j e^(s_j - m) v_j / sum_j e^(s_j - m): sums over
+// disjoint sets of keys join by their maxima, so the work is cut into items
+// (row tile, key head, key range) that leave (m, l, o) and attn_join adds
+// them.  The point of the cut: the prefix is read once for ALL rows of a key
+// head (T x G rows stacked into tiles), not once a request; a request's own
+// keys meet only its own rows.
+//
+// One item runs one of these bodies; each streams K and V tiles through a
+// three-stage cp.async ring, positions going through the block table (an
+// offset per key, computed a tile ahead; a position without a page, or past
+// the range, is filled with zeros and masked, so nothing of it is read):
+//   attn_mma_body  f16 / bf16, mma.sync m16n8k16: 16-row tiles (four warps
+//                  split the keys; memory-bound: one row group against long
+//                  own pages) or 64-row tiles (a warp 16 rows)
+//   attn_f32_body  FP32 on the CUDA cores: 1..16-row tiles, a thread a key
+// Scores, maxima, sums and outputs are FP32; the softmax weights are rounded
+// to the value type for the second tensor-core product (half a step, like
+// the values they multiply).
+#pragma once
+#include <cuda_bf16.h>
+
+#include "sb_common.cuh"
+
+#define SB_AP_THREADS 128
+#define SB_AP_STAGES 3
+
+struct AttnPages {  // strides in elements
+    const void *k, *v;
+    long long page_stride, pos_stride, head_stride;
+    int n_pages, page;
+};
+// parameter block, mirrored by the host (host/sb_serve.c)
+struct AttnParams {
+    const void *q;
+    void *out;
+    float *lse;
+    const int *cu_q, *ptable, *table, *kv_len;
+    float *ws_o;
+    float2 *ws_ml;
+    int *ws_n;
+    long long q_row, q_head, o_row, o_head;
+    AttnPages pre, suf;
+    int T, B, NH, NKV, G, HD, P, max_kv, table_stride;
+    int chunk1, S1, chunk2, S2, tiles;  // key ranges and row tiles of the items
+    float scale_log2;
+};
+
+struct AttnItem {
+    AttnPages pg;
+    const int *table;
+    int k0, k1, kvh, slot;
+    int f0, F;       // first row of the tile, rows (query row x head of the group) there are
+    int row0;        // query row of f = 0
+    int vis0;        // positions that f sees: clamp(vis0 + f / G, 0, vis1)  (prefix: vis0 = vis1 = P, step 0)
+    int vis1, step;
+};
+
+SB_DEV int ap_rows(const AttnParams &P) { return P.cu_q ? min(max(P.cu_q[P.B], 0), P.T) : P.T; }
+SB_DEV int ap_vis(const AttnItem &it, int f, int G) { return min(max(it.vis0 + it.step * (f / G), 0), it.vis1); }
+
+// Item `idx` of the prefix (row tiles fastest: neighbours read the same keys)
+SB_DEV bool ap_prefix_item(const AttnParams &P, int idx, int MT, AttnItem &it) {
+    const int tile = idx % P.tiles, rest = idx / P.tiles;
+    it.kvh = rest % P.NKV;
+    it.slot = rest / P.NKV;
+    it.pg = P.pre;
+    it.table = P.ptable;
+    it.k0 = it.slot * P.chunk1;
+    it.k1 = min(it.k0 + P.chunk1, P.P);
+    it.F = ap_rows(P) * P.G;
+    it.f0 = tile * MT;
+    it.row0 = 0;
+    it.vis0 = it.vis1 = P.P;
+    it.step = 0;
+    return it.f0 < it.F;
+}
+// Request of item `idx`, its key head and key range; row tiles are looped by the caller
+SB_DEV bool ap_own_item(const AttnParams &P, int idx, int MT, AttnItem &it, int &tile) {
+    const int s = idx % P.S2;
+    int rest = idx / P.S2;
+    tile = rest % P.tiles;
+    rest /= P.tiles;
+    it.kvh = rest % P.NKV;
+    const int b = rest / P.NKV;
+    int q0 = b, q1 = b + 1;
+    if (P.cu_q) {
+        q0 = min(max(P.cu_q[b], 0), P.T);
+        q1 = min(max(P.cu_q[b + 1], q0), P.T);
+    }
+    const int len = min(max(P.kv_len[b], 0), P.max_kv), n = q1 - q0;
+    it.slot = P.S1 + s;
+    it.pg = P.suf;
+    it.table = P.table + (long long)b * P.table_stride;
+    it.k0 = s * P.chunk2;
+    it.k1 = min(it.k0 + P.chunk2, len);
+    it.F = n * P.G;
+    it.row0 = q0;
+    it.vis0 = len - n + 1;
+    it.vis1 = len;
+    it.step = 1;
+    const int used = max(1, (len + P.chunk2 - 1) / P.chunk2);
+    if (s == 0 && it.kvh == 0 && P.ws_n)
+        for (int r = q0 + tile * SB_AP_THREADS + threadIdx.x; r < q1; r += P.tiles * SB_AP_THREADS) P.ws_n[r] = used;
+    return s < used;
+}
+
+SB_DEV unsigned ap_smem(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+SB_DEV void ap_cp16(unsigned dst, const void *src, bool ok) {  // 16 bytes, or zeros (nothing is read)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+SB_DEV void ap_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> SB_DEV void ap_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// element offset of position p in the pages (without the head), -1 where it has none
+SB_DEV long long ap_offset(const AttnItem &it, int p) {
+    if (p >= it.k1) return -1;
+    const int j = p / it.pg.page;
+    const int pg = it.table ? it.table[j] : j;
+    if (pg < 0 || pg >= it.pg.n_pages) return -1;
+    return pg * it.pg.page_stride + (p - j * it.pg.page) * it.pg.pos_stride;
+}
+
+// what a finished row leaves: the output itself where the item is the only one, else its part
+SB_DEV void ap_row_stats(const AttnParams &P, const AttnItem &it, int f, float m, float l) {
+    const int row = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
+    if (P.S1 + P.S2 == 1) {
+        if (P.lse) P.lse[(long long)row * P.NH + head] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
+    } else {
+        P.ws_ml[((long long)it.slot * P.T + row) * P.NH + head] = make_float2(m, l);
+    }
+}
+template <typename T> SB_DEV void ap_store2(T *p, float a, float b);
+template <> SB_DEV void ap_store2<float>(float *p, float a, float b) { *reinterpret_cast<float2 *>(p) = make_float2(a, b); }
+template <> SB_DEV void ap_store2<__half>(__half *p, float a, float b) { *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(a, b); }
+template <> SB_DEV void ap_store2<__nv_bfloat16>(__nv_bfloat16 *p, float a, float b) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(a, b);
+}
+// two neighbouring values (d even) of row f; a row that sees nothing gives zeros
+template <typename T>
+SB_DEV void ap_row_out(const AttnParams &P, const AttnItem &it, int f, int d, float a, float b, float l) {
+    if (d >= P.HD) return;
+    const int row = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
+    if (P.S1 + P.S2 == 1) {
+        const float w = l == 0.f ? 0.f : 1.f / l;
+        ap_store2<T>(static_cast<T *>(P.out) + row * P.o_row + head * P.o_head + d, a * w, b * w);
+    } else if (l != 0.f) {  // the join skips parts without weight
+        ap_store2<float>(P.ws_o + (((long long)it.slot * P.T + row) * P.NH + head) * P.HD + d, a, b);
+    }
+}
+
+// ---------------------------------------------------------------- f16 / bf16
+template <typename T> SB_DEV void ap_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1);
+template <> SB_DEV void ap_mma<__half>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> SB_DEV void ap_mma<__nv_bfloat16>(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> SB_DEV unsigned ap_pack(float a, float b);
+template <> SB_DEV unsigned ap_pack<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+template <> SB_DEV unsigned ap_pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const unsigned *>(&h);
+}
+SB_DEV void ap_ldsm(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+SB_DEV void ap_ldsm_t(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+SB_DEV float ap_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// HDP: head size padded to 64 or 128.  MW: warps along the rows (1: 16-row
+// tile, warps split the 64 keys of a tile; 4: 64-row tile).
+// Shared memory: SB_AP_STAGES x 2 x 64 x HDP x 2 bytes (>= the 4 x 16 x HDP
+// floats of the final join over warps), rows of 128 / 256 bytes with their
+// 16-byte chunks xor-ed by the row's low three bits (ldmatrix reads eight
+// rows of one chunk without a conflict).
+template <typename T, int HDP, int MW>
+SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
+    constexpr int KT = 64, WK = MW == 1 ? 16 : 64, NT = WK / 8, C = HDP / 8, KS = HDP / 16;
+    constexpr int TILE = KT * HDP * 2, STAGE = 2 * TILE, RING = SB_AP_STAGES + 1;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+    const int fw = it.f0 + (MW == 1 ? 0 : warp * 16);  // this warp's first row
+    const T *kb = static_cast<const T *>(it.pg.k) + it.kvh * it.pg.head_stride;
+    const T *vb = static_cast<const T *>(it.pg.v) + it.kvh * it.pg.head_stride;
+
+    // query fragments from global memory: rows fw + g and fw + g + 8
+    unsigned qa[KS][4];
+    int vis[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int f = fw + g + 8 * h;
+        vis[h] = f < it.F ? ap_vis(it, f, P.G) : 0;
+        const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = k * 16 + e * 8 + q4 * 2;
+                qa[k][h + 2 * e] = f < it.F && d < P.HD ? *reinterpret_cast<const unsigned *>(qp + d) : 0u;
+            }
+    }
+    // keys that some row of the tile sees end here; a tile of keys below every row's limit needs no mask
+    const int flast = min(it.f0 + 16 * MW, it.F) - 1;
+    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
+    const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
+
+    auto load = [&](int t) {
+        if (t < nt) {
+            const unsigned kd = ap_smem(sm) + (t % SB_AP_STAGES) * STAGE, vd = kd + TILE;
+            const long long *off = off_s[t % RING];
+#pragma unroll
+            for (int j = 0; j < KT * C / SB_AP_THREADS; j++) {
+                const int i = tid + j * SB_AP_THREADS, r = i / C, c = i % C;
+                const long long o = off[r];
+                const bool ok = o >= 0 && c * 8 < P.HD;
+                const unsigned d = r * (HDP * 2) + ((c ^ (r & 7)) << 4);
+                ap_cp16(kd + d, ok ? kb + o + c * 8 : kb, ok);
+                ap_cp16(vd + d, ok ? vb + o + c * 8 : vb, ok);
+            }
+        }
+        ap_commit();
+    };
+    float o[HDP / 8][4];
+#pragma unroll
+    for (int i = 0; i < HDP / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    __syncthreads();  // the ring and the offsets of an earlier item are no longer read
+    for (int t = 0; t < SB_AP_STAGES; t++)
+        if (tid < KT) off_s[t][tid] = ap_offset(it, it.k0 + t * KT + tid);
+    __syncthreads();
+    for (int t = 0; t < SB_AP_STAGES - 1; t++) load(t);
+    for (int t = 0; t < nt; t++) {
+        ap_wait<SB_AP_STAGES - 2>();
+        __syncthreads();  // tile t is there for all; tile t - 1 and its offsets are read
+        load(t + SB_AP_STAGES - 1);
+        long long next = -1;
+        if (tid < KT) next = ap_offset(it, it.k0 + (t + SB_AP_STAGES) * KT + tid);
+        const unsigned kt = ap_smem(sm) + (t % SB_AP_STAGES) * STAGE, vt = kt + TILE;
+        const long long *off = off_s[t % RING];
+        const int w0 = MW == 1 ? warp * 16 : 0, key0 = it.k0 + t * KT + w0;
+        float s[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        const int mid = lane >> 3, r8 = lane & 7;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int n = 0; n < NT / 2; n++) {
+                const int r = w0 + n * 16 + r8 + (mid >> 1) * 8, c = k * 2 + (mid & 1);
+                unsigned b[4];
+                ap_ldsm(b, kt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
+                ap_mma<T>(s[2 * n], qa[k], b[0], b[1]);
+                ap_mma<T>(s[2 * n + 1], qa[k], b[2], b[3]);
+            }
+        // scores in log2 units; masked where the row does not see the key or the key has no page
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = n * 8 + q4 * 2 + (e & 1);
+                const bool seen = key0 + j < vis[e >> 1] && off[w0 + j] >= 0;
+                s[n][e] = seen ? s[n][e] * P.scale_log2 : -INFINITY;
+                mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
+            }
+        float base[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(SB_FULL, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(SB_FULL, mx[h], 2));
+            base[h] = mx[h] == -INFINITY ? 0.f : mx[h];
+            const float a = ap_exp2(m[h] - base[h]);
+            m[h] = mx[h];
+            l[h] *= a;
+#pragma unroll
+            for (int i = 0; i < HDP / 8; i++) {
+                o[i][2 * h] *= a;
+                o[i][2 * h + 1] *= a;
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[n][e] = ap_exp2(s[n][e] - base[e >> 1]);
+                l[e >> 1] += s[n][e];
+            }
+#pragma unroll
+        for (int n = 0; n < NT / 2; n++) {
+            const unsigned a[4] = {ap_pack<T>(s[2 * n][0], s[2 * n][1]), ap_pack<T>(s[2 * n][2], s[2 * n][3]),
+                                   ap_pack<T>(s[2 * n + 1][0], s[2 * n + 1][1]), ap_pack<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+            for (int i = 0; i < HDP / 16; i++) {
+                const int r = w0 + n * 16 + r8 + (mid & 1) * 8, c = i * 2 + (mid >> 1);
+                unsigned b[4];
+                ap_ldsm_t(b, vt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
+                ap_mma<T>(o[2 * i], a, b[0], b[1]);
+                ap_mma<T>(o[2 * i + 1], a, b[2], b[3]);
+            }
+        }
+        if (tid < KT) off_s[(t + SB_AP_STAGES) % RING][tid] = next;
+    }
+    ap_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        l[h] += __shfl_xor_sync(SB_FULL, l[h], 1);
+        l[h] += __shfl_xor_sync(SB_FULL, l[h], 2);
+    }
+    if constexpr (MW == 4) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int f = fw + g + 8 * h;
+            if (f >= it.F) continue;
+            if (q4 == 0) ap_row_stats(P, it, f, m[h], l[h]);
+#pragma unroll
+            for (int i = 0; i < HDP / 8; i++) ap_row_out<T>(P, it, f, i * 8 + q4 * 2, o[i][2 * h], o[i][2 * h + 1], l[h]);
+        }
+    } else {  // the four warps' keys join
+        float *ow = reinterpret_cast<float *>(sm);                     // [4][16][HDP]
+        __shared__ float ms[4][16], ls[4][16];
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = g + 8 * h;
+            if (q4 == 0) {
+                ms[warp][r] = m[h];
+                ls[warp][r] = l[h];
+            }
+#pragma unroll
+            for (int i = 0; i < HDP / 8; i++)
+                *reinterpret_cast<float2 *>(ow + (warp * 16 + r) * HDP + i * 8 + q4 * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+        }
+        __syncthreads();
+        for (int i = tid; i < 16 * HDP / 2; i += SB_AP_THREADS) {
+            const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
+            if (f >= it.F) break;
+            float M = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), L = 0.f, a = 0.f, b = 0.f;
+            const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float e = ap_exp2(ms[w][r] - base);
+                const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 16 + r) * HDP + d);
+                L += e * ls[w][r];
+                a += e * x.x;
+                b += e * x.y;
+            }
+            if (d == 0) ap_row_stats(P, it, f, M, L);
+            ap_row_out<T>(P, it, f, d, a, b, L);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- FP32
+// MT rows against tiles of KT keys, 128 threads.  Scores: a thread takes a
+// key and 32 of its dimensions (DS threads a key, partial sums joined in
+// shared memory); K chunks are xor-swizzled so that 8 lanes reading 8 keys
+// touch all banks, query values are broadcast.  Weights: a warp a row.
+// Output: a thread owns four dimensions of all MT rows for every KG-th key;
+// the KG groups join at the end.  FFMA and not the tensor pipe: its FP32
+// sums are not IEEE-rounded and drift by 1e-5 over some thousand keys.
+// Sixteen rows are bound by the FMA pipe and take a two-stage ring, which
+// leaves room for a second CTA.
+template <int HDP, int MT>
+SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
+    constexpr int KT = HDP == 64 ? 64 : 32, DS = SB_AP_THREADS / KT, C = HDP / 4, KG = SB_AP_THREADS / C;
+    constexpr int TILE = KT * HDP * 4, STAGE = 2 * TILE, ST = MT >= 16 ? 2 : 3, RING = ST + 1, RW = (MT + 3) / 4;
+    __shared__ __align__(16) float q_s[MT][HDP], part[DS][MT][KT], p_s[KT][MT < 4 ? 4 : MT];
+    __shared__ float alpha_s[MT], m_s[MT], l_s[MT];
+    __shared__ int vis_s[MT];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const float *kb = static_cast<const float *>(it.pg.k) + it.kvh * it.pg.head_stride;
+    const float *vb = static_cast<const float *>(it.pg.v) + it.kvh * it.pg.head_stride;
+    __syncthreads();  // an earlier item's shared memory is no longer read
+    for (int i = tid; i < MT * HDP; i += SB_AP_THREADS) {
+        const int r = i / HDP, d = i % HDP, f = it.f0 + r;
+        q_s[r][d] = f < it.F && d < P.HD ? static_cast<const float *>(P.q)[(long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head + d] : 0.f;
+    }
+    if (tid < MT) vis_s[tid] = it.f0 + tid < it.F ? ap_vis(it, it.f0 + tid, P.G) : 0;
+    const int flast = min(it.f0 + MT, it.F) - 1;
+    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
+    const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
+    auto load = [&](int t) {
+        if (t < nt) {
+            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE, vd = kd + TILE;
+            const long long *off = off_s[t % RING];
+#pragma unroll
+            for (int j = 0; j < KT * C / SB_AP_THREADS; j++) {
+                const int i = tid + j * SB_AP_THREADS, r = i / C, c = i % C;
+                const long long o = off[r];
+                const bool ok = o >= 0 && c * 4 < P.HD;
+                const unsigned d = r * (HDP * 4) + ((c ^ (r & 7)) << 4);
+                ap_cp16(kd + d, ok ? kb + o + c * 4 : kb, ok);
+                ap_cp16(vd + d, ok ? vb + o + c * 4 : vb, ok);
+            }
+        }
+        ap_commit();
+    };
+    for (int t = 0; t < ST; t++)
+        if (tid < KT) off_s[t][tid] = ap_offset(it, it.k0 + t * KT + tid);
+    __syncthreads();
+    for (int t = 0; t < ST - 1; t++) load(t);
+
+    const int key = tid % KT, ds = tid / KT, dc = tid % C, kg = tid / C;
+    unsigned long long o[MT][2];
+#pragma unroll
+    for (int r = 0; r < MT; r++) o[r][0] = o[r][1] = 0ull;
+    float m[RW], l[RW];  // rows warp, warp + 4, ...
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+    }
+    for (int t = 0; t < nt; t++) {
+        ap_wait<ST - 2>();
+        __syncthreads();
+        load(t + ST - 1);
+        long long next = -1;
+        if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
+        const unsigned char *kt = sm + (t % ST) * STAGE, *vt = kt + TILE;
+        const long long *off = off_s[t % RING];
+        unsigned long long acc[MT];
+#pragma unroll
+        for (int r = 0; r < MT; r++) acc[r] = 0ull;
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const ulonglong2 k2 = *reinterpret_cast<const ulonglong2 *>(kt + key * (HDP * 4) + (((ds * 8 + c) ^ (key & 7)) << 4));
+#pragma unroll
+            for (int r = 0; r < MT; r++) {
+                const ulonglong2 q2 = *reinterpret_cast<const ulonglong2 *>(&q_s[r][(ds * 8 + c) * 4]);
+                acc[r] = ffma2(q2.x, k2.x, acc[r]);
+                acc[r] = ffma2(q2.y, k2.y, acc[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < MT; r++) part[ds][r][key] = f2_sum(acc[r]);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RW; i++) {
+            const int r = warp + 4 * i;
+            if (r < MT) {
+                float s[KT / 32], mx = m[i];
+#pragma unroll
+                for (int j = 0; j < KT / 32; j++) {
+                    const int kk = lane + 32 * j;
+                    float v = 0.f;
+#pragma unroll
+                    for (int e = 0; e < DS; e++) v += part[e][r][kk];
+                    s[j] = it.k0 + t * KT + kk < vis_s[r] && off[kk] >= 0 ? v * P.scale_log2 : -INFINITY;
+                    mx = fmaxf(mx, s[j]);
+                }
+                mx = warp_max(mx);
+                const float base = mx == -INFINITY ? 0.f : mx, a = ap_exp2(m[i] - base);
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < KT / 32; j++) {
+                    s[j] = ap_exp2(s[j] - base);
+                    sum += s[j];
+                    p_s[lane + 32 * j][r] = s[j];
+                }
+                l[i] = l[i] * a + sum;  // this lane's keys; the lanes join at the end
+                m[i] = mx;
+                if (lane == 0) alpha_s[r] = a;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < MT; r++) {
+            const float a = alpha_s[r];
+            const unsigned long long aa = f2_pack(a, a);
+            o[r][0] = ffma2(o[r][0], aa, 0ull);
+            o[r][1] = ffma2(o[r][1], aa, 0ull);
+        }
+#pragma unroll
+        for (int j = 0; j < KT / KG; j++) {
+            const int kk = kg + KG * j;
+            const ulonglong2 v2 = *reinterpret_cast<const ulonglong2 *>(vt + kk * (HDP * 4) + ((dc ^ (kk & 7)) << 4));
+#pragma unroll
+            for (int r = 0; r < MT; r++) {
+                const float p = p_s[kk][r];
+                const unsigned long long pp = f2_pack(p, p);
+                o[r][0] = ffma2(pp, v2.x, o[r][0]);
+                o[r][1] = ffma2(pp, v2.y, o[r][1]);
+            }
+        }
+        if (tid < KT) off_s[(t + ST) % RING][tid] = next;
+    }
+    ap_wait<0>();
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+        const int r = warp + 4 * i;
+        if (r < MT) {
+            l[i] = warp_sum(l[i]);
+            if (lane == 0) {
+                m_s[r] = m[i];
+                l_s[r] = l[i];
+            }
+        }
+    }
+    __syncthreads();
+    float *red = reinterpret_cast<float *>(sm);  // [KG][MT][HDP] floats: 32 KB at most, in the ring
+#pragma unroll
+    for (int r = 0; r < MT; r++) *reinterpret_cast<ulonglong2 *>(red + (kg * MT + r) * HDP + dc * 4) = make_ulonglong2(o[r][0], o[r][1]);
+    __syncthreads();
+    for (int i = tid; i < MT * HDP / 2; i += SB_AP_THREADS) {
+        const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
+        if (f >= it.F) break;
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int g = 0; g < KG; g++) {
+            const float2 x = *reinterpret_cast<const float2 *>(red + (g * MT + r) * HDP + d);
+            a += x.x;
+            b += x.y;
+        }
+        if (d == 0) ap_row_stats(P, it, f, m_s[r], l_s[r]);
+        ap_row_out<float>(P, it, f, d, a, b, l_s[r]);
+    }
+}
+
+// prefix: a CTA an item.  own: a CTA an item; the row tiles of a request
+// beyond the grid's are looped.  Both let the next launch start early; the
+// own kernel waits for the prefix kernel before it ends, so that the join,
+// which waits for the own kernel, has both behind it.
+#define SB_AP_BODY(MT, CALL)                                                                \
+    extern __shared__ __align__(128) unsigned char ap_sm[];                                 \
+    __shared__ long long off_s[SB_AP_STAGES + 1][64];                                       \
+    pdl_launch_dependents();                                                                \
+    AttnItem it;                                                                            \
+    if (!own) {                                                                             \
+        if (ap_prefix_item(P, blockIdx.x, MT, it)) CALL;                                    \
+    } else {                                                                                \
+        int tile;                                                                           \
+        if (ap_own_item(P, blockIdx.x, MT, it, tile))                                       \
+            for (it.f0 = tile * MT; it.f0 < it.F; it.f0 += P.tiles * MT) CALL;              \
+        pdl_wait();                                                                         \
+    }
+#define SB_AP_MMA(name, T, HDP, MW)                                                                            \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS) name(const __grid_constant__ AttnParams P, int own) { \
+        SB_AP_BODY(16 * MW, (attn_mma_body<T, HDP, MW>(P, it, ap_sm, off_s)))                                  \
+    }
+#define SB_AP_F32(name, HDP, MT)                                                                               \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS) name(const __grid_constant__ AttnParams P, int own) { \
+        SB_AP_BODY(MT, (attn_f32_body<HDP, MT>(P, it, ap_sm, off_s)))                                          \
+    }
+SB_AP_MMA(attn_f16_64_r16, __half, 64, 1)
+SB_AP_MMA(attn_f16_64_r64, __half, 64, 4)
+SB_AP_MMA(attn_f16_128_r16, __half, 128, 1)
+SB_AP_MMA(attn_f16_128_r64, __half, 128, 4)
+SB_AP_MMA(attn_bf16_64_r16, __nv_bfloat16, 64, 1)
+SB_AP_MMA(attn_bf16_64_r64, __nv_bfloat16, 64, 4)
+SB_AP_MMA(attn_bf16_128_r16, __nv_bfloat16, 128, 1)
+SB_AP_MMA(attn_bf16_128_r64, __nv_bfloat16, 128, 4)
+SB_AP_F32(attn_f32_64_r1, 64, 1)
+SB_AP_F32(attn_f32_64_r2, 64, 2)
+SB_AP_F32(attn_f32_64_r4, 64, 4)
+SB_AP_F32(attn_f32_64_r8, 64, 8)
+SB_AP_F32(attn_f32_64_r16, 64, 16)
+SB_AP_F32(attn_f32_128_r1, 128, 1)
+SB_AP_F32(attn_f32_128_r2, 128, 2)
+SB_AP_F32(attn_f32_128_r4, 128, 4)
+SB_AP_F32(attn_f32_128_r8, 128, 8)
+SB_AP_F32(attn_f32_128_r16, 128, 16)
+
+// ---------------------------------------------------------------- join
+// A warp a (row, head): parts of the prefix, then those of the request's own
+// keys that are in use; lane i takes part i's (m, l), all lanes the sums.
+// type: 0 f32, 1 f16, 2 bf16.
+extern "C" __global__ void __launch_bounds__(128) attn_join(const __grid_constant__ AttnParams P, int type) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)ap_rows(P) * P.NH, TH = (long long)P.T * P.NH;
+    for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); i < rows; i += (long long)gridDim.x * 4) {
+        const int row = (int)(i / P.NH), head = (int)(i % P.NH);
+        const int n = P.S1 + (P.S2 ? P.ws_n[row] : 0);
+        float M = -INFINITY;
+        for (int s = lane; s < n; s += 32) {
+            const float2 ml = P.ws_ml[s * TH + i];
+            if (ml.y != 0.f) M = fmaxf(M, ml.x);
+        }
+        M = warp_max(M);
+        float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < n; s0 += 32) {
+            float w = 0.f;
+            if (s0 + lane < n) {
+                const float2 ml = P.ws_ml[(s0 + lane) * TH + i];
+                if (ml.y != 0.f) {
+                    w = ap_exp2(ml.x - M);
+                    L += w * ml.y;
+                }
+            }
+            const int c = min(32, n - s0);
+            for (int s = 0; s < c; s++) {
+                const float ws = __shfl_sync(SB_FULL, w, s);
+                if (ws == 0.f) continue;  // a part without weight may not have been written
+                const float *p = P.ws_o + ((s0 + s) * TH + i) * P.HD;
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (lane + 32 * e < P.HD) acc[e] = fmaf(ws, p[lane + 32 * e], acc[e]);
+            }
+        }
+        L = warp_sum(L);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const long long at = row * P.o_row + head * P.o_head;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = lane + 32 * e;
+            if (d >= P.HD) continue;
+            const float v = acc[e] * inv;
+            if (type == 0) static_cast<float *>(P.out)[at + d] = v;
+            else if (type == 1) static_cast<__half *>(P.out)[at + d] = __float2half_rn(v);
+            else static_cast<__nv_bfloat16 *>(P.out)[at + d] = __float2bfloat16_rn(v);
+        }
+        if (P.lse && lane == 0) P.lse[i] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    }
+}

@@ -1,0 +1,135 @@
+// serve_plan.cuh -- block tables and slot maps of a batch, built on the GPU
+// from request lengths (kv_plan).
+//
+// Request b has cache_len[b] positions in have = ceil(cache_len / page)
+// pages and gets new_len[b] more, so it needs ceil((cache_len + new_len) /
+// page) pages, at most the table's width.  The missing ones come from the
+// free list in request order: request b's start at the sum of what the
+// requests before it take.  Token i of request b sits at position p =
+// cache_len[b] + i, in slot table[b][p / page] * page + p % page.
+//
+// Bound: latency.  The two prefix sums over B requests are a few
+// microseconds on one SM and the outputs are 16 bytes a token.  So every CTA
+// repeats the sums (8 B bytes of L2 reads) instead of waiting for another
+// launch, and the CTAs then share out the table rows (a warp a request) and
+// the tokens (a thread four neighbours, the request found by bisection in
+// shared memory).  A token's page is recomputed from the sums, so no CTA
+// reads what another one writes.
+#pragma once
+#include "sb_common.cuh"
+
+#define SB_PLAN_THREADS 512
+
+// exclusive sums over the block of this thread's (a, b)
+SB_DEV void plan_scan2(int &a, int &b, int *wa, int *wb) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int x = a, y = b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int p = __shfl_up_sync(SB_FULL, x, o), q = __shfl_up_sync(SB_FULL, y, o);
+        if (lane >= o) { x += p; y += q; }
+    }
+    if (lane == 31) { wa[w] = x; wb[w] = y; }
+    __syncthreads();
+    int sa = 0, sb = 0;
+    for (int i = 0; i < w; i++) { sa += wa[i]; sb += wb[i]; }
+    a = sa + x - a;
+    b = sb + y - b;
+}
+
+// dynamic shared memory: 2 (B + 1) ints
+extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
+    kv_plan(const int *__restrict__ cache_len, const int *__restrict__ new_len, int B, int page,
+            const int *__restrict__ free_pages, int n_free, int *table, int table_stride, int width,
+            long long *__restrict__ slots, int *__restrict__ pos, int *__restrict__ req, int T,
+            int *__restrict__ cu_q, int *__restrict__ kv_len, int *__restrict__ used) {
+    extern __shared__ int plan_sm[];
+    __shared__ int wa[SB_PLAN_THREADS / 32], wb[SB_PLAN_THREADS / 32], lack_s;
+    int *cu = plan_sm, *first = plan_sm + B + 1;
+    const int tid = threadIdx.x, per = (B + SB_PLAN_THREADS - 1) / SB_PLAN_THREADS;
+    if (tid == 0) lack_s = 0;
+    // this thread's requests [b0, b1): tokens and pages, negative lengths as 0
+    const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    int tok = 0, add = 0, lack = 0;
+    for (int b = b0; b < b1; b++) {
+        const int c = max(cache_len[b], 0), n = max(new_len[b], 0);
+        const int have = (int)(((long long)c + page - 1) / page), need = (int)(((long long)c + n + page - 1) / page);
+        const int got = max(min(need, width) - have, 0);
+        tok += n;
+        add += got;
+        lack += need - have - got;
+    }
+    int t0 = tok, p0 = add;
+    plan_scan2(t0, p0, wa, wb);
+    for (int b = b0; b < b1; b++) {
+        const int c = max(cache_len[b], 0), n = max(new_len[b], 0);
+        const int have = (int)(((long long)c + page - 1) / page), need = (int)(((long long)c + n + page - 1) / page);
+        cu[b] = t0;
+        first[b] = p0;
+        t0 += n;
+        p0 += max(min(need, width) - have, 0);
+    }
+    if (b1 == B && b0 < B) {  // the thread that owns the last request (B > 0)
+        cu[B] = t0;
+        first[B] = p0;
+    }
+    if (lack) atomicAdd(&lack_s, lack);
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        for (int b = tid; b <= B; b += SB_PLAN_THREADS) {
+            cu_q[b] = cu[b];
+            if (b < B) kv_len[b] = max(cache_len[b], 0) + max(new_len[b], 0);
+        }
+        if (tid == 0) {
+            const int total = first[B], taken = min(total, n_free);
+            used[0] = taken;
+            used[1] = total - taken + lack_s;
+        }
+    }
+    // new entries of the tables: a warp a request
+    const int lane = tid & 31, nw = gridDim.x * (SB_PLAN_THREADS / 32);
+    for (int b = blockIdx.x * (SB_PLAN_THREADS / 32) + (tid >> 5); b < B; b += nw) {
+        const int f = first[b], n = first[b + 1] - f;
+        if (n == 0) continue;
+        const int have = (int)(((long long)max(cache_len[b], 0) + page - 1) / page);
+        for (int j = lane; j < n; j += 32)
+            table[(size_t)b * table_stride + have + j] = f + j < n_free ? free_pages[f + j] : -1;
+    }
+    // tokens: four neighbours a thread
+    const int total = cu[B];
+    for (long long q = (long long)blockIdx.x * SB_PLAN_THREADS + tid; q * 4 < T; q += (long long)gridDim.x * SB_PLAN_THREADS) {
+        const int t = (int)(q * 4);
+        int b = -1;
+        if (t < total) {  // the last request that starts at or before t and is not empty
+            int lo = 0, hi = B;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            b = lo;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (t + i >= T) break;
+            if (t + i >= total) b = -1;
+            long long slot = -1;
+            int p = -1;
+            if (b >= 0) {
+                while (t + i >= cu[b + 1]) b++;
+                const int c = max(cache_len[b], 0);
+                p = c + (t + i - cu[b]);
+                const int j = p / page, have = (int)(((long long)c + page - 1) / page);
+                int pg = -1;
+                if (j < width) {
+                    if (j < have) pg = table[(size_t)b * table_stride + j];
+                    else if (first[b] + j - have < n_free) pg = free_pages[first[b] + j - have];
+                }
+                if (pg >= 0) slot = (long long)pg * page + p % page;
+            }
+            slots[t + i] = slot;
+            pos[t + i] = p;
+            req[t + i] = b;
+        }
+    }
+}

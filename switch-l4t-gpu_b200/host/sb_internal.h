@@ -11,7 +11,7 @@
 extern "C" {
 #endif
 
-enum { M_SWITCH = 0, M_GEMV, M_GPT2, M_QWEN, M_TC, M_COUNT };
+enum { M_SWITCH = 0, M_GEMV, M_GPT2, M_QWEN, M_TC, M_SERVE, M_SCORE, M_COUNT };
 
 typedef enum {
     F_SGEMM_B200 = 0,
@@ -83,6 +83,43 @@ typedef enum {
     F_G2PF_BIAS_GELU,
     F_G2_LAYERNORM_ROWS,
     F_GPT2_MK,
+    /* families in the order f32, f16, bf16 (rotary, logprobs) and head size, row tile (attention) */
+    F_KV_PLAN,
+    F_ROTARY_F32,
+    F_ROTARY_F16,
+    F_ROTARY_BF16,
+    F_ROTARY_F32_ANY,
+    F_ROTARY_F16_ANY,
+    F_ROTARY_BF16_ANY,
+    F_ATTN_F16_64_R16,
+    F_ATTN_F16_64_R64,
+    F_ATTN_F16_128_R16,
+    F_ATTN_F16_128_R64,
+    F_ATTN_BF16_64_R16,
+    F_ATTN_BF16_64_R64,
+    F_ATTN_BF16_128_R16,
+    F_ATTN_BF16_128_R64,
+    F_ATTN_F32_64_R1,
+    F_ATTN_F32_64_R2,
+    F_ATTN_F32_64_R4,
+    F_ATTN_F32_64_R8,
+    F_ATTN_F32_64_R16,
+    F_ATTN_F32_128_R1,
+    F_ATTN_F32_128_R2,
+    F_ATTN_F32_128_R4,
+    F_ATTN_F32_128_R8,
+    F_ATTN_F32_128_R16,
+    F_ATTN_JOIN,
+    F_LOGPROBS_F32,
+    F_LOGPROBS_F16,
+    F_LOGPROBS_BF16,
+    F_LOGPROBS_TOP_F32,
+    F_LOGPROBS_TOP_F16,
+    F_LOGPROBS_TOP_BF16,
+    F_LOGPROBS_JOIN,
+    F_LOGPROBS_GRAD_F32,
+    F_LOGPROBS_GRAD_F16,
+    F_LOGPROBS_GRAD_BF16,
     F_COUNT
 } sb_fn_id;
 
@@ -93,6 +130,7 @@ typedef struct sb_ctx {
     CUmodule mod[M_COUNT];
     CUfunction fn[F_COUNT];
     int smem_set[F_COUNT]; /* dynamic smem limit already raised to this */
+    int occ[F_COUNT];      /* co-resident CTAs per SM (sb_occupancy_of) */
     int sms;
     CUdeviceptr tc_ws; /* split-K workspace of the tensor-core GEMM (grown on demand) */
     size_t tc_ws_bytes;
@@ -123,6 +161,12 @@ int sb_launch_coop(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned bx, unsigned sme
 int sb_launch3(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned gy, unsigned gz, unsigned bx, CUstream s, void **args);
 /* max co-resident CTAs of f per SM at this block size / dynamic smem */
 int sb_occupancy(sb_ctx *c, sb_fn_id f, int block, size_t smem);
+/* the same, at least 1, kept from the first query (a kernel with one launch shape) */
+int sb_occupancy_of(sb_ctx *c, sb_fn_id f, int block, size_t smem);
+
+/* limits of sb_serve.c's launches */
+#define SB_ATTN_MAX_SPLITS 128     /* key ranges of the prefix, and of a request's own keys */
+#define SB_LOGPROBS_MAX_PARTS 256  /* parts of a row */
 
 #ifdef __cplusplus
 }

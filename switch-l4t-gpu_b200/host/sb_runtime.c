@@ -1,6 +1,6 @@
 /* sb_runtime.c -- context, module images and launches for libswitch_b200.
  *
- * The four sm_100a cubins are linked into the library (cubins.S) and loaded
+ * The sm_100a cubins are linked into the library (cubins.S) and loaded
  * with cuModuleLoadData into whichever context is current, exactly how the
  * reference's hosts load their PTX (gpu_workload.c:65-74); kernels are then
  * resolved by name with cuModuleGetFunction and launched with
@@ -17,6 +17,8 @@ extern const unsigned char sb_img_gemv[], sb_img_gemv_end[];
 extern const unsigned char sb_img_gpt2[], sb_img_gpt2_end[];
 extern const unsigned char sb_img_qwen[], sb_img_qwen_end[];
 extern const unsigned char sb_img_tc[], sb_img_tc_end[];
+extern const unsigned char sb_img_serve[], sb_img_serve_end[];
+extern const unsigned char sb_img_score[], sb_img_score_end[];
 
 static const struct {
     const char *name;
@@ -27,6 +29,8 @@ static const struct {
     {"gpt2", sb_img_gpt2, sb_img_gpt2_end},
     {"qwen", sb_img_qwen, sb_img_qwen_end},
     {"tc", sb_img_tc, sb_img_tc_end},
+    {"serve", sb_img_serve, sb_img_serve_end},
+    {"score", sb_img_score, sb_img_score_end},
 };
 
 static const struct {
@@ -102,6 +106,42 @@ static const struct {
     [F_G2PF_BIAS_GELU] = {M_GPT2, "gpt2_pf_bias_gelu"},
     [F_G2_LAYERNORM_ROWS] = {M_GPT2, "layernorm"},
     [F_GPT2_MK] = {M_GPT2, "gpt2_decode_mk"},
+    [F_KV_PLAN] = {M_SERVE, "kv_plan"},
+    [F_ROTARY_F32] = {M_SERVE, "rotary_f32"},
+    [F_ROTARY_F16] = {M_SERVE, "rotary_f16"},
+    [F_ROTARY_BF16] = {M_SERVE, "rotary_bf16"},
+    [F_ROTARY_F32_ANY] = {M_SERVE, "rotary_f32_any"},
+    [F_ROTARY_F16_ANY] = {M_SERVE, "rotary_f16_any"},
+    [F_ROTARY_BF16_ANY] = {M_SERVE, "rotary_bf16_any"},
+    [F_ATTN_F16_64_R16] = {M_SERVE, "attn_f16_64_r16"},
+    [F_ATTN_F16_64_R64] = {M_SERVE, "attn_f16_64_r64"},
+    [F_ATTN_F16_128_R16] = {M_SERVE, "attn_f16_128_r16"},
+    [F_ATTN_F16_128_R64] = {M_SERVE, "attn_f16_128_r64"},
+    [F_ATTN_BF16_64_R16] = {M_SERVE, "attn_bf16_64_r16"},
+    [F_ATTN_BF16_64_R64] = {M_SERVE, "attn_bf16_64_r64"},
+    [F_ATTN_BF16_128_R16] = {M_SERVE, "attn_bf16_128_r16"},
+    [F_ATTN_BF16_128_R64] = {M_SERVE, "attn_bf16_128_r64"},
+    [F_ATTN_F32_64_R1] = {M_SERVE, "attn_f32_64_r1"},
+    [F_ATTN_F32_64_R2] = {M_SERVE, "attn_f32_64_r2"},
+    [F_ATTN_F32_64_R4] = {M_SERVE, "attn_f32_64_r4"},
+    [F_ATTN_F32_64_R8] = {M_SERVE, "attn_f32_64_r8"},
+    [F_ATTN_F32_64_R16] = {M_SERVE, "attn_f32_64_r16"},
+    [F_ATTN_F32_128_R1] = {M_SERVE, "attn_f32_128_r1"},
+    [F_ATTN_F32_128_R2] = {M_SERVE, "attn_f32_128_r2"},
+    [F_ATTN_F32_128_R4] = {M_SERVE, "attn_f32_128_r4"},
+    [F_ATTN_F32_128_R8] = {M_SERVE, "attn_f32_128_r8"},
+    [F_ATTN_F32_128_R16] = {M_SERVE, "attn_f32_128_r16"},
+    [F_ATTN_JOIN] = {M_SERVE, "attn_join"},
+    [F_LOGPROBS_F32] = {M_SCORE, "logprobs_f32"},
+    [F_LOGPROBS_F16] = {M_SCORE, "logprobs_f16"},
+    [F_LOGPROBS_BF16] = {M_SCORE, "logprobs_bf16"},
+    [F_LOGPROBS_TOP_F32] = {M_SCORE, "logprobs_top_f32"},
+    [F_LOGPROBS_TOP_F16] = {M_SCORE, "logprobs_top_f16"},
+    [F_LOGPROBS_TOP_BF16] = {M_SCORE, "logprobs_top_bf16"},
+    [F_LOGPROBS_JOIN] = {M_SCORE, "logprobs_join"},
+    [F_LOGPROBS_GRAD_F32] = {M_SCORE, "logprobs_grad_f32"},
+    [F_LOGPROBS_GRAD_F16] = {M_SCORE, "logprobs_grad_f16"},
+    [F_LOGPROBS_GRAD_BF16] = {M_SCORE, "logprobs_grad_bf16"},
 };
 
 /* ---------------------------------------------------------------- errors */
@@ -196,10 +236,12 @@ int sb_module_image(const char *name, const void **image, size_t *size) {
 }
 
 /* ---------------------------------------------------------------- launches */
+/* dynamic shared memory up to here needs no opt-in beside 16 KB of static (48 KB together) */
+#define SB_SMEM_PLAIN (32 * 1024)
 int sb_launch(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned gy, unsigned bx, unsigned smem, CUstream s,
               void **args, int pdl) {
     if (!c->fn[f]) SB_CK(cuModuleGetFunction(&c->fn[f], c->mod[fn_table[f].mod], fn_table[f].name));
-    if (smem > 48 * 1024 && c->smem_set[f] < (int)smem) {
+    if (smem > SB_SMEM_PLAIN && c->smem_set[f] < (int)smem) {
         SB_CK(cuFuncSetAttribute(c->fn[f], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)smem));
         c->smem_set[f] = (int)smem;
     }
@@ -238,7 +280,7 @@ int sb_launch3(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned gy, unsigned gz, uns
 
 static int resolve(sb_ctx *c, sb_fn_id f, unsigned smem) {
     if (!c->fn[f]) SB_CK(cuModuleGetFunction(&c->fn[f], c->mod[fn_table[f].mod], fn_table[f].name));
-    if (smem > 48 * 1024 && c->smem_set[f] < (int)smem) {
+    if (smem > SB_SMEM_PLAIN && c->smem_set[f] < (int)smem) {
         SB_CK(cuFuncSetAttribute(c->fn[f], CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES, (int)smem));
         c->smem_set[f] = (int)smem;
     }
@@ -250,6 +292,14 @@ int sb_occupancy(sb_ctx *c, sb_fn_id f, int block, size_t smem) {
     if (resolve(c, f, (unsigned)smem)) return 0;
     if (cuOccupancyMaxActiveBlocksPerMultiprocessor(&n, c->fn[f], block, smem) != CUDA_SUCCESS) return 0;
     return n;
+}
+
+int sb_occupancy_of(sb_ctx *c, sb_fn_id f, int block, size_t smem) {
+    if (!c->occ[f]) {
+        const int n = sb_occupancy(c, f, block, smem);
+        c->occ[f] = n > 0 ? n : 1;
+    }
+    return c->occ[f];
 }
 
 int sb_launch_coop(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned bx, unsigned smem, CUstream s, void **args) {

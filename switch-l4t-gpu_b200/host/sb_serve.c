@@ -1,0 +1,531 @@
+/* sb_serve.c -- host entry points for a batch of requests that share a
+ * prompt: page plan, rotary positions with the cache write, attention over
+ * the shared prefix and each request's own pages, log probabilities and
+ * their gradient.  Each validates its arguments, picks the launch shape and
+ * issues its launches on the caller's stream; nothing is allocated, scratch
+ * comes from the caller. */
+#include <math.h>
+#include <string.h>
+
+#include "sb_internal.h"
+
+#define CEIL_DIV(a, b) (((a) + (b)-1) / (b))
+#define DP(p) ((CUdeviceptr)(uintptr_t)(p))
+#define ALIGNED(p, n) ((((uintptr_t)(p)) & ((n)-1)) == 0)
+
+static int type_size(int type) { return type == SB_F32 ? 4 : 2; }
+static int type_ok(int type) { return type == SB_F32 || type == SB_F16 || type == SB_BF16; }
+/* kernels of a family stand in the order f32, f16, bf16 */
+#define BY_TYPE(f, type) ((sb_fn_id)((f) + (type)))
+
+/* ---------------------------------------------------------------- page plan */
+int sb_kv_plan(const int *cache_len, const int *new_len, int B, int page, const int *free_pages, int n_free, int *table,
+               int table_stride, int width, int64_t *slots, int *pos, int *req, int T, int *cu_q, int *kv_len, int *used,
+               void *stream) {
+    SB_ARG(B >= 1 && B <= SB_PLAN_MAX_B, "kv_plan: B must be 1..16384");
+    SB_ARG(cache_len && new_len && table && cu_q && kv_len && used, "kv_plan: null pointer");
+    SB_ARG(page >= 1 && n_free >= 0 && (free_pages || n_free == 0), "kv_plan: bad page size or free list");
+    SB_ARG(width >= 1 && table_stride >= width, "kv_plan: table_stride must be at least the width");
+    SB_ARG(T >= 0 && ((slots && pos && req) || T == 0), "kv_plan: bad token arrays");
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    CUdeviceptr cl = DP(cache_len), nl = DP(new_len), fp = DP(free_pages), tb = DP(table), sl = DP(slots), po = DP(pos),
+                rq = DP(req), cq = DP(cu_q), kl = DP(kv_len), us = DP(used);
+    void *args[] = {&cl, &nl, &B, &page, &fp, &n_free, &tb, &table_stride, &width, &sl, &po, &rq, &T, &cq, &kl, &us};
+    /* enough CTAs for four tokens a thread and a warp a request, two per SM at most */
+    long g = CEIL_DIV((long)T, 4 * 512), gb = CEIL_DIV(B, 16);
+    if (gb > g) g = gb;
+    if (g > 2L * c->sms) g = 2L * c->sms;
+    return sb_launch(c, F_KV_PLAN, (unsigned)(g < 1 ? 1 : g), 1, 512, (unsigned)(2 * (B + 1) * 4), (CUstream)stream, args, 0);
+}
+
+/* ---------------------------------------------------------------- rotary */
+int sb_rotary_plan_init(sb_rotary_plan *r, int dim, int layout, double theta, int scaling, double factor, int orig_ctx) {
+    SB_ARG(r, "rotary_plan_init: null pointer");
+    SB_ARG(dim >= 2 && dim <= SB_ROTARY_MAX_DIM && dim % 2 == 0, "rotary_plan_init: dim must be even, 2..256");
+    SB_ARG(layout == SB_ROPE_HALF || layout == SB_ROPE_PAIRS, "rotary_plan_init: unknown layout");
+    SB_ARG(isfinite(theta) && theta > 1.0, "rotary_plan_init: theta must be above 1");
+    SB_ARG(scaling >= SB_ROPE_PLAIN && scaling <= SB_ROPE_BANDS, "rotary_plan_init: unknown scaling");
+    SB_ARG(scaling == SB_ROPE_PLAIN || (isfinite(factor) && factor >= 1.0), "rotary_plan_init: factor must be at least 1");
+    SB_ARG(scaling < SB_ROPE_YARN || orig_ctx >= 1, "rotary_plan_init: this scaling needs the trained context");
+    SB_ARG(scaling != SB_ROPE_NTK || dim > 2, "rotary_plan_init: this scaling needs dim > 2");
+    const double pi2 = 6.283185307179586476925286766559;
+    double lo = 0, hi = 0;
+    if (scaling == SB_ROPE_NTK) theta *= pow(factor, dim / (dim - 2.0));
+    if (scaling == SB_ROPE_YARN) { /* pairs that turn 32 times and once over the trained context */
+        lo = floor(dim * log(orig_ctx / (32.0 * pi2)) / (2.0 * log(theta)));
+        hi = ceil(dim * log(orig_ctx / pi2) / (2.0 * log(theta)));
+        if (lo < 0) lo = 0;
+        if (hi > dim - 1) hi = dim - 1;
+    }
+    memset(r, 0, sizeof *r);
+    r->dim = dim;
+    r->layout = layout;
+    r->mscale = 1.0f;
+    if (scaling == SB_ROPE_YARN) r->mscale = (float)(0.1 * log(factor) + 1.0);
+    for (int i = 0; i < dim / 2; i++) {
+        double f = pow(theta, -2.0 * i / dim);
+        if (scaling == SB_ROPE_LINEAR) f /= factor;
+        if (scaling == SB_ROPE_YARN) {
+            double ramp = (i - lo) / (hi > lo ? hi - lo : 0.001);
+            ramp = ramp < 0 ? 0 : ramp > 1 ? 1 : ramp;
+            f = f / factor * ramp + f * (1.0 - ramp);
+        }
+        if (scaling == SB_ROPE_BANDS) { /* turns over the trained context: 1 and fewer stretched, 4 and more kept */
+            double s = (orig_ctx * f / pi2 - 1.0) / 3.0;
+            s = s < 0 ? 0 : s > 1 ? 1 : s;
+            f = f / factor * (1.0 - s) + f * s;
+        }
+        /* the fraction of a turn per position in units of 2^-64, from a long double (64-bit mantissa) */
+        r->turn[i] = (uint64_t)(f / (long double)6.283185307179586476925286766559L * 18446744073709551616.0L + 0.5L);
+    }
+    return 0;
+}
+
+/* mirrors RotParams in csrc/serve_rotary.cuh */
+struct rot_params {
+    CUdeviceptr src[3], dst[3];
+    int64_t st[3], sh[3], dt, dh, page_stride, pos_stride, head_stride;
+    CUdeviceptr pos, slots;
+    int64_t n_slots;
+    int T, heads[3], HD, dim, layout, inverse, page, tokens_per_cta;
+    float mscale;
+    uint64_t turn[SB_ROTARY_MAX_DIM / 2];
+};
+static int rotary_launch(struct rot_params *p, const sb_rotary_plan *r, int type, int vec, void *stream) {
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    if (p->T == 0) return 0;
+    p->dim = r->dim;
+    p->layout = r->layout;
+    p->mscale = r->mscale;
+    memcpy(p->turn, r->turn, sizeof p->turn);
+    const int V = vec ? 16 / type_size(type) : 1;
+    const long H = p->heads[0] + p->heads[1] + p->heads[2], units = H * (p->HD / (2 * V));
+    /* tokens per CTA: up to 8 while that leaves two CTAs per SM; a single
+     * token's heads are spread over several CTAs when they exceed one pass */
+    int tok = 8;
+    while (tok > 1 && (CEIL_DIV(p->T, tok) < 2L * c->sms || tok * units > 8 * 256)) tok >>= 1;
+    p->tokens_per_cta = tok;
+    long gy = 1;
+    const long gx = CEIL_DIV(p->T, tok);
+    if (gx < 2L * c->sms) gy = CEIL_DIV(tok * units, 256);
+    if (gy > 64) gy = 64;
+    void *args[] = {p};
+    return sb_launch(c, vec ? BY_TYPE(F_ROTARY_F32, type) : BY_TYPE(F_ROTARY_F32_ANY, type), (unsigned)gx, (unsigned)gy, 256, 0,
+                     (CUstream)stream, args, 0);
+}
+static int rotary_args(const sb_rotary_plan *r, int type, int T, int HD) {
+    SB_ARG(r && r->dim >= 2 && r->dim <= SB_ROTARY_MAX_DIM && r->dim % 2 == 0, "rotary: plan not initialised");
+    SB_ARG(r->layout == SB_ROPE_HALF || r->layout == SB_ROPE_PAIRS, "rotary: plan not initialised");
+    SB_ARG(type_ok(type), "rotary: unknown element type");
+    SB_ARG(T >= 0 && HD >= r->dim && HD % 2 == 0, "rotary: need an even head size of at least the rotated part");
+    return 0;
+}
+/* all vectors of a row family start on 16 bytes */
+static int vec_ok(int type, const void *p, int64_t a, int64_t b, int64_t c) {
+    const int64_t V = 16 / type_size(type);
+    return ALIGNED(p, 16) && a % V == 0 && b % V == 0 && c % V == 0;
+}
+
+int sb_rotary(const void *x, int64_t x_tok, int64_t x_head, void *y, int64_t y_tok, int64_t y_head, int type, int T, int H,
+              int HD, const int *pos, const sb_rotary_plan *r, int inverse, void *stream) {
+    int rc = rotary_args(r, type, T, HD);
+    if (rc) return rc;
+    SB_ARG(H >= 1 && ((x && y && pos) || T == 0), "rotary: null pointer");
+    SB_ARG(ALIGNED(x, type_size(type)) && ALIGNED(y, type_size(type)), "rotary: misaligned rows");
+    struct rot_params p;
+    memset(&p, 0, sizeof p);
+    p.src[0] = DP(x);
+    p.dst[0] = DP(y);
+    p.st[0] = x_tok;
+    p.sh[0] = x_head;
+    p.dt = y_tok;
+    p.dh = y_head;
+    p.pos = DP(pos);
+    p.T = T;
+    p.heads[0] = H;
+    p.HD = HD;
+    p.page = 1;
+    p.inverse = inverse != 0;
+    const int V = 16 / type_size(type);
+    const int vec = vec_ok(type, x, x_tok, x_head, 0) && vec_ok(type, y, y_tok, y_head, 0) && r->dim % (2 * V) == 0 && HD % (2 * V) == 0;
+    return rotary_launch(&p, r, type, vec, stream);
+}
+
+static int pages_args(const sb_kv_pages *kv) {
+    SB_ARG(kv && kv->k && kv->v, "pages: null pointer");
+    SB_ARG(type_ok(kv->type), "pages: unknown element type");
+    SB_ARG(kv->n_pages >= 1 && kv->page >= 1 && kv->NKV >= 1 && kv->HD >= 1, "pages: bad sizes");
+    SB_ARG(kv->page_stride >= 0 && kv->pos_stride >= 0 && kv->head_stride >= 0, "pages: negative strides");
+    return 0;
+}
+
+int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int64_t qo_tok, int64_t qo_head, const void *k,
+                 int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, int T, int NH, const int *pos,
+                 const int64_t *slots, const sb_rotary_plan *r, const sb_kv_pages *kv, void *stream) {
+    int rc = pages_args(kv);
+    if (!rc) rc = rotary_args(r, kv->type, T, kv->HD);
+    if (rc) return rc;
+    SB_ARG(NH >= 1 && ((q && q_out && k && v && pos && slots) || T == 0), "rotary_kv: null pointer");
+    const int e = type_size(kv->type);
+    SB_ARG(ALIGNED(q, e) && ALIGNED(q_out, e) && ALIGNED(k, e) && ALIGNED(v, e) && ALIGNED(kv->k, e) && ALIGNED(kv->v, e),
+           "rotary_kv: misaligned rows");
+    struct rot_params p;
+    memset(&p, 0, sizeof p);
+    p.src[0] = DP(q);
+    p.src[1] = DP(k);
+    p.src[2] = DP(v);
+    p.dst[0] = DP(q_out);
+    p.dst[1] = DP(kv->k);
+    p.dst[2] = DP(kv->v);
+    p.st[0] = q_tok;
+    p.sh[0] = q_head;
+    p.st[1] = k_tok;
+    p.sh[1] = k_head;
+    p.st[2] = v_tok;
+    p.sh[2] = v_head;
+    p.dt = qo_tok;
+    p.dh = qo_head;
+    p.page_stride = kv->page_stride;
+    p.pos_stride = kv->pos_stride;
+    p.head_stride = kv->head_stride;
+    p.pos = DP(pos);
+    p.slots = DP(slots);
+    p.n_slots = (int64_t)kv->n_pages * kv->page;
+    p.T = T;
+    p.heads[0] = NH;
+    p.heads[1] = p.heads[2] = kv->NKV;
+    p.HD = kv->HD;
+    p.page = kv->page;
+    const int V = 16 / e;
+    const int vec = vec_ok(kv->type, q, q_tok, q_head, 0) && vec_ok(kv->type, q_out, qo_tok, qo_head, 0) &&
+                    vec_ok(kv->type, k, k_tok, k_head, 0) && vec_ok(kv->type, v, v_tok, v_head, 0) &&
+                    vec_ok(kv->type, kv->k, kv->page_stride, kv->pos_stride, kv->head_stride) && ALIGNED(kv->v, 16) &&
+                    r->dim % (2 * V) == 0 && kv->HD % (2 * V) == 0;
+    return rotary_launch(&p, r, kv->type, vec, stream);
+}
+
+/* ---------------------------------------------------------------- attention */
+/* mirrors AttnParams in csrc/serve_attn.cuh */
+struct attn_pages {
+    CUdeviceptr k, v;
+    int64_t page_stride, pos_stride, head_stride;
+    int n_pages, page;
+};
+struct attn_params {
+    CUdeviceptr q, out, lse, cu_q, ptable, table, kv_len, ws_o, ws_ml, ws_n;
+    int64_t q_row, q_head, o_row, o_head;
+    struct attn_pages pre, suf;
+    int T, B, NH, NKV, G, HD, P, max_kv, table_stride;
+    int chunk1, S1, chunk2, S2, tiles;
+    float scale_log2;
+};
+/* one of the two launches: kernel, row tile, row tiles per unit, key ranges */
+struct attn_part {
+    sb_fn_id f;
+    unsigned smem;
+    int tiles, S, chunk;
+    long grid;
+};
+
+/* The kernel for tiles of `rows` rows.  16-bit types: 16-row tiles (the four
+ * warps split the keys) while one holds all rows, else 64-row tiles.  FP32:
+ * the smallest of 1, 2, 4, 8, 16 rows that holds them (unused rows cost
+ * FMAs). */
+static int attn_kernel(int type, int HD, long rows, struct attn_part *a) {
+    const int wide = HD > 64;
+    if (type == SB_F32) {
+        int i = 0;
+        while (i < 4 && (1 << i) < rows) i++;
+        a->f = (sb_fn_id)(F_ATTN_F32_64_R1 + 5 * wide + i);
+        a->smem = (i == 4 ? 2 : 3) * 32768;
+        return 1 << i;
+    }
+    const int big = rows > 16;
+    a->f = (sb_fn_id)((type == SB_F16 ? F_ATTN_F16_64_R16 : F_ATTN_BF16_64_R16) + 2 * wide + big);
+    a->smem = 3 * 2 * 64 * (wide ? 128 : 64) * 2;
+    return big ? 64 : 16;
+}
+/* Key ranges of `keys` keys for `units` independent (head, row tile) pairs:
+ * one wave of items where they fit, about four where they do not (the tail
+ * of the last wave shrinks, the parts to join grow). */
+static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, int step) {
+    const long cap = (long)c->sms * sb_occupancy_of(c, a->f, 128, a->smem);
+    long S = units * 2 <= cap ? cap / units : CEIL_DIV(4 * cap, units);
+    const long most = units * 2 <= cap ? CEIL_DIV(keys, step) : CEIL_DIV(keys, 8 * step);
+    if (S > most) S = most;
+    if (S > SB_ATTN_MAX_SPLITS) S = SB_ATTN_MAX_SPLITS;
+    if (S < 1) S = 1;
+    a->chunk = (int)(CEIL_DIV(CEIL_DIV((long)keys, S), step) * step);
+    a->S = (int)CEIL_DIV((long)keys, a->chunk);
+    a->grid = units * a->S;
+}
+static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD, int max_q, int P, int max_kv,
+                      struct attn_part *pre, struct attn_part *own) {
+    const long G = NH / NKV;
+    memset(pre, 0, sizeof *pre);
+    memset(own, 0, sizeof *own);
+    if (P > 0) {
+        const int mt = attn_kernel(type, HD, T * G, pre);
+        pre->tiles = (int)CEIL_DIV(T * G, mt);
+        attn_split(c, pre, P, (long)pre->tiles * NKV, type == SB_F32 && HD > 64 ? 32 : 64);
+    }
+    if (max_kv > 0) {
+        const int mt = attn_kernel(type, HD, max_q * G, own);
+        own->tiles = (int)CEIL_DIV(max_q * G, mt);
+        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, type == SB_F32 && HD > 64 ? 32 : 64);
+    }
+    SB_ARG(pre->grid < 0x7fffffffL && own->grid < 0x7fffffffL, "attn_prefix: too many rows for one launch");
+    return 0;
+}
+static size_t attn_ws_bytes(int T, int NH, int HD, const struct attn_part *pre, const struct attn_part *own) {
+    const size_t rows = (size_t)T * NH, S = (size_t)pre->S + own->S;
+    if (S <= 1) return 0;
+    return rows * S * HD * 4 + rows * S * 8 + (size_t)T * 4;
+}
+static int attn_args(int type, int T, int B, int NH, int NKV, int HD, int max_q, int P, int max_kv) {
+    SB_ARG(type_ok(type), "attn_prefix: unknown element type");
+    SB_ARG(T >= 0 && B >= 0 && NH >= 1 && NKV >= 1 && NH % NKV == 0, "attn_prefix: need T, B >= 0 and NH % NKV == 0");
+    SB_ARG(HD >= 8 && HD <= 128 && HD % 8 == 0, "attn_prefix: the head size must be a multiple of 8, at most 128");
+    SB_ARG(max_q >= 1 && P >= 0 && max_kv >= 0 && P <= (1 << 30) && max_kv <= (1 << 30), "attn_prefix: bad lengths");
+    SB_ARG((int64_t)T * (NH / NKV) < (1 << 30) && (int64_t)max_q * (NH / NKV) < (1 << 30), "attn_prefix: too many rows");
+    return 0;
+}
+
+int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes) {
+    SB_ARG(bytes, "null pointer");
+    int rc = attn_args(type, T, B, NH, NKV, HD, max_q, prefix_len, max_kv);
+    if (rc) return rc;
+    *bytes = 0;
+    if (T == 0 || B == 0) return 0;
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    struct attn_part pre, own;
+    rc = attn_parts(c, type, T, B, NH, NKV, HD, max_q, prefix_len, max_kv, &pre, &own);
+    if (rc) return rc;
+    *bytes = attn_ws_bytes(T, NH, HD, &pre, &own);
+    return 0;
+}
+
+static int pages_for_attn(const sb_kv_pages *kv, struct attn_pages *p) {
+    const int e = type_size(kv->type);
+    SB_ARG(vec_ok(kv->type, kv->k, kv->page_stride, kv->pos_stride, kv->head_stride) && ALIGNED(kv->v, 16) && e,
+           "attn_prefix: pages need 16-byte aligned rows");
+    p->k = DP(kv->k);
+    p->v = DP(kv->v);
+    p->page_stride = kv->page_stride;
+    p->pos_stride = kv->pos_stride;
+    p->head_stride = kv->head_stride;
+    p->n_pages = kv->n_pages;
+    p->page = kv->page;
+    return 0;
+}
+
+int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
+                   int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
+                   int prefix_len, const sb_kv_pages *kv, const int *table, int table_stride, const int *kv_len, int max_kv,
+                   float scale, void *ws, size_t ws_bytes, void *stream) {
+    const sb_kv_pages *any = prefix_len > 0 ? prefix : kv;
+    int rc = pages_args(any);
+    if (!rc && prefix_len > 0 && max_kv > 0) rc = pages_args(kv);
+    if (!rc) rc = attn_args(any->type, T, B, NH, any->NKV, any->HD, max_q, prefix_len, max_kv);
+    if (rc) return rc;
+    SB_ARG(isfinite(scale), "attn_prefix: scale must be finite");
+    SB_ARG(cu_q || (T == B && max_q == 1), "attn_prefix: without cu_q there is one row a request (T == B, max_q == 1)");
+    if (T == 0 || B == 0) return 0;
+    SB_ARG(q && out && ALIGNED(lse, 4), "attn_prefix: null or misaligned pointer");
+    SB_ARG(vec_ok(any->type, q, q_row, q_head, 0) && vec_ok(any->type, out, o_row, o_head, 0),
+           "attn_prefix: query and output rows must be 16-byte aligned");
+    struct attn_params p;
+    memset(&p, 0, sizeof p);
+    if (prefix_len > 0) {
+        SB_ARG(prefix_table || prefix_len <= (int64_t)prefix->n_pages * prefix->page, "attn_prefix: the prefix exceeds its pages");
+        if ((rc = pages_for_attn(prefix, &p.pre))) return rc;
+    }
+    if (max_kv > 0) {
+        SB_ARG(table && kv_len, "attn_prefix: null table or lengths");
+        SB_ARG(kv->type == any->type && kv->NKV == any->NKV && kv->HD == any->HD,
+               "attn_prefix: prefix and own pages must have one type, head count and head size");
+        SB_ARG(table_stride >= CEIL_DIV(max_kv, kv->page), "attn_prefix: the table is narrower than max_kv positions");
+        if ((rc = pages_for_attn(kv, &p.suf))) return rc;
+    }
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    const int type = any->type, NKV = any->NKV, HD = any->HD;
+    struct attn_part pre, own;
+    rc = attn_parts(c, type, T, B, NH, NKV, HD, max_q, prefix_len, max_kv, &pre, &own);
+    if (rc) return rc;
+    const size_t need = attn_ws_bytes(T, NH, HD, &pre, &own);
+    SB_ARG(ws_bytes >= need && (ws || need == 0) && ALIGNED(ws, 16), "attn_prefix: workspace too small (sb_attn_prefix_ws) or misaligned");
+    const size_t parts = (size_t)T * NH * (pre.S + own.S);
+    p.q = DP(q);
+    p.out = DP(out);
+    p.lse = DP(lse);
+    p.cu_q = DP(cu_q);
+    p.ptable = DP(prefix_table);
+    p.table = DP(table);
+    p.kv_len = DP(kv_len);
+    if (need) {
+        p.ws_o = DP(ws);
+        p.ws_ml = p.ws_o + parts * HD * 4;
+        p.ws_n = p.ws_ml + parts * 8;
+    }
+    p.q_row = q_row;
+    p.q_head = q_head;
+    p.o_row = o_row;
+    p.o_head = o_head;
+    p.T = T;
+    p.B = B;
+    p.NH = NH;
+    p.NKV = NKV;
+    p.G = NH / NKV;
+    p.HD = HD;
+    p.P = prefix_len;
+    p.max_kv = max_kv;
+    p.table_stride = table_stride;
+    p.chunk1 = pre.chunk;
+    p.S1 = pre.S;
+    p.chunk2 = own.chunk;
+    p.S2 = own.S;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    int zero = 0, one = 1;
+    if (pre.S) {
+        p.tiles = pre.tiles;
+        void *args[] = {&p, &zero};
+        rc = sb_launch(c, pre.f, (unsigned)pre.grid, 1, 128, pre.smem, (CUstream)stream, args, 0);
+        if (rc) return rc;
+    }
+    if (own.S) { /* beside the prefix launch's last items */
+        p.tiles = own.tiles;
+        void *args[] = {&p, &one};
+        rc = sb_launch(c, own.f, (unsigned)own.grid, 1, 128, own.smem, (CUstream)stream, args, pre.S > 0);
+        if (rc) return rc;
+    }
+    if (pre.S + own.S == 1) return 0;
+    long g = CEIL_DIV((long)T * NH, 4);
+    if (g > 16L * c->sms) g = 16L * c->sms;
+    void *args[] = {&p, (void *)&type};
+    return sb_launch(c, F_ATTN_JOIN, (unsigned)g, 1, 128, 0, (CUstream)stream, args, pre.S + own.S > 0);
+}
+
+/* ---------------------------------------------------------------- log probabilities */
+/* mirrors LpParams / LpGradParams in csrc/score_kernels.cu */
+struct lp_params {
+    CUdeviceptr x;
+    int64_t stride;
+    int R, V, S, k;
+    float c;
+    CUdeviceptr tok, logp, entropy, lse, rank, top_ids, top_logp, part, keys;
+};
+struct lp_grad_params {
+    CUdeviceptr x, dx;
+    int64_t stride, dstride;
+    int R, V, S;
+    float c, inv_temp;
+    CUdeviceptr tok, lse, entropy, g_logp, g_entropy;
+};
+/* parts of a row: enough CTAs for a few waves, 4 KB of logits each at least */
+static int lp_parts(sb_ctx *c, int R, int V, int type, long waves) {
+    long S = CEIL_DIV(waves * c->sms, (long)R), most = (long)V * type_size(type) / 4096;
+    if (S > most) S = most;
+    if (S > SB_LOGPROBS_MAX_PARTS) S = SB_LOGPROBS_MAX_PARTS;
+    return (int)(S < 1 ? 1 : S);
+}
+static int lp_args(int type, int R, int V, int top_k) {
+    SB_ARG(type_ok(type), "logprobs: unknown element type");
+    SB_ARG(R >= 0 && V >= 1 && V <= (1 << 30), "logprobs: bad sizes");
+    SB_ARG(top_k >= 0 && top_k <= 64 && top_k <= V, "logprobs: top_k must be 0..64 and at most V");
+    return 0;
+}
+static size_t lp_ws_bytes(int R, int S, int k) { return S > 1 ? (size_t)R * S * (16 + 8 * (size_t)k) : 0; }
+
+int sb_logprobs_ws(int type, int R, int V, int top_k, size_t *bytes) {
+    SB_ARG(bytes, "null pointer");
+    int rc = lp_args(type, R, V, top_k);
+    if (rc) return rc;
+    *bytes = 0;
+    if (R == 0) return 0;
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    *bytes = lp_ws_bytes(R, lp_parts(c, R, V, type, 8), top_k);
+    return 0;
+}
+
+int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
+                float *logp, float *entropy, float *lse, int *rank, int top_k, int *top_ids, float *top_logp, void *ws,
+                size_t ws_bytes, void *stream) {
+    int rc = lp_args(type, R, V, top_k);
+    if (rc) return rc;
+    SB_ARG(isfinite(temperature) && temperature > 0.0f && isfinite(1.4426950408889634f / temperature),
+           "logprobs: temperature must be positive");
+    SB_ARG(tokens || (!logp && !rank), "logprobs: logp and rank need tokens");
+    SB_ARG(top_k == 0 || top_ids || top_logp, "logprobs: top_k without an output");
+    if (R == 0) return 0;
+    SB_ARG(logits && ALIGNED(logits, type_size(type)) && (row_stride >= V || R == 1), "logprobs: bad logits or row stride");
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    struct lp_params p;
+    memset(&p, 0, sizeof p);
+    p.S = lp_parts(c, R, V, type, 8);
+    const size_t need = lp_ws_bytes(R, p.S, top_k);
+    SB_ARG(ws_bytes >= need && (ws || need == 0) && ALIGNED(ws, 16), "logprobs: workspace too small (sb_logprobs_ws) or misaligned");
+    p.x = DP(logits);
+    p.stride = row_stride;
+    p.R = R;
+    p.V = V;
+    p.k = top_k;
+    p.c = 1.4426950408889634f / temperature;
+    p.tok = DP(tokens);
+    p.logp = DP(logp);
+    p.entropy = DP(entropy);
+    p.lse = DP(lse);
+    p.rank = DP(rank);
+    p.top_ids = DP(top_ids);
+    p.top_logp = DP(top_logp);
+    p.part = DP(ws);
+    p.keys = p.part + (size_t)R * p.S * 16;
+    SB_ARG((int64_t)R * p.S < 0x7fffffffL, "logprobs: too many rows");
+    void *args[] = {&p};
+    rc = sb_launch(c, top_k ? BY_TYPE(F_LOGPROBS_TOP_F32, type) : BY_TYPE(F_LOGPROBS_F32, type), (unsigned)(R * p.S), 1, 256, 0,
+                   (CUstream)stream, args, 0);
+    if (rc || p.S == 1) return rc;
+    void *jargs[] = {&p, &type};
+    return sb_launch(c, F_LOGPROBS_JOIN, (unsigned)R, 1, 256, 0, (CUstream)stream, jargs, 1);
+}
+
+int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
+                     const float *lse, const float *entropy, const float *g_logp, const float *g_entropy, void *grad,
+                     int64_t grad_stride, void *stream) {
+    int rc = lp_args(type, R, V, 0);
+    if (rc) return rc;
+    SB_ARG(isfinite(temperature) && temperature > 0.0f && isfinite(1.4426950408889634f / temperature),
+           "logprobs_grad: temperature must be positive");
+    SB_ARG(tokens || !g_logp, "logprobs_grad: g_logp needs tokens");
+    if (R == 0) return 0;
+    SB_ARG(logits && grad && lse && (entropy || !g_entropy), "logprobs_grad: null pointer");
+    SB_ARG(ALIGNED(logits, type_size(type)) && ALIGNED(grad, type_size(type)), "logprobs_grad: misaligned rows");
+    SB_ARG(R == 1 || (row_stride >= V && grad_stride >= V), "logprobs_grad: bad row stride");
+    SB_ARG(logits != grad || R == 1 || row_stride == grad_stride, "logprobs_grad: in place needs one row stride");
+    sb_ctx *c = sb_ctx_get();
+    if (!c) return SB_ERR_STATE;
+    struct lp_grad_params p;
+    memset(&p, 0, sizeof p);
+    p.x = DP(logits);
+    p.dx = DP(grad);
+    p.stride = row_stride;
+    p.dstride = grad_stride;
+    p.R = R;
+    p.V = V;
+    p.S = lp_parts(c, R, V, type, 16);
+    p.c = 1.4426950408889634f / temperature;
+    p.inv_temp = 1.0f / temperature;
+    p.tok = DP(tokens);
+    p.lse = DP(lse);
+    p.entropy = DP(entropy);
+    p.g_logp = DP(g_logp);
+    p.g_entropy = DP(g_entropy);
+    SB_ARG((int64_t)R * p.S < 0x7fffffffL, "logprobs_grad: too many rows");
+    void *args[] = {&p};
+    return sb_launch(c, BY_TYPE(F_LOGPROBS_GRAD_F32, type), (unsigned)(R * p.S), 1, 256, 0, (CUstream)stream, args, 0);
+}

@@ -17,7 +17,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(_HERE, "lib")
 BIN_DIR = os.path.join(_HERE, "bin")
 LIB_PATH = os.path.join(LIB_DIR, "libswitch_b200.so")
-CUBINS = {m: os.path.join(LIB_DIR, m + ".cubin") for m in ("switch_gpu", "gemv", "gpt2", "qwen", "tc")}
+CUBINS = {m: os.path.join(LIB_DIR, m + ".cubin") for m in
+          ("switch_gpu", "gemv", "gpt2", "qwen", "tc", "serve", "score")}
 
 MODEL_QWEN = 1
 MODEL_GPT2 = 2
@@ -31,6 +32,23 @@ GEN_STOP_EOS = 1
 QWEN = dict(V=151936, C=896, NL=24, NH=14, NKV=2, HD=64, FC=4864, CTX_FILE=8192,
             FILE_BYTES=990162688, EOT=151643, IM_END=151645)
 GPT2 = dict(V=50257, C=768, NL=12, NH=12, HD=64, FC=3072, CTX=1024, TOTAL_FLOATS=124439808, EOT=50256)
+
+F32, F16, BF16 = 0, 1, 2  # element types of the batch operators
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN, ROPE_BANDS = range(5)
+
+
+class _KvPages(ctypes.Structure):
+    """sb_kv_pages"""
+    _fields_ = ([("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+                + [(n, ctypes.c_int64) for n in ("page_stride", "pos_stride", "head_stride")]
+                + [(n, ctypes.c_int) for n in ("type", "n_pages", "page", "NKV", "HD")])
+
+
+class _RotaryPlan(ctypes.Structure):
+    """sb_rotary_plan"""
+    _fields_ = [("turn", ctypes.c_uint64 * 128), ("mscale", ctypes.c_float), ("dim", ctypes.c_int), ("layout", ctypes.c_int)]
+
 
 _lib = None
 _cuda_is_stub = False
@@ -106,6 +124,16 @@ def lib():
     _sig(L.sb_nccl_abort, I, P)
     _sig(L.sb_sgemm_panel_allgather, I, P, P, P, I, I, I, I, I, P, I, P)
     _sig(L.sb_nccl_wait, I, P, P, ctypes.c_double)
+    L64, SZ = ctypes.c_int64, ctypes.c_size_t
+    _sig(L.sb_kv_plan, I, P, P, I, I, P, I, P, I, I, P, P, P, I, P, P, P, P)
+    _sig(L.sb_rotary_plan_init, I, P, I, I, D, I, D, I)
+    _sig(L.sb_rotary, I, P, L64, L64, P, L64, L64, I, I, I, I, P, P, I, P)
+    _sig(L.sb_rotary_kv, I, P, L64, L64, P, L64, L64, P, L64, L64, P, L64, L64, I, I, P, P, P, P, P)
+    _sig(L.sb_attn_prefix_ws, I, I, I, I, I, I, I, I, I, I, ctypes.POINTER(SZ))
+    _sig(L.sb_attn_prefix, I, P, L64, L64, P, L64, L64, P, I, I, P, I, I, P, P, I, P, P, I, P, I, F, P, SZ, P)
+    _sig(L.sb_logprobs_ws, I, I, I, I, I, ctypes.POINTER(SZ))
+    _sig(L.sb_logprobs, I, P, L64, I, I, I, F, P, P, P, P, P, I, P, P, P, SZ, P)
+    _sig(L.sb_logprobs_grad, I, P, L64, I, I, I, F, P, P, P, P, P, P, L64, P)
     _sig(L.sb_engine_create, P, I, ctypes.c_char_p, I, ctypes.c_uint)
     _sig(L.sb_engine_destroy, None, P)
     _sig(L.sb_engine_reset, I, P)
@@ -312,6 +340,203 @@ def layernorm(x, w, b, y, n, eps, rows=1, stream=None):
 
 def gelu(x, y, n, stream=None):
     check(lib().sb_gelu(_p(x), _p(y), n, _s(stream)))
+
+
+# ---------------------------------------------------------------- a batch that shares a prompt
+# These take torch tensors and read sizes, strides and types from them (the
+# calls above take sizes from the caller).  Shapes, types and devices that a
+# kernel would misread raise SbError before the call.
+def _need(ok, what):
+    if not ok:
+        raise SbError(what)
+
+
+def _type(t):
+    got = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}.get(str(t.dtype))
+    _need(got is not None, f"element type {t.dtype}: need float32, float16 or bfloat16")
+    return got
+
+
+def _on_device(*tensors):
+    """Every tensor is on the current CUDA device (the one whose context runs the call)."""
+    import torch
+    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise SbError(f"tensor on {t.device}: need the current CUDA device")
+
+
+def _vector(t, name, dtype, n):
+    """A contiguous vector (or matrix) of at least n entries of a type, or None."""
+    if t is None:
+        return
+    _need(str(t.dtype) == "torch." + dtype and t.is_contiguous() and t.numel() >= n,
+          f"{name}: need a contiguous {dtype} tensor of at least {n} entries")
+
+
+def _rows3(t, name):
+    """[rows, heads, head size] whose last dimension is contiguous."""
+    _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{name}: need [rows, heads, head size], values contiguous")
+
+
+class KvPages:
+    """Keys and values in pages, from tensors [pages, page, key heads, head
+    size] of one type and layout (any strides, values contiguous).  An
+    engine's cache seen as such tensors is a pool too."""
+
+    def __init__(self, k, v):
+        _need(k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype and k.stride(3) == 1,
+              "pages: need k and v [pages, page, heads, head size] of one layout, values contiguous")
+        _need(k.device == v.device, "pages: k and v on different devices")
+        self.k, self.v = k, v  # keeps the memory alive
+        self.c = _KvPages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), _type(k), *k.shape)
+        self.ref = ctypes.byref(self.c)
+
+
+class Rotary:
+    """Frequencies of rotary positions (sb_rotary_plan): dim rotated values of
+    a head, layout ROPE_HALF / ROPE_PAIRS, scaling ROPE_PLAIN / LINEAR / NTK /
+    YARN / BANDS by `factor` from the trained context orig_ctx."""
+
+    def __init__(self, dim, theta=10000.0, layout=ROPE_HALF, scaling=ROPE_PLAIN, factor=1.0, orig_ctx=0):
+        self.c = _RotaryPlan()
+        self.ref = ctypes.byref(self.c)
+        check(lib().sb_rotary_plan_init(self.ref, dim, layout, theta, scaling, factor, orig_ctx))
+
+
+def kv_plan(cache_len, new_len, free_pages, table, page, slots, pos, req, cu_q, kv_len, used, stream=None):
+    """Block tables, slot map, positions and row offsets of a step from its
+    requests' lengths (sb_kv_plan); int32 tensors, slots int64, table [B, width]."""
+    B, T = cache_len.numel(), slots.numel()
+    _on_device(cache_len, new_len, free_pages, table, slots, pos, req, cu_q, kv_len, used)
+    for t, n, m in ((cache_len, "cache_len", B), (new_len, "new_len", B), (free_pages, "free_pages", 0), (pos, "pos", T),
+                    (req, "req", T), (cu_q, "cu_q", B + 1), (kv_len, "kv_len", B), (used, "used", 2)):
+        _vector(t, n, "int32", m)
+    _vector(slots, "slots", "int64", T)
+    _need(table.dim() == 2 and table.shape[0] >= B and str(table.dtype) == "torch.int32" and table.stride(1) == 1,
+          "table: need an int32 [B, width] tensor with contiguous rows")
+    check(lib().sb_kv_plan(_p(cache_len), _p(new_len), B, page, _p(free_pages), free_pages.numel(), _p(table),
+                           table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1], _p(slots), _p(pos), _p(req), T,
+                           _p(cu_q), _p(kv_len), _p(used), _s(stream)))
+
+
+def rotary(x, y, pos, plan, inverse=False, stream=None):
+    """y = x [T, heads, head size] turned by pos (int32 [T]); inverse turns
+    back (the gradient).  y may be x."""
+    _rows3(x, "x")
+    _rows3(y, "y")
+    _need(x.shape == y.shape and x.dtype == y.dtype, "rotary: x and y differ in shape or type")
+    T, H, HD = x.shape
+    _vector(pos, "pos", "int32", T)
+    _on_device(x, y, pos)
+    check(lib().sb_rotary(_p(x), x.stride(0), x.stride(1), _p(y), y.stride(0), y.stride(1), _type(x), T, H, HD, _p(pos), plan.ref,
+                          1 if inverse else 0, _s(stream)))
+
+
+def rotary_kv(q, q_out, k, v, pos, slots, plan, kv, stream=None):
+    """q_out = q turned; k turned and v stored in the pages at slots (int64
+    [T], -1: nowhere).  q [T, NH, HD], k and v [T, NKV, HD]."""
+    for t, n in ((q, "q"), (q_out, "q_out"), (k, "k"), (v, "v")):
+        _rows3(t, n)
+    T, NH, HD = q.shape
+    _need(q.shape == q_out.shape and k.shape == v.shape == (T, kv.c.NKV, kv.c.HD) and HD == kv.c.HD,
+          "rotary_kv: q, k, v and the pages differ in rows, heads or head size")
+    _need(q.dtype == q_out.dtype == k.dtype == v.dtype == kv.k.dtype, "rotary_kv: rows and pages differ in type")
+    _vector(pos, "pos", "int32", T)
+    _vector(slots, "slots", "int64", T)
+    _on_device(q, q_out, k, v, pos, slots, kv.k)
+    check(lib().sb_rotary_kv(_p(q), q.stride(0), q.stride(1), _p(q_out), q_out.stride(0), q_out.stride(1), _p(k), k.stride(0),
+                             k.stride(1), _p(v), v.stride(0), v.stride(1), T, NH, _p(pos), _p(slots), plan.ref, kv.ref, _s(stream)))
+
+
+def attn_prefix_ws(q, kv, prefix_len, B, max_q=1, max_kv=0):
+    """Workspace bytes of attn_prefix for these sizes (kv: the prefix' or the
+    requests' pages)."""
+    n = ctypes.c_size_t()
+    check(lib().sb_attn_prefix_ws(_type(q), q.shape[0], B, q.shape[1], kv.c.NKV, kv.c.HD, max_q, prefix_len, max_kv, ctypes.byref(n)))
+    return n.value
+
+
+def attn_prefix(q, out, prefix, prefix_table, prefix_len, kv, table, kv_len, scale, ws, cu_q=None, max_q=1, max_kv=0, lse=None,
+                stream=None):
+    """Attention of a batch over a shared prefix (pages `prefix` through
+    prefix_table, None: in order) and each request's own pages (kv, table
+    [B, width], kv_len [B]); see sb_attn_prefix.  ws: a uint8 tensor of
+    attn_prefix_ws bytes, or None when that is 0."""
+    _rows3(q, "q")
+    _rows3(out, "out")
+    T, NH, HD = q.shape
+    _need(q.shape == out.shape, "attn_prefix: q and out differ in shape")
+    pools = [p for p, n in ((prefix, prefix_len), (kv, max_kv)) if n > 0]
+    _need(bool(pools) or prefix is not None or kv is not None, "attn_prefix: no pages")
+    for p in pools or [prefix or kv]:
+        _need(p is not None and p.c.HD == HD and p.k.dtype == q.dtype == out.dtype, "attn_prefix: rows and pages differ in head size or type")
+    B = T if cu_q is None else cu_q.numel() - 1
+    if max_kv > 0:
+        _need(table is not None and table.dim() == 2 and table.shape[0] >= B and str(table.dtype) == "torch.int32"
+              and (table.stride(1) == 1 or table.shape[1] == 1) and table.shape[1] * kv.c.page >= max_kv,
+              "table: need an int32 [B, width] tensor with contiguous rows, wide enough for max_kv")
+        _need(kv_len is not None, "attn_prefix: kv_len is missing")
+        _vector(kv_len, "kv_len", "int32", B)
+    if prefix_len > 0 and prefix_table is not None:
+        _vector(prefix_table, "prefix_table", "int32", -(-prefix_len // prefix.c.page))
+    _vector(cu_q, "cu_q", "int32", B + 1)
+    _vector(lse, "lse", "float32", T * NH)
+    _on_device(q, out, prefix_table, table, kv_len, cu_q, lse, ws, *[p.k for p in pools])
+    stride = 0
+    if max_kv > 0:
+        stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
+    check(lib().sb_attn_prefix(_p(q), q.stride(0), q.stride(1), _p(out), out.stride(0), out.stride(1), _p(lse), T, NH, _p(cu_q), B,
+                               max_q, prefix.ref if prefix is not None else None, _p(prefix_table), prefix_len,
+                               kv.ref if kv is not None else None, _p(table), stride, _p(kv_len), max_kv, scale, _p(ws),
+                               0 if ws is None else ws.numel() * ws.element_size(), _s(stream)))
+
+
+def logprobs_ws(logits, top_k=0):
+    """Workspace bytes of logprobs for these logits [R, V]."""
+    n = ctypes.c_size_t()
+    check(lib().sb_logprobs_ws(_type(logits), logits.shape[0], logits.shape[1], top_k, ctypes.byref(n)))
+    return n.value
+
+
+def _logits(t, name):
+    _need(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), f"{name}: need [rows, choices], choices contiguous")
+
+
+def logprobs(logits, tokens, ws, logp=None, entropy=None, lse=None, rank=None, top_ids=None, top_logp=None, temperature=1.0, stream=None):
+    """Log probability, rank (int32) and entropy of tokens (int32 [R], -1:
+    none) under logits [R, V] / temperature, and the best alternatives
+    (top_ids int32 / top_logp [R, k], k <= 64) in one pass; see sb_logprobs."""
+    _logits(logits, "logits")
+    R, V = logits.shape
+    k = 0
+    for t in (top_ids, top_logp):
+        if t is not None:
+            _need(t.dim() == 2 and t.shape[0] == R and (k == 0 or k == t.shape[1]), "top_ids and top_logp: need [R, k]")
+            k = t.shape[1]
+    for t, n, d, m in ((tokens, "tokens", "int32", R), (logp, "logp", "float32", R), (entropy, "entropy", "float32", R),
+                       (lse, "lse", "float32", R), (rank, "rank", "int32", R), (top_ids, "top_ids", "int32", R * k),
+                       (top_logp, "top_logp", "float32", R * k)):
+        _vector(t, n, d, m)
+    _on_device(logits, tokens, ws, logp, entropy, lse, rank, top_ids, top_logp)
+    check(lib().sb_logprobs(_p(logits), logits.stride(0) if R > 1 else V, _type(logits), R, V, temperature, _p(tokens), _p(logp), _p(entropy),
+                            _p(lse), _p(rank), k, _p(top_ids), _p(top_logp), _p(ws),
+                            0 if ws is None else ws.numel() * ws.element_size(), _s(stream)))
+
+
+def logprobs_grad(logits, tokens, lse, entropy, g_logp, g_entropy, grad, temperature=1.0, stream=None):
+    """grad [R, V] = the gradient of logp and entropy (weights g_logp,
+    g_entropy [R] or None) with respect to the logits; grad may be logits."""
+    _logits(logits, "logits")
+    _logits(grad, "grad")
+    R, V = logits.shape
+    _need(grad.shape == logits.shape and grad.dtype == logits.dtype, "logprobs_grad: logits and grad differ in shape or type")
+    for t, n, d in ((tokens, "tokens", "int32"), (lse, "lse", "float32"), (entropy, "entropy", "float32"), (g_logp, "g_logp", "float32"),
+                    (g_entropy, "g_entropy", "float32")):
+        _vector(t, n, d, R)
+    _on_device(logits, tokens, lse, entropy, g_logp, g_entropy, grad)
+    check(lib().sb_logprobs_grad(_p(logits), logits.stride(0) if R > 1 else V, _type(logits), R, V, temperature, _p(tokens), _p(lse),
+                                 _p(entropy), _p(g_logp), _p(g_entropy), _p(grad), grad.stride(0) if R > 1 else V, _s(stream)))
 
 
 # ---------------------------------------------------------------- synthetic inputs

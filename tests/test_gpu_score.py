@@ -1,0 +1,348 @@
+"""Log probabilities, entropy, rank, alternatives and their gradient on the
+GPU against plain implementations in 64 bits, and a serving step of all batch
+operators together."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import sb200
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def stream():
+    return torch.cuda.current_stream()
+
+
+def run(x, tok, k=0, temperature=1.0):
+    R, V = x.shape
+    got = {n: torch.full((R,), 77.0, device="cuda") for n in ("logp", "entropy", "lse")}
+    got["rank"] = torch.full((R,), 77, dtype=torch.int32, device="cuda")
+    top = {}
+    if k:
+        top = dict(top_ids=torch.full((R, k), 77, dtype=torch.int32, device="cuda"), top_logp=torch.full((R, k), 77.0, device="cuda"))
+    ws = torch.full((sb200.logprobs_ws(x, k),), 0xFF, dtype=torch.uint8, device="cuda")
+    sb200.logprobs(x, tok, ws, temperature=temperature, stream=stream(), **got, **top)
+    return got | top
+
+
+def reference(x, tok, k, temperature):
+    y = x.double() / temperature
+    lse = torch.logsumexp(y, -1)
+    none = lse == -math.inf
+    logs = y - lse[:, None]
+    p = torch.exp(logs)
+    entropy = -torch.where(p > 0, p * logs, torch.zeros_like(p)).sum(-1)
+    V = x.shape[1]
+    given = (tok >= 0) & (tok < V)
+    at = tok.long().clamp(0, V - 1)[:, None]
+    mine, ids = x.float().gather(1, at), torch.arange(V, device="cuda")
+    logp = torch.where(none, torch.full_like(lse, -math.inf), logs.gather(1, at)[:, 0])
+    rank = ((x.float() > mine) | ((x.float() == mine) & (ids < at))).sum(-1)
+    order = torch.sort(x.float() + 0.0, dim=-1, descending=True, stable=True).indices[:, :k]
+    listed = x.float().gather(1, order) > -math.inf
+    inf = torch.full_like(order, 1).double() * -math.inf
+    return dict(lse=lse, entropy=torch.where(none, torch.zeros_like(lse), entropy), logp=torch.where(given, logp, torch.zeros_like(lse)),
+                rank=torch.where(given, rank, torch.full_like(rank, -1)), top_ids=torch.where(listed, order, torch.full_like(order, -1)),
+                top_logp=torch.where(listed, logs.gather(1, order), inf))
+
+
+def check(x, tok, k, temperature=1.0):
+    """lse: its sum is off by (V / 256 + 16) half steps of FP32 in the longest
+    chain, 2^-22 of each exponential and the products' half step of |x| /
+    temperature; logp the same, entropy the same times ln V (its terms)."""
+    got, want = run(x, tok, k, temperature), reference(x, tok, k, temperature)
+    V = x.shape[1]
+    big = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).double().abs().amax(-1) / temperature
+    bound = (V / 256 + 16) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -22 * big
+    for n in ("lse", "logp", "entropy", "top_logp"):
+        if n not in got:
+            continue
+        a, b = got[n].double(), want[n]
+        fin = torch.isfinite(b)
+        assert torch.equal(a[~fin], b[~fin]), n
+        lim = (bound if a.dim() == 1 else bound[:, None].expand_as(a)) * (1 + math.log(V) if n == "entropy" else 2)
+        assert bool(((a - b).abs()[fin] <= lim[fin]).all()), (n, float((a - b).abs()[fin].max()))
+    for n in ("rank", "top_ids"):
+        if n in got:
+            assert torch.equal(got[n].long(), want[n]), n
+    return got
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("R,V,k,temperature,odd", [
+    (1, 1, 1, 1.0, 0), (3, 5, 5, 0.5, 1), (2, 64, 64, 1.0, 3), (5, 1000, 20, 0.7, 1), (1, 151936, 20, 0.7, 0), (7, 50257, 5, 1.3, 0),
+    (2, 151936, 64, 1.0, 5), (700, 777, 1, 1.0, 2), (40, 30001, 24, 1.0, 7), (33, 4099, 25, 2.0, 1), (1500, 129, 0, 1.0, 0), (4, 65536, 0, 1.0, 0)])
+def test_logprobs(cuda_dev, kind, R, V, k, temperature, odd):
+    g = torch.Generator("cuda").manual_seed(R + V)
+    x = (torch.randn(R, V + odd, device="cuda", generator=g) * 3).to(DT[kind])[:, :V]  # odd: rows at any 2-byte place
+    tok = torch.randint(0, V, (R,), device="cuda", generator=g).to(torch.int32)
+    if R > 3:
+        tok[1], tok[2] = -1, V
+        x[3, V // 2:] = -math.inf
+        tok[3] = V - 1  # a masked choice
+    check(x, tok, k, temperature)
+
+
+@pytest.mark.parametrize("kind", list(DT))
+def test_logprobs_ties_and_orders(cuda_dev, kind):
+    """Equal, rising and falling logits, signed zeros: the list is cut on the
+    way, and equal values go by id."""
+    V, t = 20011, DT[kind]
+    ramp = torch.arange(V, device="cuda", dtype=torch.float32) / V * 8 - 4
+    zero = torch.zeros(V, device="cuda")
+    zero[1::2] = -0.0
+    step = (torch.arange(V, device="cuda") // 100).float() / 16
+    x = torch.stack([torch.full((V,), 2.5, device="cuda"), ramp, ramp.flip(0), zero, step, step.flip(0)]).to(t)
+    tok = torch.tensor([V - 1, 0, 17, 4, 9000, V // 2], dtype=torch.int32, device="cuda")
+    for k in (1, 24, 64):
+        check(x, tok, k)
+    for r in range(x.shape[0]):  # one row: cut into parts
+        check(x[r: r + 1].contiguous(), tok[r: r + 1].contiguous(), 64)
+    check(x.repeat(200, 1), tok.repeat(200), 64)  # many rows: a CTA a row
+
+
+@pytest.mark.parametrize("R", [1, 1300])
+def test_logprobs_masked_rows(cuda_dev, R):
+    """Rows with no choice, one, and fewer than k."""
+    V = 5000
+    x = torch.full((R, V), -math.inf, device="cuda")
+    tok = torch.zeros(R, dtype=torch.int32, device="cuda")
+    check(x, tok, 20)
+    x[:, V - 1] = 3.0
+    check(x, tok, 20)
+    got = check(x, tok + V - 1, 20)
+    # the one choice's exponential 2^d, d = x c less its rounding, and its log2 are each off by at most 2^-22: ln p by 2^-21
+    assert bool((got["logp"].abs() <= 2.0 ** -21).all()) and bool((got["entropy"].abs() <= 2.0 ** -21).all()) and bool((got["rank"] == 0).all())
+    x[:, 100:110] = 3.0
+    check(x, tok + 105, 20)
+
+
+def test_logprobs_nan_and_inf(cuda_dev):
+    """A NaN or +inf makes its own row's sums NaN, no other row's."""
+    x = torch.randn(6, 3001, device="cuda")
+    tok = torch.arange(6, dtype=torch.int32, device="cuda")
+    clean = run(x, tok, 5)
+    x[1, 2000], x[4, 7] = math.nan, math.inf
+    got = run(x, tok, 5)
+    for n in ("lse", "logp", "entropy"):
+        assert torch.isnan(got[n][[1, 4]]).all(), n
+        assert torch.equal(got[n][[0, 2, 3, 5]], clean[n][[0, 2, 3, 5]]), n
+    assert torch.equal(got["top_ids"][[0, 2, 3, 5]], clean["top_ids"][[0, 2, 3, 5]])
+
+
+def test_logprobs_some_outputs(cuda_dev):
+    """Any output may be absent; without tokens lse, entropy and the
+    alternatives remain."""
+    x = torch.randn(3, 40000, device="cuda")
+    full = run(x, torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"), 7)
+    ws = torch.empty(sb200.logprobs_ws(x, 7), dtype=torch.uint8, device="cuda")
+    lse, ids = torch.empty(3, device="cuda"), torch.empty(3, 7, dtype=torch.int32, device="cuda")
+    sb200.logprobs(x, None, ws, lse=lse, stream=stream())
+    sb200.logprobs(x, None, ws, top_ids=ids, stream=stream())
+    assert torch.allclose(lse, full["lse"], rtol=1e-6) and torch.equal(ids, full["top_ids"])
+    with pytest.raises(sb200.SbError, match="workspace"):
+        sb200.logprobs(x, None, None, lse=lse)
+    with pytest.raises(sb200.SbError, match="tokens"):
+        sb200.logprobs(x, None, ws, logp=lse)
+
+
+def gradient(x, tok, gl, ge, temperature):
+    y = x.double() / temperature
+    logs = torch.log_softmax(y, -1)
+    p = torch.exp(logs)
+    plogp = torch.where(p > 0, p * logs, torch.zeros_like(p))
+    h = -plogp.sum(-1, keepdim=True)
+    V = x.shape[1]
+    given = (tok >= 0) & (tok < V)
+    gl = torch.where(given, gl.double(), torch.zeros_like(gl.double()))[:, None]
+    hot = torch.zeros_like(p).scatter_(1, tok.long().clamp(0, V - 1)[:, None], gl)
+    return (hot - gl * p - ge.double()[:, None] * (plogp + p * h)) / temperature
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("R,V,temperature,odd", [(1, 1, 1.0, 0), (3, 129, 0.7, 1), (2, 151936, 1.0, 0), (300, 5001, 1.4, 0), (17, 50257, 1.0, 4)])
+def test_logprobs_gradient(cuda_dev, kind, R, V, temperature, odd):
+    """Against the formula: p is off by what lse is off (check() above; half a
+    step of FP32 of lse itself) and 2^-22 of the exponential, then one
+    rounding to the type."""
+    g = torch.Generator("cuda").manual_seed(V)
+    t = DT[kind]
+    x = (torch.randn(R, V + odd, device="cuda", generator=g) * 2).to(t)[:, :V]
+    tok = torch.randint(0, V, (R,), device="cuda", generator=g).to(torch.int32)
+    if R > 2:
+        tok[1] = -1
+        x[2, : V // 2] = -math.inf
+    gl, ge = (torch.randn(R, device="cuda", generator=g) for _ in range(2))
+    f = run(x, tok, 0, temperature)
+    want = gradient(x, tok, gl, ge, temperature)
+    big = torch.where(torch.isfinite(x), x, torch.zeros_like(x)).double().abs().amax(-1) / temperature
+    rel = (V / 256 + 16) * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -21 * (big + math.log(V) + 1)
+    p = torch.softmax(x.double() / temperature, -1)
+    size = p * (gl.double().abs()[:, None] + ge.double().abs()[:, None] * (2 * math.log(V) + 2 * big[:, None] + 2)) / temperature
+    hot = torch.zeros_like(p).scatter_(1, tok.long().clamp(0, V - 1)[:, None], gl.double().abs()[:, None] / temperature)
+    bound = rel[:, None] * size + 2.0 ** -23 * hot + torch.finfo(t).eps / 2 * want.abs() + (2.0 ** -25 if t == torch.float16 else 1e-37)
+    same = torch.empty(R, V + odd, dtype=t, device="cuda")[:, :V]     # rows placed as the logits'
+    other = torch.empty(R, V + 1 - odd % 2, dtype=t, device="cuda")[:, :V]  # and not
+    for grad in (same, other):
+        grad.fill_(7)
+        sb200.logprobs_grad(x, tok, f["lse"], f["entropy"], gl, ge, grad, temperature=temperature, stream=stream())
+        err = (grad.double() - want).abs()
+        assert bool((err <= bound).all()), float((err / bound).max())
+    z = x.clone() if odd == 0 else x
+    sb200.logprobs_grad(z, tok, f["lse"], f["entropy"], gl, ge, z, temperature=temperature, stream=stream())
+    assert torch.equal(z, same)  # in place
+
+
+def test_logprobs_gradient_against_differences(cuda_dev):
+    """Central differences of the forward call: with h = 2^-5 their own error
+    is h^2 / 6 of a third derivative below 2, the sums' rounding 2^-20 / h."""
+    R, V, h = 2, 37, 2.0 ** -5
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(R, V, device="cuda", generator=g)
+    tok = torch.tensor([3, 30], dtype=torch.int32, device="cuda")
+    gl, ge = torch.tensor([1.0, -0.5], device="cuda"), torch.tensor([0.7, 1.0], device="cuda")
+    f, grad = run(x, tok, 0, 0.8), torch.empty_like(x)
+    sb200.logprobs_grad(x, tok, f["lse"], f["entropy"], gl, ge, grad, temperature=0.8, stream=stream())
+    for v in (0, 3, 17, 30, 36):
+        vals = []
+        for s in (h, -h):
+            z = x.clone()
+            z[:, v] += s
+            r = run(z, tok, 0, 0.8)
+            vals.append((gl * r["logp"]).double() + (ge * r["entropy"]).double())
+        diff = (vals[0] - vals[1]) / (2 * h)
+        assert bool(((diff - grad[:, v].double()).abs() < h * h / 6 * 2 / 0.8 ** 3 * 1.7 + 2.0 ** -20 / h).all())
+
+
+def test_logprobs_gradient_parts(cuda_dev):
+    """One weight alone, none, and a row of masked choices."""
+    x = torch.randn(3, 1000, device="cuda")
+    x[1] = -math.inf
+    tok = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+    f = run(x, tok)
+    w = torch.tensor([1.0, 2.0, -3.0], device="cuda")
+    both, a, b, none = (torch.empty_like(x) for _ in range(4))
+    call = lambda gl, ge, out: sb200.logprobs_grad(x, tok, f["lse"], f["entropy"], gl, ge, out, stream=stream())  # noqa: E731
+    call(w, w, both), call(w, None, a), call(None, w, b), call(None, None, none)
+    assert bool((both[1] == 0).all()) and bool((a[1] == 0).all()) and bool((b[1] == 0).all()) and bool((none == 0).all())
+    # two values of each size, each sum rounded once, the exponents' 2^-20 apart
+    assert bool(((both - a - b).abs() <= 2.0 ** -19 * (a.abs() + b.abs()) + 1e-9).all())
+
+
+def test_logprobs_repeats_and_replays(cuda_dev):
+    x = torch.randn(5, 60001, device="cuda").half()
+    tok = torch.arange(5, dtype=torch.int32, device="cuda")
+    a = run(x, tok, 33)
+    k = a["top_ids"].shape[1]
+    out = {n: torch.zeros_like(v) for n, v in a.items()}
+    ws = torch.empty(sb200.logprobs_ws(x, k), dtype=torch.uint8, device="cuda")
+    sb200.logprobs(x, tok, ws, stream=stream(), **out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sb200.logprobs(x, tok, ws, stream=stream(), **out)
+    for _ in range(2):
+        for v in out.values():
+            v.fill_(3)
+        graph.replay()
+        assert all(torch.equal(out[n], a[n]) for n in a)
+    x.copy_(torch.randn(5, 60001, device="cuda"))
+    graph.replay()
+    b = run(x, tok, 33)
+    assert all(torch.equal(out[n], b[n]) for n in b)
+
+
+# ---------------------------------------------------------------- all together
+@pytest.mark.parametrize("kind,NH,NKV,HD,page", [("f32", 14, 2, 64, 16), ("f16", 8, 2, 128, 24), ("bf16", 6, 6, 64, 1)])
+def test_serving_steps_together(cuda_dev, kind, NH, NKV, HD, page):
+    """Three requests behind one prompt: the prompt's own plan and cache write,
+    a step of ragged continuations, then decode steps that grow past page
+    ends, each plan -> rotary with the cache write -> attention -> head
+    product -> log probabilities, against one attention layer in 64 bits
+    over the whole sequences."""
+    t, V, P, B = DT[kind], 997, 37, 3
+    g = torch.Generator("cuda").manual_seed(HD)
+    C = NH * HD
+    steps = [[5, 1, 9], [1, 1, 1], [1, 0, 20], [1, 1, 1]]
+    n_pages, W = 80, 64
+    kc, vc = (torch.full((n_pages, page, NKV, HD), float("nan"), dtype=t, device="cuda") for _ in range(2))
+    kv, plan = sb200.KvPages(kc, vc), sb200.Rotary(HD, theta=1e4)
+    head = (torch.randn(V, C, device="cuda", generator=g) * C ** -0.5)
+    f = torch.tensor([1e4 ** (-2.0 * i / HD) for i in range(HD // 2)], dtype=torch.float64, device="cuda")
+    e32 = lambda n, ty=torch.int32: torch.full((n,), 99, dtype=ty, device="cuda")  # noqa: E731
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    free = torch.randperm(n_pages, device="cuda", generator=g).to(torch.int32)
+    at = 0
+
+    def plan_step(cache, new, table, T):
+        nonlocal at
+        n = cache.numel()
+        o = dict(slots=e32(T, torch.int64), pos=e32(T), req=e32(T), cu_q=e32(n + 1), kv_len=e32(n), used=e32(2))
+        sb200.kv_plan(cache, new, free[at:].contiguous(), table, page, stream=stream(), **o)
+        taken, lacking = o["used"].tolist()
+        assert lacking == 0
+        at += taken
+        return o
+
+    def turn(x, pos):  # 64 bits, half layout
+        a = pos.double()[:, None, None] * f
+        u, w = x.double()[..., : HD // 2], x.double()[..., HD // 2:]
+        return torch.cat([u * torch.cos(a) - w * torch.sin(a), w * torch.cos(a) + u * torch.sin(a)], -1)
+
+    rows = lambda T: (torch.randn(T, NH + 2 * NKV, HD, device="cuda", generator=g)).to(t)  # noqa: E731
+    # the prompt: one request of its own
+    ptable = torch.full((1, W), -1, dtype=torch.int32, device="cuda")
+    x = rows(P)
+    q, k, v = x.split([NH, NKV, NKV], 1)
+    o = plan_step(i32([0]), i32([P]), ptable, P)
+    sb200.rotary_kv(q, torch.empty(P, NH, HD, dtype=t, device="cuda"), k, v, o["pos"], o["slots"], plan, kv, stream=stream())
+    u = torch.finfo(t).eps / 2
+    full_k = [turn(k, o["pos"]).to(t).double()] * B  # what the pages hold: rounded once
+    full_v = [v.double()] * B
+    table = torch.full((B, W), -1, dtype=torch.int32, device="cuda")
+    cache = i32([0] * B)
+    for new in steps:
+        T = sum(new) + 2  # two rows of padding
+        x = rows(T)
+        q, k, v = x.split([NH, NKV, NKV], 1)
+        o = plan_step(cache, i32(new), table, T)
+        pos = torch.where(o["pos"] >= 0, o["pos"] + P, o["pos"])
+        qr, out = torch.zeros(T, NH, HD, dtype=t, device="cuda"), torch.zeros(T, NH, HD, dtype=t, device="cuda")
+        sb200.rotary_kv(q, qr, k, v, pos, o["slots"], plan, kv, stream=stream())
+        most = int(o["kv_len"].max())
+        ws = torch.empty(sb200.attn_prefix_ws(qr, kv, P, B, max_q=max(new), max_kv=most), dtype=torch.uint8, device="cuda")
+        sb200.attn_prefix(qr, out, kv, ptable[0], P, kv, table, o["kv_len"], HD ** -0.5, ws, cu_q=o["cu_q"], max_q=max(new), max_kv=most,
+                          stream=stream())
+        live = sum(new)
+        logits = torch.empty(T, V, device="cuda")
+        h = out.flatten(1).float().contiguous()
+        sb200.check(sb200.lib().sb_gemv_multi_f32(head.data_ptr(), h.data_ptr(), None, logits.data_ptr(), C, V, T, stream().cuda_stream))
+        tok = torch.where(o["req"] >= 0, torch.randint(0, V, (T,), device="cuda", generator=g).to(torch.int32), -1).to(torch.int32)
+        lp, ids = torch.empty(T, device="cuda"), torch.empty(T, 3, dtype=torch.int32, device="cuda")
+        ws = torch.empty(sb200.logprobs_ws(logits, 3), dtype=torch.uint8, device="cuda")
+        sb200.logprobs(logits, tok, ws, logp=lp, top_ids=ids, stream=stream())
+        r = 0
+        for b, n in enumerate(new):
+            p = P + int(cache[b]) + torch.arange(n, device="cuda")
+            full_k[b] = torch.cat([full_k[b], turn(k[r: r + n], p).to(t).double()])
+            full_v[b] = torch.cat([full_v[b], v[r: r + n].double()])
+            for i in range(n):
+                sees = P + int(cache[b]) + i + 1
+                qd = turn(q[r: r + 1], p[i: i + 1])[0].view(NKV, NH // NKV, HD)
+                w = torch.softmax(torch.einsum("hgd,khd->hgk", qd, full_k[b][:sees]) * HD ** -0.5, -1)
+                want = torch.einsum("hgk,khd->hgd", w, full_v[b][:sees]).reshape(-1)
+                size = torch.einsum("hgk,khd->hgd", w, full_v[b][:sees].abs()).reshape(-1)
+                # query rounded once (scores of size |q k| off by half a step: 12 of it), keys at worst to the other
+                # neighbour (the same again), weights and result rounded once
+                err = (out[r].flatten().double() - want).abs()
+                assert bool((err <= (26 * u + 2e-5) * size + u * want.abs()).all()), (b, i, float((err / size).max()))
+                logs = torch.log_softmax(head.double() @ out[r].flatten().double(), -1)
+                assert abs(float(lp[r]) - float(logs[int(tok[r])])) < 1e-4  # FP32 product of C <= 1024 terms of size 1 / 32
+                best = torch.sort(logs, descending=True).values[:3]
+                assert bool(((logs[ids[r].long()] - best).abs() < 1e-4).all())
+                r += 1
+        assert bool((out[live:] == 0).all()) and lp[live:].tolist() == [0.0, 0.0]
+        cache = o["kv_len"]

@@ -1,0 +1,539 @@
+"""Page plan, rotary positions and shared-prefix attention on the GPU against
+plain implementations in 64 bits, at the sizes, masks, strides and tables
+where they can go wrong."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import sb200
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def stream():
+    return torch.cuda.current_stream()
+
+
+# ---------------------------------------------------------------- plan
+def plan_reference(cache, new, page, free, table, width, T):
+    table = [list(r) for r in table]
+    at = total = lacking = 0
+    slots, pos, req, cu = [], [], [], [0]
+    for b, (c, n) in enumerate(zip(cache, new)):
+        c, n = max(c, 0), max(n, 0)
+        have, need = -(-c // page), -(-(c + n) // page)
+        for j in range(have, need):
+            if j >= width:
+                lacking += 1
+                continue
+            table[b][j] = free[at] if at < len(free) else -1
+            lacking += at >= len(free)
+            total += at < len(free)
+            at += 1
+        for p in range(c, c + n):
+            pg = table[b][p // page] if p // page < width else -1
+            slots.append(pg * page + p % page if pg >= 0 else -1)
+            pos.append(p)
+            req.append(b)
+        cu.append(cu[-1] + n)
+    pad = lambda v: (v + [-1] * T)[:T]  # noqa: E731
+    return table, pad(slots), pad(pos), pad(req), cu, [max(c, 0) + max(n, 0) for c, n in zip(cache, new)], [total, lacking]
+
+
+@pytest.mark.parametrize("B,page,most_new,short,pad", [
+    (1, 16, 1, 0, 0), (2, 1, 3, 0, 1), (7, 16, 40, 0, 5), (33, 24, 5, 7, 0), (64, 128, 300, 0, 3), (600, 16, 9, 11, 2), (1500, 3, 2, 0, -50),
+    (16384, 8, 1, 0, 0)])
+def test_kv_plan(cuda_dev, B, page, most_new, short, pad):
+    rng = np.random.RandomState(B)
+    cache = rng.randint(0, 5 * page + 2, B).tolist()
+    new = (rng.randint(0, most_new + 1, B) if most_new > 1 else np.ones(B, int)).tolist()
+    if B > 5:
+        cache[3], new[2], new[4], new[B - 1] = -4, -1, 0, 0
+    width = 6 + most_new // page - (1 if B == 33 else 0)
+    table = np.full((B, width), -7, np.int32)
+    k = 0
+    for b in range(B):
+        n = min(-(-max(cache[b], 0) // page), width)
+        table[b, :n] = np.arange(k, k + n)
+        k += n
+    add = sum(-(-(max(c, 0) + max(n, 0)) // page) - -(-max(c, 0) // page) for c, n in zip(cache, new))
+    free = (10 ** 6 + rng.permutation(max(add - short, 1))).astype(np.int32)
+    T = max(sum(max(n, 0) for n in new) + pad, 0)
+    want = plan_reference(cache, new, page, free.tolist(), table.tolist(), width, T)
+    d_table = torch.full((B, width + 3), -9, dtype=torch.int32, device="cuda")  # rows wider than the table that is passed
+    d_table[:, :width] = torch.from_numpy(table).cuda()
+    view = d_table[:, :width]
+    slots = torch.full((T + 2,), 77, dtype=torch.int64, device="cuda")
+    pos, req = (torch.full((T + 2,), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+    cu, kv, used = i32([77] * (B + 2)), i32([77] * (B + 1)), i32([77] * 3)
+    for _ in range(2):  # a second run on its own table gives the same
+        sb200.kv_plan(i32(cache), i32(new), torch.from_numpy(free).cuda(), view, page, slots[:T], pos[:T], req[:T], cu, kv, used, stream=stream())
+        got = view.tolist(), slots[:T].tolist(), pos[:T].tolist(), req[:T].tolist(), cu[: B + 1].tolist(), kv[:B].tolist(), used[:2].tolist()
+        for name, a, b in zip(("table", "slots", "pos", "req", "cu_q", "kv_len", "used"), got, want):
+            assert a == b, name
+    # nothing past what was passed
+    assert slots[T:].tolist() == [77, 77] and pos[T:].tolist() == [77, 77] and cu[B + 1:].tolist() == [77] and kv[B:].tolist() == [77]
+    assert used[2].item() == 77 and bool((d_table[:, width:] == -9).all())
+
+
+def test_kv_plan_absent_pages_and_no_free(cuda_dev):
+    """A free list that is empty, or padded with -1, and a table entry that is
+    not there: their tokens get no slot."""
+    table = i32([[3, -1, -5], [-5, -5, -5]])
+    out = lambda n, t=torch.int32: torch.zeros(n, dtype=t, device="cuda")  # noqa: E731
+    slots, pos, req, cu, kv, used = out(6, torch.int64), out(6), out(6), out(3), out(2), out(2)
+    sb200.kv_plan(i32([3, 0]), i32([3, 2]), i32([8, -1]), table, 2, slots, pos, req, cu, kv, used, stream=stream())
+    # request 0: position 3 in its page 1 (absent), 4 and 5 in the new page 8; request 1 in the absent new page
+    assert table.tolist() == [[3, -1, 8], [-1, -5, -5]]
+    assert slots.tolist() == [-1, 16, 17, -1, -1, -1] and pos.tolist() == [3, 4, 5, 0, 1, -1] and used.tolist() == [2, 0]
+    sb200.kv_plan(i32([0, 0]), i32([1, 0]), out(0), table, 2, slots, pos, req, cu, kv, used, stream=stream())
+    assert table.tolist()[0][0] == -1 and used.tolist() == [0, 1] and slots.tolist() == [-1] * 6
+
+
+# ---------------------------------------------------------------- rotary
+def frequencies(dim, theta, scaling, factor, orig):
+    i = np.arange(dim // 2)
+    if scaling == sb200.ROPE_NTK:
+        theta = theta * factor ** (dim / (dim - 2))
+    f = theta ** (-2.0 * i / dim)
+    m = 1.0
+    if scaling == sb200.ROPE_LINEAR:
+        f = f / factor
+    elif scaling == sb200.ROPE_YARN:
+        low = max(math.floor(dim * math.log(orig / (32 * 2 * math.pi)) / (2 * math.log(theta))), 0)
+        high = min(math.ceil(dim * math.log(orig / (2 * math.pi)) / (2 * math.log(theta))), dim - 1)
+        r = np.clip((i - low) / (high - low if high > low else 0.001), 0, 1)
+        f, m = f / factor * r + f * (1 - r), 0.1 * math.log(factor) + 1
+    elif scaling == sb200.ROPE_BANDS:
+        s = np.clip((orig * f / (2 * math.pi) - 1) / 3, 0, 1)
+        f = f / factor * (1 - s) + f * s
+    return torch.tensor(f, device="cuda"), m
+
+
+def turned(x, pos, f, m, layout, inverse=False):
+    """The rotation in 64 bits, and per value the |a| + |b| of its pair."""
+    d = 2 * f.numel()
+    y, size = x.double().clone(), x.double().abs()
+    t = pos.double()[:, None, None] * f
+    c, s = torch.cos(t) * m, torch.sin(t) * m * (-1 if inverse else 1)
+    ia, ib = (slice(0, d // 2), slice(d // 2, d)) if layout == sb200.ROPE_HALF else (slice(0, d, 2), slice(1, d, 2))
+    a, b = x.double()[..., ia], x.double()[..., ib]
+    y[..., ia], y[..., ib] = a * c - b * s, b * c + a * s
+    size[..., ia] = size[..., ib] = a.abs() + b.abs()
+    return y, size
+
+
+def rotary_bound(want, size, m, t):
+    """cos and sin are off by at most 2.7e-7: the phase's 2^-25 half turns
+    (9.4e-8), two ulp of sincospif (1.2e-7), the product with m (6e-8); the
+    products add 1.2e-7 of |a| + |b|; then one rounding to the type: half a
+    step relative to the value, for fp16 below 2^-14 half of the 2^-24 that its
+    subnormals are apart."""
+    return 4e-7 * m * size + half_step(t) * want.abs() + (2.0 ** -25 if t == torch.float16 else 1e-30)
+
+
+@pytest.mark.parametrize("T,H,HD,dim,layout,scaling,far,kind", [
+    (1, 14, 64, 64, 0, 0, 100, "f32"), (5, 3, 128, 32, 1, 3, 1 << 20, "bf16"), (130, 2, 80, 80, 0, 4, 1 << 17, "f16"),
+    (33, 1, 64, 16, 1, 2, 1 << 20, "f32"), (700, 5, 256, 256, 0, 1, 1 << 30, "f32"), (3, 7, 8, 4, 0, 0, 2 ** 31 - 1, "bf16"),
+    (2500, 6, 96, 48, 1, 0, 4096, "f16"), (9, 2, 6, 2, 1, 0, 50, "f32"), (41, 4, 64, 64, 1, 3, 2 ** 31 - 1, "f16")])
+@pytest.mark.parametrize("odd", [False, True])
+def test_rotary_rows(cuda_dev, T, H, HD, dim, layout, scaling, far, kind, odd):
+    t = DT[kind]
+    g = torch.Generator("cuda").manual_seed(T + H)
+    extra = 1 if odd else 8  # odd: token strides that are no multiple of a vector
+    x = torch.randn(T, H * HD + extra, device="cuda", generator=g).to(t)[:, : H * HD].unflatten(1, (H, HD))
+    pos = torch.randint(0, far, (T,), device="cuda", generator=g).to(torch.int32)
+    pos[0] = far - 1
+    if T > 4:
+        pos[3] = -1
+    plan = sb200.Rotary(dim, theta=1e6, layout=layout, scaling=scaling, factor=16.0, orig_ctx=4096)
+    f, m = frequencies(dim, 1e6, scaling, 16.0, 4096)
+    for inverse in (False, True):
+        y = torch.full((T, H, HD), 7.0, dtype=t, device="cuda")
+        sb200.rotary(x, y, pos, plan, inverse=inverse, stream=stream())
+        want, size = turned(x, pos, f, m, layout, inverse)
+        live = pos >= 0
+        # angles of 2^31 positions: the plan's fractions are good to 2^-54 of a turn per position (pow), the reference's product to 2^-53 of it
+        slack = 2 * math.pi * far * 2.0 ** -52 * m
+        err = (y.double() - want).abs()[live]
+        assert bool((err <= (rotary_bound(want, size, m, t) + slack * size)[live]).all()), float(err.max())
+        assert torch.equal(y[..., dim:][live], x[..., dim:][live])
+        if T > 4:
+            assert bool((y[3] == 7).all())  # a row of padding is left as it was
+    z = x.clone()  # in place
+    sb200.rotary(z, z, pos, plan, inverse=True, stream=stream())
+    assert torch.equal(z[live], y[live]) and (T <= 4 or torch.equal(z[3], x[3]))
+
+
+def test_rotary_inverse_is_the_gradient(cuda_dev):
+    """<w, d rotary(x)> against differences of the rotation itself: it is
+    linear, so a step of 1 has no error but the rounding of its values."""
+    T, H, HD, dim = 3, 2, 16, 12
+    g = torch.Generator("cuda").manual_seed(0)
+    x, w = (torch.randn(T, H, HD, device="cuda", generator=g) for _ in range(2))
+    pos, plan = i32([5, 1000, 77777]), sb200.Rotary(dim, theta=1e4, layout=sb200.ROPE_PAIRS, scaling=sb200.ROPE_YARN, factor=4.0, orig_ctx=512)
+    grad, y0, y1 = (torch.empty_like(x) for _ in range(3))
+    sb200.rotary(w, grad, pos, plan, inverse=True, stream=stream())
+    sb200.rotary(x, y0, pos, plan, stream=stream())
+    for t, h, i in ((0, 0, 0), (1, 1, 7), (2, 0, 11), (2, 1, 15)):
+        z = x.clone()
+        z[t, h, i] += 1.0
+        sb200.rotary(z, y1, pos, plan, stream=stream())
+        diff = float(((y1 - y0).double() * w.double()).sum())
+        assert abs(diff - float(grad[t, h, i])) < 64 * 2.0 ** -24 * 8  # a few values of size <= 8, each off by a few half steps
+
+
+@pytest.mark.parametrize("kind,page,HD,dim", [("f32", 16, 64, 64), ("f16", 1, 128, 64), ("bf16", 24, 80, 40), ("f16", 7, 10, 6)])
+def test_rotary_kv(cuda_dev, kind, page, HD, dim):
+    t, T, NH, NKV = DT[kind], 61, 6, 2
+    g = torch.Generator("cuda").manual_seed(page)
+    qkv = torch.randn(T, NH + 2 * NKV, HD, device="cuda", generator=g).to(t)
+    q, k, v = qkv.split([NH, NKV, NKV], 1)
+    n_pages = -(-T // page) + 2
+    pool = torch.full((n_pages, page, 2, NKV, HD), 5.0, dtype=t, device="cuda")  # keys and values side by side
+    kc, vc = pool[:, :, 0], pool[:, :, 1]
+    slots = torch.randperm(n_pages * page, device="cuda", generator=g)[:T].contiguous()
+    pos = torch.randint(0, 9000, (T,), device="cuda", generator=g).to(torch.int32)
+    slots[4], slots[5], pos[6] = -1, n_pages * page, -1  # no slot, a slot outside the pool, padding
+    q_out = torch.full((T, NH, HD), 5.0, dtype=t, device="cuda")
+    plan = sb200.Rotary(dim, theta=1e5)
+    sb200.rotary_kv(q, q_out, k, v, pos, slots, plan, sb200.KvPages(kc, vc), stream=stream())
+    f, m = frequencies(dim, 1e5, 0, 1.0, 0)
+    live = pos >= 0
+    want, size = turned(q, pos, f, m, 0)
+    assert bool(((q_out.double() - want).abs() <= rotary_bound(want, size, m, t))[live].all()) and bool((q_out[6] == 5).all())
+    stored = live & (slots >= 0) & (slots < n_pages * page)
+    want, size = turned(k, pos, f, m, 0)
+    at = slots[stored]
+    got = kc[at // page, at % page].double()
+    assert bool(((got - want[stored]).abs() <= rotary_bound(want, size, m, t)[stored]).all())
+    assert torch.equal(vc[at // page, at % page], v[stored])
+    left = torch.ones(n_pages * page, dtype=torch.bool, device="cuda")
+    left[at] = False
+    left = left.view(n_pages, page)
+    assert bool((pool[left] == 5).all())  # every other place is as it was
+
+
+# ---------------------------------------------------------------- attention
+class Batch:
+    """Inputs of a call with sentinels and garbage wherever nothing may be
+    read or written, and its result in 64 bits."""
+
+    def __init__(self, kind, NH, NKV, HD, P, lens, rows=None, page=16, seed=0, pad=0, peak=1.0, pool=None):
+        self.t, self.NH, self.NKV, self.HD, self.P, self.page = DT[kind], NH, NKV, HD, P, page
+        g = torch.Generator("cuda").manual_seed(seed)
+        B = len(lens)
+        self.rows = rows or [1] * B
+        self.lens = lens
+        self.T = sum(self.rows) + pad
+        pp = -(-P // page)
+        need = [-(-n // page) for n in lens]
+        n_pages = pp + sum(need) + 3
+        perm = torch.randperm(n_pages, device="cuda", generator=g).to(torch.int32)
+        self.ptable = perm[:pp].contiguous() if P else None
+        self.table = torch.full((B, max(need + [1]) + 1), -1, dtype=torch.int32, device="cuda")
+        at = pp
+        for b, n in enumerate(need):
+            self.table[b, :n] = perm[at: at + n]
+            self.table[b, n:] = 10 ** 9  # never a page
+            at += n
+        shape = (n_pages, page, NKV, HD) if pool is None else pool
+        self.k, self.v = (torch.full(shape, float("nan"), dtype=self.t, device="cuda")[:n_pages] for _ in range(2))
+        real = lambda *s: (torch.randn(*s, device="cuda", generator=g) * peak).to(self.t)  # noqa: E731
+        self.places = []  # per request, then the prefix: pages and places of its positions
+        for b, n in list(enumerate(lens)) + [(-1, P)]:
+            i = torch.arange(n, device="cuda")
+            tab = self.table[b] if b >= 0 else self.ptable
+            pg = tab[i // page].long() if n else i
+            self.k[pg, i % page], self.v[pg, i % page] = real(n, NKV, HD), real(n, NKV, HD)
+            self.places.append((pg, i % page))
+        self.q = real(self.T, NH, HD)
+        self.cu = i32(np.concatenate([[0], np.cumsum(self.rows)]).tolist())
+        self.kv_len = i32(lens)
+        self.scale = HD ** -0.5
+        self.kv = sb200.KvPages(self.k, self.v)
+
+    def want(self):
+        """out, lse, and out of |v|: the size that rounding works on."""
+        T, G = self.T, self.NH // self.NKV
+        out = torch.zeros(T, self.NH, self.HD, dtype=torch.float64, device="cuda")
+        size, lse = out.clone(), torch.full((T, self.NH), -math.inf, dtype=torch.float64, device="cuda")
+        pg, pl = self.places[-1]
+        kp, vp = self.k[pg, pl].double(), self.v[pg, pl].double()
+        r = 0
+        for b, n in enumerate(self.rows):
+            pg, pl = self.places[b]
+            k, v = torch.cat([kp, self.k[pg, pl].double()]), torch.cat([vp, self.v[pg, pl].double()])
+            for i in range(n):
+                sees = self.P + max(min(self.lens[b] - n + i + 1, self.lens[b]), 0)
+                if sees:
+                    q = self.q[r].double().view(self.NKV, G, self.HD)
+                    s = torch.einsum("hgd,khd->hgk", q, k[:sees]) * self.scale
+                    w = torch.softmax(s, -1)
+                    lse[r] = torch.logsumexp(s, -1).flatten()
+                    out[r] = torch.einsum("hgk,khd->hgd", w, v[:sees]).reshape(self.NH, self.HD)
+                    size[r] = torch.einsum("hgk,khd->hgd", w, v[:sees].abs()).reshape(self.NH, self.HD)
+                r += 1
+        return out, lse, size
+
+    def run(self, own=True, max_q=None, out=None, lse=None, ws=None, **kw):
+        out = torch.full_like(self.q, 7.0) if out is None else out
+        lse = torch.full((self.T, self.NH), 7.0, device="cuda") if lse is None else lse
+        max_kv = max(self.lens) if own else 0
+        max_q = max_q or max(max(self.rows), 1)
+        ragged = self.rows != [1] * len(self.lens) or self.T != len(self.lens) or max_q > 1
+        n = sb200.attn_prefix_ws(self.q, self.kv, self.P, len(self.lens), max_q=max_q, max_kv=max_kv)
+        if ws is None:  # NaN: a part that is read before it is written shows
+            ws = torch.full((n // 4 + 4,), float("nan"), device="cuda")
+        sb200.attn_prefix(self.q, out, self.kv, self.ptable, self.P, self.kv, self.table, self.kv_len, self.scale, ws,
+                          cu_q=self.cu if ragged else None, max_q=max_q, max_kv=max_kv, lse=lse, stream=stream(), **kw)
+        return out, lse
+
+    def check(self, got=None, want=None):
+        """16-bit types: half a step of each weight (on |v|), half a step of the
+        result, and 6e-5 for the FP32 part (scores of size 10 off by 2^-20,
+        20 to 300 truncated sums of 2^-23).  FP32: 2e-5 (scores: 130 terms of
+        2^-24 on sums of |q k| up to 60).  lse: the same score error."""
+        out, lse = got or self.run()
+        wo, wl, size = want or self.want()
+        n = sum(self.rows)
+        u = half_step(self.t) if self.t != torch.float32 else 0.0
+        err = (out[:n].double() - wo[:n]).abs()
+        bound = u * (size[:n] + wo[:n].abs()) + (6e-5 if u else 2e-5) * size[:n] + (2.0 ** -24 if self.t == torch.float16 else 1e-30)
+        assert bool((err <= bound).all()), (float(err.max()), float((err / bound).max()))
+        fin = torch.isfinite(wl[:n])
+        assert torch.equal(fin, torch.isfinite(lse[:n])) and bool((lse[:n][~fin] == -math.inf).all())
+        assert bool(((lse[:n].double() - wl[:n]).abs()[fin] <= 6e-5 + 2.0 ** -22 * wl[:n].abs()[fin]).all())
+        assert bool((out[n:] == 7).all()) and bool((lse[n:] == 7).all())  # padding is left as it was
+
+
+KINDS = ["f32", "f16", "bf16"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("NH,NKV,HD,P,lens,page", [
+    (14, 2, 64, 300, [64, 1, 0, 33], 16),       # the Qwen heads; a request without positions of its own
+    (12, 12, 64, 1, [1], 16),                   # one position each
+    (1, 1, 8, 0, [1], 1),                       # the smallest call
+    (4, 4, 64, 0, [0, 5, 0], 16),               # rows that see nothing
+    (8, 1, 128, 129, [127, 128, 129, 1000], 24),
+    (6, 2, 80, 65, [17, 63], 7),                # odd head size, pages that end inside a tile
+    (32, 8, 128, 2050, [300] * 3, 64),
+    (9, 3, 40, 700, [5, 2], 1024),
+    (20, 1, 64, 100, [50, 70], 32),             # more than 16 heads on one key head
+])
+def test_attn_prefix_single_rows(cuda_dev, kind, NH, NKV, HD, P, lens, page):
+    Batch(kind, NH, NKV, HD, P, lens, page=page, seed=P + HD).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("NH,NKV,HD,P,lens,rows,page,pad", [
+    (14, 2, 64, 200, [40, 9, 0, 130], [3, 9, 0, 33], 16, 5),   # causal among a request's rows; an empty one; padding
+    (4, 1, 128, 0, [70, 1], [70, 1], 32, 0),                   # no prefix: plain causal prefill
+    (2, 2, 64, 77, [3, 300], [5, 2], 16, 1),                   # more rows than positions: the first rows see only the prefix
+    (2, 2, 32, 0, [2, 0], [4, 3], 8, 0),                       # and without a prefix nothing
+    (8, 2, 96, 1500, [65, 64, 63], [17, 16, 15], 48, 0),
+])
+def test_attn_prefix_many_rows(cuda_dev, kind, NH, NKV, HD, P, lens, rows, page, pad):
+    b = Batch(kind, NH, NKV, HD, P, lens, rows=rows, page=page, seed=P + HD, pad=pad)
+    want = b.want()
+    b.check(want=want)
+    b.check(got=b.run(max_q=1), want=want)  # max_q sizes the launch only
+    b.check(got=b.run(max_q=200), want=want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_large_batch(cuda_dev, kind):
+    """Many row tiles on one key head, a long prefix cut into ranges, ragged
+    own lengths."""
+    lens = [(i * 37) % 200 for i in range(150)]
+    Batch(kind, 14, 2, 64, 3001, lens, page=16, seed=1).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_peaked_scores(cuda_dev, kind):
+    """Scores of size 60: the running maximum moves far from tile to tile.
+    Their FP32 rounding grows with them, so only values of the formula count
+    here: weights that sum to 1 on values of 1."""
+    b = Batch(kind, 4, 2, 64, 500, [100, 37], seed=3)
+    b.q *= 8
+    for pg, pl in b.places:
+        b.v[pg, pl] = 1.0
+    out, lse = b.run()
+    assert bool(((out.double() - 1).abs() <= 4 * half_step(b.t) + 1e-5).all())
+    wl = b.want()[1]
+    # |q k| sums reach 64 x 8 x 3: 130 terms of 2^-24 of that, times the scale
+    assert bool(((lse.double() - wl).abs() <= 130 * 2.0 ** -24 * 1536 * b.scale + 2.0 ** -21 * wl.abs()).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_missing_pages(cuda_dev, kind):
+    """A page number outside the pool: its positions are skipped, as if they
+    were not there; a request whose pages are all missing sees the prefix."""
+    b = Batch(kind, 6, 2, 64, 100, [70, 40, 33], page=16, seed=5)
+    missing = [(0, 1), (1, 0), (1, 1), (1, 2), (2, 2)]
+    for r, j in missing:
+        keep = b.places[r][0] != int(b.table[r, j])
+        b.places[r] = (b.places[r][0][keep], b.places[r][1][keep])
+        b.table[r, j] = [-1, 10 ** 6, -2 ** 31, b.k.shape[0], -1][(r + j) % 5]
+    b.ptable[2] = -1
+    i = torch.arange(100, device="cuda")
+    b.places[-1] = tuple(x[i // 16 != 2] for x in b.places[-1])
+    lens, P = b.lens, b.P
+    got = b.run()
+    b.lens, b.P = [len(p[0]) for p in b.places[:-1]], len(b.places[-1][0])
+    want = b.want()
+    b.lens, b.P = lens, P
+    b.check(got=got, want=want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_only_one_side(cuda_dev, kind):
+    """No own positions at all (max_kv 0), or no prefix: the other side's
+    arguments may be absent; nothing on both sides gives zeros."""
+    b = Batch(kind, 4, 2, 64, 333, [0, 0], seed=7)
+    want = b.want()
+    out, lse = torch.full_like(b.q, 7.0), torch.full((2, 4), 7.0, device="cuda")
+    ws = torch.empty(sb200.attn_prefix_ws(b.q, b.kv, 333, 2), dtype=torch.uint8, device="cuda")
+    sb200.attn_prefix(b.q, out, b.kv, b.ptable, 333, None, None, None, b.scale, ws, lse=lse, stream=stream())
+    b.check(got=(out, lse), want=want)
+    c = Batch(kind, 4, 2, 64, 0, [90, 31], seed=8)
+    out, lse = torch.full_like(c.q, 7.0), torch.full((2, 4), 7.0, device="cuda")
+    ws = torch.empty(sb200.attn_prefix_ws(c.q, c.kv, 0, 2, max_kv=90), dtype=torch.uint8, device="cuda")
+    sb200.attn_prefix(c.q, out, None, None, 0, c.kv, c.table, c.kv_len, c.scale, ws, max_kv=90, lse=lse, stream=stream())
+    c.check(got=(out, lse))
+    sb200.attn_prefix(c.q, out, c.kv, None, 0, c.kv, None, None, c.scale, None, lse=lse, stream=stream())
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attn_prefix_strides_and_lengths(cuda_dev, kind):
+    """Query and output rows inside wider ones, keys and values side by side,
+    pages in order (no prefix table), negative and too long lengths."""
+    t, g = DT[kind], torch.Generator("cuda").manual_seed(9)
+    NH, NKV, HD, page, P, lens = 4, 2, 64, 16, 40, [20, 16]
+    b = Batch(kind, NH, NKV, HD, P, lens, page=page, seed=9)
+    pool = torch.full((8, NKV, page, 2, HD), float("nan"), dtype=t, device="cuda").permute(0, 2, 1, 3, 4)
+    k, v = pool[..., 0, :], pool[..., 1, :]
+    table, at = i32([[5, 3, 10 ** 6], [6, 4, 7]]), 0
+    for r, n in list(enumerate(lens)) + [(-1, P)]:
+        i = torch.arange(n, device="cuda")
+        pg = table[r][i // page].long() if r >= 0 else i // page
+        k[pg, i % page], v[pg, i % page] = b.k[b.places[r]], b.v[b.places[r]]
+    wide = torch.full((2, NH + 3, HD + 8), 7.0, dtype=t, device="cuda")
+    q, out = wide[:, :NH, :HD], torch.full((2, NH + 1, HD), 7.0, dtype=t, device="cuda")
+    q.copy_(b.q)
+    kv = sb200.KvPages(k, v)
+    ws = torch.empty(sb200.attn_prefix_ws(q, kv, P, 2, max_kv=20), dtype=torch.uint8, device="cuda")
+    lse = torch.full((2, NH), 7.0, device="cuda")
+    # request 0's length is cut to max_kv = 20, as the 20 that it has
+    sb200.attn_prefix(q, out[:, :NH], kv, None, P, kv, table, i32([10 ** 9, 16]), b.scale, ws, max_kv=20, lse=lse, stream=stream())
+    b.check(got=(out[:, :NH], lse))
+    assert bool((out[:, NH:] == 7).all())
+    sb200.attn_prefix(q, out[:, :NH], kv, None, P, kv, table, i32([-3, 16]), b.scale, ws, max_kv=20, lse=lse, stream=stream())
+    b.lens = [0, 16]
+    b.places[0] = tuple(x[:0] for x in b.places[0])
+    b.check(got=(out[:, :NH], lse))
+
+
+def test_attn_prefix_offsets_past_32_bits(cuda_dev):
+    """Pages whose elements lie past 2^32 bytes and 2^31 elements."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    NKV, HD, page = 2, 64, 16
+    big = torch.empty(2, 2_200_000_000, dtype=torch.float16, device="cuda")
+    stride = 2_200_000_000 // 4 // 8 * 8
+    k, v = (x.as_strided((4, page, NKV, HD), (stride, NKV * HD, HD, 1)) for x in big)
+    b = Batch("f16", 4, NKV, HD, 20, [30], page=page, seed=11)
+    table = i32([[3, 2, -1]])
+    for r, n in ((0, 30), (-1, 20)):
+        i = torch.arange(n, device="cuda")
+        pg = table[0][i // page].long() if r == 0 else i32([3, 1])[i // page].long()
+        at = i % page
+        if r:
+            pg, at = i32([1, 0])[i // page].long(), at
+        k[pg, at], v[pg, at] = b.k[b.places[r]], b.v[b.places[r]]
+    kv, lse = sb200.KvPages(k, v), torch.empty(1, 4, device="cuda")
+    out, ws = torch.empty_like(b.q), torch.empty(sb200.attn_prefix_ws(b.q, kv, 20, 1, max_kv=30), dtype=torch.uint8, device="cuda")
+    sb200.attn_prefix(b.q, out, kv, i32([1, 0]), 20, kv, table, b.kv_len, b.scale, ws, max_kv=30, lse=lse, stream=stream())
+    b.check(got=(out, lse))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_repeats_and_replays(cuda_dev, kind):
+    """The same bits on every run (no sums in an order of arrival), on another
+    stream, and from a captured graph whose lengths change between replays."""
+    lens = [50, 0, 200, 31]
+    b = Batch(kind, 14, 2, 64, 1000, lens, rows=[2, 1, 4, 3], page=16, seed=13)
+    out, lse = b.run()
+    ws = torch.empty(sb200.attn_prefix_ws(b.q, b.kv, 1000, 4, max_q=4, max_kv=200), dtype=torch.uint8, device="cuda")
+    o2, l2 = torch.zeros_like(out), torch.zeros_like(lse)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            b.run(out=o2, lse=l2, ws=ws)
+    side.synchronize()
+    assert torch.equal(out, o2) and torch.equal(lse, l2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.run(out=o2, lse=l2, ws=ws)
+    for change in ([20, 0, 200, 31], [50, 0, 3, 0]):
+        b.kv_len.copy_(i32(change))
+        o2.fill_(9)
+        graph.replay()
+        places, was = list(b.places), b.lens
+        b.lens, b.places = change, [tuple(x[:n] for x in p) for p, n in zip(places, change)] + [places[-1]]
+        want = b.want()
+        b.lens, b.places = was, places
+        b.check(got=(o2, l2), want=want)
+
+
+def test_attn_prefix_workspace_too_small(cuda_dev):
+    b = Batch("f16", 14, 2, 64, 1000, [50, 20])
+    n = sb200.attn_prefix_ws(b.q, b.kv, 1000, 2, max_kv=50)
+    assert n > 0
+    for ws in (None, torch.empty(n - 1, dtype=torch.uint8, device="cuda"), torch.empty(n + 9, dtype=torch.uint8, device="cuda")[8:]):
+        with pytest.raises(sb200.SbError, match="workspace"):
+            sb200.attn_prefix(b.q, torch.empty_like(b.q), b.kv, b.ptable, 1000, b.kv, b.table, b.kv_len, b.scale, ws, max_kv=50)
+
+
+def test_attn_prefix_reads_an_engine_cache(cuda_dev, qwen_weights):
+    """A prompt that an engine has prefilled, as the shared prefix of a batch:
+    the same attention as the single-sequence kernel on the same cache."""
+    Q = sb200.QWEN
+    eng = sb200.Engine(sb200.MODEL_QWEN, qwen_weights, 256)
+    ids = sb200.synth_ids(100, Q["V"], 3)
+    eng.begin(ids, 1)
+    eng.prefill(99)
+    ptr, nbytes, NL, ctx, width = eng.kv_cache()
+    torch.cuda.synchronize()
+
+    class Memory:
+        __cuda_array_interface__ = {"shape": (2, NL, ctx // 16, 16, 2, 64), "typestr": "<f4", "data": (ptr, False), "version": 3}
+    cache = torch.as_tensor(Memory(), device="cuda")
+    for layer in (0, 23):
+        kv = sb200.KvPages(cache[0, layer], cache[1, layer])
+        g = torch.Generator("cuda").manual_seed(layer)
+        q = torch.randn(5, 14, 64, device="cuda", generator=g)
+        out = torch.empty_like(q)
+        ws = torch.empty(sb200.attn_prefix_ws(q, kv, 99, 5), dtype=torch.uint8, device="cuda")
+        sb200.attn_prefix(q, out, kv, None, 99, None, None, None, 0.125, ws, stream=stream())
+        part, tickets = torch.zeros(2 * 7 * 7 * 66, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+        one = torch.empty(14 * 64, device="cuda")
+        for r in range(5):
+            sb200.attn_decode(q[r].contiguous(), cache[0, layer], cache[1, layer], one, 99, 14, 2, 64, 128, 0.125, part, tickets)
+            torch.testing.assert_close(out[r].flatten(), one, rtol=1e-5, atol=2e-6)
+    eng.close()
