@@ -3,27 +3,31 @@
 // alternatives, from one pass over the logits, and their gradient.  No
 // counterpart in the reference, which samples one token a step.
 //
-// With y = x log2(e) / temperature of a row and m its maximum,
-//   s = sum 2^(y - m),  t = sum 2^(y - m) (y - m)
-//   lse = ln2 (m + log2 s),  logp = ln2 (y_tok - m - log2 s)
+// With c = log2(e) / temperature and m the maximum of a row,
+//   s = sum 2^(c (x - m)),  t = sum 2^(c (x - m)) c (x - m)
+//   lse = m / temperature + ln2 log2 s,  logp = ln2 (c (x_tok - m) - log2 s)
 //   entropy = ln2 (log2 s - t / s)
-// and a change of m turns (s, t) into f s, f (t + s (m - m')), f = 2^(m - m'):
-// a thread keeps (m, s, t) of its values and looks at m once per vector.
-// y - m is one fma with m's own rounded product, so the rounding of m is the
-// same in every term and cancels.  Sums are FP32.
+// and a change of m turns (s, t) into f s, f (t + s d), f = 2^d: a thread
+// keeps (m, s, t) of its values and looks at m once per four vectors.
+// c (x - m) is one fma with the rounded product c m, the same in every term,
+// so that rounding cancels; values whose product could overflow (masks of the
+// type's lowest value, -inf) take a guarded form, chosen by the vector's
+// minimum.  Sums are FP32.
 //
-// Bound: HBM (one read of the logits); for 16-bit logits the 16 exponentials
-// per SM and cycle are close behind (5.5 against 4.2 us for 10^7 values).
+// Bound: HBM (one read of the logits).  For 16-bit logits the 16 exponentials
+// per SM and cycle are close behind, and issue slots too: about eight
+// instructions a value, with maxima, minima and rank compares on packed pairs.
 //
 // The k best in the same pass.  A key is the value's order-preserving bits
 // above the complemented id, so a larger key is a better candidate and equal
 // values go to the lower id (-0 counts as +0); masked choices (-inf) are not
-// listed.  The k-th best of the
-// threads' (or thread groups') maxima so far is a lower bound of the k-th
-// best value: k holders each have a value at least that good.  Only values
+// listed.  The k-th best of the threads' (or thread groups') maxima so far is
+// a lower bound of the k-th best value: k holders each have a value at least
+// that good.  Only vectors that reach it are looked into, and only values
 // that reach it go to a list in shared memory -- about k per doubling of the
-// values seen, as the bound is renewed after tiles 0, 1, 3, 7, ...  A list
-// that would overflow (rising or equal logits) is cut to its k best first.
+// values seen, as the bound is renewed after tiles 0, 1, 3, 7, ...  Where the
+// list overflows (rising or equal logits), the part's k best are taken by k
+// passes instead.
 #include <cfloat>
 #include <cuda_bf16.h>
 
@@ -40,7 +44,7 @@ struct LpParams {
     const void *x;
     long long stride;  // elements
     int R, V, S, k;    // S parts per row, one CTA each
-    float c;           // log2(e) / temperature
+    float c, inv_temp;  // log2(e) / temperature
     const int *tok;
     float *logp, *entropy, *lse;
     int *rank, *top_ids;
@@ -49,7 +53,6 @@ struct LpParams {
     unsigned long long *keys;    // [R][S][k]
 };
 
-template <typename T> struct LpVec { static constexpr int N = 16 / sizeof(T); };
 SB_DEV float lp_f(float v) { return v; }
 SB_DEV float lp_f(__half v) { return __half2float(v); }
 SB_DEV float lp_f(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -58,13 +61,11 @@ SB_DEV float lp_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-SB_DEV float lp_max_nan(float a, float b) {  // a NaN stays: the row's results become NaN
+SB_DEV float lp_max_nan(float a, float b) {  // a NaN stays
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
-// y - m; -inf logits (and m = -inf) become a power of two that is 0
-SB_DEV float lp_diff(float x, float c, float mc) { return fmaxf(fmaf(x, c, -mc), -200.f); }
 SB_DEV unsigned long long lp_key(float v, int id) {
     const unsigned u = __float_as_uint(v == 0.f ? 0.f : v);
     return ((unsigned long long)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32) | (unsigned)~id;
@@ -75,129 +76,261 @@ SB_DEV float lp_key_value(unsigned long long k) {
 }
 SB_DEV int lp_key_id(unsigned long long k) { return (int)~(unsigned)k; }
 
+// sixteen bytes of a row: maximum and minimum (a NaN loses), values, and how
+// many reach a bound (counted in the type itself: exact for the 16 of a tile)
+template <typename T> struct LpVec;
+template <> struct LpVec<float> {
+    static constexpr int N = 4;
+    static constexpr unsigned NEG_INF = 0xff800000u;
+    using Count = int;
+    using Bound = float;
+    static SB_DEV float max(const uint4 &r) {
+        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+    static SB_DEV float min(const uint4 &r) {
+        return fminf(fminf(__uint_as_float(r.x), __uint_as_float(r.y)), fminf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+    static SB_DEV float max(const uint4 (&r)[LP_U]) { return fmaxf(fmaxf(max(r[0]), max(r[1])), fmaxf(max(r[2]), max(r[3]))); }
+    static SB_DEV float min(const uint4 (&r)[LP_U]) { return fminf(fminf(min(r[0]), min(r[1])), fminf(min(r[2]), min(r[3]))); }
+    static SB_DEV void values(const uint4 &r, float (&v)[4]) {
+        v[0] = __uint_as_float(r.x);
+        v[1] = __uint_as_float(r.y);
+        v[2] = __uint_as_float(r.z);
+        v[3] = __uint_as_float(r.w);
+    }
+    static SB_DEV uint4 packed(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    static SB_DEV Bound bound(float v) { return v; }
+    static SB_DEV Bound above(float v) {  // the next value up
+        const unsigned u = __float_as_uint(v);
+        return __uint_as_float(v == 0.f ? 1u : u & 0x80000000u ? u - 1 : u + 1);
+    }
+    static SB_DEV Count zero() { return 0; }
+    static SB_DEV void count(const uint4 &r, Bound b, Count &n) {
+        n += __uint_as_float(r.x) >= b;
+        n += __uint_as_float(r.y) >= b;
+        n += __uint_as_float(r.z) >= b;
+        n += __uint_as_float(r.w) >= b;
+    }
+    static SB_DEV int total(Count n) { return n; }
+};
+template <typename T, typename T2> struct LpVec16 {
+    static constexpr int N = 8;
+    using Count = T2;
+    using Bound = T2;
+    static SB_DEV T2 pair(unsigned u) { return *reinterpret_cast<const T2 *>(&u); }
+    static SB_DEV T2 max2(const uint4 &r) { return __hmax2(__hmax2(pair(r.x), pair(r.y)), __hmax2(pair(r.z), pair(r.w))); }
+    static SB_DEV T2 min2(const uint4 &r) { return __hmin2(__hmin2(pair(r.x), pair(r.y)), __hmin2(pair(r.z), pair(r.w))); }
+    static SB_DEV float max(const uint4 &r) {
+        const T2 m = max2(r);
+        return fmaxf(lp_f(m.x), lp_f(m.y));
+    }
+    static SB_DEV float max(const uint4 (&r)[LP_U]) {
+        const T2 m = __hmax2(__hmax2(max2(r[0]), max2(r[1])), __hmax2(max2(r[2]), max2(r[3])));
+        return fmaxf(lp_f(m.x), lp_f(m.y));
+    }
+    static SB_DEV float min(const uint4 (&r)[LP_U]) {
+        const T2 m = __hmin2(__hmin2(min2(r[0]), min2(r[1])), __hmin2(min2(r[2]), min2(r[3])));
+        return fminf(lp_f(m.x), lp_f(m.y));
+    }
+    static SB_DEV void values(const uint4 &r, float (&v)[8]) {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = lp_f(pair(w[i]).x);
+            v[2 * i + 1] = lp_f(pair(w[i]).y);
+        }
+    }
+    static SB_DEV unsigned pack(float a, float b) {
+        if constexpr (__is_same(T, __half)) {
+            const __half2 h = __floats2half2_rn(a, b);
+            return *reinterpret_cast<const unsigned *>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            return *reinterpret_cast<const unsigned *>(&h);
+        }
+    }
+    static SB_DEV uint4 packed(const float (&v)[8]) { return make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7])); }
+    static SB_DEV Bound both(unsigned short b) { return pair(b * 0x10001u); }
+    static SB_DEV unsigned short bits(float v) {  // v is a value of the type
+        if constexpr (__is_same(T, __half)) return __half_as_ushort(__float2half_rn(v));
+        else return __bfloat16_as_ushort(__float2bfloat16_rn(v));
+    }
+    static SB_DEV Bound bound(float v) { return both(bits(v)); }
+    static SB_DEV Bound above(float v) {
+        const unsigned short u = bits(v);
+        return both(v == 0.f ? 1 : u & 0x8000 ? u - 1 : u + 1);
+    }
+    static SB_DEV Count zero() { return pair(0u); }
+    static SB_DEV void count(const uint4 &r, Bound b, Count &n) {
+        n = __hadd2(n, __hge2(pair(r.x), b));
+        n = __hadd2(n, __hge2(pair(r.y), b));
+        n = __hadd2(n, __hge2(pair(r.z), b));
+        n = __hadd2(n, __hge2(pair(r.w), b));
+    }
+    static SB_DEV int total(Count n) { return (int)(lp_f(n.x) + lp_f(n.y)); }
+};
+template <> struct LpVec<__half> : LpVec16<__half, __half2> { static constexpr unsigned NEG_INF = 0xfc00fc00u; };
+template <> struct LpVec<__nv_bfloat16> : LpVec16<__nv_bfloat16, __nv_bfloat162> { static constexpr unsigned NEG_INF = 0xff80ff80u; };
+
+// value e of a vector, e not known at compile time (an indexed register array would live in memory)
+template <typename T>
+SB_DEV float lp_at(const uint4 &r, int e) {
+    const int w = sizeof(T) == 4 ? e : e >> 1;
+    const unsigned u = w & 2 ? (w & 1 ? r.w : r.z) : (w & 1 ? r.y : r.x);
+    if constexpr (sizeof(T) == 4) return __uint_as_float(u);
+    const unsigned short h = (unsigned short)(e & 1 ? u >> 16 : u);
+    return lp_f(*reinterpret_cast<const T *>(&h));
+}
+// vector j of a row, counted from the 16-byte boundary at or below its start;
+// values outside the row are -inf
+template <typename T>
+SB_DEV uint4 lp_load(const T *x, int lead, int V, int j) {
+    constexpr int N = LpVec<T>::N;
+    const int e0 = j * N - lead;
+    if (e0 >= 0 && e0 + N <= V) return ld_stream_u4(x + e0);
+    uint4 r = make_uint4(LpVec<T>::NEG_INF, LpVec<T>::NEG_INF, LpVec<T>::NEG_INF, LpVec<T>::NEG_INF);
+    T *h = reinterpret_cast<T *>(&r);
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (e0 + e >= 0 && e0 + e < V) h[e] = x[e0 + e];
+    return r;
+}
+
+// (m, s, t) of a set of values; m in logits, s and t as at the top
 struct LpSum { float m, s, t; };
-SB_DEV void lp_raise(LpSum &a, float m) {  // m >= a.m
+SB_DEV bool lp_sane(float m) { return fabsf(m) < 1e30f; }  // c m does not overflow (temperature > 1e-8)
+SB_DEV unsigned long long lp_add2(unsigned long long a, unsigned long long b) {  // two FP32 sums in one instruction
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+SB_DEV unsigned long long lp_mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// c (a - b), for b the maximum that sums are held against
+SB_DEV float lp_gap(float a, float b, float c) { return lp_sane(a) && lp_sane(b) ? __fmul_rn(a, c) - __fmul_rn(b, c) : (a - b) * c; }
+SB_DEV void lp_raise(LpSum &a, float m, float c) {  // m >= a.m
     if (a.s != 0.f) {
-        const float d = fmaxf(a.m - m, -200.f), f = lp_exp2(d);
+        const float d = lp_max_nan(lp_gap(a.m, m, c), -200.f), f = lp_exp2(d);
         a.t = f * fmaf(a.s, d, a.t);
         a.s *= f;
     }
     a.m = m;
 }
-SB_DEV LpSum lp_join(LpSum a, LpSum b) {
-    const float m = lp_max_nan(a.m, b.m);
-    lp_raise(a, m);
-    lp_raise(b, m);
-    return {m, a.s + b.s, a.t + b.t};
-}
-SB_DEV LpSum lp_warp(LpSum a) {
+// all threads' sums and counts: the common maximum first, then plain sums.
+// lp_s: [3][warps]; a barrier must stand before its next use.
+struct LpShared { float m[LP_THREADS / 32], s[LP_THREADS / 32], t[LP_THREADS / 32]; int n[LP_THREADS / 32]; };
+SB_DEV void lp_block(LpSum &a, int &above, float c, LpShared &sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float m = warp_max(a.m);
+    if (lane == 0) sh.m[warp] = m;
+    __syncthreads();
+    m = sh.m[0];
+#pragma unroll
+    for (int w = 1; w < LP_THREADS / 32; w++) m = fmaxf(m, sh.m[w]);
+    lp_raise(a, m, c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const LpSum b = {__shfl_xor_sync(SB_FULL, a.m, o), __shfl_xor_sync(SB_FULL, a.s, o), __shfl_xor_sync(SB_FULL, a.t, o)};
-        a = lp_join(a, b);
+        a.s += __shfl_xor_sync(SB_FULL, a.s, o);
+        a.t += __shfl_xor_sync(SB_FULL, a.t, o);
     }
-    return a;
+    above = __reduce_add_sync(SB_FULL, above);
+    if (lane == 0) {
+        sh.s[warp] = a.s;
+        sh.t[warp] = a.t;
+        sh.n[warp] = above;
+    }
+    __syncthreads();
+    a = {m, 0.f, 0.f};
+    above = 0;
+#pragma unroll
+    for (int w = 0; w < LP_THREADS / 32; w++) {
+        a.s += sh.s[w];
+        a.t += sh.t[w];
+        above += sh.n[w];
+    }
 }
 
+// ln2 (c (x - m) - l2) of a value against finished sums
+SB_DEV float lp_logp(float x, float m, float l2, float c) {
+    return ((lp_sane(x) && lp_sane(m) ? fmaf(x, c, -__fmul_rn(m, c)) : (x - m) * c) - l2) * LP_LN2;
+}
+// results of a row from its joined sums; a row of masked choices has m = -inf and s = 0
+SB_DEV void lp_finish(const LpParams &P, int r, LpSum a, int above, float xt, bool given) {
+    const bool none = a.m == -INFINITY && a.s == 0.f;
+    const float l2 = log2f(a.s);
+    if (P.lse) P.lse[r] = none ? -INFINITY : lp_sane(a.m) ? (__fmul_rn(a.m, P.c) + l2) * LP_LN2 : fmaf(l2, LP_LN2, a.m * P.inv_temp);
+    if (P.entropy) P.entropy[r] = none ? 0.f : (l2 - a.t / a.s) * LP_LN2;
+    if (P.logp) P.logp[r] = !given ? 0.f : none ? -INFINITY : lp_logp(xt, a.m, l2, P.c);
+    if (P.rank) P.rank[r] = given ? above : -1;
+}
+SB_DEV void lp_top(const LpParams &P, int r, int i, unsigned long long key, float m, float l2) {
+    if (P.top_ids) P.top_ids[(long long)r * P.k + i] = key ? lp_key_id(key) : -1;
+    if (P.top_logp) P.top_logp[(long long)r * P.k + i] = key ? lp_logp(lp_key_value(key), m, l2, P.c) : -INFINITY;
+}
 // the first k of n keys in a list, ranked by counting, as emit(rank, key)
-template <int THREADS, typename F>
+template <typename F>
 SB_DEV void lp_rank(const unsigned long long *list, int n, int k, F emit) {
-    for (int i = threadIdx.x; i < n; i += THREADS) {
+    for (int i = threadIdx.x; i < n; i += LP_THREADS) {
         const unsigned long long me = list[i];
         int r = 0;
         for (int j = 0; j < n; j++) r += list[j] > me;
         if (r < k) emit(r, me);
     }
 }
-// the list cut to its k best (in any case to at most k); returns how many
-template <int THREADS>
-SB_DEV int lp_cut(unsigned long long *list, int n, int k) {
-    unsigned long long mine[(LP_LIST + THREADS - 1) / THREADS];
-    int rank[(LP_LIST + THREADS - 1) / THREADS];
-#pragma unroll
-    for (int q = 0; q < (LP_LIST + THREADS - 1) / THREADS; q++) {
-        const int i = threadIdx.x + q * THREADS;
-        mine[q] = i < n ? list[i] : 0ull;
-        rank[q] = 0;
-        if (i < n)
-            for (int j = 0; j < n; j++) rank[q] += list[j] > mine[q];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < (LP_LIST + THREADS - 1) / THREADS; q++)
-        if ((int)threadIdx.x + q * THREADS < n && rank[q] < k) list[rank[q]] = mine[q];
-    __syncthreads();
-    return min(n, k);
-}
 
-// results of a row from its joined sums
-SB_DEV void lp_finish(const LpParams &P, int r, LpSum a, int above, float xt, bool given) {
-    const bool none = a.m == -INFINITY;  // every choice is masked
-    const float l2 = log2f(a.s);
-    if (P.lse) P.lse[r] = none ? -INFINITY : (a.m + l2) * LP_LN2;
-    if (P.entropy) P.entropy[r] = none ? 0.f : (l2 - a.t / a.s) * LP_LN2;
-    if (P.logp) P.logp[r] = !given ? 0.f : none ? -INFINITY : (fmaf(xt, P.c, -a.m) - l2) * LP_LN2;
-    if (P.rank) P.rank[r] = given ? above : -1;
-}
-SB_DEV void lp_top(const LpParams &P, int r, int i, unsigned long long key, float m, float l2) {
-    const bool ok = key != 0ull;
-    if (P.top_ids) P.top_ids[(long long)r * P.k + i] = ok ? lp_key_id(key) : -1;
-    if (P.top_logp)
-        P.top_logp[(long long)r * P.k + i] = !ok || m == -INFINITY ? -INFINITY : (fmaf(lp_key_value(key), P.c, -m) - l2) * LP_LN2;
-}
-
-// CTA = part s of row r: vectors [n s / S, n (s + 1) / S) of the row, counted
-// from the 16-byte boundary at or below its start (the partial first and
-// last vectors are read value by value).
+// CTA = part s of row r: vectors [n s / S, n (s + 1) / S) of the row
 template <typename T, bool TOP>
 SB_DEV void logprobs_body(const LpParams &P) {
-    constexpr int N = LpVec<T>::N;
-    __shared__ LpSum sum_s[LP_THREADS / 32];
-    __shared__ int cnt_s[LP_THREADS / 32];
+    using Vec = LpVec<T>;
+    constexpr int N = Vec::N, TILE = LP_THREADS * LP_U;
+    __shared__ LpShared sum_s;
     __shared__ unsigned long long list[TOP ? LP_LIST : 1];
     __shared__ __align__(16) float best_s[TOP ? LP_THREADS : 4];
     __shared__ int n_s;
     __shared__ float thr_s;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x;
     const int r = blockIdx.x / P.S, part = blockIdx.x % P.S;
     pdl_launch_dependents();
     const T *x = static_cast<const T *>(P.x) + r * P.stride;
-    const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));  // values of the first vector that are not the row's
-    const T *x0 = x - lead;
+    const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));  // places of the first vector that are not the row's
     const int nv = (int)(((long long)lead + P.V + N - 1) / N);
     const int v0 = (int)((long long)nv * part / P.S), v1 = (int)((long long)nv * (part + 1) / P.S);
+    const int whole0 = lead ? 1 : 0, whole1 = min((int)(((long long)lead + P.V) / N), v1);  // vectors inside the row
     const int tok = P.tok ? P.tok[r] : -1;
-    const bool given = tok >= 0 && tok < P.V;
-    const float xt = given ? lp_f(x[tok]) : 0.f;
-    const bool count = P.rank && given;
+    const bool given = tok >= 0 && tok < P.V, count = P.rank && given;
+    const float xt = given ? lp_f(x[tok]) : 0.f, c = P.c;
+    const int jt = given ? (tok + lead) / N : -1;  // the token's vector
+    // ids before the token's vector count when equal, later ones do not; equal ids inside it, and
+    // masked ones where the token is masked itself, are added behind the loop
+    const typename Vec::Bound more = Vec::above(xt), at_least = xt == -INFINITY ? more : Vec::bound(xt);
 
     LpSum a = {-INFINITY, 0.f, 0.f};
-    float best = -INFINITY;  // this thread's best raw value
     int above = 0;
-    float thr = -FLT_MAX;  // masked choices (-inf) are never listed
-    unsigned long long cut = 0ull;  // keys at or below it are out
+    float best = -INFINITY, thr = -FLT_MAX;
+    // group maxima: one per thread, per 4 lanes or per 8 (fewer are looser and cheaper to rank)
+    const int per = P.k > 24 ? 1 : P.k > 8 ? 4 : 8, groups = LP_THREADS / per;
+    int renew = 0, tile = 0;
     if (TOP && tid == 0) n_s = 0;
-    const int groups = P.k > 24 ? LP_THREADS : LP_THREADS / 4;
-    int renew = 0, tile = 0, held = 0;  // held: keys in the list
 
     // the k-th best group maximum bounds the k-th best value from below
     auto raise_bound = [&]() {
         float g = best;
-        if (groups != LP_THREADS) {
-            g = fmaxf(g, __shfl_xor_sync(SB_FULL, g, 1));
-            g = fmaxf(g, __shfl_xor_sync(SB_FULL, g, 2));
-        }
-        const bool lead_lane = groups == LP_THREADS || (tid & 3) == 0;
-        const int gi = groups == LP_THREADS ? tid : tid >> 2;
-        if (lead_lane) best_s[gi] = g;
+        for (int o = 1; o < per; o <<= 1) g = fmaxf(g, __shfl_xor_sync(SB_FULL, g, o));
+        if (tid % per == 0) best_s[tid / per] = g;
         if (tid == 0) thr_s = -FLT_MAX;
         __syncthreads();
-        if (lead_lane) {
+        if (tid < groups) {
+            g = best_s[tid];
             int rk = 0;
             for (int i = 0; i < groups; i += 4) {
                 const float4 o = *reinterpret_cast<const float4 *>(best_s + i);
-                rk += (o.x > g || (o.x == g && i < gi)) + (o.y > g || (o.y == g && i + 1 < gi)) +
-                      (o.z > g || (o.z == g && i + 2 < gi)) + (o.w > g || (o.w == g && i + 3 < gi));
+                rk += (o.x > g || (o.x == g && i < tid)) + (o.y > g || (o.y == g && i + 1 < tid)) +
+                      (o.z > g || (o.z == g && i + 2 < tid)) + (o.w > g || (o.w == g && i + 3 < tid));
             }
             if (rk == P.k - 1) thr_s = g;
         }
@@ -205,151 +338,164 @@ SB_DEV void logprobs_body(const LpParams &P) {
         thr = fmaxf(thr, thr_s);
     };
 
-    for (int b = v0; b < v1; b += LP_THREADS * LP_U, tile++) {
-        float v[LP_U][N];
+    for (int b = v0; b < v1; b += TILE, tile++) {
         uint4 raw[LP_U];
+        if (b >= whole0 && b + TILE <= whole1) {
 #pragma unroll
-        for (int u = 0; u < LP_U; u++) {
-            const int j = b + u * LP_THREADS + tid;
-            const int e0 = j * N - lead;
-            if (j < v1 && e0 >= 0 && e0 + N <= P.V) raw[u] = ld_stream_u4(x0 + (long long)j * N);
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < LP_U; u++) {
-            const int j = b + u * LP_THREADS + tid;
-            const int e0 = j * N - lead;
-            if (j < v1 && e0 >= 0 && e0 + N <= P.V) {
-                const T *h = reinterpret_cast<const T *>(&raw[u]);
-#pragma unroll
-                for (int e = 0; e < N; e++) v[u][e] = lp_f(h[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; e++) v[u][e] = j < v1 && e0 + e >= 0 && e0 + e < P.V ? lp_f(x[e0 + e]) : -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < N; e++) mx = lp_max_nan(mx, v[u][e]);
-        }
-        best = lp_max_nan(best, mx);
-        if (best * P.c > a.m || best != best) lp_raise(a, best * P.c);
-#pragma unroll
-        for (int u = 0; u < LP_U; u++)
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float d = lp_diff(v[u][e], P.c, a.m), w = lp_exp2(d);
-                a.s += w;
-                a.t = fmaf(w, d, a.t);
-            }
-        if (count) {
+            for (int u = 0; u < LP_U; u++) raw[u] = ld_stream_u4(x + ((b + u * LP_THREADS + tid) * N - lead));
+        } else {
 #pragma unroll
             for (int u = 0; u < LP_U; u++) {
-                const int j = b + u * LP_THREADS + tid, e0 = j * N - lead;
-#pragma unroll
-                for (int e = 0; e < N; e++)
-                    above += v[u][e] > xt || (v[u][e] == xt && e0 + e < tok && e0 + e >= 0 && j < v1);
+                const int j = b + u * LP_THREADS + tid;
+                raw[u] = make_uint4(Vec::NEG_INF, Vec::NEG_INF, Vec::NEG_INF, Vec::NEG_INF);
+                if (j < v1) raw[u] = lp_load(x, lead, P.V, j);
             }
+        }
+        const float mx = Vec::max(raw), mn = Vec::min(raw);
+        best = fmaxf(best, mx);
+        if (best > a.m) lp_raise(a, best, c);
+        const float mc = __fmul_rn(a.m, c);
+        const bool sane = lp_sane(a.m);
+        if (sane) {
+            const unsigned long long c2 = f2_pack(c, c), mc2 = f2_pack(-mc, -mc);
+            unsigned long long s2 = 0ull, t2 = 0ull;
+            if (mn > -1e30f) {
+#pragma unroll
+                for (int u = 0; u < LP_U; u++) {
+                    float v[N];
+                    Vec::values(raw[u], v);
+#pragma unroll
+                    for (int e = 0; e < N; e += 2) {
+                        const unsigned long long d2 = ffma2(f2_pack(v[e], v[e + 1]), c2, mc2);
+                        float d0, d1;
+                        f2_unpack(d2, d0, d1);
+                        const unsigned long long w2 = f2_pack(lp_exp2(d0), lp_exp2(d1));
+                        s2 = lp_add2(s2, w2);
+                        t2 = ffma2(w2, d2, t2);
+                    }
+                }
+            } else {  // masked or absent values among them: a product of -inf becomes a power of two that is 0
+#pragma unroll
+                for (int u = 0; u < LP_U; u++) {
+                    float v[N];
+                    Vec::values(raw[u], v);
+#pragma unroll
+                    for (int e = 0; e < N; e += 2) {
+                        const float d0 = lp_max_nan(fmaf(v[e], c, -mc), -200.f), d1 = lp_max_nan(fmaf(v[e + 1], c, -mc), -200.f);
+                        const unsigned long long w2 = f2_pack(lp_exp2(d0), lp_exp2(d1));
+                        s2 = lp_add2(s2, w2);
+                        t2 = ffma2(w2, f2_pack(d0, d1), t2);
+                    }
+                }
+            }
+            a.s += f2_sum(s2);
+            a.t += f2_sum(t2);
+        } else {  // no value yet, or maxima that c would overflow
+#pragma unroll
+            for (int u = 0; u < LP_U; u++) {
+                if (b + u * LP_THREADS + tid >= v1) continue;
+#pragma unroll 1
+                for (int e = 0; e < N; e++) {
+                    const float y = lp_at<T>(raw[u], e);
+                    // before any choice that is not masked: weight 0, a NaN stays
+                    const float d = a.m == -INFINITY ? (y == y ? -200.f : y) : lp_max_nan((y - a.m) * c, -200.f);
+                    const float w = lp_exp2(d);
+                    a.s += w;
+                    a.t = fmaf(w, d, a.t);
+                }
+            }
+        }
+        if (count) {
+            typename Vec::Count n = Vec::zero();
+#pragma unroll
+            for (int u = 0; u < LP_U; u++) Vec::count(raw[u], b + u * LP_THREADS + tid < jt ? at_least : more, n);
+            above += Vec::total(n);
         }
         if constexpr (TOP) {
             if (tile == renew) {
                 renew = 2 * renew + 1;
                 raise_bound();
             }
-            int pass = 0;
             if (mx >= thr) {
 #pragma unroll
                 for (int u = 0; u < LP_U; u++) {
-                    const int j = b + u * LP_THREADS + tid, e0 = j * N - lead;
+                    float v[N];
+                    Vec::values(raw[u], v);
+                    unsigned hits = 0;
 #pragma unroll
-                    for (int e = 0; e < N; e++)
-                        pass += v[u][e] >= thr && j < v1 && e0 + e >= 0 && e0 + e < P.V && lp_key(v[u][e], e0 + e) > cut;
-                }
-            }
-            if (__syncthreads_or(pass)) {
-                int at = pass ? atomicAdd(&n_s, pass) : 0;
-                __syncthreads();
-                const int n = n_s;
-                if (n <= LP_LIST) {
-                    held = n;
-                    if (pass) {
-#pragma unroll
-                        for (int u = 0; u < LP_U; u++) {
-                            const int j = b + u * LP_THREADS + tid, e0 = j * N - lead;
-#pragma unroll
-                            for (int e = 0; e < N; e++) {
-                                const unsigned long long key = lp_key(v[u][e], e0 + e);
-                                if (v[u][e] >= thr && j < v1 && e0 + e >= 0 && e0 + e < P.V && key > cut) list[at++] = key;
-                            }
-                        }
+                    for (int e = 0; e < N; e++) hits |= (unsigned)(v[e] >= thr) << e;
+                    while (hits) {
+                        const int e = __ffs(hits) - 1, at = atomicAdd(&n_s, 1);
+                        hits &= hits - 1;
+                        if (at < LP_LIST) list[at] = lp_key(lp_at<T>(raw[u], e), (b + u * LP_THREADS + tid) * N - lead + e);
                     }
-                    __syncthreads();
-                } else {  // too many at once: value by value, the list cut to its k best whenever 256 more might not fit
-                    int have = held;
-                    __syncthreads();  // n_s is read
-#pragma unroll 1
-                    for (int u = 0; u < LP_U; u++)
-#pragma unroll 1
-                        for (int e = 0; e < N; e++) {
-                            if (have + LP_THREADS > LP_LIST) {
-                                have = lp_cut<LP_THREADS>(list, have, P.k);
-                                if (have == P.k) cut = max(cut, list[P.k - 1]);
-                            }
-                            if (tid == 0) n_s = have;
-                            __syncthreads();
-                            const int j = b + u * LP_THREADS + tid, id = j * N - lead + e;
-                            if (j < v1 && id >= 0 && id < P.V) {
-                                const float w = lp_f(x[id]);
-                                const unsigned long long key = lp_key(w, id);
-                                if (w >= thr && key > cut) list[atomicAdd(&n_s, 1)] = key;
-                            }
-                            __syncthreads();
-                            have = n_s;
-                            __syncthreads();
-                        }
-                    held = have;
                 }
             }
         }
     }
-    // join over the block
-    a = lp_warp(a);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(SB_FULL, above, o);
-    if (lane == 0) {
-        sum_s[warp] = a;
-        cnt_s[warp] = above;
+    if (count) {
+        if (tid < N && jt >= v0 && jt < v1) {
+            const int id = jt * N - lead + tid;
+            above += id >= 0 && id < tok && lp_f(x[id]) == xt;
+        }
+        if (xt == -INFINITY)
+            for (int id = max(v0 * N - lead, 0) + tid; id < min(v1, jt) * N - lead; id += LP_THREADS) above += lp_f(x[id]) == xt;
     }
-    __syncthreads();
-    a = sum_s[0];
-    above = cnt_s[0];
-#pragma unroll
-    for (int w = 1; w < LP_THREADS / 32; w++) {
-        a = lp_join(a, sum_s[w]);
-        above += cnt_s[w];
-    }
+    lp_block(a, above, c, sum_s);
     if (tid == 0) {
         if (P.S == 1) lp_finish(P, r, a, above, xt, given);
         else P.part[(long long)r * P.S + part] = make_float4(a.m, a.s, a.t, __int_as_float(above));
     }
     if constexpr (TOP) {
-        // what the final bound leaves of the list, ranked
-        raise_bound();
-        unsigned long long mine[LP_LIST / LP_THREADS];
+        int n = n_s;  // (the barriers above stand between the appends and this)
+        if (n > LP_LIST) {  // k passes: the best key below the last one
+            unsigned long long last = ~0ull;
+            for (n = 0; n < P.k; n++) {
+                unsigned long long top = 0ull;
+                for (int j = v0 + tid; j < v1; j += LP_THREADS) {
+                    const uint4 w = lp_load(x, lead, P.V, j);
+                    if (Vec::max(w) < thr) continue;
+#pragma unroll 1
+                    for (int e = 0; e < N; e++) {
+                        const float y = lp_at<T>(w, e);
+                        const unsigned long long key = y >= thr ? lp_key(y, j * N - lead + e) : 0ull;
+                        if (key < last && key > top) top = key;
+                    }
+                }
 #pragma unroll
-        for (int q = 0; q < LP_LIST / LP_THREADS; q++) {
-            const int i = tid + q * LP_THREADS;
-            mine[q] = i < held ? list[i] : 0ull;
+                for (int o = 16; o > 0; o >>= 1) {
+                    const unsigned long long other = __shfl_xor_sync(SB_FULL, top, o);
+                    top = other > top ? other : top;
+                }
+                __syncthreads();
+                if ((tid & 31) == 0) list[LP_KMAX + (tid >> 5)] = top;
+                __syncthreads();
+                for (int w = 0; w < LP_THREADS / 32; w++) top = list[LP_KMAX + w] > top ? list[LP_KMAX + w] : top;
+                if (top == 0ull) break;
+                if (tid == 0) list[n] = top;
+                last = top;
+            }
+            __syncthreads();
+        } else if (n > LP_THREADS / 4) {  // what the final bound leaves
+            raise_bound();
+            unsigned long long mine[LP_LIST / LP_THREADS];
+#pragma unroll
+            for (int q = 0; q < LP_LIST / LP_THREADS; q++) {
+                const int i = tid + q * LP_THREADS;
+                mine[q] = i < n ? list[i] : 0ull;
+            }
+            __syncthreads();
+            if (tid == 0) n_s = 0;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < LP_LIST / LP_THREADS; q++)
+                if (mine[q] && lp_key_value(mine[q]) >= thr) list[atomicAdd(&n_s, 1)] = mine[q];
+            __syncthreads();
+            n = n_s;
         }
-        __syncthreads();
-        if (tid == 0) n_s = 0;
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < LP_LIST / LP_THREADS; q++)
-            if (mine[q] && lp_key_value(mine[q]) >= thr) list[atomicAdd(&n_s, 1)] = mine[q];
-        __syncthreads();
-        const int n = n_s;
         const float l2 = log2f(a.s);
         unsigned long long *out = P.keys + ((long long)r * P.S + part) * P.k;
-        lp_rank<LP_THREADS>(list, n, P.k, [&](int i, unsigned long long key) {
+        lp_rank(list, n, P.k, [&](int i, unsigned long long key) {
             if (P.S == 1) lp_top(P, r, i, key, a.m, l2);
             else out[i] = key;
         });
@@ -359,86 +505,71 @@ SB_DEV void logprobs_body(const LpParams &P) {
         }
     }
 }
-#define LP_KERNEL(name, T, TOP) \
-    extern "C" __global__ void __launch_bounds__(LP_THREADS) name(const __grid_constant__ LpParams P) { logprobs_body<T, TOP>(P); }
-LP_KERNEL(logprobs_f32, float, false)
-LP_KERNEL(logprobs_f16, __half, false)
-LP_KERNEL(logprobs_bf16, __nv_bfloat16, false)
-LP_KERNEL(logprobs_top_f32, float, true)
-LP_KERNEL(logprobs_top_f16, __half, true)
-LP_KERNEL(logprobs_top_bf16, __nv_bfloat16, true)
+#define LP_KERNEL(name, T, TOP, CTAS) \
+    extern "C" __global__ void __launch_bounds__(LP_THREADS, CTAS) name(const __grid_constant__ LpParams P) { logprobs_body<T, TOP>(P); }
+LP_KERNEL(logprobs_f32, float, false, 5)
+LP_KERNEL(logprobs_f16, __half, false, 5)
+LP_KERNEL(logprobs_bf16, __nv_bfloat16, false, 5)
+LP_KERNEL(logprobs_top_f32, float, true, 5)
+LP_KERNEL(logprobs_top_f16, __half, true, 5)
+LP_KERNEL(logprobs_top_bf16, __nv_bfloat16, true, 5)
 
 // A CTA a row: the parts' sums, and the k best of their S sorted lists.  The
 // k-th best list head bounds the k-th best key from below, so at most k
 // lists matter and k x k keys are kept.
 // type: 0 f32, 1 f16, 2 bf16.
 extern "C" __global__ void __launch_bounds__(LP_THREADS) logprobs_join(const __grid_constant__ LpParams P, int type) {
-    __shared__ LpSum sum_s[LP_THREADS / 32];
-    __shared__ int cnt_s[LP_THREADS / 32];
-    __shared__ unsigned long long list[LP_KMAX * LP_KMAX];
+    __shared__ LpShared sum_s;
+    __shared__ unsigned long long list[LP_KMAX * LP_KMAX], head_s[LP_THREADS];
     __shared__ unsigned long long bound_s;
     __shared__ int n_s;
+    const int tid = threadIdx.x, r = blockIdx.x;
+    const int tok = P.tok ? P.tok[r] : -1;
+    const bool given = tok >= 0 && tok < P.V;
+    float xt = 0.f;
+    if (given) {
+        const long long at = r * P.stride + tok;
+        xt = type == 0 ? static_cast<const float *>(P.x)[at]
+                       : type == 1 ? lp_f(static_cast<const __half *>(P.x)[at]) : lp_f(static_cast<const __nv_bfloat16 *>(P.x)[at]);
+    }
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = blockIdx.x;
+    // S <= LP_THREADS: a part a thread
     LpSum a = {-INFINITY, 0.f, 0.f};
     int above = 0;
-    for (int s = tid; s < P.S; s += LP_THREADS) {
-        const float4 p = P.part[(long long)r * P.S + s];
-        a = lp_join(a, {p.x, p.y, p.z});
-        above += __float_as_int(p.w);
+    unsigned long long head = 0ull;
+    const unsigned long long *keys = P.keys + (long long)r * P.S * P.k;
+    if (tid < P.S) {
+        const float4 p = P.part[(long long)r * P.S + tid];
+        if (P.k) head = keys[(long long)tid * P.k];
+        a = {p.x, p.y, p.z};
+        above = __float_as_int(p.w);
     }
+    head_s[tid] = head;
     if (tid == 0) {
         n_s = 0;
         bound_s = 0ull;
     }
-    a = lp_warp(a);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(SB_FULL, above, o);
-    if (lane == 0) {
-        sum_s[warp] = a;
-        cnt_s[warp] = above;
-    }
-    __syncthreads();
-    a = sum_s[0];
-    above = cnt_s[0];
-#pragma unroll
-    for (int w = 1; w < LP_THREADS / 32; w++) {
-        a = lp_join(a, sum_s[w]);
-        above += cnt_s[w];
-    }
-    const int tok = P.tok ? P.tok[r] : -1;
-    const bool given = tok >= 0 && tok < P.V;
-    if (tid == 0) {
-        float xt = 0.f;
-        if (given) {
-            const long long at = r * P.stride + tok;
-            xt = type == 0 ? static_cast<const float *>(P.x)[at]
-                           : type == 1 ? lp_f(static_cast<const __half *>(P.x)[at]) : lp_f(static_cast<const __nv_bfloat16 *>(P.x)[at]);
-        }
-        lp_finish(P, r, a, above, xt, given);
-    }
+    lp_block(a, above, P.c, sum_s);
+    if (tid == 0) lp_finish(P, r, a, above, xt, given);
     if (P.k == 0) return;
-    const unsigned long long *keys = P.keys + (long long)r * P.S * P.k;
-    if (P.S >= P.k)
-        for (int s = tid; s < P.S; s += LP_THREADS) {
-            const unsigned long long me = keys[(long long)s * P.k];
-            int rk = 0;
-            for (int j = 0; j < P.S; j++) {
-                const unsigned long long o = keys[(long long)j * P.k];
-                rk += o > me || (o == me && j < s);
-            }
-            if (rk == P.k - 1) bound_s = me;
-        }
+    if (P.S >= P.k && tid < P.S) {
+        int rk = 0;
+        for (int j = 0; j < P.S; j++) rk += head_s[j] > head || (head_s[j] == head && j < tid);
+        if (rk == P.k - 1) bound_s = head;
+    }
     __syncthreads();
     const unsigned long long bound = bound_s;
-    for (int i = tid; i < P.S * P.k; i += LP_THREADS) {
-        const unsigned long long key = keys[i];
-        if (key && key >= bound) list[atomicAdd(&n_s, 1)] = key;
+    if (tid < P.S && head && head >= bound) {  // a sorted list: as far as it reaches the bound
+        for (int i = 0; i < P.k; i++) {
+            const unsigned long long key = i ? keys[(long long)tid * P.k + i] : head;
+            if (!key || key < bound) break;
+            list[atomicAdd(&n_s, 1)] = key;
+        }
     }
     __syncthreads();
     const int n = n_s;
     const float l2 = log2f(a.s);
-    lp_rank<LP_THREADS>(list, n, P.k, [&](int i, unsigned long long key) { lp_top(P, r, i, key, a.m, l2); });
+    lp_rank(list, n, P.k, [&](int i, unsigned long long key) { lp_top(P, r, i, key, a.m, l2); });
     for (int i = n + tid; i < P.k; i += LP_THREADS) lp_top(P, r, i, 0ull, a.m, l2);
 }
 
@@ -462,7 +593,8 @@ template <> SB_DEV __nv_bfloat16 lp_to<__nv_bfloat16>(float v) { return __float2
 
 template <typename T>
 SB_DEV void logprobs_grad_body(const LpGradParams &P) {
-    constexpr int N = LpVec<T>::N;
+    using Vec = LpVec<T>;
+    constexpr int N = Vec::N, TILE = LP_THREADS * LP_U;
     const int r = blockIdx.x / P.S, part = blockIdx.x % P.S, tid = threadIdx.x;
     const T *x = static_cast<const T *>(P.x) + r * P.stride;
     T *dx = static_cast<T *>(P.dx) + r * P.dstride;
@@ -470,38 +602,72 @@ SB_DEV void logprobs_grad_body(const LpGradParams &P) {
     const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;  // else the vectors of dx would straddle
     const int nv = (int)(((long long)lead + P.V + N - 1) / N);
     const int v0 = (int)((long long)nv * part / P.S), v1 = (int)((long long)nv * (part + 1) / P.S);
+    const int whole0 = lead ? 1 : 0, whole1 = min((int)(((long long)lead + P.V) / N), v1);
     const int tok = P.tok ? P.tok[r] : -1;
     const bool given = tok >= 0 && tok < P.V;
+    const int jt = given ? (tok + lead) / N : -1;
     const float lse = P.lse[r], H = P.g_entropy ? P.entropy[r] : 0.f;
     const float gl = given && P.g_logp ? P.g_logp[r] * P.inv_temp : 0.f, ge = P.g_entropy ? P.g_entropy[r] * P.inv_temp : 0.f;
-    const bool none = lse == -INFINITY;
+    const bool none = lse == -INFINITY, sane = lp_sane(lse);
     constexpr float L2E = 1.4426950408889634f, L2E_LO = 1.925963033500e-08f;
-    const float hi = none ? 0.f : lse * L2E, lo = none ? 0.f : fmaf(lse, L2E, -hi) + lse * L2E_LO;
-    const float a0 = gl + ge * H, a1 = ge * LP_LN2;  // dx = -p (a0 + a1 d), d = log2 p
-    auto grad = [&](float v, int id) {
-        const float d = fmaxf(fmaf(v, P.c, -hi) - lo, -200.f);
-        const float p = none ? 0.f : lp_exp2(d);
-        const float g = -p * fmaf(a1, d, a0);
-        return id == tok && !none ? g + gl : g;
+    const float hi = sane ? lse * L2E : 0.f, lo = sane ? fmaf(lse, L2E, -hi) + lse * L2E_LO : 0.f;
+    // dx = -p (a0 + a1 log2 p) with log2 p = d - lo, d = c x - hi: 2^-lo goes into the factors
+    const float a1 = ge * LP_LN2, a0 = gl + ge * H, f = lp_exp2(-lo), b1 = -a1 * f, b0 = -(a0 - a1 * lo) * f;
+    auto grad = [&](float v, int id) {  // one value, any range
+        const float d = lp_max_nan(sane ? fmaf(v, P.c, -hi) : (v * P.inv_temp - lse) * L2E, -200.f);
+        const float g = lp_exp2(d) * fmaf(b1, d, b0);
+        return none ? 0.f : id == tok ? g + gl : g;
     };
-    for (int b = v0; b < v1; b += LP_THREADS * LP_U) {
+    const unsigned long long c2 = f2_pack(P.c, P.c), hi2 = f2_pack(-hi, -hi), b12 = f2_pack(b1, b1), b02 = f2_pack(b0, b0);
+    for (int b = v0; b < v1; b += TILE) {
         uint4 raw[LP_U];
+        const bool whole = same && sane && b >= whole0 && b + TILE <= whole1;
+        if (whole) {
 #pragma unroll
-        for (int u = 0; u < LP_U; u++) {
-            const int j = b + u * LP_THREADS + tid, e0 = j * N - lead;
-            if (same && j < v1 && e0 >= 0 && e0 + N <= P.V) raw[u] = *reinterpret_cast<const uint4 *>(x + e0);
+            for (int u = 0; u < LP_U; u++) raw[u] = *reinterpret_cast<const uint4 *>(x + ((b + u * LP_THREADS + tid) * N - lead));
+            if (Vec::min(raw) > -1e30f) {
+#pragma unroll
+                for (int u = 0; u < LP_U; u++) {
+                    const int j = b + u * LP_THREADS + tid;
+                    float v[N];
+                    Vec::values(raw[u], v);
+                    if (j == jt) continue;  // written below
+#pragma unroll
+                    for (int e = 0; e < N; e += 2) {
+                        const unsigned long long d2 = ffma2(f2_pack(v[e], v[e + 1]), c2, hi2);
+                        float d0, d1;
+                        f2_unpack(d2, d0, d1);
+                        const unsigned long long g2 = lp_mul2(f2_pack(lp_exp2(d0), lp_exp2(d1)), ffma2(b12, d2, b02));
+                        f2_unpack(g2, v[e], v[e + 1]);
+                    }
+                    *reinterpret_cast<uint4 *>(dx + (j * N - lead)) = Vec::packed(v);
+                }
+                if (jt >= b && jt < b + TILE && (jt - b) % LP_THREADS == tid) {
+#pragma unroll
+                    for (int u = 0; u < LP_U; u++) {
+                        const int j = b + u * LP_THREADS + tid;
+                        float v[N];
+                        Vec::values(raw[u], v);
+                        if (j != jt) continue;
+#pragma unroll
+                        for (int e = 0; e < N; e++) v[e] = grad(v[e], j * N - lead + e);
+                        *reinterpret_cast<uint4 *>(dx + (j * N - lead)) = Vec::packed(v);
+                    }
+                }
+                continue;
+            }
         }
 #pragma unroll
         for (int u = 0; u < LP_U; u++) {
             const int j = b + u * LP_THREADS + tid, e0 = j * N - lead;
             if (j >= v1) break;
             if (same && e0 >= 0 && e0 + N <= P.V) {
-                const T *h = reinterpret_cast<const T *>(&raw[u]);
-                uint4 o;
-                T *w = reinterpret_cast<T *>(&o);
+                if (!whole) raw[u] = *reinterpret_cast<const uint4 *>(x + e0);
+                float v[N];
+                Vec::values(raw[u], v);
 #pragma unroll
-                for (int e = 0; e < N; e++) w[e] = lp_to<T>(grad(lp_f(h[e]), e0 + e));
-                *reinterpret_cast<uint4 *>(dx + e0) = o;
+                for (int e = 0; e < N; e++) v[e] = grad(v[e], e0 + e);
+                *reinterpret_cast<uint4 *>(dx + e0) = Vec::packed(v);
             } else {
                 for (int e = 0; e < N; e++)
                     if (e0 + e >= 0 && e0 + e < P.V) dx[e0 + e] = lp_to<T>(grad(lp_f(x[e0 + e]), e0 + e));

@@ -415,7 +415,7 @@ struct lp_params {
     CUdeviceptr x;
     int64_t stride;
     int R, V, S, k;
-    float c;
+    float c, inv_temp;
     CUdeviceptr tok, logp, entropy, lse, rank, top_ids, top_logp, part, keys;
 };
 struct lp_grad_params {
@@ -425,9 +425,11 @@ struct lp_grad_params {
     float c, inv_temp;
     CUdeviceptr tok, lse, entropy, g_logp, g_entropy;
 };
-/* parts of a row: enough CTAs for a few waves, 4 KB of logits each at least */
+/* parts of a row: one where the rows fill the SMs (no join, and the bound of
+ * the alternatives is renewed less often), else enough for `waves` CTAs per
+ * SM, 4 KB of logits each at least */
 static int lp_parts(sb_ctx *c, int R, int V, int type, long waves) {
-    long S = CEIL_DIV(waves * c->sms, (long)R), most = (long)V * type_size(type) / 4096;
+    long S = R >= 4L * c->sms ? 1 : CEIL_DIV(waves * c->sms, (long)R), most = (long)V * type_size(type) / 4096;
     if (S > most) S = most;
     if (S > SB_LOGPROBS_MAX_PARTS) S = SB_LOGPROBS_MAX_PARTS;
     return (int)(S < 1 ? 1 : S);
@@ -476,6 +478,7 @@ int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, 
     p.V = V;
     p.k = top_k;
     p.c = 1.4426950408889634f / temperature;
+    p.inv_temp = 1.0f / temperature;
     p.tok = DP(tokens);
     p.logp = DP(logp);
     p.entropy = DP(entropy);
@@ -517,7 +520,9 @@ int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, in
     p.dstride = grad_stride;
     p.R = R;
     p.V = V;
-    p.S = lp_parts(c, R, V, type, 16);
+    /* the gradient has nothing to join: 16 CTAs per SM even out the last wave */
+    long S = CEIL_DIV(16L * c->sms, (long)R), most = CEIL_DIV((long)V * type_size(type), 16384);
+    p.S = (int)(S < most ? S : most);
     p.c = 1.4426950408889634f / temperature;
     p.inv_temp = 1.0f / temperature;
     p.tok = DP(tokens);

@@ -121,6 +121,40 @@ def test_logprobs_masked_rows(cuda_dev, R):
     check(x, tok + 105, 20)
 
 
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("R", [1, 700])
+def test_logprobs_lowest_value_masks(cuda_dev, kind, R):
+    """Masks of the type's lowest value: weight 0 beside other choices; alone
+    they are equal choices, and -inf beside them still has weight 0."""
+    V, t = 3001, DT[kind]
+    low = torch.finfo(t).min
+    x = torch.full((R, V), low, dtype=t, device="cuda")
+    tok = torch.full((R,), 2000, dtype=torch.int32, device="cuda")
+    grad, one = torch.empty_like(x), torch.ones(R, device="cuda")
+    for n, ids in ((V, [0, 1, 2, 3, 4]), (V - V // 2, [1500, 1501, 1502, 1503, 1504])):
+        got = run(x, tok, 5)
+        # equal choices: ln n to the FP32 sum's (n / 256 + 16) half steps and 2^-22 of the logarithm
+        for name in ("logp", "entropy", "top_logp"):
+            assert bool(((got[name].double().abs() - math.log(n)).abs() <= 2.0 ** -18).all()), name
+        assert bool((got["top_ids"] == torch.tensor(ids, device="cuda")).all()) and bool((got["rank"] == 2000 - ids[0]).all())
+        sb200.logprobs_grad(x, tok, got["lse"], got["entropy"], one, one, grad, stream=stream())
+        # lse = lowest + ln n rounds to the lowest value itself: a probability there means nothing, but nothing is NaN
+        assert not bool(torch.isnan(grad).any())
+        x[:, : V // 2] = -math.inf
+    x[:, 10] = 1.5
+    x[:, 2999] = -0.5
+    # two choices of size 1 are left
+    want = reference(x, tok - 1990, 5, 1.0)
+    got = run(x, tok - 1990, 5)
+    for name in ("lse", "logp", "entropy"):
+        assert bool(((got[name].double() - want[name]).abs() <= 2.0 ** -20).all()), name
+    assert torch.equal(got["top_ids"].long(), want["top_ids"]) and torch.equal(got["rank"].long(), want["rank"])
+    sb200.logprobs_grad(x, tok - 1990, got["lse"], got["entropy"], one, one, grad, stream=stream())
+    want = gradient(x, tok - 1990, one, one, 1.0)
+    # values of size 1, one rounding each and 2^-20 of the exponentials
+    assert bool(((grad.double() - want).abs() <= torch.finfo(t).eps / 2 * want.abs() + 2.0 ** -19).all())
+
+
 def test_logprobs_nan_and_inf(cuda_dev):
     """A NaN or +inf makes its own row's sums NaN, no other row's."""
     x = torch.randn(6, 3001, device="cuda")
