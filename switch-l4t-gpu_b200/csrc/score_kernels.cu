@@ -25,8 +25,8 @@
 // a lower bound of the k-th best value: k holders each have a value at least
 // that good.  Only vectors that reach it are looked into, and only values
 // that reach it go to a list in shared memory -- about k per doubling of the
-// values seen, as the bound is renewed after tiles 0, 1, 3, 7, ...  Where the
-// list overflows (rising or equal logits), the part's k best are taken by k
+// values seen, as the bound is renewed with each of the first tiles, later with
+// every fourth.  Where the list overflows (rising or equal logits), the part's k best are taken by k
 // passes instead.
 #include <cfloat>
 #include <cuda_bf16.h>
@@ -312,9 +312,10 @@ SB_DEV void logprobs_body(const LpParams &P) {
     LpSum a = {-INFINITY, 0.f, 0.f};
     int above = 0;
     float best = -INFINITY, thr = -FLT_MAX;
-    // group maxima: one per thread, per 4 lanes or per 8 (fewer are looser and cheaper to rank)
-    const int per = P.k > 24 ? 1 : P.k > 8 ? 4 : 8, groups = LP_THREADS / per;
-    int renew = 0, tile = 0;
+    // group maxima, one per 2, 4 or 8 lanes: 2 to 4 times k of them leave 1.2 to 1.4 k values above the
+    // k-th, and a tighter bound from more groups costs more to rank than it saves
+    const int per = P.k > 24 ? 2 : P.k > 8 ? 4 : 8, groups = LP_THREADS / per;
+    int tile = 0;
     if (TOP && tid == 0) n_s = 0;
 
     // the k-th best group maximum bounds the k-th best value from below
@@ -390,16 +391,24 @@ SB_DEV void logprobs_body(const LpParams &P) {
             }
             a.s += f2_sum(s2);
             a.t += f2_sum(t2);
-        } else {  // no value yet, or maxima that c would overflow
+        } else if (a.m == -INFINITY) {  // masked choices only so far: no weight, but a NaN among them stays
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < LP_U; u++) {
+                float v[N];
+                Vec::values(raw[u], v);
+#pragma unroll
+                for (int e = 0; e < N; e++) sum += v[e];
+            }
+            if (sum != sum) a.s = sum;
+        } else {  // maxima that c would overflow
 #pragma unroll
             for (int u = 0; u < LP_U; u++) {
                 if (b + u * LP_THREADS + tid >= v1) continue;
 #pragma unroll 1
                 for (int e = 0; e < N; e++) {
                     const float y = lp_at<T>(raw[u], e);
-                    // before any choice that is not masked: weight 0, a NaN stays
-                    const float d = a.m == -INFINITY ? (y == y ? -200.f : y) : lp_max_nan((y - a.m) * c, -200.f);
-                    const float w = lp_exp2(d);
+                    const float d = lp_max_nan((y - a.m) * c, -200.f), w = lp_exp2(d);
                     a.s += w;
                     a.t = fmaf(w, d, a.t);
                 }
@@ -412,10 +421,7 @@ SB_DEV void logprobs_body(const LpParams &P) {
             above += Vec::total(n);
         }
         if constexpr (TOP) {
-            if (tile == renew) {
-                renew = 2 * renew + 1;
-                raise_bound();
-            }
+            if (tile < 4 || (tile & 3) == 3 || thr == -FLT_MAX) raise_bound();
             if (mx >= thr) {
 #pragma unroll
                 for (int u = 0; u < LP_U; u++) {

@@ -36,6 +36,8 @@ SB_DEV void plan_scan2(int &a, int &b, int *wa, int *wb) {
     a = sa + x - a;
     b = sb + y - b;
 }
+// pages that n positions fill; n + page - 1 < 2^32 (a 64-bit division costs 100 cycles)
+SB_DEV int plan_pages(unsigned n, unsigned page) { return (int)((n + page - 1) / page); }
 
 // dynamic shared memory: 2 (B + 1) ints
 extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
@@ -46,39 +48,41 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
     extern __shared__ int plan_sm[];
     __shared__ int wa[SB_PLAN_THREADS / 32], wb[SB_PLAN_THREADS / 32], lack_s;
     int *cu = plan_sm, *first = plan_sm + B + 1;
-    const int tid = threadIdx.x, per = (B + SB_PLAN_THREADS - 1) / SB_PLAN_THREADS;
+    const int tid = threadIdx.x, nthreads = blockDim.x, per = (B + nthreads - 1) / nthreads;
     if (tid == 0) lack_s = 0;
     // this thread's requests [b0, b1): tokens and pages, negative lengths as 0
     const int b0 = min(tid * per, B), b1 = min(b0 + per, B);
-    int tok = 0, add = 0, lack = 0;
+    int tok = 0, add = 0, lack = 0, len = 0;
     for (int b = b0; b < b1; b++) {
         const int c = max(cache_len[b], 0), n = max(new_len[b], 0);
-        const int have = (int)(((long long)c + page - 1) / page), need = (int)(((long long)c + n + page - 1) / page);
-        const int got = max(min(need, width) - have, 0);
+        const int have = plan_pages(c, page), need = plan_pages((unsigned)c + n, page), got = max(min(need, width) - have, 0);
+        cu[b] = n;
+        first[b] = got;
         tok += n;
         add += got;
         lack += need - have - got;
+        len = c + n;
     }
     int t0 = tok, p0 = add;
     plan_scan2(t0, p0, wa, wb);
-    for (int b = b0; b < b1; b++) {
-        const int c = max(cache_len[b], 0), n = max(new_len[b], 0);
-        const int have = (int)(((long long)c + page - 1) / page), need = (int)(((long long)c + n + page - 1) / page);
+    for (int b = b0; b < b1; b++) {  // lengths turn into sums in place
+        const int n = cu[b], got = first[b];
         cu[b] = t0;
         first[b] = p0;
         t0 += n;
-        p0 += max(min(need, width) - have, 0);
+        p0 += got;
     }
     if (b1 == B && b0 < B) {  // the thread that owns the last request (B > 0)
         cu[B] = t0;
         first[B] = p0;
     }
     if (lack) atomicAdd(&lack_s, lack);
+    if (blockIdx.x == 0 && per == 1 && b0 < B) kv_len[b0] = len;
     __syncthreads();
     if (blockIdx.x == 0) {
-        for (int b = tid; b <= B; b += SB_PLAN_THREADS) {
+        for (int b = tid; b <= B; b += nthreads) {
             cu_q[b] = cu[b];
-            if (b < B) kv_len[b] = max(cache_len[b], 0) + max(new_len[b], 0);
+            if (b < B && per > 1) kv_len[b] = max(cache_len[b], 0) + max(new_len[b], 0);
         }
         if (tid == 0) {
             const int total = first[B], taken = min(total, n_free);
@@ -87,17 +91,17 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
         }
     }
     // new entries of the tables: a warp a request
-    const int lane = tid & 31, nw = gridDim.x * (SB_PLAN_THREADS / 32);
-    for (int b = blockIdx.x * (SB_PLAN_THREADS / 32) + (tid >> 5); b < B; b += nw) {
+    const int lane = tid & 31, nw = gridDim.x * (nthreads / 32);
+    for (int b = blockIdx.x * (nthreads / 32) + (tid >> 5); b < B; b += nw) {
         const int f = first[b], n = first[b + 1] - f;
         if (n == 0) continue;
-        const int have = (int)(((long long)max(cache_len[b], 0) + page - 1) / page);
+        const int have = plan_pages(max(cache_len[b], 0), page);
         for (int j = lane; j < n; j += 32)
             table[(size_t)b * table_stride + have + j] = f + j < n_free ? free_pages[f + j] : -1;
     }
     // tokens: four neighbours a thread
     const int total = cu[B];
-    for (long long q = (long long)blockIdx.x * SB_PLAN_THREADS + tid; q * 4 < T; q += (long long)gridDim.x * SB_PLAN_THREADS) {
+    for (long long q = (long long)blockIdx.x * nthreads + tid; q * 4 < T; q += (long long)gridDim.x * nthreads) {
         const int t = (int)(q * 4);
         int b = -1;
         if (t < total) {  // the last request that starts at or before t and is not empty
@@ -109,27 +113,50 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
             }
             b = lo;
         }
+        long long slot[4];
+        int p[4], rq[4], c = -1, have = 0, j = 0, off = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (t + i >= T) break;
-            if (t + i >= total) b = -1;
-            long long slot = -1;
-            int p = -1;
-            if (b >= 0) {
-                while (t + i >= cu[b + 1]) b++;
-                const int c = max(cache_len[b], 0);
-                p = c + (t + i - cu[b]);
-                const int j = p / page, have = (int)(((long long)c + page - 1) / page);
-                int pg = -1;
-                if (j < width) {
-                    if (j < have) pg = table[(size_t)b * table_stride + j];
-                    else if (first[b] + j - have < n_free) pg = free_pages[first[b] + j - have];
-                }
-                if (pg >= 0) slot = (long long)pg * page + p % page;
+            slot[i] = -1;
+            p[i] = rq[i] = -1;
+            if (t + i >= total) continue;
+            bool fresh = i == 0;
+            while (t + i >= cu[b + 1]) {
+                b++;
+                fresh = true;
             }
-            slots[t + i] = slot;
-            pos[t + i] = p;
-            req[t + i] = b;
+            if (fresh) {
+                c = max(cache_len[b], 0);
+                have = plan_pages(c, page);
+                const int at = c + (t + i - cu[b]);
+                j = at / page;
+                off = at - j * page;
+            } else if (++off == page) {
+                off = 0;
+                j++;
+            }
+            int pg = -1;
+            if (j < width) {
+                if (j < have) pg = table[(size_t)b * table_stride + j];
+                else if (first[b] + j - have < n_free) pg = free_pages[first[b] + j - have];
+            }
+            if (pg >= 0) slot[i] = (long long)pg * page + off;
+            p[i] = c + (t + i - cu[b]);
+            rq[i] = b;
+        }
+        if (t + 4 <= T && ((uintptr_t)slots & 15) == 0 && (((uintptr_t)pos | (uintptr_t)req) & 15) == 0) {
+            reinterpret_cast<longlong2 *>(slots + t)[0] = make_longlong2(slot[0], slot[1]);
+            reinterpret_cast<longlong2 *>(slots + t)[1] = make_longlong2(slot[2], slot[3]);
+            *reinterpret_cast<int4 *>(pos + t) = make_int4(p[0], p[1], p[2], p[3]);
+            *reinterpret_cast<int4 *>(req + t) = make_int4(rq[0], rq[1], rq[2], rq[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (t + i >= T) break;
+                slots[t + i] = slot[i];
+                pos[t + i] = p[i];
+                req[t + i] = rq[i];
+            }
         }
     }
 }

@@ -32,11 +32,14 @@ int sb_kv_plan(const int *cache_len, const int *new_len, int B, int page, const 
     CUdeviceptr cl = DP(cache_len), nl = DP(new_len), fp = DP(free_pages), tb = DP(table), sl = DP(slots), po = DP(pos),
                 rq = DP(req), cq = DP(cu_q), kl = DP(kv_len), us = DP(used);
     void *args[] = {&cl, &nl, &B, &page, &fp, &n_free, &tb, &table_stride, &width, &sl, &po, &rq, &T, &cq, &kl, &us};
-    /* enough CTAs for four tokens a thread and a warp a request, two per SM at most */
-    long g = CEIL_DIV((long)T, 4 * 512), gb = CEIL_DIV(B, 16);
-    if (gb > g) g = gb;
+    /* a decode step of up to 128 requests is one small CTA (its barriers are
+     * cheaper); else enough CTAs for four tokens a thread and a warp a
+     * request, two per SM at most */
+    const int threads = B <= 128 && T <= 512 ? 128 : 512;
+    long g = CEIL_DIV((long)T, 4L * threads), gb = CEIL_DIV(B, threads / 32);
+    if (gb > g && threads == 512) g = gb;
     if (g > 2L * c->sms) g = 2L * c->sms;
-    return sb_launch(c, F_KV_PLAN, (unsigned)(g < 1 ? 1 : g), 1, 512, (unsigned)(2 * (B + 1) * 4), (CUstream)stream, args, 0);
+    return sb_launch(c, F_KV_PLAN, (unsigned)(g < 1 ? 1 : g), 1, (unsigned)threads, (unsigned)(2 * (B + 1) * 4), (CUstream)stream, args, 0);
 }
 
 /* ---------------------------------------------------------------- rotary */

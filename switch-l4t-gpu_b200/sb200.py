@@ -351,32 +351,54 @@ def _need(ok, what):
         raise SbError(what)
 
 
+class _Torch:
+    """torch's names that every call needs, looked up once."""
+    dev = None
+
+    def __init__(self):
+        import torch
+        self.i32, self.i64, self.f32 = torch.int32, torch.int64, torch.float32
+        self.types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+        self.current_device = torch.cuda.current_device if torch.cuda.is_available() else lambda: None
+
+
+_torch_names = None
+
+
+def _tn():
+    global _torch_names
+    if _torch_names is None:
+        _torch_names = _Torch()
+    return _torch_names
+
+
 def _type(t):
-    got = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}.get(str(t.dtype))
-    _need(got is not None, f"element type {t.dtype}: need float32, float16 or bfloat16")
+    got = _tn().types.get(t.dtype)
+    if got is None:
+        raise SbError(f"element type {t.dtype}: need float32, float16 or bfloat16")
     return got
 
 
 def _on_device(*tensors):
     """Every tensor is on the current CUDA device (the one whose context runs the call)."""
-    import torch
-    dev = torch.cuda.current_device() if torch.cuda.is_available() else None
+    dev = _tn().current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise SbError(f"tensor on {t.device}: need the current CUDA device")
 
 
 def _vector(t, name, dtype, n):
-    """A contiguous vector (or matrix) of at least n entries of a type, or None."""
-    if t is None:
-        return
-    _need(str(t.dtype) == "torch." + dtype and t.is_contiguous() and t.numel() >= n,
-          f"{name}: need a contiguous {dtype} tensor of at least {n} entries")
+    """A contiguous tensor of at least n entries of a type, or None."""
+    if t is not None and (t.dtype is not dtype or t.numel() < n or not t.is_contiguous()):
+        raise SbError(f"{name}: need a contiguous {dtype} tensor of at least {n} entries")
 
 
 def _rows3(t, name):
-    """[rows, heads, head size] whose last dimension is contiguous."""
-    _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{name}: need [rows, heads, head size], values contiguous")
+    """[rows, heads, head size] whose last dimension is contiguous; its shape and strides."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] != 1):
+        raise SbError(f"{name}: need [rows, heads, head size], values contiguous")
+    return shape, stride
 
 
 class KvPages:
@@ -390,6 +412,8 @@ class KvPages:
         _need(k.device == v.device, "pages: k and v on different devices")
         self.k, self.v = k, v  # keeps the memory alive
         self.c = _KvPages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), _type(k), *k.shape)
+        self.dtype = k.dtype
+        _, self.page, self.NKV, self.HD = k.shape
         self.ref = ctypes.byref(self.c)
 
 
@@ -407,53 +431,71 @@ class Rotary:
 def kv_plan(cache_len, new_len, free_pages, table, page, slots, pos, req, cu_q, kv_len, used, stream=None):
     """Block tables, slot map, positions and row offsets of a step from its
     requests' lengths (sb_kv_plan); int32 tensors, slots int64, table [B, width]."""
+    n = _tn()
     B, T = cache_len.numel(), slots.numel()
     _on_device(cache_len, new_len, free_pages, table, slots, pos, req, cu_q, kv_len, used)
-    for t, n, m in ((cache_len, "cache_len", B), (new_len, "new_len", B), (free_pages, "free_pages", 0), (pos, "pos", T),
-                    (req, "req", T), (cu_q, "cu_q", B + 1), (kv_len, "kv_len", B), (used, "used", 2)):
-        _vector(t, n, "int32", m)
-    _vector(slots, "slots", "int64", T)
-    _need(table.dim() == 2 and table.shape[0] >= B and str(table.dtype) == "torch.int32" and table.stride(1) == 1,
-          "table: need an int32 [B, width] tensor with contiguous rows")
-    check(lib().sb_kv_plan(_p(cache_len), _p(new_len), B, page, _p(free_pages), free_pages.numel(), _p(table),
-                           table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[1], _p(slots), _p(pos), _p(req), T,
-                           _p(cu_q), _p(kv_len), _p(used), _s(stream)))
+    i32 = n.i32
+    _vector(cache_len, "cache_len", i32, B)
+    _vector(new_len, "new_len", i32, B)
+    _vector(free_pages, "free_pages", i32, 0)
+    _vector(slots, "slots", n.i64, T)
+    _vector(pos, "pos", i32, T)
+    _vector(req, "req", i32, T)
+    _vector(cu_q, "cu_q", i32, B + 1)
+    _vector(kv_len, "kv_len", i32, B)
+    _vector(used, "used", i32, 2)
+    stride, width = _table(table, B)
+    check(lib().sb_kv_plan(cache_len.data_ptr(), new_len.data_ptr(), B, page, free_pages.data_ptr(), free_pages.numel(), table.data_ptr(),
+                           stride, width, slots.data_ptr(), pos.data_ptr(), req.data_ptr(), T, cu_q.data_ptr(), kv_len.data_ptr(),
+                           used.data_ptr(), _s(stream)))
+
+
+def _table(t, B):
+    """Row stride and width of an int32 [B, width] table."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] < B or t.dtype is not _tn().i32 or (stride[1] != 1 and shape[1] != 1):
+        raise SbError("table: need an int32 [B, width] tensor with contiguous rows")
+    return (stride[0] if shape[0] > 1 else shape[1]), shape[1]
 
 
 def rotary(x, y, pos, plan, inverse=False, stream=None):
     """y = x [T, heads, head size] turned by pos (int32 [T]); inverse turns
     back (the gradient).  y may be x."""
-    _rows3(x, "x")
-    _rows3(y, "y")
-    _need(x.shape == y.shape and x.dtype == y.dtype, "rotary: x and y differ in shape or type")
-    T, H, HD = x.shape
-    _vector(pos, "pos", "int32", T)
+    shape, xs = _rows3(x, "x")
+    _, ys = _rows3(y, "y")
+    _need(shape == y.shape and x.dtype is y.dtype, "rotary: x and y differ in shape or type")
+    T, H, HD = shape
+    _vector(pos, "pos", _tn().i32, T)
     _on_device(x, y, pos)
-    check(lib().sb_rotary(_p(x), x.stride(0), x.stride(1), _p(y), y.stride(0), y.stride(1), _type(x), T, H, HD, _p(pos), plan.ref,
+    check(lib().sb_rotary(x.data_ptr(), xs[0], xs[1], y.data_ptr(), ys[0], ys[1], _type(x), T, H, HD, pos.data_ptr(), plan.ref,
                           1 if inverse else 0, _s(stream)))
 
 
 def rotary_kv(q, q_out, k, v, pos, slots, plan, kv, stream=None):
     """q_out = q turned; k turned and v stored in the pages at slots (int64
     [T], -1: nowhere).  q [T, NH, HD], k and v [T, NKV, HD]."""
-    for t, n in ((q, "q"), (q_out, "q_out"), (k, "k"), (v, "v")):
-        _rows3(t, n)
-    T, NH, HD = q.shape
-    _need(q.shape == q_out.shape and k.shape == v.shape == (T, kv.c.NKV, kv.c.HD) and HD == kv.c.HD,
+    shape, qs = _rows3(q, "q")
+    oshape, os_ = _rows3(q_out, "q_out")
+    kshape, ks = _rows3(k, "k")
+    vshape, vs = _rows3(v, "v")
+    T, NH, HD = shape
+    _need(shape == oshape and kshape == vshape == (T, kv.NKV, kv.HD) and HD == kv.HD,
           "rotary_kv: q, k, v and the pages differ in rows, heads or head size")
-    _need(q.dtype == q_out.dtype == k.dtype == v.dtype == kv.k.dtype, "rotary_kv: rows and pages differ in type")
-    _vector(pos, "pos", "int32", T)
-    _vector(slots, "slots", "int64", T)
+    t = kv.dtype
+    _need(q.dtype is t and q_out.dtype is t and k.dtype is t and v.dtype is t, "rotary_kv: rows and pages differ in type")
+    n = _tn()
+    _vector(pos, "pos", n.i32, T)
+    _vector(slots, "slots", n.i64, T)
     _on_device(q, q_out, k, v, pos, slots, kv.k)
-    check(lib().sb_rotary_kv(_p(q), q.stride(0), q.stride(1), _p(q_out), q_out.stride(0), q_out.stride(1), _p(k), k.stride(0),
-                             k.stride(1), _p(v), v.stride(0), v.stride(1), T, NH, _p(pos), _p(slots), plan.ref, kv.ref, _s(stream)))
+    check(lib().sb_rotary_kv(q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os_[0], os_[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+                             vs[1], T, NH, pos.data_ptr(), slots.data_ptr(), plan.ref, kv.ref, _s(stream)))
 
 
 def attn_prefix_ws(q, kv, prefix_len, B, max_q=1, max_kv=0):
     """Workspace bytes of attn_prefix for these sizes (kv: the prefix' or the
     requests' pages)."""
     n = ctypes.c_size_t()
-    check(lib().sb_attn_prefix_ws(_type(q), q.shape[0], B, q.shape[1], kv.c.NKV, kv.c.HD, max_q, prefix_len, max_kv, ctypes.byref(n)))
+    check(lib().sb_attn_prefix_ws(_type(q), q.shape[0], B, q.shape[1], kv.NKV, kv.HD, max_q, prefix_len, max_kv, ctypes.byref(n)))
     return n.value
 
 
@@ -463,33 +505,32 @@ def attn_prefix(q, out, prefix, prefix_table, prefix_len, kv, table, kv_len, sca
     prefix_table, None: in order) and each request's own pages (kv, table
     [B, width], kv_len [B]); see sb_attn_prefix.  ws: a uint8 tensor of
     attn_prefix_ws bytes, or None when that is 0."""
-    _rows3(q, "q")
-    _rows3(out, "out")
-    T, NH, HD = q.shape
-    _need(q.shape == out.shape, "attn_prefix: q and out differ in shape")
-    pools = [p for p, n in ((prefix, prefix_len), (kv, max_kv)) if n > 0]
-    _need(bool(pools) or prefix is not None or kv is not None, "attn_prefix: no pages")
-    for p in pools or [prefix or kv]:
-        _need(p is not None and p.c.HD == HD and p.k.dtype == q.dtype == out.dtype, "attn_prefix: rows and pages differ in head size or type")
+    shape, qs = _rows3(q, "q")
+    oshape, os_ = _rows3(out, "out")
+    T, NH, HD = shape
+    _need(shape == oshape and q.dtype is out.dtype, "attn_prefix: q and out differ in shape or type")
+    _need(prefix is not None or kv is not None, "attn_prefix: no pages")
+    i32 = _tn().i32
     B = T if cu_q is None else cu_q.numel() - 1
-    if max_kv > 0:
-        _need(table is not None and table.dim() == 2 and table.shape[0] >= B and str(table.dtype) == "torch.int32"
-              and (table.stride(1) == 1 or table.shape[1] == 1) and table.shape[1] * kv.c.page >= max_kv,
-              "table: need an int32 [B, width] tensor with contiguous rows, wide enough for max_kv")
-        _need(kv_len is not None, "attn_prefix: kv_len is missing")
-        _vector(kv_len, "kv_len", "int32", B)
-    if prefix_len > 0 and prefix_table is not None:
-        _vector(prefix_table, "prefix_table", "int32", -(-prefix_len // prefix.c.page))
-    _vector(cu_q, "cu_q", "int32", B + 1)
-    _vector(lse, "lse", "float32", T * NH)
-    _on_device(q, out, prefix_table, table, kv_len, cu_q, lse, ws, *[p.k for p in pools])
+    _on_device(q, out, prefix_table, table, kv_len, cu_q, lse, ws, None if prefix is None else prefix.k, None if kv is None else kv.k)
     stride = 0
     if max_kv > 0:
-        stride = table.stride(0) if table.shape[0] > 1 else table.shape[1]
-    check(lib().sb_attn_prefix(_p(q), q.stride(0), q.stride(1), _p(out), out.stride(0), out.stride(1), _p(lse), T, NH, _p(cu_q), B,
-                               max_q, prefix.ref if prefix is not None else None, _p(prefix_table), prefix_len,
-                               kv.ref if kv is not None else None, _p(table), stride, _p(kv_len), max_kv, scale, _p(ws),
-                               0 if ws is None else ws.numel() * ws.element_size(), _s(stream)))
+        _need(kv is not None and kv.HD == HD and kv.dtype is q.dtype, "attn_prefix: rows and pages differ in head size or type")
+        _need(table is not None and kv_len is not None, "attn_prefix: table or kv_len is missing")
+        stride, width = _table(table, B)
+        _need(width * kv.page >= max_kv, "attn_prefix: the table is narrower than max_kv positions")
+        _vector(kv_len, "kv_len", i32, B)
+    if prefix_len > 0 or max_kv <= 0:
+        p = prefix if prefix is not None else kv
+        _need(p.HD == HD and p.dtype is q.dtype, "attn_prefix: rows and pages differ in head size or type")
+        _need(prefix is not None or prefix_len <= 0, "attn_prefix: no pages of the prefix")
+        if prefix_table is not None:
+            _vector(prefix_table, "prefix_table", i32, -(-prefix_len // p.page))
+    _vector(cu_q, "cu_q", i32, B + 1)
+    _vector(lse, "lse", _tn().f32, T * NH)
+    check(lib().sb_attn_prefix(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0], os_[1], _p(lse), T, NH, _p(cu_q), B, max_q,
+                               None if prefix is None else prefix.ref, _p(prefix_table), prefix_len, None if kv is None else kv.ref,
+                               _p(table), stride, _p(kv_len), max_kv, scale, _p(ws), 0 if ws is None else ws.nbytes, _s(stream)))
 
 
 def logprobs_ws(logits, top_k=0):
@@ -500,43 +541,50 @@ def logprobs_ws(logits, top_k=0):
 
 
 def _logits(t, name):
-    _need(t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1), f"{name}: need [rows, choices], choices contiguous")
+    """Rows, choices and row stride of [R, V] logits."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] != 1):
+        raise SbError(f"{name}: need [rows, choices], choices contiguous")
+    return shape[0], shape[1], (stride[0] if shape[0] > 1 else shape[1])
 
 
 def logprobs(logits, tokens, ws, logp=None, entropy=None, lse=None, rank=None, top_ids=None, top_logp=None, temperature=1.0, stream=None):
     """Log probability, rank (int32) and entropy of tokens (int32 [R], -1:
     none) under logits [R, V] / temperature, and the best alternatives
     (top_ids int32 / top_logp [R, k], k <= 64) in one pass; see sb_logprobs."""
-    _logits(logits, "logits")
-    R, V = logits.shape
-    k = 0
+    R, V, stride = _logits(logits, "logits")
+    n, k = _tn(), 0
     for t in (top_ids, top_logp):
         if t is not None:
             _need(t.dim() == 2 and t.shape[0] == R and (k == 0 or k == t.shape[1]), "top_ids and top_logp: need [R, k]")
             k = t.shape[1]
-    for t, n, d, m in ((tokens, "tokens", "int32", R), (logp, "logp", "float32", R), (entropy, "entropy", "float32", R),
-                       (lse, "lse", "float32", R), (rank, "rank", "int32", R), (top_ids, "top_ids", "int32", R * k),
-                       (top_logp, "top_logp", "float32", R * k)):
-        _vector(t, n, d, m)
+    _vector(tokens, "tokens", n.i32, R)
+    _vector(logp, "logp", n.f32, R)
+    _vector(entropy, "entropy", n.f32, R)
+    _vector(lse, "lse", n.f32, R)
+    _vector(rank, "rank", n.i32, R)
+    _vector(top_ids, "top_ids", n.i32, R * k)
+    _vector(top_logp, "top_logp", n.f32, R * k)
     _on_device(logits, tokens, ws, logp, entropy, lse, rank, top_ids, top_logp)
-    check(lib().sb_logprobs(_p(logits), logits.stride(0) if R > 1 else V, _type(logits), R, V, temperature, _p(tokens), _p(logp), _p(entropy),
-                            _p(lse), _p(rank), k, _p(top_ids), _p(top_logp), _p(ws),
-                            0 if ws is None else ws.numel() * ws.element_size(), _s(stream)))
+    check(lib().sb_logprobs(logits.data_ptr(), stride, _type(logits), R, V, temperature, _p(tokens), _p(logp), _p(entropy), _p(lse), _p(rank),
+                            k, _p(top_ids), _p(top_logp), _p(ws), 0 if ws is None else ws.nbytes, _s(stream)))
 
 
 def logprobs_grad(logits, tokens, lse, entropy, g_logp, g_entropy, grad, temperature=1.0, stream=None):
     """grad [R, V] = the gradient of logp and entropy (weights g_logp,
     g_entropy [R] or None) with respect to the logits; grad may be logits."""
-    _logits(logits, "logits")
-    _logits(grad, "grad")
-    R, V = logits.shape
-    _need(grad.shape == logits.shape and grad.dtype == logits.dtype, "logprobs_grad: logits and grad differ in shape or type")
-    for t, n, d in ((tokens, "tokens", "int32"), (lse, "lse", "float32"), (entropy, "entropy", "float32"), (g_logp, "g_logp", "float32"),
-                    (g_entropy, "g_entropy", "float32")):
-        _vector(t, n, d, R)
+    R, V, stride = _logits(logits, "logits")
+    gR, gV, gstride = _logits(grad, "grad")
+    _need(R == gR and V == gV and grad.dtype is logits.dtype, "logprobs_grad: logits and grad differ in shape or type")
+    n = _tn()
+    _vector(tokens, "tokens", n.i32, R)
+    _vector(lse, "lse", n.f32, R)
+    _vector(entropy, "entropy", n.f32, R)
+    _vector(g_logp, "g_logp", n.f32, R)
+    _vector(g_entropy, "g_entropy", n.f32, R)
     _on_device(logits, tokens, lse, entropy, g_logp, g_entropy, grad)
-    check(lib().sb_logprobs_grad(_p(logits), logits.stride(0) if R > 1 else V, _type(logits), R, V, temperature, _p(tokens), _p(lse),
-                                 _p(entropy), _p(g_logp), _p(g_entropy), _p(grad), grad.stride(0) if R > 1 else V, _s(stream)))
+    check(lib().sb_logprobs_grad(logits.data_ptr(), stride, _type(logits), R, V, temperature, _p(tokens), _p(lse), _p(entropy), _p(g_logp),
+                                 _p(g_entropy), grad.data_ptr(), gstride, _s(stream)))
 
 
 # ---------------------------------------------------------------- synthetic inputs
