@@ -18,24 +18,27 @@
 // per SM and cycle are close behind, and issue slots too: about eight
 // instructions a value, with maxima, minima and rank compares on packed pairs.
 //
-// The k best in the same pass.  A key is the value's order-preserving bits
-// above the complemented id, so a larger key is a better candidate and equal
-// values go to the lower id (-0 counts as +0); masked choices (-inf) are not
-// listed.  The k-th best of the threads' (or thread groups') maxima so far is
-// a lower bound of the k-th best value: k holders each have a value at least
-// that good.  Only vectors that reach it are looked into, and only values
-// that reach it go to a list in shared memory -- about k per doubling of the
-// values seen, as the bound is renewed with each of the first tiles, later with
-// every fourth.  Where the list overflows (rising or equal logits), the part's k best are taken by k
-// passes instead.
+// The k best without a second pass.  A key is the value's order-preserving
+// bits above the complemented id, so a larger key is a better candidate and
+// equal values go to the lower id (-0 counts as +0); masked choices (-inf) are
+// not listed.  On the way every thread leaves the maximum of each of its cells
+// (a few tiles) in shared memory.  The k-th best of the threads' (or thread
+// groups') maxima bounds the k-th best value from below: k holders each have a
+// value at least that good.  So only cells that reach it -- 1.2 to 1.4 k of
+// them -- are looked into again, a thread a vector, and what reaches it there
+// is ranked by counting.  (Collecting candidates on the way, against a bound
+// renewed tile by tile, cost three times as much: each hit stalls a warp, each
+// renewal the block.)  Where too many reach it (equal or rising logits), the
+// part's k best are taken by k passes instead.
 #include <cfloat>
 #include <cuda_bf16.h>
 
 #include "sb_common.cuh"
 
-#define LP_THREADS 256
+#define LP_THREADS 128
 #define LP_U 4        // vectors of a thread per tile
-#define LP_LIST 1024  // keys
+#define LP_LIST 512   // keys, and cells
+#define LP_CELLS 32    // cells of a thread
 #define LP_KMAX 64
 #define LP_LN2 0.6931471805599453f
 
@@ -56,6 +59,10 @@ struct LpParams {
 SB_DEV float lp_f(float v) { return v; }
 SB_DEV float lp_f(__half v) { return __half2float(v); }
 SB_DEV float lp_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> SB_DEV T lp_to(float v);
+template <> SB_DEV float lp_to<float>(float v) { return v; }
+template <> SB_DEV __half lp_to<__half>(float v) { return __float2half_rn(v); }
+template <> SB_DEV __nv_bfloat16 lp_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 SB_DEV float lp_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -290,8 +297,10 @@ SB_DEV void logprobs_body(const LpParams &P) {
     constexpr int N = Vec::N, TILE = LP_THREADS * LP_U;
     __shared__ LpShared sum_s;
     __shared__ unsigned long long list[TOP ? LP_LIST : 1];
+    __shared__ T cell_s[TOP ? LP_CELLS : 1][LP_THREADS];
     __shared__ __align__(16) float best_s[TOP ? LP_THREADS : 4];
-    __shared__ int n_s;
+    __shared__ unsigned short hit_s[TOP ? LP_LIST : 1];
+    __shared__ int n_s, hits_s;
     __shared__ float thr_s;
     const int tid = threadIdx.x;
     const int r = blockIdx.x / P.S, part = blockIdx.x % P.S;
@@ -299,7 +308,7 @@ SB_DEV void logprobs_body(const LpParams &P) {
     const T *x = static_cast<const T *>(P.x) + r * P.stride;
     const int lead = (int)(((uintptr_t)x & 15) / sizeof(T));  // places of the first vector that are not the row's
     const int nv = (int)(((long long)lead + P.V + N - 1) / N);
-    const int v0 = (int)((long long)nv * part / P.S), v1 = (int)((long long)nv * (part + 1) / P.S);
+    const int v0 = P.S == 1 ? 0 : (int)((long long)nv * part / P.S), v1 = P.S == 1 ? nv : (int)((long long)nv * (part + 1) / P.S);
     const int whole0 = lead ? 1 : 0, whole1 = min((int)(((long long)lead + P.V) / N), v1);  // vectors inside the row
     const int tok = P.tok ? P.tok[r] : -1;
     const bool given = tok >= 0 && tok < P.V, count = P.rank && given;
@@ -311,33 +320,13 @@ SB_DEV void logprobs_body(const LpParams &P) {
 
     LpSum a = {-INFINITY, 0.f, 0.f};
     int above = 0;
-    float best = -INFINITY, thr = -FLT_MAX;
-    // group maxima, one per 2, 4 or 8 lanes: 2 to 4 times k of them leave 1.2 to 1.4 k values above the
-    // k-th, and a tighter bound from more groups costs more to rank than it saves
-    const int per = P.k > 24 ? 2 : P.k > 8 ? 4 : 8, groups = LP_THREADS / per;
-    int tile = 0;
-    if (TOP && tid == 0) n_s = 0;
-
-    // the k-th best group maximum bounds the k-th best value from below
-    auto raise_bound = [&]() {
-        float g = best;
-        for (int o = 1; o < per; o <<= 1) g = fmaxf(g, __shfl_xor_sync(SB_FULL, g, o));
-        if (tid % per == 0) best_s[tid / per] = g;
-        if (tid == 0) thr_s = -FLT_MAX;
-        __syncthreads();
-        if (tid < groups) {
-            g = best_s[tid];
-            int rk = 0;
-            for (int i = 0; i < groups; i += 4) {
-                const float4 o = *reinterpret_cast<const float4 *>(best_s + i);
-                rk += (o.x > g || (o.x == g && i < tid)) + (o.y > g || (o.y == g && i + 1 < tid)) +
-                      (o.z > g || (o.z == g && i + 2 < tid)) + (o.w > g || (o.w == g && i + 3 < tid));
-            }
-            if (rk == P.k - 1) thr_s = g;
-        }
-        __syncthreads();
-        thr = fmaxf(thr, thr_s);
-    };
+    float best = -INFINITY, cell_best = -INFINITY;
+    const int tiles = (v1 - v0 + TILE - 1) / TILE, per_cell = (tiles + LP_CELLS - 1) / LP_CELLS;  // tiles of a cell
+    int tile = 0, cell = 0, cell_end = per_cell;
+    if (TOP && tid == 0) {
+        n_s = hits_s = 0;
+        thr_s = -FLT_MAX;
+    }
 
     for (int b = v0; b < v1; b += TILE, tile++) {
         uint4 raw[LP_U];
@@ -421,21 +410,11 @@ SB_DEV void logprobs_body(const LpParams &P) {
             above += Vec::total(n);
         }
         if constexpr (TOP) {
-            if (tile < 4 || (tile & 3) == 3 || thr == -FLT_MAX) raise_bound();
-            if (mx >= thr) {
-#pragma unroll
-                for (int u = 0; u < LP_U; u++) {
-                    float v[N];
-                    Vec::values(raw[u], v);
-                    unsigned hits = 0;
-#pragma unroll
-                    for (int e = 0; e < N; e++) hits |= (unsigned)(v[e] >= thr) << e;
-                    while (hits) {
-                        const int e = __ffs(hits) - 1, at = atomicAdd(&n_s, 1);
-                        hits &= hits - 1;
-                        if (at < LP_LIST) list[at] = lp_key(lp_at<T>(raw[u], e), (b + u * LP_THREADS + tid) * N - lead + e);
-                    }
-                }
+            cell_best = fmaxf(cell_best, mx);
+            if (tile + 1 == cell_end || b + TILE >= v1) {
+                cell_s[cell++][tid] = lp_to<T>(cell_best);  // exact: a value of the type
+                cell_best = -INFINITY;
+                cell_end += per_cell;
             }
         }
     }
@@ -453,8 +432,51 @@ SB_DEV void logprobs_body(const LpParams &P) {
         else P.part[(long long)r * P.S + part] = make_float4(a.m, a.s, a.t, __int_as_float(above));
     }
     if constexpr (TOP) {
-        int n = n_s;  // (the barriers above stand between the appends and this)
-        if (n > LP_LIST) {  // k passes: the best key below the last one
+        // group maxima, one per 1, 2 or 4 threads: 2 to 4 times k of them leave 1.2 to 1.4 k cells
+        const int per = P.k > 24 ? 1 : P.k > 8 ? 2 : 4, groups = LP_THREADS / per;
+        float g = best;
+        for (int o = 1; o < per; o <<= 1) g = fmaxf(g, __shfl_xor_sync(SB_FULL, g, o));
+        if (tid % per == 0) best_s[tid / per] = g;
+        __syncthreads();
+        if (tid < groups) {
+            g = best_s[tid];
+            int rk = 0;
+            for (int i = 0; i < groups; i += 4) {
+                const float4 o = *reinterpret_cast<const float4 *>(best_s + i);
+                rk += (o.x > g || (o.x == g && i < tid)) + (o.y > g || (o.y == g && i + 1 < tid)) +
+                      (o.z > g || (o.z == g && i + 2 < tid)) + (o.w > g || (o.w == g && i + 3 < tid));
+            }
+            if (rk == P.k - 1 && g > thr_s) thr_s = g;
+        }
+        __syncthreads();
+        const float thr = thr_s;  // at least the lowest finite value
+        if (best >= thr)
+            for (int i = 0; i < cell; i++)
+                if (lp_f(cell_s[i][tid]) >= thr) {
+                    const int at = atomicAdd(&hits_s, 1);
+                    if (at < LP_LIST) hit_s[at] = (unsigned short)(i * LP_THREADS + tid);
+                }
+        __syncthreads();
+        const int hits = hits_s, vecs = per_cell * LP_U;  // vectors of a cell
+        if (hits <= LP_LIST)
+            for (int i = tid; i < hits * vecs; i += LP_THREADS) {
+                const int h = i / vecs, u = i - h * vecs, at = hit_s[h];
+                const int j = v0 + ((at / LP_THREADS) * vecs + u) * LP_THREADS + at % LP_THREADS;
+                if (j >= v1) continue;
+                const uint4 w = lp_load(x, lead, P.V, j);
+                if (Vec::max(w) < thr) continue;
+                float v[N];
+                Vec::values(w, v);
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (v[e] >= thr) {
+                        const int slot = atomicAdd(&n_s, 1);
+                        if (slot < LP_LIST) list[slot] = lp_key(v[e], j * N - lead + e);
+                    }
+            }
+        __syncthreads();
+        int n = n_s;
+        if (hits > LP_LIST || n > LP_LIST) {  // k passes: the best key below the last one
             unsigned long long last = ~0ull;
             for (n = 0; n < P.k; n++) {
                 unsigned long long top = 0ull;
@@ -482,22 +504,6 @@ SB_DEV void logprobs_body(const LpParams &P) {
                 last = top;
             }
             __syncthreads();
-        } else if (n > LP_THREADS / 4) {  // what the final bound leaves
-            raise_bound();
-            unsigned long long mine[LP_LIST / LP_THREADS];
-#pragma unroll
-            for (int q = 0; q < LP_LIST / LP_THREADS; q++) {
-                const int i = tid + q * LP_THREADS;
-                mine[q] = i < n ? list[i] : 0ull;
-            }
-            __syncthreads();
-            if (tid == 0) n_s = 0;
-            __syncthreads();
-#pragma unroll
-            for (int q = 0; q < LP_LIST / LP_THREADS; q++)
-                if (mine[q] && lp_key_value(mine[q]) >= thr) list[atomicAdd(&n_s, 1)] = mine[q];
-            __syncthreads();
-            n = n_s;
         }
         const float l2 = log2f(a.s);
         unsigned long long *out = P.keys + ((long long)r * P.S + part) * P.k;
@@ -513,12 +519,12 @@ SB_DEV void logprobs_body(const LpParams &P) {
 }
 #define LP_KERNEL(name, T, TOP, CTAS) \
     extern "C" __global__ void __launch_bounds__(LP_THREADS, CTAS) name(const __grid_constant__ LpParams P) { logprobs_body<T, TOP>(P); }
-LP_KERNEL(logprobs_f32, float, false, 5)
-LP_KERNEL(logprobs_f16, __half, false, 5)
-LP_KERNEL(logprobs_bf16, __nv_bfloat16, false, 5)
-LP_KERNEL(logprobs_top_f32, float, true, 5)
-LP_KERNEL(logprobs_top_f16, __half, true, 5)
-LP_KERNEL(logprobs_top_bf16, __nv_bfloat16, true, 5)
+LP_KERNEL(logprobs_f32, float, false, 10)
+LP_KERNEL(logprobs_f16, __half, false, 10)
+LP_KERNEL(logprobs_bf16, __nv_bfloat16, false, 10)
+LP_KERNEL(logprobs_top_f32, float, true, 10)
+LP_KERNEL(logprobs_top_f16, __half, true, 10)
+LP_KERNEL(logprobs_top_bf16, __nv_bfloat16, true, 10)
 
 // A CTA a row: the parts' sums, and the k best of their S sorted lists.  The
 // k-th best list head bounds the k-th best key from below, so at most k
@@ -592,11 +598,6 @@ struct LpGradParams {
     const int *tok;
     const float *lse, *entropy, *g_logp, *g_entropy;
 };
-template <typename T> SB_DEV T lp_to(float v);
-template <> SB_DEV float lp_to<float>(float v) { return v; }
-template <> SB_DEV __half lp_to<__half>(float v) { return __float2half_rn(v); }
-template <> SB_DEV __nv_bfloat16 lp_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
 template <typename T>
 SB_DEV void logprobs_grad_body(const LpGradParams &P) {
     using Vec = LpVec<T>;

@@ -166,7 +166,8 @@ int sb_occupancy_of(sb_ctx *c, sb_fn_id f, int block, size_t smem);
 
 /* limits of sb_serve.c's launches */
 #define SB_ATTN_MAX_SPLITS 128     /* key ranges of the prefix, and of a request's own keys */
-#define SB_LOGPROBS_MAX_PARTS 256  /* parts of a row */
+#define SB_LOGPROBS_THREADS 128     /* LP_THREADS in csrc/score_kernels.cu */
+#define SB_LOGPROBS_MAX_PARTS 128   /* parts of a row: one a thread of the join */
 
 #ifdef __cplusplus
 }

@@ -493,11 +493,11 @@ int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, 
     p.keys = p.part + (size_t)R * p.S * 16;
     SB_ARG((int64_t)R * p.S < 0x7fffffffL, "logprobs: too many rows");
     void *args[] = {&p};
-    rc = sb_launch(c, top_k ? BY_TYPE(F_LOGPROBS_TOP_F32, type) : BY_TYPE(F_LOGPROBS_F32, type), (unsigned)(R * p.S), 1, 256, 0,
+    rc = sb_launch(c, top_k ? BY_TYPE(F_LOGPROBS_TOP_F32, type) : BY_TYPE(F_LOGPROBS_F32, type), (unsigned)(R * p.S), 1, SB_LOGPROBS_THREADS, 0,
                    (CUstream)stream, args, 0);
     if (rc || p.S == 1) return rc;
     void *jargs[] = {&p, &type};
-    return sb_launch(c, F_LOGPROBS_JOIN, (unsigned)R, 1, 256, 0, (CUstream)stream, jargs, 1);
+    return sb_launch(c, F_LOGPROBS_JOIN, (unsigned)R, 1, SB_LOGPROBS_THREADS, 0, (CUstream)stream, jargs, 1);
 }
 
 int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
@@ -535,5 +535,5 @@ int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, in
     p.g_entropy = DP(g_entropy);
     SB_ARG((int64_t)R * p.S < 0x7fffffffL, "logprobs_grad: too many rows");
     void *args[] = {&p};
-    return sb_launch(c, BY_TYPE(F_LOGPROBS_GRAD_F32, type), (unsigned)(R * p.S), 1, 256, 0, (CUstream)stream, args, 0);
+    return sb_launch(c, BY_TYPE(F_LOGPROBS_GRAD_F32, type), (unsigned)(R * p.S), 1, SB_LOGPROBS_THREADS, 0, (CUstream)stream, args, 0);
 }
