@@ -1,0 +1,389 @@
+// serve_attn_tc.cuh -- the shared prefix of attn_prefix on the tcgen05 tensor
+// cores (f16 / bf16): many query rows of a key head against a range of keys.
+//
+// Item = (key head, 256 stacked query rows, key range), one CTA of 16 warps:
+//   warps 0-3, 4-7  softmax of row tile A / B (128 rows each, a thread a row)
+//   warps 8-11      loaders: K and V tiles of 128 keys through the page table
+//                   (cp.async, 128-byte swizzle; TMA boxes cannot follow pages
+//                   of any size), two (HD 128) or four (HD 64) stages
+//   warp 12         issues the tcgen05.mma of both products
+// S = Q K^T (128 x 128, FP32) and P V run on the tensor pipe with S, P and O
+// in tensor memory: the softmax threads read S, write P as 16-bit pairs over
+// it (the A operand of the second product), and O stays there until the end.
+// While one tile's softmax runs, the pipe works on the other tile: PV(t) and
+// S(t + 1) of a tile are issued together as soon as its weights are there.
+//
+// The running maximum is lazy: O is rescaled only when a row's maximum has
+// grown by more than 2^8 since the last time (weights up to 256 are as exact
+// as weights up to 1 in floating point), which leaves a few rescales a row.
+//
+// Bound: 16 exponentials per SM and cycle (1024 cycles for a tile of 128 x
+// 128), against 512 (HD 64) or 1024 (HD 128) cycles of the tensor pipe.
+//
+// Every wait is bounded; after a timeout tc_err is set, the roles stop, what
+// was issued drains, and the tensor memory is freed.
+#pragma once
+#include "serve_attn.cuh"
+
+__device__ int tc_err;  // nonzero after a wait timed out (sb_tc_error reads and clears it)
+
+namespace atc {
+constexpr int THREADS = 512, BM = 128, KT = 128;
+constexpr unsigned long long WAIT_NS = 2000000000ull;
+template <int HDP> struct Cfg {
+    static constexpr int ST = HDP == 128 ? 2 : 4, SUB = HDP / 64, TILE = KT * HDP * 2;
+    static constexpr int SMEM = 1024 + (2 * ST + 2) * TILE;
+};
+SB_DEV void mbar_init(uint64_t *mb, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(ap_smem(mb)), "r"(count) : "memory");
+}
+SB_DEV void mbar_arrive(uint64_t *mb) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ap_smem(mb)) : "memory");
+}
+SB_DEV unsigned long long now() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// false after WAIT_NS, or (abortable) once any wait has given up
+SB_DEV bool mbar_wait(uint64_t *mb, unsigned ph, bool abortable = true) {
+    unsigned long long t0 = 0;
+    for (long spin = 0; spin < (1l << 26); spin++) {
+        unsigned done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(ap_smem(mb)), "r"(ph)
+            : "memory");
+        if (done) return true;
+        if ((spin & 1023) == 1023) {
+            if (abortable && *(volatile int *)&tc_err) return false;
+            const unsigned long long t = now();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > WAIT_NS) break;
+        }
+    }
+    atomicExch(&tc_err, 1);
+    return false;
+}
+// the same for a converged warp, one answer for all lanes
+SB_DEV bool warp_wait(uint64_t *mb, unsigned ph, bool abortable = true) { return __all_sync(SB_FULL, mbar_wait(mb, ph, abortable)); }
+SB_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+SB_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+SB_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 128-byte swizzled operand: rows (K-major: query rows or keys; MN-major: keys)
+// of 128 bytes, 8-row atoms 1024 bytes apart, 64-value column blocks 16 KB apart
+SB_DEV uint64_t desc(unsigned addr) {
+    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// f32 accumulator, M = 128; B K-major (keys as rows) or MN-major (values along N)
+template <typename T> SB_DEV uint32_t idesc(int n, bool b_mn) {
+    constexpr uint32_t fmt = __is_same(T, __half) ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+}
+SB_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "r"(id), "r"(acc)
+        : "memory");
+}
+SB_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
+        "r"(id), "r"(acc)
+        : "memory");
+}
+SB_DEV void commit(uint64_t *mb) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(ap_smem(mb)) : "memory");
+}
+#define ATC_R32(r) \
+    "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), \
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), \
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), \
+        "=r"(r[31])
+// 32 columns of this warp's 32 lanes; wait_ld before the registers are read
+SB_DEV void ld32(uint32_t addr, unsigned (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+        "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : ATC_R32(r)
+        : "r"(addr));
+}
+#define ATC_W32(r) \
+    "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), \
+        "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), \
+        "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+// waits for every load of this thread; r's values are used behind it only
+SB_DEV void wait_ld(unsigned (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : ATC_W32(r)::"memory");
+    asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
+}
+SB_DEV void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+SB_DEV void st16(uint32_t addr, const unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+}  // namespace atc
+
+template <typename T, int HDP>
+SB_DEV void attn_tc_body(const AttnParams &P) {
+    using namespace atc;
+    using C = Cfg<HDP>;
+    constexpr int ST = C::ST, TILE = C::TILE;
+    extern __shared__ unsigned char tc_sm_raw[];
+    __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], pfull[2], ofull;
+    __shared__ uint32_t tmem_s;
+    __shared__ __align__(16) uint32_t valid_s[2 * ST][4];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_launch_dependents();
+    AttnItem it;
+    if (!ap_prefix_item(P, blockIdx.x, 2 * BM, it)) return;
+    const unsigned sm = (ap_smem(tc_sm_raw) + 1023u) & ~1023u;
+    const unsigned vst = sm, kst = sm + ST * TILE, qst = sm + 2 * ST * TILE;  // stages of V and K, both query tiles
+    const int nt = (it.k1 - it.k0 + KT - 1) / KT;
+    const int nx = it.f0 + BM < it.F ? 2 : 1;  // row tiles with rows
+
+    if (tid == 0) {
+        for (int s = 0; s < ST; s++) {
+            mbar_init(&kfull[s], 4);
+            mbar_init(&vfull[s], 4);
+            mbar_init(&kempty[s], 1);
+            mbar_init(&vempty[s], 1);
+        }
+        for (int x = 0; x < 2; x++) {
+            mbar_init(&sfull[x], 1);
+            mbar_init(&pfull[x], 4);
+        }
+        mbar_init(&ofull, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ap_smem(&tmem_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp < 8) {  // a thread its query row, negated for a negative scale; rows behind the last as zeros
+        const int f = it.f0 + tid;
+        const unsigned flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
+        const unsigned row = qst + (tid >> 7) * TILE + (tid & 127) * 128;
+#pragma unroll
+        for (int c = 0; c < HDP / 8; c++) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (f < it.F && c * 8 < P.HD) v = *reinterpret_cast<const uint4 *>(qp + c * 8);
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + (c >> 3) * 16384 + (((c & 7) ^ (tid & 7)) << 4)), "r"(v.x ^ flip),
+                         "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
+                         : "memory");
+        }
+        fence_async();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_s;
+    // 512 threads x 128 registers = 256 x 144 + 256 x 112: no role spills
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+
+    if (warp >= 8 && warp < 12) {
+        // ---- loaders: warp w the keys 32 w .. 32 w + 31 of a tile
+        const int w = warp - 8;
+        const T *kb = static_cast<const T *>(it.pg.k) + it.kvh * it.pg.head_stride;
+        const T *vb = static_cast<const T *>(it.pg.v) + it.kvh * it.pg.head_stride;
+        constexpr int CH = HDP / 8, RPI = 32 / CH;  // chunks of a row, rows an instruction
+        const int c = lane % CH, rsub = lane / CH;
+        const bool cok = c * 8 < P.HD;
+        auto rows = [&](unsigned stage, const T *base, long long off) {
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int r = i * RPI + rsub;
+                const long long o = __shfl_sync(SB_FULL, off, r);
+                const bool ok = o >= 0 && cok;
+                ap_cp16(stage + (c >> 3) * 16384 + (w * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), ok ? base + o + c * 8 : base, ok);
+            }
+            ap_commit();
+        };
+        long long off = ap_offset(it, it.k0 + w * 32 + lane);
+        bool ok = true;
+        uint64_t *landed = nullptr;  // full barrier of the group issued last
+        auto landed_now = [&]() {
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(landed);
+        };
+        for (int t = 0; t < nt && ok; t++) {
+            const int s = t % ST;
+            const unsigned ph = (unsigned)((t / ST) - 1) & 1u;
+            if (t >= ST) ok = warp_wait(&kempty[s], ph);
+            if (!ok) break;
+            const unsigned valid = __ballot_sync(SB_FULL, off >= 0);
+            if (lane == 0) valid_s[t % (2 * ST)][w] = valid;
+            rows(kst + s * TILE, kb, off);
+            if (landed) {
+                ap_wait<1>();
+                landed_now();
+            }
+            landed = &kfull[s];
+            if (t >= ST) ok = warp_wait(&vempty[s], ph);
+            if (!ok) break;
+            rows(vst + s * TILE, vb, off);
+            off = ap_offset(it, it.k0 + (t + 1) * KT + w * 32 + lane);
+            ap_wait<1>();
+            landed_now();
+            landed = &vfull[s];
+        }
+        ap_wait<0>();
+        if (ok && landed) landed_now();
+    } else if (warp == 12) {
+        if (lane == 0) {
+            // ---- issuer
+            const uint32_t id_s = idesc<T>(KT, false), id_o = idesc<T>(HDP, true);
+            auto scores = [&](int x, int t) {
+#pragma unroll
+                for (int k = 0; k < HDP / 16; k++) {
+                    const uint64_t a = desc(qst + x * TILE + (k >> 2) * 16384) + 2 * (k & 3);
+                    const uint64_t b = desc(kst + (t % ST) * TILE + (k >> 2) * 16384) + 2 * (k & 3);
+                    mma_ss(tmem + x * 128, a, b, id_s, k > 0);
+                }
+                commit(&sfull[x]);
+            };
+            bool ok = nt > 0 && mbar_wait(&kfull[0], 0);
+            if (ok) {
+                fence_after();
+                for (int x = 0; x < nx; x++) scores(x, 0);
+                commit(&kempty[0]);
+            }
+            for (int t = 0; t < nt && ok; t++) {
+                ok = mbar_wait(&vfull[t % ST], (t / ST) & 1);
+                if (ok && t + 1 < nt) ok = mbar_wait(&kfull[(t + 1) % ST], ((t + 1) / ST) & 1);
+                for (int x = 0; x < nx && ok; x++) {
+                    ok = mbar_wait(&pfull[x], t & 1);
+                    if (!ok) break;
+                    fence_after();
+#pragma unroll
+                    for (int k = 0; k < KT / 16; k++)
+                        mma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, desc(vst + (t % ST) * TILE + k * 2048), id_o, t > 0 || k > 0);
+                    if (t + 1 < nt) scores(x, t + 1);
+                }
+                if (!ok) break;
+                commit(&vempty[t % ST]);
+                if (t + 1 < nt) commit(&kempty[(t + 1) % ST]);
+            }
+            commit(&ofull);  // when everything issued above has completed, also after giving up
+        }
+        __syncwarp();
+    } else if (warp < 8 && (warp >> 2) < nx) {
+        // ---- softmax and epilogue: a thread a row
+        const int x = warp >> 2, f = it.f0 + tid;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
+        const float sc = fabsf(P.scale_log2);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int t = 0; t < nt && ok; t++) {
+            ok = warp_wait(&sfull[x], t & 1);
+            if (!ok) break;
+            fence_after();
+            const uint4 valid = *reinterpret_cast<const uint4 *>(valid_s[t % (2 * ST)]);
+            const bool whole = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu;
+            // two column blocks in registers: one is read while the other is worked on
+            unsigned r[2][32];
+            float mx = -INFINITY;
+            ld32(s_at, r[0]);
+            wait_ld(r[0]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (c < 3) ld32(s_at + (c + 1) * 32, r[(c + 1) & 1]);
+                const unsigned bits = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (!(bits >> i & 1)) r[c & 1][i] = 0xff800000u;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(r[c & 1][i]));
+                if (c < 3) wait_ld(r[(c + 1) & 1]);
+            }
+            mx *= sc;
+            if (t == 0) {
+                m = mx;
+            } else if (__any_sync(SB_FULL, mx > m + 8.f)) {  // S(t) is complete, so PV(t - 1) is
+                const float to = fmaxf(m, mx), a = m == to ? 1.f : ap_exp2(m - to);
+                m = to;
+                l *= a;
+#pragma unroll
+                for (int c = 0; c < HDP / 32; c++) {
+                    ld32(o_at + c * 32, r[0]);
+                    wait_ld(r[0]);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        unsigned w[16];
+#pragma unroll
+                        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(r[0][16 * h + i]) * a);
+                        st16(o_at + c * 32 + 16 * h, w);
+                    }
+                }
+            }
+            const float b = m == -INFINITY ? 0.f : m;
+            const unsigned long long sc2 = f2_pack(sc, sc), b2 = f2_pack(-b, -b), one2 = f2_pack(1.f, 1.f);
+            unsigned long long l2 = 0ull;
+            ld32(s_at, r[0]);
+            wait_ld(r[0]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                if (c < 3) ld32(s_at + (c + 1) * 32, r[(c + 1) & 1]);
+                const unsigned bits = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (!(bits >> i & 1)) r[c & 1][i] = 0xff800000u;
+                }
+                unsigned w[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float p0, p1;
+                    f2_unpack(ffma2(f2_pack(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), sc2, b2), p0, p1);
+                    p0 = ap_exp2(p0);
+                    p1 = ap_exp2(p1);
+                    l2 = ffma2(one2, f2_pack(p0, p1), l2);
+                    w[i] = ap_pack<T>(p0, p1);
+                }
+                if (c < 3) wait_ld(r[(c + 1) & 1]);  // the block after this one is read before P goes over it
+                st16(s_at + c * 16, w);
+            }
+            l += f2_sum(l2);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[x]);
+        }
+        ok = __all_sync(SB_FULL, mbar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
+        fence_after();
+        if (f < it.F && ok) ap_row_stats(P, it, f, m, l);
+#pragma unroll
+        for (int c = 0; c < HDP / 32; c++) {
+            unsigned r[32];
+            ld32(o_at + c * 32, r);
+            wait_ld(r);
+            if (f < it.F && ok) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2)
+                    ap_row_out<T>(P, it, f, c * 32 + i, __uint_as_float(r[i]), __uint_as_float(r[i + 1]), l);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        fence_after();
+        mbar_wait(&ofull, 0, false);
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+#define ATC_KERNEL(name, T, HDP) \
+    extern "C" __global__ void __launch_bounds__(atc::THREADS, 1) name(const __grid_constant__ AttnParams P, int own) { attn_tc_body<T, HDP>(P); }
+ATC_KERNEL(attn_tc_f16_64, __half, 64)
+ATC_KERNEL(attn_tc_f16_128, __half, 128)
+ATC_KERNEL(attn_tc_bf16_64, __nv_bfloat16, 64)
+ATC_KERNEL(attn_tc_bf16_128, __nv_bfloat16, 128)

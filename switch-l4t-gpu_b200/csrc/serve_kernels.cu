@@ -6,3 +6,4 @@
 #include "serve_plan.cuh"
 #include "serve_rotary.cuh"
 #include "serve_attn.cuh"
+#include "serve_attn_tc.cuh"

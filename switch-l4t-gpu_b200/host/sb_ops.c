@@ -529,12 +529,20 @@ int sb_tc_error(int *err) {
     SB_ARG(err, "null pointer");
     sb_ctx *c = sb_ctx_get();
     if (!c) return SB_ERR_STATE;
-    CUdeviceptr p;
-    size_t bytes;
     SB_CK(cuCtxSynchronize());
-    SB_CK(cuModuleGetGlobal(&p, &bytes, c->mod[M_TC], "tc_err"));
-    SB_CK(cuMemcpyDtoH(err, p, 4));
-    if (*err) SB_CK(cuMemsetD32(p, 0, 1));
+    *err = 0;
+    const int mods[] = {M_TC, M_SERVE};
+    for (int i = 0; i < 2; i++) {
+        CUdeviceptr p;
+        size_t bytes;
+        int e = 0;
+        SB_CK(cuModuleGetGlobal(&p, &bytes, c->mod[mods[i]], "tc_err"));
+        SB_CK(cuMemcpyDtoH(&e, p, 4));
+        if (e) {
+            *err = e;
+            SB_CK(cuMemsetD32(p, 0, 1));
+        }
+    }
     return 0;
 }
 

@@ -131,6 +131,10 @@ static const struct {
     [F_ATTN_F32_128_R4] = {M_SERVE, "attn_f32_128_r4"},
     [F_ATTN_F32_128_R8] = {M_SERVE, "attn_f32_128_r8"},
     [F_ATTN_F32_128_R16] = {M_SERVE, "attn_f32_128_r16"},
+    [F_ATTN_TC_F16_64] = {M_SERVE, "attn_tc_f16_64"},
+    [F_ATTN_TC_F16_128] = {M_SERVE, "attn_tc_f16_128"},
+    [F_ATTN_TC_BF16_64] = {M_SERVE, "attn_tc_bf16_64"},
+    [F_ATTN_TC_BF16_128] = {M_SERVE, "attn_tc_bf16_128"},
     [F_ATTN_JOIN] = {M_SERVE, "attn_join"},
     [F_LOGPROBS_F32] = {M_SCORE, "logprobs_f32"},
     [F_LOGPROBS_F16] = {M_SCORE, "logprobs_f16"},

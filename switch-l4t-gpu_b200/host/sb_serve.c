@@ -224,43 +224,61 @@ struct attn_params {
     int chunk1, S1, chunk2, S2, tiles;
     float scale_log2;
 };
-/* one of the two launches: kernel, row tile, row tiles per unit, key ranges */
+/* one of the two launches: kernel, row tiles, key ranges, items */
 struct attn_part {
     sb_fn_id f;
-    unsigned smem;
-    int tiles, S, chunk;
+    unsigned smem, threads;
+    int rows, step, tiles, S, chunk;
     long grid;
 };
 
-/* The kernel for tiles of `rows` rows.  16-bit types: 16-row tiles (the four
- * warps split the keys) while one holds all rows, else 64-row tiles.  FP32:
- * the smallest of 1, 2, 4, 8, 16 rows that holds them (unused rows cost
- * FMAs). */
-static int attn_kernel(int type, int HD, long rows, struct attn_part *a) {
-    const int wide = HD > 64;
+/* The kernel for `rows` query rows of a key head.  FP32: row tiles of 1, 2,
+ * 4, 8 or 16, the smallest that holds them (unused rows cost FMAs).  16-bit
+ * types: 16-row tiles (the four warps split the keys) while one holds all
+ * rows, 64-row tiles up to SB_ATTN_TC_ROWS, and for a prefix behind more rows
+ * the tcgen05 kernel's 256. */
+static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_part *a) {
+    const int wide = HD > 64, second = type == SB_BF16;
+    a->threads = 128;
     if (type == SB_F32) {
         int i = 0;
         while (i < 4 && (1 << i) < rows) i++;
         a->f = (sb_fn_id)(F_ATTN_F32_64_R1 + 5 * wide + i);
         a->smem = (i == 4 ? 2 : 3) * 32768;
-        return 1 << i;
+        a->rows = 1 << i;
+        a->step = wide ? 32 : 64;
+    } else if (prefix && rows >= SB_ATTN_TC_ROWS) {
+        a->f = (sb_fn_id)(F_ATTN_TC_F16_64 + 2 * second + wide);
+        a->smem = 1024 + (wide ? 6 * 32768 : 10 * 16384);
+        a->threads = 512;
+        a->rows = 256;
+        a->step = 128;
+    } else {
+        const int big = rows > 16;
+        a->f = (sb_fn_id)((second ? F_ATTN_BF16_64_R16 : F_ATTN_F16_64_R16) + 2 * wide + big);
+        a->smem = 3 * 2 * 64 * (wide ? 128 : 64) * 2;
+        a->rows = big ? 64 : 16;
+        a->step = 64;
     }
-    const int big = rows > 16;
-    a->f = (sb_fn_id)((type == SB_F16 ? F_ATTN_F16_64_R16 : F_ATTN_BF16_64_R16) + 2 * wide + big);
-    a->smem = 3 * 2 * 64 * (wide ? 128 : 64) * 2;
-    return big ? 64 : 16;
+    a->tiles = (int)CEIL_DIV(rows, a->rows);
 }
-/* Key ranges of `keys` keys for `units` independent (head, row tile) pairs:
- * one wave of items where they fit, about four where they do not (the tail
- * of the last wave shrinks, the parts to join grow). */
-static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, int step) {
-    const long cap = (long)c->sms * sb_occupancy_of(c, a->f, 128, a->smem);
-    long S = units * 2 <= cap ? cap / units : CEIL_DIV(4 * cap, units);
-    const long most = units * 2 <= cap ? CEIL_DIV(keys, step) : CEIL_DIV(keys, 8 * step);
-    if (S > most) S = most;
-    if (S > SB_ATTN_MAX_SPLITS) S = SB_ATTN_MAX_SPLITS;
-    if (S < 1) S = 1;
-    a->chunk = (int)(CEIL_DIV(CEIL_DIV((long)keys, S), step) * step);
+/* Key ranges of `keys` keys for `units` independent (head, row tile) pairs.
+ * An item of n tiles of keys costs about n + SB_ATTN_ITEM tile times (its
+ * queries, its part to write and join), and the launch as many rounds of
+ * items as the SMs need: the count with the least of that is taken. */
+static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units) {
+    const long cap = (long)c->sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
+    long best = 0, best_cost = 0;
+    for (long S = 1; S <= SB_ATTN_MAX_SPLITS && S <= tiles; S++) {
+        const long n = CEIL_DIV(tiles, S), items = units * CEIL_DIV(tiles, n);
+        const long cost = CEIL_DIV(items, cap) * (n + SB_ATTN_ITEM) + CEIL_DIV(tiles, n) / 8;
+        if (!best || cost < best_cost) {
+            best = n;
+            best_cost = cost;
+        }
+        if (items > 16 * cap) break;
+    }
+    a->chunk = (int)(best * a->step);
     a->S = (int)CEIL_DIV((long)keys, a->chunk);
     a->grid = units * a->S;
 }
@@ -270,14 +288,12 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
     memset(pre, 0, sizeof *pre);
     memset(own, 0, sizeof *own);
     if (P > 0) {
-        const int mt = attn_kernel(type, HD, T * G, pre);
-        pre->tiles = (int)CEIL_DIV(T * G, mt);
-        attn_split(c, pre, P, (long)pre->tiles * NKV, type == SB_F32 && HD > 64 ? 32 : 64);
+        attn_kernel(type, HD, T * G, 1, pre);
+        attn_split(c, pre, P, (long)pre->tiles * NKV);
     }
     if (max_kv > 0) {
-        const int mt = attn_kernel(type, HD, max_q * G, own);
-        own->tiles = (int)CEIL_DIV(max_q * G, mt);
-        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, type == SB_F32 && HD > 64 ? 32 : 64);
+        attn_kernel(type, HD, max_q * G, 0, own);
+        attn_split(c, own, max_kv, (long)own->tiles * NKV * B);
     }
     SB_ARG(pre->grid < 0x7fffffffL && own->grid < 0x7fffffffL, "attn_prefix: too many rows for one launch");
     return 0;
@@ -396,13 +412,13 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     if (pre.S) {
         p.tiles = pre.tiles;
         void *args[] = {&p, &zero};
-        rc = sb_launch(c, pre.f, (unsigned)pre.grid, 1, 128, pre.smem, (CUstream)stream, args, 0);
+        rc = sb_launch(c, pre.f, (unsigned)pre.grid, 1, pre.threads, pre.smem, (CUstream)stream, args, 0);
         if (rc) return rc;
     }
     if (own.S) { /* beside the prefix launch's last items */
         p.tiles = own.tiles;
         void *args[] = {&p, &one};
-        rc = sb_launch(c, own.f, (unsigned)own.grid, 1, 128, own.smem, (CUstream)stream, args, pre.S > 0);
+        rc = sb_launch(c, own.f, (unsigned)own.grid, 1, own.threads, own.smem, (CUstream)stream, args, pre.S > 0);
         if (rc) return rc;
     }
     if (pre.S + own.S == 1) return 0;

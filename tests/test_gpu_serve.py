@@ -362,6 +362,37 @@ def test_attn_prefix_large_batch(cuda_dev, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,NH,NKV,HD,P,page", [
+    (128, 1, 1, 64, 1, 16), (129, 2, 1, 128, 127, 7), (64, 8, 2, 80, 128, 24), (257, 1, 1, 128, 129, 1), (33, 16, 2, 64, 1300, 64),
+    (40, 14, 2, 40, 700, 700), (20, 32, 2, 128, 5000, 128)])
+def test_attn_prefix_many_rows_a_key_head(cuda_dev, kind, B, NH, NKV, HD, P, page):
+    """128 query rows of a key head and more, one row tile full, over, or
+    partly filled; one key, a tile less one, a tile, one more."""
+    lens = [(i * 5) % 9 for i in range(B)]
+    b = Batch(kind, NH, NKV, HD, P, lens, page=page, seed=B + P)
+    want = b.want()
+    b.check(want=want)
+    b.scale = -b.scale
+    b.check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_growing_scores(cuda_dev, kind):
+    """Keys whose scores rise along the prefix: the maximum that a row's parts
+    are held against moves again and again, and a first part of low scores is
+    scaled down to nothing."""
+    b = Batch(kind, 16, 1, 64, 2000, [3] * 10, seed=21)
+    b.q = b.q.abs()
+    b.k[b.places[-1]] = (torch.linspace(-2, 2, 2000, device="cuda")[:, None, None] + 0.1 * b.k[b.places[-1]].float()).to(b.t)
+    out, lse = b.run()
+    wo, wl, size = b.want()
+    # scores up to 64 x 0.8 x 2 / 8 = 13 either way, on |q k| sums of 100: 2^-24 x 70 terms x 100 / 8 = 5e-5, twice (key, query)
+    u = half_step(b.t) if b.t != torch.float32 else 0.0
+    assert bool(((out.double() - wo).abs() <= u * (size + wo.abs()) + 2e-4 * size + 2.0 ** -24).all())
+    assert bool(((lse.double() - wl).abs() <= 2e-4).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attn_prefix_peaked_scores(cuda_dev, kind):
     """Scores of size 60: the running maximum moves far from tile to tile.
     Their FP32 rounding grows with them, so only values of the formula count
@@ -381,7 +412,11 @@ def test_attn_prefix_peaked_scores(cuda_dev, kind):
 def test_attn_prefix_missing_pages(cuda_dev, kind):
     """A page number outside the pool: its positions are skipped, as if they
     were not there; a request whose pages are all missing sees the prefix."""
-    b = Batch(kind, 6, 2, 64, 100, [70, 40, 33], page=16, seed=5)
+    _missing_pages(Batch(kind, 6, 2, 64, 100, [70, 40, 33], page=16, seed=5))
+    _missing_pages(Batch(kind, 100, 2, 64, 100, [70, 40, 33], page=16, seed=6))  # 150 rows a key head
+
+
+def _missing_pages(b):
     missing = [(0, 1), (1, 0), (1, 1), (1, 2), (2, 2)]
     for r, j in missing:
         keep = b.places[r][0] != int(b.table[r, j])
