@@ -3,7 +3,7 @@
 //
 // Item = (key head, 256 stacked query rows, key range), one CTA of 16 warps:
 //   warps 0-3, 4-7  softmax of row tile A / B (128 rows each, a thread a row)
-//   warps 8-11      loaders: K and V tiles of 128 keys through the page table
+//   warps 8-9, 10-11  loaders of K and V: tiles of 128 keys through the page table
 //                   (cp.async, 128-byte swizzle; TMA boxes cannot follow pages
 //                   of any size), two (HD 128) or four (HD 64) stages
 //   warp 12         issues the tcgen05.mma of both products
@@ -118,6 +118,15 @@ SB_DEV void wait_ld(unsigned (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : ATC_W32(r)::"memory");
     asm volatile("" : "+r"(r[30]), "+r"(r[31])::"memory");
 }
+SB_DEV void ld16(uint32_t addr, unsigned (&r)[16]) {  // and waits
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+}
 SB_DEV void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 SB_DEV void st16(uint32_t addr, const unsigned (&r)[16]) {
     asm volatile(
@@ -127,6 +136,9 @@ SB_DEV void st16(uint32_t addr, const unsigned (&r)[16]) {
         : "memory");
 }
 }  // namespace atc
+
+#define ATC_MORE asm volatile("setmaxnreg.inc.sync.aligned.u32 200;")
+#define ATC_FEWER asm volatile("setmaxnreg.dec.sync.aligned.u32 56;")
 
 template <typename T, int HDP>
 SB_DEV void attn_tc_body(const AttnParams &P) {
@@ -148,8 +160,8 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
 
     if (tid == 0) {
         for (int s = 0; s < ST; s++) {
-            mbar_init(&kfull[s], 4);
-            mbar_init(&vfull[s], 4);
+            mbar_init(&kfull[s], 2);
+            mbar_init(&vfull[s], 2);
             mbar_init(&kempty[s], 1);
             mbar_init(&vempty[s], 1);
         }
@@ -183,69 +195,62 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_s;
-    // 512 threads x 128 registers = 256 x 144 + 256 x 112: no role spills
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
-
+    // 512 threads x 128 registers = 256 x 200 + 256 x 56 (inside each role: the compiler goes by it)
     if (warp >= 8 && warp < 12) {
-        // ---- loaders: warp w the keys 32 w .. 32 w + 31 of a tile
-        const int w = warp - 8;
-        const T *kb = static_cast<const T *>(it.pg.k) + it.kvh * it.pg.head_stride;
-        const T *vb = static_cast<const T *>(it.pg.v) + it.kvh * it.pg.head_stride;
+        ATC_FEWER;
+        // ---- loaders: warps 8, 9 the keys, warps 10, 11 the values; each 64 positions of a tile.  A tile is
+        // waited for right after its copies are issued: its stage came free a whole tile time before it is needed
+        const bool is_k = warp < 10;
+        const int p0 = (warp & 1) * 64;
+        const T *base = static_cast<const T *>(is_k ? it.pg.k : it.pg.v) + it.kvh * it.pg.head_stride;
+        uint64_t *full = is_k ? kfull : vfull, *empty = is_k ? kempty : vempty;
         constexpr int CH = HDP / 8, RPI = 32 / CH;  // chunks of a row, rows an instruction
         const int c = lane % CH, rsub = lane / CH;
         const bool cok = c * 8 < P.HD;
-        auto rows = [&](unsigned stage, const T *base, long long off) {
+        const T *col = base + c * 8;
+        long long off[2];
 #pragma unroll
-            for (int i = 0; i < CH; i++) {
-                const int r = i * RPI + rsub;
-                const long long o = __shfl_sync(SB_FULL, off, r);
-                const bool ok = o >= 0 && cok;
-                ap_cp16(stage + (c >> 3) * 16384 + (w * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), ok ? base + o + c * 8 : base, ok);
+        for (int h = 0; h < 2; h++) off[h] = ap_offset(it, it.k0 + p0 + h * 32 + lane);
+        bool ok = true;
+        for (int t = 0; t < nt; t++) {
+            const int s = t % ST;
+            if (t >= ST) ok = warp_wait(&empty[s], (unsigned)((t / ST) - 1) & 1u);
+            if (!ok) break;
+            const unsigned stage = (is_k ? kst : vst) + s * TILE + (c >> 3) * 16384;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (is_k) {
+                    const unsigned valid = __ballot_sync(SB_FULL, off[h] >= 0);
+                    if (lane == 0) valid_s[t % (2 * ST)][(warp & 1) * 2 + h] = valid;
+                }
+#pragma unroll 4
+                for (int i = 0; i < CH; i++) {
+                    const int r = i * RPI + rsub;
+                    const long long o = __shfl_sync(SB_FULL, off[h], r);
+                    const bool there = o >= 0 && cok;
+                    ap_cp16(stage + (p0 + h * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), there ? col + o : base, there);
+                }
             }
             ap_commit();
-        };
-        long long off = ap_offset(it, it.k0 + w * 32 + lane);
-        bool ok = true;
-        uint64_t *landed = nullptr;  // full barrier of the group issued last
-        auto landed_now = [&]() {
+#pragma unroll
+            for (int h = 0; h < 2; h++) off[h] = ap_offset(it, it.k0 + (t + 1) * KT + p0 + h * 32 + lane);
+            ap_wait<0>();
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(landed);
-        };
-        for (int t = 0; t < nt && ok; t++) {
-            const int s = t % ST;
-            const unsigned ph = (unsigned)((t / ST) - 1) & 1u;
-            if (t >= ST) ok = warp_wait(&kempty[s], ph);
-            if (!ok) break;
-            const unsigned valid = __ballot_sync(SB_FULL, off >= 0);
-            if (lane == 0) valid_s[t % (2 * ST)][w] = valid;
-            rows(kst + s * TILE, kb, off);
-            if (landed) {
-                ap_wait<1>();
-                landed_now();
-            }
-            landed = &kfull[s];
-            if (t >= ST) ok = warp_wait(&vempty[s], ph);
-            if (!ok) break;
-            rows(vst + s * TILE, vb, off);
-            off = ap_offset(it, it.k0 + (t + 1) * KT + w * 32 + lane);
-            ap_wait<1>();
-            landed_now();
-            landed = &vfull[s];
+            if (lane == 0) mbar_arrive(&full[s]);
         }
         ap_wait<0>();
-        if (ok && landed) landed_now();
-    } else if (warp == 12) {
-        if (lane == 0) {
+    } else if (warp >= 12) {
+        ATC_FEWER;
+        if (tid == 12 * 32) {
             // ---- issuer
             const uint32_t id_s = idesc<T>(KT, false), id_o = idesc<T>(HDP, true);
-            auto scores = [&](int x, int t) {
+            const uint64_t qd = desc(qst), kd = desc(kst), vd = desc(vst);
+            auto scores = [&](int x, int s) {
 #pragma unroll
                 for (int k = 0; k < HDP / 16; k++) {
-                    const uint64_t a = desc(qst + x * TILE + (k >> 2) * 16384) + 2 * (k & 3);
-                    const uint64_t b = desc(kst + (t % ST) * TILE + (k >> 2) * 16384) + 2 * (k & 3);
-                    mma_ss(tmem + x * 128, a, b, id_s, k > 0);
+                    const uint32_t in = (k >> 2) * 1024 + 2 * (k & 3);
+                    mma_ss(tmem + x * 128, qd + (x * (TILE >> 4) + in), kd + (s * (TILE >> 4) + in), id_s, k > 0);
                 }
                 commit(&sfull[x]);
             };
@@ -255,26 +260,37 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
                 for (int x = 0; x < nx; x++) scores(x, 0);
                 commit(&kempty[0]);
             }
+            int s = 0, s1 = ST > 1 ? 1 : 0;  // stages of t and t + 1
+            unsigned ph = 0, ph1 = 0;
             for (int t = 0; t < nt && ok; t++) {
-                ok = mbar_wait(&vfull[t % ST], (t / ST) & 1);
-                if (ok && t + 1 < nt) ok = mbar_wait(&kfull[(t + 1) % ST], ((t + 1) / ST) & 1);
+                ok = mbar_wait(&vfull[s], ph);
+                if (ok && t + 1 < nt) ok = mbar_wait(&kfull[s1], ph1);
+#pragma unroll 1
                 for (int x = 0; x < nx && ok; x++) {
                     ok = mbar_wait(&pfull[x], t & 1);
                     if (!ok) break;
                     fence_after();
+                    const uint64_t vs = vd + s * (TILE >> 4);
 #pragma unroll
                     for (int k = 0; k < KT / 16; k++)
-                        mma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, desc(vst + (t % ST) * TILE + k * 2048), id_o, t > 0 || k > 0);
-                    if (t + 1 < nt) scores(x, t + 1);
+                        mma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, vs + k * 128, id_o, t > 0 || k > 0);
+                    if (t + 1 < nt) scores(x, s1);
                 }
                 if (!ok) break;
-                commit(&vempty[t % ST]);
-                if (t + 1 < nt) commit(&kempty[(t + 1) % ST]);
+                commit(&vempty[s]);
+                if (t + 1 < nt) commit(&kempty[s1]);
+                s = s1;
+                ph = ph1;
+                if (++s1 == ST) {
+                    s1 = 0;
+                    ph1 ^= 1;
+                }
             }
             commit(&ofull);  // when everything issued above has completed, also after giving up
         }
         __syncwarp();
-    } else if (warp < 8 && (warp >> 2) < nx) {
+    } else if ((warp >> 2) < nx) {
+        ATC_MORE;
         // ---- softmax and epilogue: a thread a row
         const int x = warp >> 2, f = it.f0 + tid;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
@@ -286,73 +302,61 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
             if (!ok) break;
             fence_after();
             const uint4 valid = *reinterpret_cast<const uint4 *>(valid_s[t % (2 * ST)]);
-            const bool whole = (valid.x & valid.y & valid.z & valid.w) == 0xffffffffu;
-            // two column blocks in registers: one is read while the other is worked on
-            unsigned r[2][32];
-            float mx = -INFINITY;
-            ld32(s_at, r[0]);
-            wait_ld(r[0]);
+            unsigned r[4][32];
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                if (c < 3) ld32(s_at + (c + 1) * 32, r[(c + 1) & 1]);
-                const unsigned bits = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
-                if (!whole) {
+            for (int c = 0; c < 4; c++) ld32(s_at + c * 32, r[c]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) wait_ld(r[c]);
+            if ((valid.x & valid.y & valid.z & valid.w) != 0xffffffffu) {  // the end of the range, or a page that is not there
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const unsigned bits = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
 #pragma unroll
                     for (int i = 0; i < 32; i++)
-                        if (!(bits >> i & 1)) r[c & 1][i] = 0xff800000u;
+                        if (!(bits >> i & 1)) r[c][i] = 0xff800000u;
                 }
-#pragma unroll
-                for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(r[c & 1][i]));
-                if (c < 3) wait_ld(r[(c + 1) & 1]);
             }
-            mx *= sc;
+            float mx4[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                mx4[c] = fmaxf(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
+#pragma unroll
+                for (int i = 2; i < 32; i += 2) mx4[c] = fmaxf(fmaxf(mx4[c], __uint_as_float(r[c][i])), __uint_as_float(r[c][i + 1]));
+            }
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
             if (t == 0) {
                 m = mx;
             } else if (__any_sync(SB_FULL, mx > m + 8.f)) {  // S(t) is complete, so PV(t - 1) is
                 const float to = fmaxf(m, mx), a = m == to ? 1.f : ap_exp2(m - to);
                 m = to;
                 l *= a;
+#pragma unroll 1
+                for (int c = 0; c < HDP / 16; c++) {
+                    unsigned w[16];
+                    ld16(o_at + c * 16, w);
 #pragma unroll
-                for (int c = 0; c < HDP / 32; c++) {
-                    ld32(o_at + c * 32, r[0]);
-                    wait_ld(r[0]);
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        unsigned w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(r[0][16 * h + i]) * a);
-                        st16(o_at + c * 32 + 16 * h, w);
-                    }
+                    for (int i = 0; i < 16; i++) w[i] = __float_as_uint(__uint_as_float(w[i]) * a);
+                    st16(o_at + c * 16, w);
                 }
             }
             const float b = m == -INFINITY ? 0.f : m;
             const unsigned long long sc2 = f2_pack(sc, sc), b2 = f2_pack(-b, -b), one2 = f2_pack(1.f, 1.f);
-            unsigned long long l2 = 0ull;
-            ld32(s_at, r[0]);
-            wait_ld(r[0]);
+            unsigned long long l2[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                if (c < 3) ld32(s_at + (c + 1) * 32, r[(c + 1) & 1]);
-                const unsigned bits = c == 0 ? valid.x : c == 1 ? valid.y : c == 2 ? valid.z : valid.w;
-                if (!whole) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (!(bits >> i & 1)) r[c & 1][i] = 0xff800000u;
-                }
                 unsigned w[16];
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     float p0, p1;
-                    f2_unpack(ffma2(f2_pack(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), sc2, b2), p0, p1);
+                    f2_unpack(ffma2(f2_pack(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), sc2, b2), p0, p1);
                     p0 = ap_exp2(p0);
                     p1 = ap_exp2(p1);
-                    l2 = ffma2(one2, f2_pack(p0, p1), l2);
+                    l2[i & 1] = ffma2(one2, f2_pack(p0, p1), l2[i & 1]);
                     w[i] = ap_pack<T>(p0, p1);
                 }
-                if (c < 3) wait_ld(r[(c + 1) & 1]);  // the block after this one is read before P goes over it
-                st16(s_at + c * 16, w);
+                st16(s_at + c * 16, w);  // P over S, which is in registers
             }
-            l += f2_sum(l2);
+            l += f2_sum(l2[0]) + f2_sum(l2[1]);
             wait_st();
             fence_before();
             __syncwarp();
