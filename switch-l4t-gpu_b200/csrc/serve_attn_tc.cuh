@@ -2,11 +2,12 @@
 // cores (f16 / bf16): many query rows of a key head against a range of keys.
 //
 // Item = (key head, 256 stacked query rows, key range), one CTA of 16 warps:
-//   warps 0-3, 4-7  softmax of row tile A / B (128 rows each, a thread a row)
-//   warps 8-9, 10-11  loaders of K and V: tiles of 128 keys through the page table
-//                   (cp.async, 128-byte swizzle; TMA boxes cannot follow pages
-//                   of any size), two (HD 128) or four (HD 64) stages
-//   warp 12         issues the tcgen05.mma of both products
+//   warps 0-3, 4-7    softmax of row tile A / B (128 rows each, a thread a row)
+//   warps 8-9, 10-11  loaders of K and V: tiles of 128 keys, two (HD 128) or
+//                     four (HD 64) stages with the 128-byte swizzle; whole
+//                     pages by TMA boxes, tiles that end inside a page, miss
+//                     one, or have pages of other sizes by cp.async
+//   warp 12           issues the tcgen05.mma of both products
 // S = Q K^T (128 x 128, FP32) and P V run on the tensor pipe with S, P and O
 // in tensor memory: the softmax threads read S, write P as 16-bit pairs over
 // it (the A operand of the second product), and O stays there until the end.
@@ -23,7 +24,11 @@
 // Every wait is bounded; after a timeout tc_err is set, the roles stop, what
 // was issued drains, and the tensor memory is freed.
 #pragma once
+#include <cuda.h>
+
 #include "serve_attn.cuh"
+
+#define ATC_POLY 4
 
 __device__ int tc_err;  // nonzero after a wait timed out (sb_tc_error reads and clears it)
 
@@ -45,17 +50,21 @@ SB_DEV unsigned long long now() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
+SB_DEV bool mbar_try(uint64_t *mb, unsigned ph) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(ap_smem(mb)), "r"(ph)
+                 : "memory");
+    return done;
+}
 // false after WAIT_NS, or (abortable) once any wait has given up
 SB_DEV bool mbar_wait(uint64_t *mb, unsigned ph, bool abortable = true) {
+    if (mbar_try(mb, ph)) return true;
     unsigned long long t0 = 0;
-    for (long spin = 0; spin < (1l << 26); spin++) {
-        unsigned done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(ap_smem(mb)), "r"(ph)
-            : "memory");
-        if (done) return true;
+#pragma unroll 1
+    for (int spin = 0; spin < (1 << 26); spin++) {
+        if (mbar_try(mb, ph)) return true;
         if ((spin & 1023) == 1023) {
             if (abortable && *(volatile int *)&tc_err) return false;
             const unsigned long long t = now();
@@ -65,6 +74,16 @@ SB_DEV bool mbar_wait(uint64_t *mb, unsigned ph, bool abortable = true) {
     }
     atomicExch(&tc_err, 1);
     return false;
+}
+SB_DEV void expect_tx(uint64_t *mb, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(ap_smem(mb)), "r"(bytes) : "memory");
+}
+// box {64 values, one head, rows of a page, one page}
+SB_DEV void tma_rows(unsigned dst, const CUtensorMap *tm, int d, int head, int row, int page, uint64_t *mb) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(tm), "r"(d), "r"(head), "r"(row), "r"(page), "r"(ap_smem(mb))
+        : "memory");
 }
 // the same for a converged warp, one answer for all lanes
 SB_DEV bool warp_wait(uint64_t *mb, unsigned ph, bool abortable = true) { return __all_sync(SB_FULL, mbar_wait(mb, ph, abortable)); }
@@ -135,13 +154,69 @@ SB_DEV void st16(uint32_t addr, const unsigned (&r)[16]) {
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+SB_DEV float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+SB_DEV unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// Two powers of two on the FMA pipe, x <= 8: 2^x = 2^n 2^f, n = x rounded,
+// |f| <= 1/2, 2^f as 1 + f q(f), q cubic with the least largest relative error
+// (2.8e-6, 0.01 of a half step of the weights' type); n goes into the
+// exponent.  At x <= -127 it is exactly 0.
+SB_DEV void exp2_pair(unsigned long long x2, float &p0, float &p1) {
+    float x0, x1;
+    f2_unpack(x2, x0, x1);
+    const unsigned long long x = f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+    constexpr float R = 12582912.f;  // 1.5 x 2^23: adding it rounds to a whole number in the low bits
+    const unsigned long long t = add2(x, f2_pack(R, R)), f = add2(x, ffma2(t, f2_pack(-1.f, -1.f), f2_pack(R, R)));
+    unsigned long long q = ffma2(f, f2_pack(0.009582852944731712f, 0.009582852944731712f), f2_pack(0.055906426161527634f, 0.055906426161527634f));
+    q = ffma2(f, q, f2_pack(0.24024099111557007f, 0.24024099111557007f));
+    q = ffma2(f, q, f2_pack(0.6931241750717163f, 0.6931241750717163f));
+    q = ffma2(f, q, f2_pack(1.f, 1.f));
+    float q0, q1, t0, t1;
+    f2_unpack(q, q0, q1);
+    f2_unpack(t, t0, t1);
+    p0 = __uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23));
+    p1 = __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23));
+}
+// weights 2^(sc s - b) of 128 scores as 16-bit pairs over the scores' columns;
+// returns their sum (two halves).  Every fourth pair leaves the exponential unit to the others.
+template <typename T> SB_DEV unsigned long long weights(const unsigned (&r)[4][32], float sc, float b, uint32_t at) {
+    const unsigned long long sc2 = f2_pack(sc, sc), b2 = f2_pack(-b, -b);
+    unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        unsigned w[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const unsigned long long x = ffma2(f2_pack(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), sc2, b2);
+            float p0, p1;
+            if (i % ATC_POLY == ATC_POLY - 1) {
+                exp2_pair(x, p0, p1);
+            } else {
+                f2_unpack(x, p0, p1);
+                p0 = ap_exp2(p0);
+                p1 = ap_exp2(p1);
+            }
+            sum[i & 1] = add2(sum[i & 1], f2_pack(p0, p1));
+            w[i] = ap_pack<T>(p0, p1);
+        }
+        st16(at + c * 16, w);
+    }
+    return add2(sum[0], sum[1]);
+}
 }  // namespace atc
 
 #define ATC_MORE asm volatile("setmaxnreg.inc.sync.aligned.u32 200;")
 #define ATC_FEWER asm volatile("setmaxnreg.dec.sync.aligned.u32 56;")
 
 template <typename T, int HDP>
-SB_DEV void attn_tc_body(const AttnParams &P) {
+SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUtensorMap *tm_v, int box) {
     using namespace atc;
     using C = Cfg<HDP>;
     constexpr int ST = C::ST, TILE = C::TILE;
@@ -203,54 +278,76 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
         const bool is_k = warp < 10;
         const int p0 = (warp & 1) * 64;
         const T *base = static_cast<const T *>(is_k ? it.pg.k : it.pg.v) + it.kvh * it.pg.head_stride;
+        const CUtensorMap *tm = is_k ? tm_k : tm_v;
         uint64_t *full = is_k ? kfull : vfull, *empty = is_k ? kempty : vempty;
         constexpr int CH = HDP / 8, RPI = 32 / CH;  // chunks of a row, rows an instruction
         const int c = lane % CH, rsub = lane / CH;
         const bool cok = c * 8 < P.HD;
         const T *col = base + c * 8;
-        long long off[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) off[h] = ap_offset(it, it.k0 + p0 + h * 32 + lane);
-        bool ok = true;
-        for (int t = 0; t < nt; t++) {
-            const int s = t % ST;
+        // TMA: lane i takes rows [box i, box i + box) of these 64 in column block i / pieces
+        const int pieces = box ? 64 / box : 1, sub = lane / pieces, row = lane % pieces * box;
+        const bool mine = box && sub < C::SUB;
+        bool ok = true, any_tma = false;
+        int t = 0;
+        for (; t < nt; t++) {
+            const int s = t % ST, key = it.k0 + t * KT + p0;
+            int page = -1, in_page = 0;
+            if (mine && key + 64 <= it.k1) {
+                const int j = (key + row) / it.pg.page;
+                page = it.table ? it.table[j] : j;
+                in_page = key + row - j * it.pg.page;
+            }
+            const bool by_tma = __all_sync(SB_FULL, box && (!mine || (page >= 0 && page < it.pg.n_pages)));
             if (t >= ST) ok = warp_wait(&empty[s], (unsigned)((t / ST) - 1) & 1u);
             if (!ok) break;
-            const unsigned stage = (is_k ? kst : vst) + s * TILE + (c >> 3) * 16384;
-#pragma unroll
+            const unsigned stage = (is_k ? kst : vst) + s * TILE;
+            if (by_tma) {
+                any_tma = true;
+                if (lane == 0) {
+                    if (is_k) *reinterpret_cast<uint2 *>(&valid_s[t % (2 * ST)][(warp & 1) * 2]) = make_uint2(~0u, ~0u);
+                    expect_tx(&full[s], 64 * HDP * 2);
+                }
+                __syncwarp();
+                if (mine) tma_rows(stage + sub * 16384 + (p0 + row) * 128, tm, sub * 64, it.kvh, in_page, page, &full[s]);
+                continue;
+            }
+#pragma unroll 1
             for (int h = 0; h < 2; h++) {
+                const long long off = ap_offset(it, key + h * 32 + lane);
                 if (is_k) {
-                    const unsigned valid = __ballot_sync(SB_FULL, off[h] >= 0);
+                    const unsigned valid = __ballot_sync(SB_FULL, off >= 0);
                     if (lane == 0) valid_s[t % (2 * ST)][(warp & 1) * 2 + h] = valid;
                 }
 #pragma unroll 4
                 for (int i = 0; i < CH; i++) {
                     const int r = i * RPI + rsub;
-                    const long long o = __shfl_sync(SB_FULL, off[h], r);
+                    const long long o = __shfl_sync(SB_FULL, off, r);
                     const bool there = o >= 0 && cok;
-                    ap_cp16(stage + (p0 + h * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), there ? col + o : base, there);
+                    ap_cp16(stage + (c >> 3) * 16384 + (p0 + h * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), there ? col + o : base, there);
                 }
             }
             ap_commit();
-#pragma unroll
-            for (int h = 0; h < 2; h++) off[h] = ap_offset(it, it.k0 + (t + 1) * KT + p0 + h * 32 + lane);
             ap_wait<0>();
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[s]);
         }
         ap_wait<0>();
+        if (!ok && any_tma)  // given up: the copies that were issued still have to land
+            for (int i = t > ST ? t - ST : 0; i < t; i++) mbar_wait(&full[i % ST], (i / ST) & 1, false);
     } else if (warp >= 12) {
         ATC_FEWER;
         if (tid == 12 * 32) {
-            // ---- issuer
+            // ---- issuer.  One for both tiles: it keeps their phases apart (with an issuer each they fell into step,
+            // both in their softmax, then both on the tensor pipe)
             const uint32_t id_s = idesc<T>(KT, false), id_o = idesc<T>(HDP, true);
             const uint64_t qd = desc(qst), kd = desc(kst), vd = desc(vst);
             auto scores = [&](int x, int s) {
+                const uint64_t qs = qd + x * (TILE >> 4), ks = kd + s * (TILE >> 4);
 #pragma unroll
                 for (int k = 0; k < HDP / 16; k++) {
                     const uint32_t in = (k >> 2) * 1024 + 2 * (k & 3);
-                    mma_ss(tmem + x * 128, qd + (x * (TILE >> 4) + in), kd + (s * (TILE >> 4) + in), id_s, k > 0);
+                    mma_ss(tmem + x * 128, qs + in, ks + in, id_s, k > 0);
                 }
                 commit(&sfull[x]);
             };
@@ -260,11 +357,13 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
                 for (int x = 0; x < nx; x++) scores(x, 0);
                 commit(&kempty[0]);
             }
-            int s = 0, s1 = ST > 1 ? 1 : 0;  // stages of t and t + 1
-            unsigned ph = 0, ph1 = 0;
+            int s = 0;
+            unsigned ph = 0;
             for (int t = 0; t < nt && ok; t++) {
-                ok = mbar_wait(&vfull[s], ph);
-                if (ok && t + 1 < nt) ok = mbar_wait(&kfull[s1], ph1);
+                const int s1 = s + 1 == ST ? 0 : s + 1;
+                const unsigned ph1 = s1 ? ph : ph ^ 1;
+                const bool more = t + 1 < nt;
+                ok = mbar_wait(&vfull[s], ph) && (!more || mbar_wait(&kfull[s1], ph1));
 #pragma unroll 1
                 for (int x = 0; x < nx && ok; x++) {
                     ok = mbar_wait(&pfull[x], t & 1);
@@ -274,17 +373,12 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
 #pragma unroll
                     for (int k = 0; k < KT / 16; k++)
                         mma_ts(tmem + 256 + x * 128, tmem + x * 128 + k * 8, vs + k * 128, id_o, t > 0 || k > 0);
-                    if (t + 1 < nt) scores(x, s1);
+                    if (more) scores(x, s1);
                 }
-                if (!ok) break;
                 commit(&vempty[s]);
-                if (t + 1 < nt) commit(&kempty[s1]);
+                if (more) commit(&kempty[s1]);
                 s = s1;
                 ph = ph1;
-                if (++s1 == ST) {
-                    s1 = 0;
-                    ph1 ^= 1;
-                }
             }
             commit(&ofull);  // when everything issued above has completed, also after giving up
         }
@@ -319,19 +413,24 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
             float mx4[4];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                mx4[c] = fmaxf(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
+                mx4[c] = max_nan(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
 #pragma unroll
-                for (int i = 2; i < 32; i += 2) mx4[c] = fmaxf(fmaxf(mx4[c], __uint_as_float(r[c][i])), __uint_as_float(r[c][i + 1]));
+                for (int i = 2; i < 32; i += 2) mx4[c] = max_nan(max_nan(mx4[c], __uint_as_float(r[c][i])), __uint_as_float(r[c][i + 1]));
             }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-            if (t == 0) {
-                m = mx;
-            } else if (__any_sync(SB_FULL, mx > m + 8.f)) {  // S(t) is complete, so PV(t - 1) is
-                const float to = fmaxf(m, mx), a = m == to ? 1.f : ap_exp2(m - to);
+            const float mx = max_nan(max_nan(mx4[0], mx4[1]), max_nan(mx4[2], mx4[3])) * sc;
+            if (t == 0) m = mx;
+            // the weights are taken against the maximum so far, beside the search for the new one; where that has
+            // grown too far (or a NaN turns up) they are taken again
+            unsigned long long l2;
+            for (;;) {
+                l2 = weights<T>(r, sc, m == -INFINITY ? 0.f : m, s_at);
+                if (!__any_sync(SB_FULL, mx > m + 8.f || (mx != mx && m == m))) break;
+                const float to = max_nan(m, mx), a = m == to ? 1.f : ap_exp2(m - to);
                 m = to;
                 l *= a;
+                wait_st();
 #pragma unroll 1
-                for (int c = 0; c < HDP / 16; c++) {
+                for (int c = 0; c < HDP / 16; c++) {  // S(t) is complete, so PV(t - 1) is
                     unsigned w[16];
                     ld16(o_at + c * 16, w);
 #pragma unroll
@@ -339,29 +438,13 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
                     st16(o_at + c * 16, w);
                 }
             }
-            const float b = m == -INFINITY ? 0.f : m;
-            const unsigned long long sc2 = f2_pack(sc, sc), b2 = f2_pack(-b, -b), one2 = f2_pack(1.f, 1.f);
-            unsigned long long l2[2] = {0ull, 0ull};
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                unsigned w[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float p0, p1;
-                    f2_unpack(ffma2(f2_pack(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), sc2, b2), p0, p1);
-                    p0 = ap_exp2(p0);
-                    p1 = ap_exp2(p1);
-                    l2[i & 1] = ffma2(one2, f2_pack(p0, p1), l2[i & 1]);
-                    w[i] = ap_pack<T>(p0, p1);
-                }
-                st16(s_at + c * 16, w);  // P over S, which is in registers
-            }
-            l += f2_sum(l2[0]) + f2_sum(l2[1]);
+            l += f2_sum(l2);
             wait_st();
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&pfull[x]);
         }
+        if (m == INFINITY) l = __int_as_float(0x7fc00000);  // an infinite score: NaN, as its softmax
         ok = __all_sync(SB_FULL, mbar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
         fence_after();
         if (f < it.F && ok) ap_row_stats(P, it, f, m, l);
@@ -385,8 +468,12 @@ SB_DEV void attn_tc_body(const AttnParams &P) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
-#define ATC_KERNEL(name, T, HDP) \
-    extern "C" __global__ void __launch_bounds__(atc::THREADS, 1) name(const __grid_constant__ AttnParams P, int own) { attn_tc_body<T, HDP>(P); }
+#define ATC_KERNEL(name, T, HDP)                                                                                                     \
+    extern "C" __global__ void __launch_bounds__(atc::THREADS, 1)                                                                       \
+        name(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,  \
+             int box) {                                                                                                                 \
+        attn_tc_body<T, HDP>(P, &tm_k, &tm_v, box);                                                                                     \
+    }
 ATC_KERNEL(attn_tc_f16_64, __half, 64)
 ATC_KERNEL(attn_tc_f16_128, __half, 128)
 ATC_KERNEL(attn_tc_bf16_64, __nv_bfloat16, 64)

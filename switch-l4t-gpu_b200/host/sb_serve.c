@@ -341,6 +341,17 @@ static int pages_for_attn(const sb_kv_pages *kv, struct attn_pages *p) {
     return 0;
 }
 
+/* pages as {HD, heads, positions, pages}, boxes of 64 values of one head of
+ * `box` positions, 128-byte swizzle; what is past HD reads as zero */
+static int encode_pages(CUtensorMap *tm, const void *base, const sb_kv_pages *kv, int box) {
+    const cuuint64_t dims[4] = {(cuuint64_t)kv->HD, (cuuint64_t)kv->NKV, (cuuint64_t)kv->page, (cuuint64_t)kv->n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)kv->head_stride * 2, (cuuint64_t)kv->pos_stride * 2, (cuuint64_t)kv->page_stride * 2};
+    const cuuint32_t size[4] = {64, 1, (cuuint32_t)box, 1}, estr[4] = {1, 1, 1, 1};
+    return cuTensorMapEncodeTiled(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void *)base, dims, strides, size, estr,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
                    int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
                    int prefix_len, const sb_kv_pages *kv, const int *table, int table_stride, const int *kv_len, int max_kv,
@@ -411,8 +422,19 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     int zero = 0, one = 1;
     if (pre.S) {
         p.tiles = pre.tiles;
-        void *args[] = {&p, &zero};
-        rc = sb_launch(c, pre.f, (unsigned)pre.grid, 1, pre.threads, pre.smem, (CUstream)stream, args, 0);
+        CUtensorMap tk, tv;
+        /* whole pages (or 64-position parts of one) by TMA, in at most 32 boxes
+         * of a warp; other page sizes, and strides that a map cannot hold, by
+         * the kernel's own copies (box 0) */
+        const int pg = prefix->page;
+        int box = pg % 64 == 0 ? 64 : 64 % pg == 0 && pg >= 8 ? pg : 0;
+        if (pre.threads != 512 || !encode_pages(&tk, prefix->k, prefix, box ? box : 1) || !encode_pages(&tv, prefix->v, prefix, box ? box : 1)) {
+            box = 0;
+            memset(&tk, 0, sizeof tk);
+            memset(&tv, 0, sizeof tv);
+        }
+        void *args[] = {&p, &zero}, *tc_args[] = {&p, &tk, &tv, &box};
+        rc = sb_launch(c, pre.f, (unsigned)pre.grid, 1, pre.threads, pre.smem, (CUstream)stream, pre.threads == 512 ? tc_args : args, 0);
         if (rc) return rc;
     }
     if (own.S) { /* beside the prefix launch's last items */
