@@ -326,7 +326,7 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * requests are still right; kv_len is cut to max_kv.  A row that sees nothing
  * gives zeros and lse = -inf; rows from cu_q[B] on are left as they were.
  * lse [T][NH] (natural log of the softmax denominator) may be NULL.
- * ws: sb_attn_prefix_ws bytes for the same sizes (16-byte aligned).  FP32
+ * ws: sb_attn_prefix_ws bytes for the same sizes (32-byte aligned).  FP32
  * runs on CUDA cores in FP32 throughout; 16-bit types use the tensor cores
  * with FP32 scores, sums and outputs and 16-bit softmax weights. */
 int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes);

@@ -583,11 +583,14 @@ SB_AP_F32(attn_f32_128_r16, 128, 16)
 
 // ---------------------------------------------------------------- join
 // A warp a (row, head): parts of the prefix, then those of the request's own
-// keys that are in use; lane i takes part i's (m, l), all lanes the sums.
+// keys that are in use.  Four values a lane; head sizes up to 64, 32, ... let
+// 2, 4, ... groups of lanes take parts side by side.  A part without weight
+// may not have been written and is not read.
 // type: 0 f32, 1 f16, 2 bf16.
 extern "C" __global__ void __launch_bounds__(128) attn_join(const __grid_constant__ AttnParams P, int type) {
-    pdl_wait();
     const int lane = threadIdx.x & 31;
+    const int width = P.HD > 64 ? 32 : P.HD > 32 ? 16 : P.HD > 16 ? 8 : 4, groups = 32 / width, d = (lane & (width - 1)) * 4;
+    pdl_wait();
     const long long rows = (long long)ap_rows(P) * P.NH, TH = (long long)P.T * P.NH;
     for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); i < rows; i += (long long)gridDim.x * 4) {
         const int row = (int)(i / P.NH), head = (int)(i % P.NH);
@@ -598,37 +601,37 @@ extern "C" __global__ void __launch_bounds__(128) attn_join(const __grid_constan
             if (ml.y != 0.f) M = fmaxf(M, ml.x);
         }
         M = warp_max(M);
-        float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < n; s0 += 32) {
-            float w = 0.f;
-            if (s0 + lane < n) {
-                const float2 ml = P.ws_ml[(s0 + lane) * TH + i];
-                if (ml.y != 0.f) {
-                    w = ap_exp2(ml.x - M);
-                    L += w * ml.y;
-                }
-            }
-            const int c = min(32, n - s0);
-            for (int s = 0; s < c; s++) {
-                const float ws = __shfl_sync(SB_FULL, w, s);
-                if (ws == 0.f) continue;  // a part without weight may not have been written
-                const float *p = P.ws_o + ((s0 + s) * TH + i) * P.HD;
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (lane + 32 * e < P.HD) acc[e] = fmaf(ws, p[lane + 32 * e], acc[e]);
-            }
+        float L = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int s = lane / width; s < n; s += groups) {
+            const float2 ml = P.ws_ml[s * TH + i];
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (ml.y != 0.f && d < P.HD) o = *reinterpret_cast<const float4 *>(P.ws_o + (s * TH + i) * P.HD + d);
+            const float w = ml.y != 0.f ? ap_exp2(ml.x - M) : 0.f;
+            L = fmaf(w, ml.y, L);
+            acc.x = fmaf(w, o.x, acc.x);
+            acc.y = fmaf(w, o.y, acc.y);
+            acc.z = fmaf(w, o.z, acc.z);
+            acc.w = fmaf(w, o.w, acc.w);
         }
-        L = warp_sum(L);
+        for (int o = width; o < 32; o <<= 1) {
+            L += __shfl_xor_sync(SB_FULL, L, o);
+            acc.x += __shfl_xor_sync(SB_FULL, acc.x, o);
+            acc.y += __shfl_xor_sync(SB_FULL, acc.y, o);
+            acc.z += __shfl_xor_sync(SB_FULL, acc.z, o);
+            acc.w += __shfl_xor_sync(SB_FULL, acc.w, o);
+        }
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        const long long at = row * P.o_row + head * P.o_head;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int d = lane + 32 * e;
-            if (d >= P.HD) continue;
-            const float v = acc[e] * inv;
-            if (type == 0) static_cast<float *>(P.out)[at + d] = v;
-            else if (type == 1) static_cast<__half *>(P.out)[at + d] = __float2half_rn(v);
-            else static_cast<__nv_bfloat16 *>(P.out)[at + d] = __float2bfloat16_rn(v);
+        const long long at = row * P.o_row + head * P.o_head + d;
+        if (lane < width && d < P.HD) {
+            const float a = acc.x * inv, b = acc.y * inv, e = acc.z * inv, f = acc.w * inv;
+            if (type == 0) *reinterpret_cast<float4 *>(static_cast<float *>(P.out) + at) = make_float4(a, b, e, f);
+            else if (type == 1)
+                *reinterpret_cast<uint2 *>(static_cast<__half *>(P.out) + at) = make_uint2(ap_pack<__half>(a, b), ap_pack<__half>(e, f));
+            else
+                *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(P.out) + at) =
+                    make_uint2(ap_pack<__nv_bfloat16>(a, b), ap_pack<__nv_bfloat16>(e, f));
         }
         if (P.lse && lane == 0) P.lse[i] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }

@@ -221,7 +221,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
     using C = Cfg<HDP>;
     constexpr int ST = C::ST, TILE = C::TILE;
     extern __shared__ unsigned char tc_sm_raw[];
-    __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], pfull[2], ofull;
+    __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], pfull[2], qfull, ofull;
     __shared__ uint32_t tmem_s;
     __shared__ __align__(16) uint32_t valid_s[2 * ST][4];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -245,26 +245,12 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             mbar_init(&pfull[x], 4);
         }
         mbar_init(&ofull, 1);
+        mbar_init(&qfull, 4 * nx);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ap_smem(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    if (warp < 8) {  // a thread its query row, negated for a negative scale; rows behind the last as zeros
-        const int f = it.f0 + tid;
-        const unsigned flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;
-        const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
-        const unsigned row = qst + (tid >> 7) * TILE + (tid & 127) * 128;
-#pragma unroll
-        for (int c = 0; c < HDP / 8; c++) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (f < it.F && c * 8 < P.HD) v = *reinterpret_cast<const uint4 *>(qp + c * 8);
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + (c >> 3) * 16384 + (((c & 7) ^ (tid & 7)) << 4)), "r"(v.x ^ flip),
-                         "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
-                         : "memory");
-        }
-        fence_async();
     }
     fence_before();
     __syncthreads();
@@ -351,7 +337,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 }
                 commit(&sfull[x]);
             };
-            bool ok = nt > 0 && mbar_wait(&kfull[0], 0);
+            bool ok = nt > 0 && mbar_wait(&qfull, 0) && mbar_wait(&kfull[0], 0);
             if (ok) {
                 fence_after();
                 for (int x = 0; x < nx; x++) scores(x, 0);
@@ -389,6 +375,25 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         const int x = warp >> 2, f = it.f0 + tid;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
         const float sc = fabsf(P.scale_log2);
+        {  // this warp's 32 query rows, neighbouring lanes on one row; negated for a negative scale, zeros behind the last
+            constexpr int CH = HDP / 8, RPI = 32 / CH;
+            const int c = lane % CH;
+            const unsigned flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const int r = (warp & 3) * 32 + i * RPI + lane / CH, fr = it.f0 + x * BM + r;
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (fr < it.F && c * 8 < P.HD)
+                    v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(P.q) + (long long)(it.row0 + fr / P.G) * P.q_row +
+                                                         (it.kvh * P.G + fr % P.G) * P.q_head + c * 8);
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qst + x * TILE + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                             "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
+                             : "memory");
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&qfull);
+        }
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int t = 0; t < nt && ok; t++) {
@@ -447,16 +452,32 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         if (m == INFINITY) l = __int_as_float(0x7fc00000);  // an infinite score: NaN, as its softmax
         ok = __all_sync(SB_FULL, mbar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
         fence_after();
-        if (f < it.F && ok) ap_row_stats(P, it, f, m, l);
-#pragma unroll
+        const bool live = f < it.F && ok;
+        if (live) ap_row_stats(P, it, f, m, l);
+        const int qrow = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
+        const bool whole = P.S1 + P.S2 == 1;  // the result itself, else this range's part of it
+        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        float *po = P.ws_o + (((long long)it.slot * P.T + qrow) * P.NH + head) * P.HD;
+        T *out = static_cast<T *>(P.out) + qrow * P.o_row + head * P.o_head;
+#pragma unroll 1
         for (int c = 0; c < HDP / 32; c++) {
             unsigned r[32];
             ld32(o_at + c * 32, r);
             wait_ld(r);
-            if (f < it.F && ok) {
+            if (!live) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i += 2)
-                    ap_row_out<T>(P, it, f, c * 32 + i, __uint_as_float(r[i]), __uint_as_float(r[i + 1]), l);
+            for (int i = 0; i < 32; i += 8) {  // 32-byte stores (a lane a row: full sectors)
+                if (c * 32 + i >= P.HD) break;
+                if (whole) {
+                    unsigned w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = ap_pack<T>(__uint_as_float(r[i + 2 * e]) * inv, __uint_as_float(r[i + 2 * e + 1]) * inv);
+                    *reinterpret_cast<uint4 *>(out + c * 32 + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else if (l != 0.f) {
+                    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(po + c * 32 + i), "r"(r[i]), "r"(r[i + 1]),
+                                 "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+                                 : "memory");
+                }
             }
         }
     }

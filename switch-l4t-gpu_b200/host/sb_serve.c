@@ -387,7 +387,7 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     rc = attn_parts(c, type, T, B, NH, NKV, HD, max_q, prefix_len, max_kv, &pre, &own);
     if (rc) return rc;
     const size_t need = attn_ws_bytes(T, NH, HD, &pre, &own);
-    SB_ARG(ws_bytes >= need && (ws || need == 0) && ALIGNED(ws, 16), "attn_prefix: workspace too small (sb_attn_prefix_ws) or misaligned");
+    SB_ARG(ws_bytes >= need && (ws || need == 0) && ALIGNED(ws, 32), "attn_prefix: workspace too small (sb_attn_prefix_ws) or misaligned");
     const size_t parts = (size_t)T * NH * (pre.S + own.S);
     p.q = DP(q);
     p.out = DP(out);

@@ -540,7 +540,7 @@ def test_attn_prefix_workspace_too_small(cuda_dev):
     b = Batch("f16", 14, 2, 64, 1000, [50, 20])
     n = sb200.attn_prefix_ws(b.q, b.kv, 1000, 2, max_kv=50)
     assert n > 0
-    for ws in (None, torch.empty(n - 1, dtype=torch.uint8, device="cuda"), torch.empty(n + 9, dtype=torch.uint8, device="cuda")[8:]):
+    for ws in (None, torch.empty(n - 1, dtype=torch.uint8, device="cuda"), torch.empty(n + 17, dtype=torch.uint8, device="cuda")[16:]):
         with pytest.raises(sb200.SbError, match="workspace"):
             sb200.attn_prefix(b.q, torch.empty_like(b.q), b.kv, b.ptable, 1000, b.kv, b.table, b.kv_len, b.scale, ws, max_kv=50)
 
