@@ -11,12 +11,13 @@
 // keys meet only its own rows.
 //
 // One item runs one of these bodies; each streams K and V tiles through a
-// three-stage cp.async ring, positions going through the block table (an
+// cp.async ring of two or three stages, positions going through the block table (an
 // offset per key, computed a tile ahead; a position without a page, or past
 // the range, is filled with zeros and masked, so nothing of it is read):
-//   attn_mma_body  f16 / bf16, mma.sync m16n8k16: 16-row tiles (four warps
-//                  split the keys; memory-bound: one row group against long
-//                  own pages) or 64-row tiles (a warp 16 rows)
+//   attn_mma8_body f16 / bf16, mma.sync m16n8k16, up to eight rows (the head
+//                  group of a decode step) against long own pages: memory-bound
+//   attn_mma_body  the same for 16-row tiles (four warps split the keys) or
+//                  64-row tiles (a warp 16 rows)
 //   attn_f32_body  FP32 on the CUDA cores: 1..16-row tiles, a thread a key
 // Scores, maxima, sums and outputs are FP32; the softmax weights are rounded
 // to the value type for the second tensor-core product (half a step, like
@@ -27,7 +28,9 @@
 #include "sb_common.cuh"
 
 #define SB_AP_THREADS 128
-#define SB_AP_STAGES 3
+// stages of the K / V ring: two of 32 KB for 128 values leave room for three CTAs on an SM
+#define SB_AP_ST(HDP) ((HDP) == 128 ? 2 : 3)
+#define SB_AP_RING 4  // offsets of the tiles in flight
 
 struct AttnPages {  // strides in elements
     const void *k, *v;
@@ -116,14 +119,47 @@ SB_DEV void ap_cp16(unsigned dst, const void *src, bool ok) {  // 16 bytes, or z
 SB_DEV void ap_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> SB_DEV void ap_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// element offset of position p in the pages (without the head), -1 where it has none
+// element offset of position p in the pages (without the head) with the lowest
+// bit set (offsets are multiples of 16 bytes), 0 where it has none
 SB_DEV long long ap_offset(const AttnItem &it, int p) {
-    if (p >= it.k1) return -1;
+    if (p >= it.k1) return 0;
     const int j = p / it.pg.page;
     const int pg = it.table ? it.table[j] : j;
-    if (pg < 0 || pg >= it.pg.n_pages) return -1;
-    return pg * it.pg.page_stride + (p - j * it.pg.page) * it.pg.pos_stride;
+    if (pg < 0 || pg >= it.pg.n_pages) return 0;
+    return (pg * it.pg.page_stride + (p - j * it.pg.page) * it.pg.pos_stride) | 1;
 }
+// A thread's share of the copies of a K and a V tile of KT positions, rows of
+// HDP values of E bytes: its 16-byte chunk of every STEP-th row, swizzled by
+// the row's low three bits.  Places that are not
+// there are filled with zeros, nothing of them is read.
+template <int KT, int HDP, int E> struct ApCopy {
+    static constexpr int C = HDP * E / 16, STEP = SB_AP_THREADS / C, N = KT / STEP;
+    const char *k;
+    long long to_v;
+    unsigned dst;
+    int row;
+    bool in;
+    SB_DEV ApCopy(const AttnItem &it, int HD) {
+        static_assert(STEP % 8 == 0 || STEP == 4, "rows of a thread share their low three bits, or differ in the third");
+        const int c = threadIdx.x % C;
+        row = threadIdx.x / C;
+        k = static_cast<const char *>(it.pg.k) + it.kvh * it.pg.head_stride * E + c * 16;
+        to_v = static_cast<const char *>(it.pg.v) - static_cast<const char *>(it.pg.k);
+        dst = row * (HDP * E) + ((c ^ (row & 7)) << 4);
+        in = c * 16 < HD * E;
+    }
+    SB_DEV void copy(unsigned kd, unsigned vd, const long long *off) const {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const long long o = off[row + j * STEP];
+            const bool ok = (o & 1) && in;
+            const char *p = k + (o & ~1ll) * E;
+            const unsigned at = (dst ^ ((j * STEP & 4) << 4)) + j * STEP * HDP * E;  // chunk ^ 4 where the row's third bit is set
+            ap_cp16(kd + at, p, ok);
+            ap_cp16(vd + at, p + to_v, ok);
+        }
+    }
+};
 
 // what a finished row leaves: the output itself where the item is the only one, else its part
 SB_DEV void ap_row_stats(const AttnParams &P, const AttnItem &it, int f, float m, float l) {
@@ -190,18 +226,17 @@ SB_DEV float ap_exp2(float x) {
 
 // HDP: head size padded to 64 or 128.  MW: warps along the rows (1: 16-row
 // tile, warps split the 64 keys of a tile; 4: 64-row tile).
-// Shared memory: SB_AP_STAGES x 2 x 64 x HDP x 2 bytes (>= the 4 x 16 x HDP
+// Shared memory: SB_AP_ST x 2 x 64 x HDP x 2 bytes (>= the 4 x 16 x HDP
 // floats of the final join over warps), rows of 128 / 256 bytes with their
 // 16-byte chunks xor-ed by the row's low three bits (ldmatrix reads eight
 // rows of one chunk without a conflict).
 template <typename T, int HDP, int MW>
 SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
-    constexpr int KT = 64, WK = MW == 1 ? 16 : 64, NT = WK / 8, C = HDP / 8, KS = HDP / 16;
-    constexpr int TILE = KT * HDP * 2, STAGE = 2 * TILE, RING = SB_AP_STAGES + 1;
+    constexpr int KT = 64, WK = MW == 1 ? 16 : 64, NT = WK / 8, KS = HDP / 16, ST = SB_AP_ST(HDP);
+    constexpr int TILE = KT * HDP * 2, STAGE = 2 * TILE, RING = SB_AP_RING;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     const int fw = it.f0 + (MW == 1 ? 0 : warp * 16);  // this warp's first row
-    const T *kb = static_cast<const T *>(it.pg.k) + it.kvh * it.pg.head_stride;
-    const T *vb = static_cast<const T *>(it.pg.v) + it.kvh * it.pg.head_stride;
+    const ApCopy<KT, HDP, 2> copier(it, P.HD);
 
     // query fragments from global memory: rows fw + g and fw + g + 8
     unsigned qa[KS][4];
@@ -226,17 +261,8 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
 
     auto load = [&](int t) {
         if (t < nt) {
-            const unsigned kd = ap_smem(sm) + (t % SB_AP_STAGES) * STAGE, vd = kd + TILE;
-            const long long *off = off_s[t % RING];
-#pragma unroll
-            for (int j = 0; j < KT * C / SB_AP_THREADS; j++) {
-                const int i = tid + j * SB_AP_THREADS, r = i / C, c = i % C;
-                const long long o = off[r];
-                const bool ok = o >= 0 && c * 8 < P.HD;
-                const unsigned d = r * (HDP * 2) + ((c ^ (r & 7)) << 4);
-                ap_cp16(kd + d, ok ? kb + o + c * 8 : kb, ok);
-                ap_cp16(vd + d, ok ? vb + o + c * 8 : vb, ok);
-            }
+            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE;
+            copier.copy(kd, kd + TILE, off_s[t % RING]);
         }
         ap_commit();
     };
@@ -246,17 +272,17 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
     __syncthreads();  // the ring and the offsets of an earlier item are no longer read
-    for (int t = 0; t < SB_AP_STAGES; t++)
+    for (int t = 0; t < ST; t++)
         if (tid < KT) off_s[t][tid] = ap_offset(it, it.k0 + t * KT + tid);
     __syncthreads();
-    for (int t = 0; t < SB_AP_STAGES - 1; t++) load(t);
+    for (int t = 0; t < ST - 1; t++) load(t);
     for (int t = 0; t < nt; t++) {
-        ap_wait<SB_AP_STAGES - 2>();
+        ap_wait<ST - 2>();
         __syncthreads();  // tile t is there for all; tile t - 1 and its offsets are read
-        load(t + SB_AP_STAGES - 1);
-        long long next = -1;
-        if (tid < KT) next = ap_offset(it, it.k0 + (t + SB_AP_STAGES) * KT + tid);
-        const unsigned kt = ap_smem(sm) + (t % SB_AP_STAGES) * STAGE, vt = kt + TILE;
+        load(t + ST - 1);
+        long long next = 0;
+        if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
+        const unsigned kt = ap_smem(sm) + (t % ST) * STAGE, vt = kt + TILE;
         const long long *off = off_s[t % RING];
         const int w0 = MW == 1 ? warp * 16 : 0, key0 = it.k0 + t * KT + w0;
         float s[NT][4];
@@ -280,7 +306,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int j = n * 8 + q4 * 2 + (e & 1);
-                const bool seen = key0 + j < vis[e >> 1] && off[w0 + j] >= 0;
+                const bool seen = key0 + j < vis[e >> 1] && (off[w0 + j] & 1);
                 s[n][e] = seen ? s[n][e] * P.scale_log2 : -INFINITY;
                 mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
             }
@@ -319,7 +345,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
                 ap_mma<T>(o[2 * i + 1], a, b[2], b[3]);
             }
         }
-        if (tid < KT) off_s[(t + SB_AP_STAGES) % RING][tid] = next;
+        if (tid < KT) off_s[(t + ST) % RING][tid] = next;
     }
     ap_wait<0>();
 #pragma unroll
@@ -371,6 +397,152 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
     }
 }
 
+// Up to eight rows against their own keys, the products the other way round:
+// S^T = K Q^T (keys along m, rows along n = 8) and O^T = V^T P^T.  Nothing is
+// spent on rows that are not there (a group of 4 or 7 heads filled a quarter
+// or half of 16), and the outputs take half the registers.  P^T turns from
+// accumulator into operand by movmatrix.  The four warps split the 64 keys of
+// a tile.  Like the tcgen05 kernel it rescales only when a row's maximum has
+// grown by more than 2^8; a tile without that costs one vote.
+SB_DEV unsigned ap_movmatrix(unsigned a) {
+    unsigned d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+template <typename T, int HDP>
+SB_DEV void attn_mma8_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
+    constexpr int KT = 64, KS = HDP / 16, ST = SB_AP_ST(HDP), TILE = KT * HDP * 2, STAGE = 2 * TILE, RING = SB_AP_RING;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
+    const ApCopy<KT, HDP, 2> copier(it, P.HD);
+    unsigned qb[KS][2];  // row f0 + g
+    int vis[2];          // of rows f0 + 2 q4, + 1
+    {
+        const int f = it.f0 + g;
+        const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = k * 16 + e * 8 + q4 * 2;
+                qb[k][e] = f < it.F && d < P.HD ? *reinterpret_cast<const unsigned *>(qp + d) : 0u;
+            }
+#pragma unroll
+        for (int h = 0; h < 2; h++) vis[h] = it.f0 + 2 * q4 + h < it.F ? ap_vis(it, it.f0 + 2 * q4 + h, P.G) : 0;
+    }
+    const int flast = min(it.f0 + 8, it.F) - 1;
+    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
+    const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
+    auto load = [&](int t) {
+        if (t < nt) {
+            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE;
+            copier.copy(kd, kd + TILE, off_s[t % RING]);
+        }
+        ap_commit();
+    };
+    float o[KS][4];
+#pragma unroll
+    for (int i = 0; i < KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    __syncthreads();  // the ring and the offsets of an earlier item are no longer read
+    for (int t = 0; t < ST; t++)
+        if (tid < KT) off_s[t][tid] = ap_offset(it, it.k0 + t * KT + tid);
+    __syncthreads();
+    for (int t = 0; t < ST - 1; t++) load(t);
+    const int w0 = warp * 16;
+    for (int t = 0; t < nt; t++) {
+        ap_wait<ST - 2>();
+        __syncthreads();  // tile t is there for all; tile t - 1 and its offsets are read
+        load(t + ST - 1);
+        long long next = 0;
+        if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
+        const unsigned kt = ap_smem(sm) + (t % ST) * STAGE, vt = kt + TILE;
+        const long long *off = off_s[t % RING];
+        const int key = it.k0 + t * KT + w0 + g;
+        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // two chains
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const int r = w0 + (lane & 15), c = 2 * k + (lane >> 4);
+            unsigned a[4];
+            ap_ldsm(a, kt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
+            ap_mma<T>(s[k & 1], a, qb[k][0], qb[k][1]);
+        }
+        const bool there0 = off[w0 + g] & 1, there1 = off[w0 + g + 8] & 1;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {  // key g + 8 (e >> 1), row 2 q4 + (e & 1)
+            const bool seen = ((e >> 1) ? there1 : there0) && key + 8 * (e >> 1) < vis[e & 1];
+            s[0][e] = seen ? (s[0][e] + s[1][e]) * P.scale_log2 : -INFINITY;
+        }
+        float mx[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
+        if (__any_sync(SB_FULL, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(SB_FULL, mx[h], x));
+                const float to = fmaxf(m[h], mx[h]), a = to == m[h] ? 1.f : ap_exp2(m[h] - to);
+                m[h] = to;
+                l[h] *= a;
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    o[i][h] *= a;
+                    o[i][2 + h] *= a;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            s[0][e] = ap_exp2(s[0][e] - (m[e & 1] == -INFINITY ? 0.f : m[e & 1]));
+            l[e & 1] += s[0][e];
+        }
+        const unsigned b0 = ap_movmatrix(ap_pack<T>(s[0][0], s[0][1])), b1 = ap_movmatrix(ap_pack<T>(s[0][2], s[0][3]));
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const int mid = lane >> 3, r = w0 + (mid >> 1) * 8 + (lane & 7), c = 2 * i + (mid & 1);
+            unsigned a[4];
+            ap_ldsm_t(a, vt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
+            ap_mma<T>(o[i], a, b0, b1);
+        }
+        if (tid < KT) off_s[(t + ST) % RING][tid] = next;
+    }
+    ap_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(SB_FULL, l[h], x);
+    float *ow = reinterpret_cast<float *>(sm);  // [4 warps][8 rows][HDP]
+    __shared__ float ms[4][8], ls[4][8];
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = 2 * q4 + h;
+        if (g == 0) {
+            ms[warp][r] = m[h];
+            ls[warp][r] = l[h];
+        }
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            ow[(warp * 8 + r) * HDP + i * 16 + g] = o[i][h];
+            ow[(warp * 8 + r) * HDP + i * 16 + g + 8] = o[i][2 + h];
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < 8 * HDP / 2; i += SB_AP_THREADS) {
+        const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
+        if (f >= it.F) break;
+        float M = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), L = 0.f, a = 0.f, b = 0.f;
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float e = ap_exp2(ms[w][r] - base);
+            const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 8 + r) * HDP + d);
+            L += e * ls[w][r];
+            a += e * x.x;
+            b += e * x.y;
+        }
+        if (d == 0) ap_row_stats(P, it, f, M, L);
+        ap_row_out<T>(P, it, f, d, a, b, L);
+    }
+}
+
 // ---------------------------------------------------------------- FP32
 // MT rows against tiles of KT keys, 128 threads.  Scores: a thread takes a
 // key and 32 of its dimensions (DS threads a key, partial sums joined in
@@ -384,13 +556,12 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
 template <int HDP, int MT>
 SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
     constexpr int KT = HDP == 64 ? 64 : 32, DS = SB_AP_THREADS / KT, C = HDP / 4, KG = SB_AP_THREADS / C;
-    constexpr int TILE = KT * HDP * 4, STAGE = 2 * TILE, ST = MT >= 16 ? 2 : 3, RING = ST + 1, RW = (MT + 3) / 4;
+    constexpr int TILE = KT * HDP * 4, STAGE = 2 * TILE, ST = MT >= 16 ? 2 : 3, RING = SB_AP_RING, RW = (MT + 3) / 4;
     __shared__ __align__(16) float q_s[MT][HDP], part[DS][MT][KT], p_s[KT][MT < 4 ? 4 : MT];
     __shared__ float alpha_s[MT], m_s[MT], l_s[MT];
     __shared__ int vis_s[MT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const float *kb = static_cast<const float *>(it.pg.k) + it.kvh * it.pg.head_stride;
-    const float *vb = static_cast<const float *>(it.pg.v) + it.kvh * it.pg.head_stride;
+    const ApCopy<KT, HDP, 4> copier(it, P.HD);
     __syncthreads();  // an earlier item's shared memory is no longer read
     for (int i = tid; i < MT * HDP; i += SB_AP_THREADS) {
         const int r = i / HDP, d = i % HDP, f = it.f0 + r;
@@ -402,17 +573,8 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
     auto load = [&](int t) {
         if (t < nt) {
-            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE, vd = kd + TILE;
-            const long long *off = off_s[t % RING];
-#pragma unroll
-            for (int j = 0; j < KT * C / SB_AP_THREADS; j++) {
-                const int i = tid + j * SB_AP_THREADS, r = i / C, c = i % C;
-                const long long o = off[r];
-                const bool ok = o >= 0 && c * 4 < P.HD;
-                const unsigned d = r * (HDP * 4) + ((c ^ (r & 7)) << 4);
-                ap_cp16(kd + d, ok ? kb + o + c * 4 : kb, ok);
-                ap_cp16(vd + d, ok ? vb + o + c * 4 : vb, ok);
-            }
+            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE;
+            copier.copy(kd, kd + TILE, off_s[t % RING]);
         }
         ap_commit();
     };
@@ -435,7 +597,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
         ap_wait<ST - 2>();
         __syncthreads();
         load(t + ST - 1);
-        long long next = -1;
+        long long next = 0;
         if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
         const unsigned char *kt = sm + (t % ST) * STAGE, *vt = kt + TILE;
         const long long *off = off_s[t % RING];
@@ -466,7 +628,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
                     float v = 0.f;
 #pragma unroll
                     for (int e = 0; e < DS; e++) v += part[e][r][kk];
-                    s[j] = it.k0 + t * KT + kk < vis_s[r] && off[kk] >= 0 ? v * P.scale_log2 : -INFINITY;
+                    s[j] = it.k0 + t * KT + kk < vis_s[r] && (off[kk] & 1) ? v * P.scale_log2 : -INFINITY;
                     mx = fmaxf(mx, s[j]);
                 }
                 mx = warp_max(mx);
@@ -543,7 +705,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 // which waits for the own kernel, has both behind it.
 #define SB_AP_BODY(MT, CALL)                                                                \
     extern __shared__ __align__(128) unsigned char ap_sm[];                                 \
-    __shared__ long long off_s[SB_AP_STAGES + 1][64];                                       \
+    __shared__ long long off_s[SB_AP_RING][64];                                       \
     pdl_launch_dependents();                                                                \
     AttnItem it;                                                                            \
     if (!own) {                                                                             \
@@ -554,14 +716,22 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             for (it.f0 = tile * MT; it.f0 < it.F; it.f0 += P.tiles * MT) CALL;              \
         pdl_wait();                                                                         \
     }
+#define SB_AP_MMA8(name, T, HDP)                                                                               \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, 4) name(const __grid_constant__ AttnParams P, int own) { \
+        SB_AP_BODY(8, (attn_mma8_body<T, HDP>(P, it, ap_sm, off_s)))                                           \
+    }
 #define SB_AP_MMA(name, T, HDP, MW)                                                                            \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS) name(const __grid_constant__ AttnParams P, int own) { \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, HDP == 128 ? 2 : 3) name(const __grid_constant__ AttnParams P, int own) { \
         SB_AP_BODY(16 * MW, (attn_mma_body<T, HDP, MW>(P, it, ap_sm, off_s)))                                  \
     }
 #define SB_AP_F32(name, HDP, MT)                                                                               \
     extern "C" __global__ void __launch_bounds__(SB_AP_THREADS) name(const __grid_constant__ AttnParams P, int own) { \
         SB_AP_BODY(MT, (attn_f32_body<HDP, MT>(P, it, ap_sm, off_s)))                                          \
     }
+SB_AP_MMA8(attn_f16_64_r8, __half, 64)
+SB_AP_MMA8(attn_f16_128_r8, __half, 128)
+SB_AP_MMA8(attn_bf16_64_r8, __nv_bfloat16, 64)
+SB_AP_MMA8(attn_bf16_128_r8, __nv_bfloat16, 128)
 SB_AP_MMA(attn_f16_64_r16, __half, 64, 1)
 SB_AP_MMA(attn_f16_64_r64, __half, 64, 4)
 SB_AP_MMA(attn_f16_128_r16, __half, 128, 1)

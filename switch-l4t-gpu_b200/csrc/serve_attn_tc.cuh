@@ -301,15 +301,15 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             for (int h = 0; h < 2; h++) {
                 const long long off = ap_offset(it, key + h * 32 + lane);
                 if (is_k) {
-                    const unsigned valid = __ballot_sync(SB_FULL, off >= 0);
+                    const unsigned valid = __ballot_sync(SB_FULL, off & 1);
                     if (lane == 0) valid_s[t % (2 * ST)][(warp & 1) * 2 + h] = valid;
                 }
 #pragma unroll 4
                 for (int i = 0; i < CH; i++) {
                     const int r = i * RPI + rsub;
                     const long long o = __shfl_sync(SB_FULL, off, r);
-                    const bool there = o >= 0 && cok;
-                    ap_cp16(stage + (c >> 3) * 16384 + (p0 + h * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), there ? col + o : base, there);
+                    const bool there = (o & 1) && cok;
+                    ap_cp16(stage + (c >> 3) * 16384 + (p0 + h * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), col + (o & ~1ll), there);
                 }
             }
             ap_commit();

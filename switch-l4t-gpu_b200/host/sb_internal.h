@@ -91,6 +91,10 @@ typedef enum {
     F_ROTARY_F32_ANY,
     F_ROTARY_F16_ANY,
     F_ROTARY_BF16_ANY,
+    F_ATTN_F16_64_R8,
+    F_ATTN_F16_128_R8,
+    F_ATTN_BF16_64_R8,
+    F_ATTN_BF16_128_R8,
     F_ATTN_F16_64_R16,
     F_ATTN_F16_64_R64,
     F_ATTN_F16_128_R16,

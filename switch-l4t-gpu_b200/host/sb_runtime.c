@@ -113,6 +113,10 @@ static const struct {
     [F_ROTARY_F32_ANY] = {M_SERVE, "rotary_f32_any"},
     [F_ROTARY_F16_ANY] = {M_SERVE, "rotary_f16_any"},
     [F_ROTARY_BF16_ANY] = {M_SERVE, "rotary_bf16_any"},
+    [F_ATTN_F16_64_R8] = {M_SERVE, "attn_f16_64_r8"},
+    [F_ATTN_F16_128_R8] = {M_SERVE, "attn_f16_128_r8"},
+    [F_ATTN_BF16_64_R8] = {M_SERVE, "attn_bf16_64_r8"},
+    [F_ATTN_BF16_128_R8] = {M_SERVE, "attn_bf16_128_r8"},
     [F_ATTN_F16_64_R16] = {M_SERVE, "attn_f16_64_r16"},
     [F_ATTN_F16_64_R64] = {M_SERVE, "attn_f16_64_r64"},
     [F_ATTN_F16_128_R16] = {M_SERVE, "attn_f16_128_r16"},

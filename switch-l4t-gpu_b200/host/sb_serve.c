@@ -234,9 +234,9 @@ struct attn_part {
 
 /* The kernel for `rows` query rows of a key head.  FP32: row tiles of 1, 2,
  * 4, 8 or 16, the smallest that holds them (unused rows cost FMAs).  16-bit
- * types: 16-row tiles (the four warps split the keys) while one holds all
- * rows, 64-row tiles up to SB_ATTN_TC_ROWS, and for a prefix behind more rows
- * the tcgen05 kernel's 256. */
+ * types: a tile of 8 or 16 rows (the four warps split the keys) while it holds
+ * all rows, 64-row tiles up to SB_ATTN_TC_ROWS, and for a prefix behind more
+ * rows the tcgen05 kernel's 256. */
 static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_part *a) {
     const int wide = HD > 64, second = type == SB_BF16;
     a->threads = 128;
@@ -255,9 +255,10 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
         a->step = 128;
     } else {
         const int big = rows > 16;
-        a->f = (sb_fn_id)((second ? F_ATTN_BF16_64_R16 : F_ATTN_F16_64_R16) + 2 * wide + big);
-        a->smem = 3 * 2 * 64 * (wide ? 128 : 64) * 2;
-        a->rows = big ? 64 : 16;
+        a->f = rows <= 8 ? (sb_fn_id)(F_ATTN_F16_64_R8 + 2 * second + wide)
+                         : (sb_fn_id)((second ? F_ATTN_BF16_64_R16 : F_ATTN_F16_64_R16) + 2 * wide + big);
+        a->smem = 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64); /* SB_AP_ST stages of K and V */
+        a->rows = rows <= 8 ? 8 : big ? 64 : 16;
         a->step = 64;
     }
     a->tiles = (int)CEIL_DIV(rows, a->rows);
