@@ -14,10 +14,9 @@
 // cp.async ring of two or three stages, positions going through the block table (an
 // offset per key, computed a tile ahead; a position without a page, or past
 // the range, is filled with zeros and masked, so nothing of it is read):
-//   attn_mma8_body f16 / bf16, mma.sync m16n8k16, up to eight rows (the head
+//   attn_mmaw_body f16 / bf16, mma.sync m16n8k16, up to 8 or 16 rows (the head
 //                  group of a decode step) against long own pages: memory-bound
-//   attn_mma_body  the same for 16-row tiles (four warps split the keys) or
-//                  64-row tiles (a warp 16 rows)
+//   attn_mma_body  64-row tiles, a warp 16 rows
 //   attn_f32_body  FP32 on the CUDA cores: 1..16-row tiles, a thread a key
 // Scores, maxima, sums and outputs are FP32; the softmax weights are rounded
 // to the value type for the second tensor-core product (half a step, like
@@ -161,6 +160,47 @@ template <int KT, int HDP, int E> struct ApCopy {
     }
 };
 
+// The same for a warp that reads its keys alone: KW positions of a tile, K and V
+// each a group of their own, in a ring of ST tiles a warp.  The block never
+// meets: a tile of K is asked for as soon as the warp has its scores, one of V
+// as soon as it has its outputs, so nearly 2 ST groups are always in flight.
+template <int KW, int HDP, int E, int ST> struct ApWarpCopy {
+    static constexpr int C = HDP * E / 16, STEP = 32 / C, N = KW / STEP, TILE = KW * HDP * E, RING = 8;
+    static_assert(ST + 2 <= RING, "offsets of the tiles in flight");
+    const char *k, *v;
+    unsigned sm;         // this warp's ring: K tiles, then V tiles
+    long long *off;      // [RING][KW]
+    int row, c;
+    bool in;
+    SB_DEV ApWarpCopy(const AttnItem &it, int HD, unsigned char *ring, long long *offsets) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        c = lane % C;
+        row = lane / C;
+        k = static_cast<const char *>(it.pg.k) + it.kvh * it.pg.head_stride * E + c * 16;
+        v = static_cast<const char *>(it.pg.v) + it.kvh * it.pg.head_stride * E + c * 16;
+        sm = ap_smem(ring) + warp * (2 * ST * TILE);
+        off = offsets + warp * (RING * KW);
+        in = c * 16 < HD * E;
+    }
+    SB_DEV unsigned k_tile(int t) const { return sm + (t % ST) * TILE; }
+    SB_DEV unsigned v_tile(int t) const { return sm + (ST + t % ST) * TILE; }
+    SB_DEV const long long *offs(int t) const { return off + (t % RING) * KW; }
+    SB_DEV void copy(unsigned dst, const char *base, int t, bool live) const {
+        if (live) {
+            const long long *o = offs(t);
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                const int r = row + j * STEP;
+                const long long w = o[r];
+                ap_cp16(dst + r * (HDP * E) + ((c ^ (r & 7)) << 4), base + (w & ~1ll) * E, (w & 1) && in);
+            }
+        }
+        ap_commit();
+    }
+    SB_DEV void copy_k(int t, bool live) const { copy(k_tile(t), k, t, live); }
+    SB_DEV void copy_v(int t, bool live) const { copy(v_tile(t), v, t, live); }
+};
+
 // what a finished row leaves: the output itself where the item is the only one, else its part
 SB_DEV void ap_row_stats(const AttnParams &P, const AttnItem &it, int f, float m, float l) {
     const int row = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
@@ -224,18 +264,16 @@ SB_DEV float ap_exp2(float x) {
     return y;
 }
 
-// HDP: head size padded to 64 or 128.  MW: warps along the rows (1: 16-row
-// tile, warps split the 64 keys of a tile; 4: 64-row tile).
-// Shared memory: SB_AP_ST x 2 x 64 x HDP x 2 bytes (>= the 4 x 16 x HDP
-// floats of the final join over warps), rows of 128 / 256 bytes with their
-// 16-byte chunks xor-ed by the row's low three bits (ldmatrix reads eight
-// rows of one chunk without a conflict).
-template <typename T, int HDP, int MW>
+// 64-row tiles, a warp 16 rows against all keys.  HDP: head size padded to 64
+// or 128.  Shared memory: SB_AP_ST x 2 x 64 x HDP x 2 bytes, rows of 128 / 256
+// bytes with their 16-byte chunks xor-ed by the row's low three bits (ldmatrix
+// reads eight rows of one chunk without a conflict).
+template <typename T, int HDP>
 SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
-    constexpr int KT = 64, WK = MW == 1 ? 16 : 64, NT = WK / 8, KS = HDP / 16, ST = SB_AP_ST(HDP);
+    constexpr int KT = 64, NT = KT / 8, KS = HDP / 16, ST = SB_AP_ST(HDP);
     constexpr int TILE = KT * HDP * 2, STAGE = 2 * TILE, RING = SB_AP_RING;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    const int fw = it.f0 + (MW == 1 ? 0 : warp * 16);  // this warp's first row
+    const int fw = it.f0 + warp * 16;  // this warp's first row
     const ApCopy<KT, HDP, 2> copier(it, P.HD);
 
     // query fragments from global memory: rows fw + g and fw + g + 8
@@ -255,7 +293,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
             }
     }
     // keys that some row of the tile sees end here; a tile of keys below every row's limit needs no mask
-    const int flast = min(it.f0 + 16 * MW, it.F) - 1;
+    const int flast = min(it.f0 + 64, it.F) - 1;
     const int k1 = min(it.k1, ap_vis(it, flast, P.G));
     const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
 
@@ -284,7 +322,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
         if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
         const unsigned kt = ap_smem(sm) + (t % ST) * STAGE, vt = kt + TILE;
         const long long *off = off_s[t % RING];
-        const int w0 = MW == 1 ? warp * 16 : 0, key0 = it.k0 + t * KT + w0;
+        const int key0 = it.k0 + t * KT;
         float s[NT][4];
 #pragma unroll
         for (int i = 0; i < NT; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
@@ -293,7 +331,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int n = 0; n < NT / 2; n++) {
-                const int r = w0 + n * 16 + r8 + (mid >> 1) * 8, c = k * 2 + (mid & 1);
+                const int r = n * 16 + r8 + (mid >> 1) * 8, c = k * 2 + (mid & 1);
                 unsigned b[4];
                 ap_ldsm(b, kt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
                 ap_mma<T>(s[2 * n], qa[k], b[0], b[1]);
@@ -306,7 +344,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int j = n * 8 + q4 * 2 + (e & 1);
-                const bool seen = key0 + j < vis[e >> 1] && (off[w0 + j] & 1);
+                const bool seen = key0 + j < vis[e >> 1] && (off[j] & 1);
                 s[n][e] = seen ? s[n][e] * P.scale_log2 : -INFINITY;
                 mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
             }
@@ -338,7 +376,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
                                    ap_pack<T>(s[2 * n + 1][0], s[2 * n + 1][1]), ap_pack<T>(s[2 * n + 1][2], s[2 * n + 1][3])};
 #pragma unroll
             for (int i = 0; i < HDP / 16; i++) {
-                const int r = w0 + n * 16 + r8 + (mid & 1) * 8, c = i * 2 + (mid >> 1);
+                const int r = n * 16 + r8 + (mid & 1) * 8, c = i * 2 + (mid >> 1);
                 unsigned b[4];
                 ap_ldsm_t(b, vt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
                 ap_mma<T>(o[2 * i], a, b[0], b[1]);
@@ -353,179 +391,168 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
         l[h] += __shfl_xor_sync(SB_FULL, l[h], 1);
         l[h] += __shfl_xor_sync(SB_FULL, l[h], 2);
     }
-    if constexpr (MW == 4) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int f = fw + g + 8 * h;
-            if (f >= it.F) continue;
-            if (q4 == 0) ap_row_stats(P, it, f, m[h], l[h]);
+    for (int h = 0; h < 2; h++) {
+        const int f = fw + g + 8 * h;
+        if (f >= it.F) continue;
+        if (q4 == 0) ap_row_stats(P, it, f, m[h], l[h]);
 #pragma unroll
-            for (int i = 0; i < HDP / 8; i++) ap_row_out<T>(P, it, f, i * 8 + q4 * 2, o[i][2 * h], o[i][2 * h + 1], l[h]);
-        }
-    } else {  // the four warps' keys join
-        float *ow = reinterpret_cast<float *>(sm);                     // [4][16][HDP]
-        __shared__ float ms[4][16], ls[4][16];
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = g + 8 * h;
-            if (q4 == 0) {
-                ms[warp][r] = m[h];
-                ls[warp][r] = l[h];
-            }
-#pragma unroll
-            for (int i = 0; i < HDP / 8; i++)
-                *reinterpret_cast<float2 *>(ow + (warp * 16 + r) * HDP + i * 8 + q4 * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-        }
-        __syncthreads();
-        for (int i = tid; i < 16 * HDP / 2; i += SB_AP_THREADS) {
-            const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
-            if (f >= it.F) break;
-            float M = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), L = 0.f, a = 0.f, b = 0.f;
-            const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float e = ap_exp2(ms[w][r] - base);
-                const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 16 + r) * HDP + d);
-                L += e * ls[w][r];
-                a += e * x.x;
-                b += e * x.y;
-            }
-            if (d == 0) ap_row_stats(P, it, f, M, L);
-            ap_row_out<T>(P, it, f, d, a, b, L);
-        }
+        for (int i = 0; i < HDP / 8; i++) ap_row_out<T>(P, it, f, i * 8 + q4 * 2, o[i][2 * h], o[i][2 * h + 1], l[h]);
     }
 }
 
-// Up to eight rows against their own keys, the products the other way round:
-// S^T = K Q^T (keys along m, rows along n = 8) and O^T = V^T P^T.  Nothing is
-// spent on rows that are not there (a group of 4 or 7 heads filled a quarter
-// or half of 16), and the outputs take half the registers.  P^T turns from
-// accumulator into operand by movmatrix.  The four warps split the 64 keys of
-// a tile.  Like the tcgen05 kernel it rescales only when a row's maximum has
-// grown by more than 2^8; a tile without that costs one vote.
+// Up to 8 NB rows, a warp a quarter of the keys of every 64, the products with
+// the keys along m: S^T = K Q^T (rows along n = 8) and O^T = V^T P^T.  Nothing
+// is spent on rows that are not there (a group of 4 or 7 heads filled a
+// quarter or half of a 16-row tile), and the outputs take half the registers.
+// P^T turns from accumulator into operand by movmatrix.  Like the tcgen05
+// kernel it rescales only when a row's maximum has grown by more than 2^8; a
+// tile without that costs one vote.
 SB_DEV unsigned ap_movmatrix(unsigned a) {
     unsigned d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
-template <typename T, int HDP>
-SB_DEV void attn_mma8_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
-    constexpr int KT = 64, KS = HDP / 16, ST = SB_AP_ST(HDP), TILE = KT * HDP * 2, STAGE = 2 * TILE, RING = SB_AP_RING;
+template <typename T, int HDP, int NB>
+SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long *off_s) {
+    constexpr int KS = HDP / 16, ST = HDP == 128 ? 2 : 4;
+    using Copy = ApWarpCopy<16, HDP, 2, ST>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    const ApCopy<KT, HDP, 2> copier(it, P.HD);
-    unsigned qb[KS][2];  // row f0 + g
-    int vis[2];          // of rows f0 + 2 q4, + 1
-    {
-        const int f = it.f0 + g;
+    const Copy cp(it, P.HD, sm, off_s);
+    unsigned qb[NB][KS][2];  // rows f0 + 8 b + g
+    int vis[NB][2];          // of rows f0 + 8 b + 2 q4, + 1
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int f = it.f0 + b * 8 + g;
         const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const int d = k * 16 + e * 8 + q4 * 2;
-                qb[k][e] = f < it.F && d < P.HD ? *reinterpret_cast<const unsigned *>(qp + d) : 0u;
+                qb[b][k][e] = f < it.F && d < P.HD ? *reinterpret_cast<const unsigned *>(qp + d) : 0u;
             }
 #pragma unroll
-        for (int h = 0; h < 2; h++) vis[h] = it.f0 + 2 * q4 + h < it.F ? ap_vis(it, it.f0 + 2 * q4 + h, P.G) : 0;
-    }
-    const int flast = min(it.f0 + 8, it.F) - 1;
-    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
-    const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
-    auto load = [&](int t) {
-        if (t < nt) {
-            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE;
-            copier.copy(kd, kd + TILE, off_s[t % RING]);
+        for (int h = 0; h < 2; h++) {
+            const int fh = it.f0 + b * 8 + 2 * q4 + h;
+            vis[b][h] = fh < it.F ? ap_vis(it, fh, P.G) : 0;
         }
-        ap_commit();
-    };
-    float o[KS][4];
+    }
+    const int flast = min(it.f0 + 8 * NB, it.F) - 1, first = it.k0 + warp * 16;
+    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
+    const int nt = k1 > first ? (k1 - first + 63) / 64 : 0;  // this warp's tiles: 16 keys of every 64
+    float o[NB][KS][4], m[NB][2], l[NB][2];
 #pragma unroll
-    for (int i = 0; i < KS; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    __syncthreads();  // the ring and the offsets of an earlier item are no longer read
-    for (int t = 0; t < ST; t++)
-        if (tid < KT) off_s[t][tid] = ap_offset(it, it.k0 + t * KT + tid);
-    __syncthreads();
-    for (int t = 0; t < ST - 1; t++) load(t);
-    const int w0 = warp * 16;
+    for (int b = 0; b < NB; b++) {
+#pragma unroll
+        for (int i = 0; i < KS; i++) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.f;
+        m[b][0] = m[b][1] = -INFINITY;
+        l[b][0] = l[b][1] = 0.f;
+    }
+    __syncthreads();  // an earlier item's join has been read
+    for (int t = lane / 16; t <= ST; t += 2) cp.off[(t % Copy::RING) * 16 + lane % 16] = ap_offset(it, first + t * 64 + lane % 16);
+    __syncwarp();
+    for (int t = 0; t < ST; t++) {
+        cp.copy_k(t, t < nt);
+        cp.copy_v(t, t < nt);
+    }
     for (int t = 0; t < nt; t++) {
-        ap_wait<ST - 2>();
-        __syncthreads();  // tile t is there for all; tile t - 1 and its offsets are read
-        load(t + ST - 1);
-        long long next = 0;
-        if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
-        const unsigned kt = ap_smem(sm) + (t % ST) * STAGE, vt = kt + TILE;
-        const long long *off = off_s[t % RING];
-        const int key = it.k0 + t * KT + w0 + g;
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // two chains
+        long long next = 0;  // the offsets of tile t + ST + 1, a tile ahead of their use
+        if (lane < 16) next = ap_offset(it, first + (t + ST + 1) * 64 + lane);
+        const unsigned kt = cp.k_tile(t), vt = cp.v_tile(t);
+        const int key = first + t * 64 + g;
+        ap_wait<2 * ST - 1>();
+        __syncwarp();
+        const bool there0 = cp.offs(t)[g] & 1, there1 = cp.offs(t)[g + 8] & 1;
+        float s[NB][4];
+#pragma unroll
+        for (int b = 0; b < NB; b++) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const int r = w0 + (lane & 15), c = 2 * k + (lane >> 4);
+            const int r = lane & 15, c = 2 * k + (lane >> 4);
             unsigned a[4];
             ap_ldsm(a, kt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
-            ap_mma<T>(s[k & 1], a, qb[k][0], qb[k][1]);
+#pragma unroll
+            for (int b = 0; b < NB; b++) ap_mma<T>(s[b], a, qb[b][k][0], qb[b][k][1]);
         }
-        const bool there0 = off[w0 + g] & 1, there1 = off[w0 + g + 8] & 1;
+        __syncwarp();
+        cp.copy_k(t + ST, t + ST < nt);
+        bool grown = false;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {  // key g + 8 (e >> 1), row 2 q4 + (e & 1)
-            const bool seen = ((e >> 1) ? there1 : there0) && key + 8 * (e >> 1) < vis[e & 1];
-            s[0][e] = seen ? (s[0][e] + s[1][e]) * P.scale_log2 : -INFINITY;
-        }
-        float mx[2] = {fmaxf(s[0][0], s[0][2]), fmaxf(s[0][1], s[0][3])};
-        if (__any_sync(SB_FULL, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(SB_FULL, mx[h], x));
-                const float to = fmaxf(m[h], mx[h]), a = to == m[h] ? 1.f : ap_exp2(m[h] - to);
-                m[h] = to;
-                l[h] *= a;
-#pragma unroll
-                for (int i = 0; i < KS; i++) {
-                    o[i][h] *= a;
-                    o[i][2 + h] *= a;
-                }
+            for (int e = 0; e < 4; e++) {  // key g + 8 (e >> 1), row 2 q4 + (e & 1)
+                const bool seen = ((e >> 1) ? there1 : there0) && key + 8 * (e >> 1) < vis[b][e & 1];
+                s[b][e] = seen ? s[b][e] * P.scale_log2 : -INFINITY;
+                grown |= s[b][e] > m[b][e & 1] + 8.f;
             }
-        }
+        if (__any_sync(SB_FULL, grown)) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            s[0][e] = ap_exp2(s[0][e] - (m[e & 1] == -INFINITY ? 0.f : m[e & 1]));
-            l[e & 1] += s[0][e];
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float mx = fmaxf(s[b][h], s[b][2 + h]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(SB_FULL, mx, x));
+                    const float to = fmaxf(m[b][h], mx), a = to == m[b][h] ? 1.f : ap_exp2(m[b][h] - to);
+                    m[b][h] = to;
+                    l[b][h] *= a;
+#pragma unroll
+                    for (int i = 0; i < KS; i++) {
+                        o[b][i][h] *= a;
+                        o[b][i][2 + h] *= a;
+                    }
+                }
         }
-        const unsigned b0 = ap_movmatrix(ap_pack<T>(s[0][0], s[0][1])), b1 = ap_movmatrix(ap_pack<T>(s[0][2], s[0][3]));
+        unsigned p[NB][2];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[b][e] = ap_exp2(s[b][e] - (m[b][e & 1] == -INFINITY ? 0.f : m[b][e & 1]));
+                l[b][e & 1] += s[b][e];
+            }
+            p[b][0] = ap_movmatrix(ap_pack<T>(s[b][0], s[b][1]));
+            p[b][1] = ap_movmatrix(ap_pack<T>(s[b][2], s[b][3]));
+        }
+        ap_wait<2 * ST - 1>();
+        __syncwarp();
 #pragma unroll
         for (int i = 0; i < KS; i++) {
-            const int mid = lane >> 3, r = w0 + (mid >> 1) * 8 + (lane & 7), c = 2 * i + (mid & 1);
+            const int mid = lane >> 3, r = (mid >> 1) * 8 + (lane & 7), c = 2 * i + (mid & 1);
             unsigned a[4];
             ap_ldsm_t(a, vt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
-            ap_mma<T>(o[i], a, b0, b1);
+#pragma unroll
+            for (int b = 0; b < NB; b++) ap_mma<T>(o[b][i], a, p[b][0], p[b][1]);
         }
-        if (tid < KT) off_s[(t + ST) % RING][tid] = next;
+        __syncwarp();
+        cp.copy_v(t + ST, t + ST < nt);
+        if (lane < 16) cp.off[((t + ST + 1) % Copy::RING) * 16 + lane] = next;
+        __syncwarp();
     }
     ap_wait<0>();
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l[h] += __shfl_xor_sync(SB_FULL, l[h], x);
-    float *ow = reinterpret_cast<float *>(sm);  // [4 warps][8 rows][HDP]
-    __shared__ float ms[4][8], ls[4][8];
+    float *ow = reinterpret_cast<float *>(sm);  // [4 warps][8 NB rows][HDP]
+    __shared__ float ms[4][8 * NB], ls[4][8 * NB];
     __syncthreads();
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int r = 2 * q4 + h;
-        if (g == 0) {
-            ms[warp][r] = m[h];
-            ls[warp][r] = l[h];
-        }
+    for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            ow[(warp * 8 + r) * HDP + i * 16 + g] = o[i][h];
-            ow[(warp * 8 + r) * HDP + i * 16 + g + 8] = o[i][2 + h];
+        for (int h = 0; h < 2; h++) {
+            const int r = b * 8 + 2 * q4 + h;
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[b][h] += __shfl_xor_sync(SB_FULL, l[b][h], x);
+            if (g == 0) {
+                ms[warp][r] = m[b][h];
+                ls[warp][r] = l[b][h];
+            }
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                ow[(warp * 8 * NB + r) * HDP + i * 16 + g] = o[b][i][h];
+                ow[(warp * 8 * NB + r) * HDP + i * 16 + g + 8] = o[b][i][2 + h];
+            }
         }
-    }
     __syncthreads();
-    for (int i = tid; i < 8 * HDP / 2; i += SB_AP_THREADS) {
+    for (int i = tid; i < 8 * NB * HDP / 2; i += SB_AP_THREADS) {
         const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
         if (f >= it.F) break;
         float M = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), L = 0.f, a = 0.f, b = 0.f;
@@ -533,7 +560,7 @@ SB_DEV void attn_mma8_body(const AttnParams &P, const AttnItem &it, unsigned cha
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float e = ap_exp2(ms[w][r] - base);
-            const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 8 + r) * HDP + d);
+            const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 8 * NB + r) * HDP + d);
             L += e * ls[w][r];
             a += e * x.x;
             b += e * x.y;
@@ -544,158 +571,164 @@ SB_DEV void attn_mma8_body(const AttnParams &P, const AttnItem &it, unsigned cha
 }
 
 // ---------------------------------------------------------------- FP32
-// MT rows against tiles of KT keys, 128 threads.  Scores: a thread takes a
-// key and 32 of its dimensions (DS threads a key, partial sums joined in
-// shared memory); K chunks are xor-swizzled so that 8 lanes reading 8 keys
-// touch all banks, query values are broadcast.  Weights: a warp a row.
-// Output: a thread owns four dimensions of all MT rows for every KG-th key;
-// the KG groups join at the end.  FFMA and not the tensor pipe: its FP32
-// sums are not IEEE-rounded and drift by 1e-5 over some thousand keys.
-// Sixteen rows are bound by the FMA pipe and take a two-stage ring, which
-// leaves room for a second CTA.
+// MT rows, a warp a quarter of the keys of every KT from the scores to the
+// outputs (the block meets only for the join).  Scores: a lane takes a key and 32 of its dimensions; K chunks are
+// xor-swizzled so that eight lanes reading eight keys touch all banks, query
+// values are broadcast (the DQ parts of a row 36 floats apart, on banks of
+// their own).  Outputs: a lane owns HDP / 32 dimensions of all rows, the
+// weights come as pairs from shared memory for two-wide FMAs.  Rows rescale
+// when their maximum has grown by more than 2^8, as in the other kernels.
+// Bound: HBM up to eight rows (46 of the 24 bytes per SM and cycle that HBM
+// gives at MT = 8), the shared-memory and FMA pipes beyond.  FFMA and not the
+// tensor pipe: its FP32 sums are not IEEE-rounded and drift by 1e-5 over some
+// thousand keys.
 template <int HDP, int MT>
-SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long (*off_s)[64]) {
-    constexpr int KT = HDP == 64 ? 64 : 32, DS = SB_AP_THREADS / KT, C = HDP / 4, KG = SB_AP_THREADS / C;
-    constexpr int TILE = KT * HDP * 4, STAGE = 2 * TILE, ST = MT >= 16 ? 2 : 3, RING = SB_AP_RING, RW = (MT + 3) / 4;
-    __shared__ __align__(16) float q_s[MT][HDP], part[DS][MT][KT], p_s[KT][MT < 4 ? 4 : MT];
-    __shared__ float alpha_s[MT], m_s[MT], l_s[MT];
+SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long *off_s) {
+    constexpr int KT = HDP == 64 ? 64 : 32, KW = KT / 4, DQ = 32 / KW, DP = HDP / 64;  // keys a warp, parts of a key, pairs of a lane
+    constexpr int ST = 2;
+    using Copy = ApWarpCopy<KW, HDP, 4, ST>;
+    __shared__ __align__(16) float q_s[MT][DQ][36];
+    __shared__ __align__(16) float2 p_s[4][KW][MT < 2 ? 2 : MT];
+    __shared__ float m_s[4][MT], l_s[4][MT];
     __shared__ int vis_s[MT];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const ApCopy<KT, HDP, 4> copier(it, P.HD);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = lane % KW, dq = lane / KW;
+    const Copy cp(it, P.HD, sm, off_s);
     __syncthreads();  // an earlier item's shared memory is no longer read
     for (int i = tid; i < MT * HDP; i += SB_AP_THREADS) {
         const int r = i / HDP, d = i % HDP, f = it.f0 + r;
-        q_s[r][d] = f < it.F && d < P.HD ? static_cast<const float *>(P.q)[(long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head + d] : 0.f;
+        q_s[r][d / 32][d % 32] = f < it.F && d < P.HD ? static_cast<const float *>(P.q)[(long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head + d] * P.scale_log2 : 0.f;
     }
     if (tid < MT) vis_s[tid] = it.f0 + tid < it.F ? ap_vis(it, it.f0 + tid, P.G) : 0;
     const int flast = min(it.f0 + MT, it.F) - 1;
-    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
-    const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
-    auto load = [&](int t) {
-        if (t < nt) {
-            const unsigned kd = ap_smem(sm) + (t % ST) * STAGE;
-            copier.copy(kd, kd + TILE, off_s[t % RING]);
-        }
-        ap_commit();
-    };
-    for (int t = 0; t < ST; t++)
-        if (tid < KT) off_s[t][tid] = ap_offset(it, it.k0 + t * KT + tid);
+    const int k1 = min(it.k1, ap_vis(it, flast, P.G)), vmin = ap_vis(it, it.f0, P.G);  // rows in order see more and more
+    const int first = it.k0 + warp * KW, nt = k1 > first ? (k1 - first + KT - 1) / KT : 0;  // this warp's KW keys of every KT
+    for (int t = lane / KW; t <= ST; t += 32 / KW) cp.off[(t % Copy::RING) * KW + key] = ap_offset(it, first + t * KT + key);
     __syncthreads();
-    for (int t = 0; t < ST - 1; t++) load(t);
-
-    const int key = tid % KT, ds = tid / KT, dc = tid % C, kg = tid / C;
-    unsigned long long o[MT][2];
+    for (int t = 0; t < ST; t++) {
+        cp.copy_k(t, t < nt);
+        cp.copy_v(t, t < nt);
+    }
+    unsigned long long o[MT][DP];
+    float m[MT], l[MT];
 #pragma unroll
-    for (int r = 0; r < MT; r++) o[r][0] = o[r][1] = 0ull;
-    float m[RW], l[RW];  // rows warp, warp + 4, ...
+    for (int r = 0; r < MT; r++) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
 #pragma unroll
-    for (int i = 0; i < RW; i++) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
+        for (int e = 0; e < DP; e++) o[r][e] = 0ull;
     }
     for (int t = 0; t < nt; t++) {
-        ap_wait<ST - 2>();
-        __syncthreads();
-        load(t + ST - 1);
-        long long next = 0;
-        if (tid < KT) next = ap_offset(it, it.k0 + (t + ST) * KT + tid);
-        const unsigned char *kt = sm + (t % ST) * STAGE, *vt = kt + TILE;
-        const long long *off = off_s[t % RING];
+        long long next = 0;  // the offsets of tile t + ST + 1, a tile ahead of their use
+        if (lane < KW) next = ap_offset(it, first + (t + ST + 1) * KT + lane);
+        const unsigned char *kt = sm + (cp.k_tile(t) - ap_smem(sm)), *vt = sm + (cp.v_tile(t) - ap_smem(sm));
+        ap_wait<2 * ST - 1>();
+        __syncwarp();
+        const bool there = cp.offs(t)[key] & 1;
         unsigned long long acc[MT];
 #pragma unroll
         for (int r = 0; r < MT; r++) acc[r] = 0ull;
 #pragma unroll
         for (int c = 0; c < 8; c++) {
-            const ulonglong2 k2 = *reinterpret_cast<const ulonglong2 *>(kt + key * (HDP * 4) + (((ds * 8 + c) ^ (key & 7)) << 4));
+            const ulonglong2 k2 = *reinterpret_cast<const ulonglong2 *>(kt + key * (HDP * 4) + (((dq * 8 + c) ^ (key & 7)) << 4));
 #pragma unroll
             for (int r = 0; r < MT; r++) {
-                const ulonglong2 q2 = *reinterpret_cast<const ulonglong2 *>(&q_s[r][(ds * 8 + c) * 4]);
+                const ulonglong2 q2 = *reinterpret_cast<const ulonglong2 *>(&q_s[r][dq][c * 4]);
                 acc[r] = ffma2(q2.x, k2.x, acc[r]);
                 acc[r] = ffma2(q2.y, k2.y, acc[r]);
             }
         }
-#pragma unroll
-        for (int r = 0; r < MT; r++) part[ds][r][key] = f2_sum(acc[r]);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < RW; i++) {
-            const int r = warp + 4 * i;
-            if (r < MT) {
-                float s[KT / 32], mx = m[i];
-#pragma unroll
-                for (int j = 0; j < KT / 32; j++) {
-                    const int kk = lane + 32 * j;
-                    float v = 0.f;
-#pragma unroll
-                    for (int e = 0; e < DS; e++) v += part[e][r][kk];
-                    s[j] = it.k0 + t * KT + kk < vis_s[r] && (off[kk] & 1) ? v * P.scale_log2 : -INFINITY;
-                    mx = fmaxf(mx, s[j]);
-                }
-                mx = warp_max(mx);
-                const float base = mx == -INFINITY ? 0.f : mx, a = ap_exp2(m[i] - base);
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < KT / 32; j++) {
-                    s[j] = ap_exp2(s[j] - base);
-                    sum += s[j];
-                    p_s[lane + 32 * j][r] = s[j];
-                }
-                l[i] = l[i] * a + sum;  // this lane's keys; the lanes join at the end
-                m[i] = mx;
-                if (lane == 0) alpha_s[r] = a;
-            }
-        }
-        __syncthreads();
+        __syncwarp();
+        cp.copy_k(t + ST, t + ST < nt);
+        float s[MT];
+        bool grown = false;
+        const int at = first + t * KT + key;
+        const bool all = there && at < vmin;
 #pragma unroll
         for (int r = 0; r < MT; r++) {
-            const float a = alpha_s[r];
-            const unsigned long long aa = f2_pack(a, a);
-            o[r][0] = ffma2(o[r][0], aa, 0ull);
-            o[r][1] = ffma2(o[r][1], aa, 0ull);
-        }
+            s[r] = f2_sum(acc[r]);
 #pragma unroll
-        for (int j = 0; j < KT / KG; j++) {
-            const int kk = kg + KG * j;
-            const ulonglong2 v2 = *reinterpret_cast<const ulonglong2 *>(vt + kk * (HDP * 4) + ((dc ^ (kk & 7)) << 4));
+            for (int x = KW; x < 32; x <<= 1) s[r] += __shfl_xor_sync(SB_FULL, s[r], x);
+            if (!all && !(there && at < vis_s[r])) s[r] = -INFINITY;
+            grown |= s[r] > m[r] + 8.f;
+        }
+        if (__any_sync(SB_FULL, grown)) {
 #pragma unroll
             for (int r = 0; r < MT; r++) {
-                const float p = p_s[kk][r];
-                const unsigned long long pp = f2_pack(p, p);
-                o[r][0] = ffma2(pp, v2.x, o[r][0]);
-                o[r][1] = ffma2(pp, v2.y, o[r][1]);
+                const float to = fmaxf(m[r], warp_max(s[r])), a = to == m[r] ? 1.f : ap_exp2(m[r] - to);
+                m[r] = to;
+                l[r] *= a;
+#pragma unroll
+                for (int e = 0; e < DP; e++) o[r][e] = ffma2(o[r][e], f2_pack(a, a), 0ull);
             }
         }
-        if (tid < KT) off_s[(t + ST) % RING][tid] = next;
+#pragma unroll
+        for (int r = 0; r < MT; r++) {
+            s[r] = ap_exp2(s[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] += s[r];
+            if (r % DQ == dq) p_s[warp][key][r] = make_float2(s[r], s[r]);
+        }
+        ap_wait<2 * ST - 1>();
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < KW; k++) {
+                        unsigned long long v[DP];
+            if constexpr (DP == 1) {
+                v[0] = *reinterpret_cast<const unsigned long long *>(vt + k * (HDP * 4) + (((lane >> 1) ^ (k & 7)) << 4) + (lane & 1) * 8);
+            } else {
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(vt + k * (HDP * 4) + ((lane ^ (k & 7)) << 4));
+                v[0] = w.x;
+                v[DP - 1] = w.y;
+            }
+            if constexpr (MT == 1) {
+                const unsigned long long p = *reinterpret_cast<const unsigned long long *>(&p_s[warp][k][0]);
+#pragma unroll
+                for (int e = 0; e < DP; e++) o[0][e] = ffma2(p, v[e], o[0][e]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < MT; r += 2) {
+                    const ulonglong2 p = *reinterpret_cast<const ulonglong2 *>(&p_s[warp][k][r]);
+#pragma unroll
+                    for (int e = 0; e < DP; e++) {
+                        o[r][e] = ffma2(p.x, v[e], o[r][e]);
+                        o[r + (MT > 1)][e] = ffma2(p.y, v[e], o[r + (MT > 1)][e]);
+                    }
+                }
+            }
+        }
+        __syncwarp();  // values and weights are read
+        cp.copy_v(t + ST, t + ST < nt);
+        if (lane < KW) cp.off[((t + ST + 1) % Copy::RING) * KW + lane] = next;
+        __syncwarp();
     }
     ap_wait<0>();
-#pragma unroll
-    for (int i = 0; i < RW; i++) {
-        const int r = warp + 4 * i;
-        if (r < MT) {
-            l[i] = warp_sum(l[i]);
-            if (lane == 0) {
-                m_s[r] = m[i];
-                l_s[r] = l[i];
-            }
-        }
-    }
     __syncthreads();
-    float *red = reinterpret_cast<float *>(sm);  // [KG][MT][HDP] floats: 32 KB at most, in the ring
+    float *red = reinterpret_cast<float *>(sm);  // [4 warps][MT][HDP] floats: 32 KB at most, in the ring
 #pragma unroll
-    for (int r = 0; r < MT; r++) *reinterpret_cast<ulonglong2 *>(red + (kg * MT + r) * HDP + dc * 4) = make_ulonglong2(o[r][0], o[r][1]);
+    for (int r = 0; r < MT; r++) {
+        const float sum = warp_sum(l[r]) * (1.f / DQ);  // every key is held by DQ lanes
+        if (lane == 0) {
+            m_s[warp][r] = m[r];
+            l_s[warp][r] = sum;
+        }
+#pragma unroll
+        for (int e = 0; e < DP; e++) *reinterpret_cast<unsigned long long *>(red + (warp * MT + r) * HDP + lane * (2 * DP) + 2 * e) = o[r][e];
+    }
     __syncthreads();
     for (int i = tid; i < MT * HDP / 2; i += SB_AP_THREADS) {
         const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
         if (f >= it.F) break;
-        float a = 0.f, b = 0.f;
+        const float M = fmaxf(fmaxf(m_s[0][r], m_s[1][r]), fmaxf(m_s[2][r], m_s[3][r])), base = M == -INFINITY ? 0.f : M;
+        float L = 0.f, a = 0.f, b = 0.f;
 #pragma unroll
-        for (int g = 0; g < KG; g++) {
-            const float2 x = *reinterpret_cast<const float2 *>(red + (g * MT + r) * HDP + d);
-            a += x.x;
-            b += x.y;
+        for (int w = 0; w < 4; w++) {
+            const float e = ap_exp2(m_s[w][r] - base);
+            const float2 x = *reinterpret_cast<const float2 *>(red + (w * MT + r) * HDP + d);
+            L = fmaf(e, l_s[w][r], L);
+            a = fmaf(e, x.x, a);
+            b = fmaf(e, x.y, b);
         }
-        if (d == 0) ap_row_stats(P, it, f, m_s[r], l_s[r]);
-        ap_row_out<float>(P, it, f, d, a, b, l_s[r]);
+        if (d == 0) ap_row_stats(P, it, f, M, L);
+        ap_row_out<float>(P, it, f, d, a, b, L);
     }
 }
 
@@ -705,7 +738,6 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 // which waits for the own kernel, has both behind it.
 #define SB_AP_BODY(MT, CALL)                                                                \
     extern __shared__ __align__(128) unsigned char ap_sm[];                                 \
-    __shared__ long long off_s[SB_AP_RING][64];                                       \
     pdl_launch_dependents();                                                                \
     AttnItem it;                                                                            \
     if (!own) {                                                                             \
@@ -716,30 +748,33 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             for (it.f0 = tile * MT; it.f0 < it.F; it.f0 += P.tiles * MT) CALL;              \
         pdl_wait();                                                                         \
     }
-#define SB_AP_MMA8(name, T, HDP)                                                                               \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, 4) name(const __grid_constant__ AttnParams P, int own) { \
-        SB_AP_BODY(8, (attn_mma8_body<T, HDP>(P, it, ap_sm, off_s)))                                           \
+#define SB_AP_MMAW(name, T, HDP, NB, CTAS)                                                                     \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, CTAS) name(const __grid_constant__ AttnParams P, int own) { \
+        __shared__ long long off_s[4 * 8 * 16];                                                                \
+        SB_AP_BODY(8 * NB, (attn_mmaw_body<T, HDP, NB>(P, it, ap_sm, off_s)))                                  \
     }
-#define SB_AP_MMA(name, T, HDP, MW)                                                                            \
+#define SB_AP_MMA(name, T, HDP)                                                                                \
     extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, HDP == 128 ? 2 : 3) name(const __grid_constant__ AttnParams P, int own) { \
-        SB_AP_BODY(16 * MW, (attn_mma_body<T, HDP, MW>(P, it, ap_sm, off_s)))                                  \
+        __shared__ long long off_s[SB_AP_RING][64];                                                            \
+        SB_AP_BODY(64, (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))                                           \
     }
 #define SB_AP_F32(name, HDP, MT)                                                                               \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS) name(const __grid_constant__ AttnParams P, int own) { \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, 3) name(const __grid_constant__ AttnParams P, int own) { \
+        __shared__ long long off_s[4 * 8 * 16];                                                                \
         SB_AP_BODY(MT, (attn_f32_body<HDP, MT>(P, it, ap_sm, off_s)))                                          \
     }
-SB_AP_MMA8(attn_f16_64_r8, __half, 64)
-SB_AP_MMA8(attn_f16_128_r8, __half, 128)
-SB_AP_MMA8(attn_bf16_64_r8, __nv_bfloat16, 64)
-SB_AP_MMA8(attn_bf16_128_r8, __nv_bfloat16, 128)
-SB_AP_MMA(attn_f16_64_r16, __half, 64, 1)
-SB_AP_MMA(attn_f16_64_r64, __half, 64, 4)
-SB_AP_MMA(attn_f16_128_r16, __half, 128, 1)
-SB_AP_MMA(attn_f16_128_r64, __half, 128, 4)
-SB_AP_MMA(attn_bf16_64_r16, __nv_bfloat16, 64, 1)
-SB_AP_MMA(attn_bf16_64_r64, __nv_bfloat16, 64, 4)
-SB_AP_MMA(attn_bf16_128_r16, __nv_bfloat16, 128, 1)
-SB_AP_MMA(attn_bf16_128_r64, __nv_bfloat16, 128, 4)
+SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 3)
+SB_AP_MMAW(attn_f16_64_r16, __half, 64, 2, 3)
+SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 3)
+SB_AP_MMAW(attn_f16_128_r16, __half, 128, 2, 2)
+SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 3)
+SB_AP_MMAW(attn_bf16_64_r16, __nv_bfloat16, 64, 2, 3)
+SB_AP_MMAW(attn_bf16_128_r8, __nv_bfloat16, 128, 1, 3)
+SB_AP_MMAW(attn_bf16_128_r16, __nv_bfloat16, 128, 2, 2)
+SB_AP_MMA(attn_f16_64_r64, __half, 64)
+SB_AP_MMA(attn_f16_128_r64, __half, 128)
+SB_AP_MMA(attn_bf16_64_r64, __nv_bfloat16, 64)
+SB_AP_MMA(attn_bf16_128_r64, __nv_bfloat16, 128)
 SB_AP_F32(attn_f32_64_r1, 64, 1)
 SB_AP_F32(attn_f32_64_r2, 64, 2)
 SB_AP_F32(attn_f32_64_r4, 64, 4)

@@ -244,7 +244,7 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
         int i = 0;
         while (i < 4 && (1 << i) < rows) i++;
         a->f = (sb_fn_id)(F_ATTN_F32_64_R1 + 5 * wide + i);
-        a->smem = (i == 4 ? 2 : 3) * 32768;
+        a->smem = 2 * 32768;
         a->rows = 1 << i;
         a->step = wide ? 32 : 64;
     } else if (prefix && rows >= SB_ATTN_TC_ROWS) {
@@ -257,7 +257,7 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
         const int big = rows > 16;
         a->f = rows <= 8 ? (sb_fn_id)(F_ATTN_F16_64_R8 + 2 * second + wide)
                          : (sb_fn_id)((second ? F_ATTN_BF16_64_R16 : F_ATTN_F16_64_R16) + 2 * wide + big);
-        a->smem = 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64); /* SB_AP_ST stages of K and V */
+        a->smem = big ? 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64) : 65536; /* the kernels' rings */
         a->rows = rows <= 8 ? 8 : big ? 64 : 16;
         a->step = 64;
     }
@@ -266,13 +266,16 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
 /* Key ranges of `keys` keys for `units` independent (head, row tile) pairs.
  * An item of n tiles of keys costs about n + SB_ATTN_ITEM tile times (its
  * queries, its part to write and join), and the launch as many rounds of
- * items as the SMs need: the count with the least of that is taken. */
-static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units) {
-    const long cap = (long)c->sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
+ * items as the SMs need: the count with the least of that is taken.  `fill`:
+ * how many items stand for one that is there (requests are shorter than the
+ * longest, their last ranges empty).  `alone`: one range would need no join. */
+static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, int fill, int alone) {
+    const long cap = (long)fill * c->sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
     long best = 0, best_cost = 0;
     for (long S = 1; S <= SB_ATTN_MAX_SPLITS && S <= tiles; S++) {
         const long n = CEIL_DIV(tiles, S), items = units * CEIL_DIV(tiles, n);
-        const long cost = CEIL_DIV(items, cap) * (n + SB_ATTN_ITEM) + CEIL_DIV(tiles, n) / 8;
+        const long parts = CEIL_DIV(tiles, n);
+        const long cost = CEIL_DIV(items, cap) * (n + SB_ATTN_ITEM) + parts / 8 + (alone && parts > 1 ? SB_ATTN_ITEM : 0);
         if (!best || cost < best_cost) {
             best = n;
             best_cost = cost;
@@ -290,11 +293,11 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
     memset(own, 0, sizeof *own);
     if (P > 0) {
         attn_kernel(type, HD, T * G, 1, pre);
-        attn_split(c, pre, P, (long)pre->tiles * NKV);
+        attn_split(c, pre, P, (long)pre->tiles * NKV, 1, max_kv == 0);
     }
     if (max_kv > 0) {
         attn_kernel(type, HD, max_q * G, 0, own);
-        attn_split(c, own, max_kv, (long)own->tiles * NKV * B);
+        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, 2, P == 0);
     }
     SB_ARG(pre->grid < 0x7fffffffL && own->grid < 0x7fffffffL, "attn_prefix: too many rows for one launch");
     return 0;
