@@ -48,7 +48,8 @@ struct AttnParams {
     long long q_row, q_head, o_row, o_head;
     AttnPages pre, suf;
     int T, B, NH, NKV, G, HD, P, max_kv, table_stride;
-    int chunk1, S1, chunk2, S2, tiles;  // key ranges and row tiles of the items
+    int chunk1, S1, tiles1, chunk2, S2, tiles2;  // key ranges and row tiles of the items
+    int items1;                                  // prefix items in this launch; own items follow them
     float scale_log2;
 };
 
@@ -67,7 +68,7 @@ SB_DEV int ap_vis(const AttnItem &it, int f, int G) { return min(max(it.vis0 + i
 
 // Item `idx` of the prefix (row tiles fastest: neighbours read the same keys)
 SB_DEV bool ap_prefix_item(const AttnParams &P, int idx, int MT, AttnItem &it) {
-    const int tile = idx % P.tiles, rest = idx / P.tiles;
+    const int tile = idx % P.tiles1, rest = idx / P.tiles1;
     it.kvh = rest % P.NKV;
     it.slot = rest / P.NKV;
     it.pg = P.pre;
@@ -85,8 +86,8 @@ SB_DEV bool ap_prefix_item(const AttnParams &P, int idx, int MT, AttnItem &it) {
 SB_DEV bool ap_own_item(const AttnParams &P, int idx, int MT, AttnItem &it, int &tile) {
     const int s = idx % P.S2;
     int rest = idx / P.S2;
-    tile = rest % P.tiles;
-    rest /= P.tiles;
+    tile = rest % P.tiles2;
+    rest /= P.tiles2;
     it.kvh = rest % P.NKV;
     const int b = rest / P.NKV;
     int q0 = b, q1 = b + 1;
@@ -107,7 +108,7 @@ SB_DEV bool ap_own_item(const AttnParams &P, int idx, int MT, AttnItem &it, int 
     it.step = 1;
     const int used = max(1, (len + P.chunk2 - 1) / P.chunk2);
     if (s == 0 && it.kvh == 0 && P.ws_n)
-        for (int r = q0 + tile * SB_AP_THREADS + threadIdx.x; r < q1; r += P.tiles * SB_AP_THREADS) P.ws_n[r] = used;
+        for (int r = q0 + tile * (int)blockDim.x + (int)threadIdx.x; r < q1; r += P.tiles2 * (int)blockDim.x) P.ws_n[r] = used;
     return s < used;
 }
 
@@ -415,7 +416,7 @@ SB_DEV unsigned ap_movmatrix(unsigned a) {
 }
 template <typename T, int HDP, int NB>
 SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long *off_s) {
-    constexpr int KS = HDP / 16, ST = HDP == 128 ? 2 : 4;
+    constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, ST = HDP == 128 ? 2 : 4, KT = 16 * NW;
     using Copy = ApWarpCopy<16, HDP, 2, ST>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     const Copy cp(it, P.HD, sm, off_s);
@@ -440,7 +441,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
     }
     const int flast = min(it.f0 + 8 * NB, it.F) - 1, first = it.k0 + warp * 16;
     const int k1 = min(it.k1, ap_vis(it, flast, P.G));
-    const int nt = k1 > first ? (k1 - first + 63) / 64 : 0;  // this warp's tiles: 16 keys of every 64
+    const int nt = k1 > first ? (k1 - first + KT - 1) / KT : 0;  // this warp's tiles: 16 keys of every KT
     float o[NB][KS][4], m[NB][2], l[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
@@ -450,7 +451,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
         l[b][0] = l[b][1] = 0.f;
     }
     __syncthreads();  // an earlier item's join has been read
-    for (int t = lane / 16; t <= ST; t += 2) cp.off[(t % Copy::RING) * 16 + lane % 16] = ap_offset(it, first + t * 64 + lane % 16);
+    for (int t = lane / 16; t <= ST; t += 2) cp.off[(t % Copy::RING) * 16 + lane % 16] = ap_offset(it, first + t * KT + lane % 16);
     __syncwarp();
     for (int t = 0; t < ST; t++) {
         cp.copy_k(t, t < nt);
@@ -458,9 +459,9 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
     }
     for (int t = 0; t < nt; t++) {
         long long next = 0;  // the offsets of tile t + ST + 1, a tile ahead of their use
-        if (lane < 16) next = ap_offset(it, first + (t + ST + 1) * 64 + lane);
+        if (lane < 16) next = ap_offset(it, first + (t + ST + 1) * KT + lane);
         const unsigned kt = cp.k_tile(t), vt = cp.v_tile(t);
-        const int key = first + t * 64 + g;
+        const int key = first + t * KT + g;
         ap_wait<2 * ST - 1>();
         __syncwarp();
         const bool there0 = cp.offs(t)[g] & 1, there1 = cp.offs(t)[g + 8] & 1;
@@ -531,8 +532,8 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
         __syncwarp();
     }
     ap_wait<0>();
-    float *ow = reinterpret_cast<float *>(sm);  // [4 warps][8 NB rows][HDP]
-    __shared__ float ms[4][8 * NB], ls[4][8 * NB];
+    float *ow = reinterpret_cast<float *>(sm);  // [NW][8 NB rows][HDP]
+    __shared__ float ms[NW][8 * NB], ls[NW][8 * NB];
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -552,13 +553,15 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             }
         }
     __syncthreads();
-    for (int i = tid; i < 8 * NB * HDP / 2; i += SB_AP_THREADS) {
+    for (int i = tid; i < 8 * NB * HDP / 2; i += 32 * NW) {
         const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
         if (f >= it.F) break;
-        float M = fmaxf(fmaxf(ms[0][r], ms[1][r]), fmaxf(ms[2][r], ms[3][r])), L = 0.f, a = 0.f, b = 0.f;
+        float M = ms[0][r], L = 0.f, a = 0.f, b = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, ms[w][r]);
         const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             const float e = ap_exp2(ms[w][r] - base);
             const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 8 * NB + r) * HDP + d);
             L += e * ls[w][r];
@@ -584,17 +587,17 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
 // thousand keys.
 template <int HDP, int MT>
 SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long *off_s) {
-    constexpr int KT = HDP == 64 ? 64 : 32, KW = KT / 4, DQ = 32 / KW, DP = HDP / 64;  // keys a warp, parts of a key, pairs of a lane
+    constexpr int NW = SB_AP_THREADS / 32, KW = HDP == 64 ? 16 : 8, KT = KW * NW, DQ = 32 / KW, DP = HDP / 64;  // keys a warp, parts of a key, pairs of a lane
     constexpr int ST = 2;
     using Copy = ApWarpCopy<KW, HDP, 4, ST>;
     __shared__ __align__(16) float q_s[MT][DQ][36];
-    __shared__ __align__(16) float2 p_s[4][KW][MT < 2 ? 2 : MT];
-    __shared__ float m_s[4][MT], l_s[4][MT];
+    __shared__ __align__(16) float2 p_s[NW][KW][MT < 2 ? 2 : MT];
+    __shared__ float m_s[NW][MT], l_s[NW][MT];
     __shared__ int vis_s[MT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = lane % KW, dq = lane / KW;
     const Copy cp(it, P.HD, sm, off_s);
     __syncthreads();  // an earlier item's shared memory is no longer read
-    for (int i = tid; i < MT * HDP; i += SB_AP_THREADS) {
+    for (int i = tid; i < MT * HDP; i += 32 * NW) {
         const int r = i / HDP, d = i % HDP, f = it.f0 + r;
         q_s[r][d / 32][d % 32] = f < it.F && d < P.HD ? static_cast<const float *>(P.q)[(long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head + d] * P.scale_log2 : 0.f;
     }
@@ -702,7 +705,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     }
     ap_wait<0>();
     __syncthreads();
-    float *red = reinterpret_cast<float *>(sm);  // [4 warps][MT][HDP] floats: 32 KB at most, in the ring
+    float *red = reinterpret_cast<float *>(sm);  // [NW][MT][HDP] floats: 32 KB at most, in the ring
 #pragma unroll
     for (int r = 0; r < MT; r++) {
         const float sum = warp_sum(l[r]) * (1.f / DQ);  // every key is held by DQ lanes
@@ -714,13 +717,16 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
         for (int e = 0; e < DP; e++) *reinterpret_cast<unsigned long long *>(red + (warp * MT + r) * HDP + lane * (2 * DP) + 2 * e) = o[r][e];
     }
     __syncthreads();
-    for (int i = tid; i < MT * HDP / 2; i += SB_AP_THREADS) {
+    for (int i = tid; i < MT * HDP / 2; i += 32 * NW) {
         const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
         if (f >= it.F) break;
-        const float M = fmaxf(fmaxf(m_s[0][r], m_s[1][r]), fmaxf(m_s[2][r], m_s[3][r])), base = M == -INFINITY ? 0.f : M;
+        float M = m_s[0][r];
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, m_s[w][r]);
+        const float base = M == -INFINITY ? 0.f : M;
         float L = 0.f, a = 0.f, b = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < NW; w++) {
             const float e = ap_exp2(m_s[w][r] - base);
             const float2 x = *reinterpret_cast<const float2 *>(red + (w * MT + r) * HDP + d);
             L = fmaf(e, l_s[w][r], L);
@@ -732,44 +738,47 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     }
 }
 
-// prefix: a CTA an item.  own: a CTA an item; the row tiles of a request
-// beyond the grid's are looped.  Both let the next launch start early; the
-// own kernel waits for the prefix kernel before it ends, so that the join,
-// which waits for the own kernel, has both behind it.
+// A CTA an item: the prefix items of the launch, then own ones (either may be
+// none; row tiles of a request beyond the grid's are looped).  Each launch lets
+// the next start early and waits, before it ends, for the one before it, so
+// that the join, which waits for the last, has all of them behind it.
 #define SB_AP_BODY(MT, CALL)                                                                \
     extern __shared__ __align__(128) unsigned char ap_sm[];                                 \
     pdl_launch_dependents();                                                                \
     AttnItem it;                                                                            \
-    if (!own) {                                                                             \
-        if (ap_prefix_item(P, blockIdx.x, MT, it)) CALL;                                    \
+    const int item = (int)blockIdx.x - P.items1;                                            \
+    it.f0 = 0;                                                                              \
+    if (item < 0) {                                                                         \
+        if (!ap_prefix_item(P, blockIdx.x, MT, it)) it.F = 0;                               \
     } else {                                                                                \
         int tile;                                                                           \
-        if (ap_own_item(P, blockIdx.x, MT, it, tile))                                       \
-            for (it.f0 = tile * MT; it.f0 < it.F; it.f0 += P.tiles * MT) CALL;              \
-        pdl_wait();                                                                         \
-    }
+        if (ap_own_item(P, item, MT, it, tile)) it.f0 = tile * MT;                          \
+        else it.F = 0;                                                                      \
+    }                                                                                       \
+    for (const int step = item < 0 ? 1 << 30 : P.tiles2 * MT; it.f0 < it.F; it.f0 += step) CALL; \
+    pdl_wait();
 #define SB_AP_MMAW(name, T, HDP, NB, CTAS)                                                                     \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, CTAS) name(const __grid_constant__ AttnParams P, int own) { \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, CTAS) name(const __grid_constant__ AttnParams P) { \
         __shared__ long long off_s[4 * 8 * 16];                                                                \
         SB_AP_BODY(8 * NB, (attn_mmaw_body<T, HDP, NB>(P, it, ap_sm, off_s)))                                  \
     }
 #define SB_AP_MMA(name, T, HDP)                                                                                \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, HDP == 128 ? 2 : 3) name(const __grid_constant__ AttnParams P, int own) { \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, HDP == 128 ? 2 : 3) name(const __grid_constant__ AttnParams P) { \
         __shared__ long long off_s[SB_AP_RING][64];                                                            \
         SB_AP_BODY(64, (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))                                           \
     }
 #define SB_AP_F32(name, HDP, MT)                                                                               \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, 3) name(const __grid_constant__ AttnParams P, int own) { \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, 3) name(const __grid_constant__ AttnParams P) { \
         __shared__ long long off_s[4 * 8 * 16];                                                                \
         SB_AP_BODY(MT, (attn_f32_body<HDP, MT>(P, it, ap_sm, off_s)))                                          \
     }
 SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 3)
-SB_AP_MMAW(attn_f16_64_r16, __half, 64, 2, 3)
 SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 3)
-SB_AP_MMAW(attn_f16_128_r16, __half, 128, 2, 2)
 SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 3)
-SB_AP_MMAW(attn_bf16_64_r16, __nv_bfloat16, 64, 2, 3)
 SB_AP_MMAW(attn_bf16_128_r8, __nv_bfloat16, 128, 1, 3)
+SB_AP_MMAW(attn_f16_64_r16, __half, 64, 2, 3)
+SB_AP_MMAW(attn_f16_128_r16, __half, 128, 2, 2)
+SB_AP_MMAW(attn_bf16_64_r16, __nv_bfloat16, 64, 2, 3)
 SB_AP_MMAW(attn_bf16_128_r16, __nv_bfloat16, 128, 2, 2)
 SB_AP_MMA(attn_f16_64_r64, __half, 64)
 SB_AP_MMA(attn_f16_128_r64, __half, 128)

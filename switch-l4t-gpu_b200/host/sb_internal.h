@@ -96,12 +96,12 @@ typedef enum {
     F_ATTN_BF16_64_R8,
     F_ATTN_BF16_128_R8,
     F_ATTN_F16_64_R16,
-    F_ATTN_F16_64_R64,
     F_ATTN_F16_128_R16,
-    F_ATTN_F16_128_R64,
     F_ATTN_BF16_64_R16,
-    F_ATTN_BF16_64_R64,
     F_ATTN_BF16_128_R16,
+    F_ATTN_F16_64_R64,
+    F_ATTN_F16_128_R64,
+    F_ATTN_BF16_64_R64,
     F_ATTN_BF16_128_R64,
     F_ATTN_F32_64_R1,
     F_ATTN_F32_64_R2,
