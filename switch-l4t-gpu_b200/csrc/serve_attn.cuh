@@ -22,6 +22,7 @@
 // to the value type for the second tensor-core product (half a step, like
 // the values they multiply).
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "sb_common.cuh"
@@ -30,6 +31,8 @@
 // stages of the K / V ring: two of 32 KB for 128 values leave room for three CTAs on an SM
 #define SB_AP_ST(HDP) ((HDP) == 128 ? 2 : 3)
 #define SB_AP_RING 4  // offsets of the tiles in flight
+
+__device__ int tc_err;  // nonzero after a wait timed out
 
 struct AttnPages {  // strides in elements
     const void *k, *v;
@@ -119,6 +122,60 @@ SB_DEV void ap_cp16(unsigned dst, const void *src, bool ok) {  // 16 bytes, or z
 SB_DEV void ap_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> SB_DEV void ap_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// ---- barriers.  Every wait is bounded: after two seconds it sets tc_err
+// (sb_tc_error reads and clears it) and the caller stops.
+SB_DEV void ap_bar_init(uint64_t *b, unsigned count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(ap_smem(b)), "r"(count) : "memory");
+}
+SB_DEV void ap_arrive(uint64_t *b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ap_smem(b)) : "memory"); }
+SB_DEV void ap_expect(uint64_t *b, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(ap_smem(b)), "r"(bytes) : "memory");
+}
+SB_DEV bool ap_bar_try(uint64_t *b, unsigned ph) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(ap_smem(b)), "r"(ph)
+                 : "memory");
+    return done;
+}
+SB_DEV unsigned long long ap_now() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+// false after WAIT_NS, or (abortable) once any wait has given up
+SB_DEV bool ap_bar_wait(uint64_t *b, unsigned ph, bool abortable = true) {
+    constexpr unsigned long long WAIT_NS = 2000000000ull;
+    if (ap_bar_try(b, ph)) return true;
+    unsigned long long t0 = 0;
+#pragma unroll 1
+    for (int spin = 0; spin < (1 << 26); spin++) {
+        if (ap_bar_try(b, ph)) return true;
+        if ((spin & 1023) == 1023) {
+            if (abortable && *(volatile int *)&tc_err) return false;
+            const unsigned long long t = ap_now();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > WAIT_NS) break;
+        }
+    }
+    atomicExch(&tc_err, 1);
+    return false;
+}
+SB_DEV void ap_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// box {128 bytes of values, one head, rows of a page, one page}
+SB_DEV void ap_tma(unsigned dst, const CUtensorMap *tm, int d, int head, int row, int page, uint64_t *b) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(tm), "r"(d), "r"(head), "r"(row), "r"(page), "r"(ap_smem(b))
+        : "memory");
+}
+// a warp's ring: K and V tiles that have landed (32 arrivals and the bytes), and which keys of a tile are there
+struct ApBars {
+    uint64_t full[2][4];
+    unsigned valid[4];
+};
+
 // element offset of position p in the pages (without the head) with the lowest
 // bit set (offsets are multiples of 16 bytes), 0 where it has none
 SB_DEV long long ap_offset(const AttnItem &it, int p) {
@@ -161,45 +218,87 @@ template <int KT, int HDP, int E> struct ApCopy {
     }
 };
 
-// The same for a warp that reads its keys alone: KW positions of a tile, K and V
-// each a group of their own, in a ring of ST tiles a warp.  The block never
-// meets: a tile of K is asked for as soon as the warp has its scores, one of V
-// as soon as it has its outputs, so nearly 2 ST groups are always in flight.
-template <int KW, int HDP, int E, int ST> struct ApWarpCopy {
-    static constexpr int C = HDP * E / 16, STEP = 32 / C, N = KW / STEP, TILE = KW * HDP * E, RING = 8;
-    static_assert(ST + 2 <= RING, "offsets of the tiles in flight");
-    const char *k, *v;
-    unsigned sm;         // this warp's ring: K tiles, then V tiles
-    long long *off;      // [RING][KW]
-    int row, c;
-    bool in;
-    SB_DEV ApWarpCopy(const AttnItem &it, int HD, unsigned char *ring, long long *offsets) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        c = lane % C;
-        row = lane / C;
-        k = static_cast<const char *>(it.pg.k) + it.kvh * it.pg.head_stride * E + c * 16;
-        v = static_cast<const char *>(it.pg.v) + it.kvh * it.pg.head_stride * E + c * 16;
+// The keys of one warp: KW positions of every KT, K and V tiles in a ring of ST
+// each.  The block never meets: a tile of K is asked for as soon as the warp
+// has its scores, one of V as soon as it has its outputs, so nearly 2 ST tiles
+// are always in flight.  A tile is rows of 128 bytes in column blocks, 16-byte
+// chunks xor-ed by the row's low three bits (ldmatrix, or eight lanes on eight
+// keys, touch all banks).  Whole pages come by TMA boxes, one lane a box:
+// copies by the lanes (tiles that end inside a page or miss one, other page
+// sizes, calls too small to encode a map for) cost a third of all
+// instructions of a decode tile.
+template <int KW, int HDP, int E, int ST> struct ApRing {
+    static constexpr int SUB = HDP * E / 128, BLOCK = KW * 128, TILE = SUB * BLOCK, KT = KW * (SB_AP_THREADS / 32);
+    static constexpr int C = HDP * E / 16, STEP = 32 / C, N = KW / STEP;
+    const AttnItem &it;
+    const CUtensorMap *tm[2];
+    ApBars *bars;
+    unsigned sm;
+    int first, box, HD, seq;  // seq: tiles that went through the ring before this item
+    int pg, in_pg, row, sub;  // this lane's box of the tile looked up last
+    bool mine;
+    SB_DEV ApRing(const AttnItem &item, int hd, unsigned char *ring, ApBars *b, int seq0, const CUtensorMap *k, const CUtensorMap *v, int bx)
+        : it(item), bars(b + (threadIdx.x >> 5)), box(min(bx, KW)), HD(hd), seq(seq0) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = box ? KW / box : 1;
+        tm[0] = k;
+        tm[1] = v;
         sm = ap_smem(ring) + warp * (2 * ST * TILE);
-        off = offsets + warp * (RING * KW);
-        in = c * 16 < HD * E;
+        first = it.k0 + warp * KW;
+        sub = lane / pieces;
+        row = lane % pieces * box;
+        mine = box && sub < SUB;
     }
-    SB_DEV unsigned k_tile(int t) const { return sm + (t % ST) * TILE; }
-    SB_DEV unsigned v_tile(int t) const { return sm + (ST + t % ST) * TILE; }
-    SB_DEV const long long *offs(int t) const { return off + (t % RING) * KW; }
-    SB_DEV void copy(unsigned dst, const char *base, int t, bool live) const {
-        if (live) {
-            const long long *o = offs(t);
-#pragma unroll
-            for (int j = 0; j < N; j++) {
-                const int r = row + j * STEP;
-                const long long w = o[r];
-                ap_cp16(dst + r * (HDP * E) + ((c ^ (r & 7)) << 4), base + (w & ~1ll) * E, (w & 1) && in);
-            }
+    SB_DEV int tiles(int k1) const { return k1 > first ? (k1 - first + KT - 1) / KT : 0; }
+    SB_DEV unsigned tile(int which, int t) const { return sm + (which * ST + (seq + t) % ST) * TILE; }
+    SB_DEV void look(int t) {  // a tile ahead of its use
+        const int p = first + t * KT + row;
+        pg = -1;
+        if (mine && p - row + KW <= it.k1) {
+            const int j = p / it.pg.page;
+            pg = it.table ? it.table[j] : j;
+            in_pg = p - j * it.pg.page;
         }
-        ap_commit();
     }
-    SB_DEV void copy_k(int t, bool live) const { copy(k_tile(t), k, t, live); }
-    SB_DEV void copy_v(int t, bool live) const { copy(v_tile(t), v, t, live); }
+    SB_DEV void copy(int which, int t) {  // tile t, looked up
+        const int lane = threadIdx.x & 31, n = (seq + t) % ST;
+        const unsigned dst = tile(which, t);
+        uint64_t *bar = &bars->full[which][n];
+        if (__all_sync(SB_FULL, box && (!mine || (pg >= 0 && pg < it.pg.n_pages)))) {
+            if (lane == 0) {
+                if (which == 0) bars->valid[n] = ~0u;
+                ap_expect(bar, TILE);
+            } else {
+                ap_arrive(bar);
+            }
+            __syncwarp();
+            if (mine) ap_tma(dst + sub * BLOCK + row * 128, tm[which], sub * (128 / E), it.kvh, in_pg, pg, bar);
+            return;
+        }
+        const long long off = ap_offset(it, first + t * KT + lane % KW);
+        const unsigned valid = __ballot_sync(SB_FULL, off & 1);
+        if (which == 0 && lane == 0) bars->valid[n] = valid;
+        const int c = lane % C, r0 = lane / C;
+        const char *base = static_cast<const char *>(which ? it.pg.v : it.pg.k) + it.kvh * it.pg.head_stride * E + c * 16;
+        ap_fence_async();  // the ring's place may have been written by TMA, or will be
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int r = r0 + j * STEP;
+            const long long o = __shfl_sync(SB_FULL, off, r);
+            ap_cp16(dst + (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o & ~1ll) * E, (o & 1) && c * 16 < HD * E);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ap_smem(bar)) : "memory");
+    }
+    SB_DEV bool wait(int which, int t) const {
+        return __all_sync(SB_FULL, ap_bar_wait(&bars->full[which][(seq + t) % ST], (unsigned)((seq + t) / ST) & 1u));
+    }
+    SB_DEV void drain(int t, int nt) {  // given up at tile t: what was asked for still has to land
+        for (int u = t; u < min(t + ST + 1, nt); u++) {
+            ap_bar_wait(&bars->full[0][(seq + u) % ST], (unsigned)((seq + u) / ST) & 1u, false);
+            ap_bar_wait(&bars->full[1][(seq + u) % ST], (unsigned)((seq + u) / ST) & 1u, false);
+        }
+        __syncwarp();
+    }
+    SB_DEV unsigned valid(int t) const { return bars->valid[(seq + t) % ST]; }
 };
 
 // what a finished row leaves: the output itself where the item is the only one, else its part
@@ -415,11 +514,11 @@ SB_DEV unsigned ap_movmatrix(unsigned a) {
     return d;
 }
 template <typename T, int HDP, int NB>
-SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long *off_s) {
+SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, ApBars *bars, int &seq, const CUtensorMap *tm_k,
+                           const CUtensorMap *tm_v, int box) {
     constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, ST = HDP == 128 ? 2 : 4, KT = 16 * NW;
-    using Copy = ApWarpCopy<16, HDP, 2, ST>;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    const Copy cp(it, P.HD, sm, off_s);
+    ApRing<16, HDP, 2, ST> ring(it, P.HD, sm, bars, seq, tm_k, tm_v, box);
     unsigned qb[NB][KS][2];  // rows f0 + 8 b + g
     int vis[NB][2];          // of rows f0 + 8 b + 2 q4, + 1
 #pragma unroll
@@ -439,9 +538,8 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             vis[b][h] = fh < it.F ? ap_vis(it, fh, P.G) : 0;
         }
     }
-    const int flast = min(it.f0 + 8 * NB, it.F) - 1, first = it.k0 + warp * 16;
-    const int k1 = min(it.k1, ap_vis(it, flast, P.G));
-    const int nt = k1 > first ? (k1 - first + KT - 1) / KT : 0;  // this warp's tiles: 16 keys of every KT
+    const int flast = min(it.f0 + 8 * NB, it.F) - 1, first = ring.first;
+    const int nt = ring.tiles(min(it.k1, ap_vis(it, flast, P.G)));  // this warp's tiles: 16 keys of every KT
     float o[NB][KS][4], m[NB][2], l[NB][2];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
@@ -450,21 +548,24 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
         m[b][0] = m[b][1] = -INFINITY;
         l[b][0] = l[b][1] = 0.f;
     }
+    ap_fence_async();
     __syncthreads();  // an earlier item's join has been read
-    for (int t = lane / 16; t <= ST; t += 2) cp.off[(t % Copy::RING) * 16 + lane % 16] = ap_offset(it, first + t * KT + lane % 16);
-    __syncwarp();
     for (int t = 0; t < ST; t++) {
-        cp.copy_k(t, t < nt);
-        cp.copy_v(t, t < nt);
+        ring.look(t);
+        if (t < nt) {
+            ring.copy(0, t);
+            ring.copy(1, t);
+        }
     }
-    for (int t = 0; t < nt; t++) {
-        long long next = 0;  // the offsets of tile t + ST + 1, a tile ahead of their use
-        if (lane < 16) next = ap_offset(it, first + (t + ST + 1) * KT + lane);
-        const unsigned kt = cp.k_tile(t), vt = cp.v_tile(t);
+    ring.look(ST);
+    bool ok = true;
+    int t = 0;
+    for (; t < nt; t++) {
+        const unsigned kt = ring.tile(0, t), vt = ring.tile(1, t);
         const int key = first + t * KT + g;
-        ap_wait<2 * ST - 1>();
-        __syncwarp();
-        const bool there0 = cp.offs(t)[g] & 1, there1 = cp.offs(t)[g + 8] & 1;
+        if (!(ok = ring.wait(0, t))) break;
+        const unsigned valid = ring.valid(t);
+        const bool there0 = valid >> g & 1, there1 = valid >> (g + 8) & 1;
         float s[NB][4];
 #pragma unroll
         for (int b = 0; b < NB; b++) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
@@ -472,12 +573,12 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
         for (int k = 0; k < KS; k++) {
             const int r = lane & 15, c = 2 * k + (lane >> 4);
             unsigned a[4];
-            ap_ldsm(a, kt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
+            ap_ldsm(a, kt + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 #pragma unroll
             for (int b = 0; b < NB; b++) ap_mma<T>(s[b], a, qb[b][k][0], qb[b][k][1]);
         }
         __syncwarp();
-        cp.copy_k(t + ST, t + ST < nt);
+        if (t + ST < nt) ring.copy(0, t + ST);
         bool grown = false;
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -516,22 +617,26 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             p[b][0] = ap_movmatrix(ap_pack<T>(s[b][0], s[b][1]));
             p[b][1] = ap_movmatrix(ap_pack<T>(s[b][2], s[b][3]));
         }
-        ap_wait<2 * ST - 1>();
-        __syncwarp();
+        if (!(ok = ring.wait(1, t))) break;
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             const int mid = lane >> 3, r = (mid >> 1) * 8 + (lane & 7), c = 2 * i + (mid & 1);
             unsigned a[4];
-            ap_ldsm_t(a, vt + r * (HDP * 2) + ((c ^ (r & 7)) << 4));
+            ap_ldsm_t(a, vt + (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 #pragma unroll
             for (int b = 0; b < NB; b++) ap_mma<T>(o[b][i], a, p[b][0], p[b][1]);
         }
         __syncwarp();
-        cp.copy_v(t + ST, t + ST < nt);
-        if (lane < 16) cp.off[((t + ST + 1) % Copy::RING) * 16 + lane] = next;
-        __syncwarp();
+        if (t + ST < nt) {
+            ring.copy(1, t + ST);
+            ring.look(t + ST + 1);
+        }
     }
-    ap_wait<0>();
+    seq += nt;
+    if (!ok) {  // given up (tc_err): nothing that passes for a result
+        ring.drain(t, nt);
+        l[0][0] = l[0][1] = __int_as_float(0x7fc00000);
+    }
     float *ow = reinterpret_cast<float *>(sm);  // [NW][8 NB rows][HDP]
     __shared__ float ms[NW][8 * NB], ls[NW][8 * NB];
     __syncthreads();
@@ -586,16 +691,16 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
 // tensor pipe: its FP32 sums are not IEEE-rounded and drift by 1e-5 over some
 // thousand keys.
 template <int HDP, int MT>
-SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, long long *off_s) {
+SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, ApBars *bars, int &seq, const CUtensorMap *tm_k,
+                          const CUtensorMap *tm_v, int box) {
     constexpr int NW = SB_AP_THREADS / 32, KW = HDP == 64 ? 16 : 8, KT = KW * NW, DQ = 32 / KW, DP = HDP / 64;  // keys a warp, parts of a key, pairs of a lane
-    constexpr int ST = 2;
-    using Copy = ApWarpCopy<KW, HDP, 4, ST>;
+    constexpr int ST = 2, BLOCK = KW * 128;
     __shared__ __align__(16) float q_s[MT][DQ][36];
     __shared__ __align__(16) float2 p_s[NW][KW][MT < 2 ? 2 : MT];
     __shared__ float m_s[NW][MT], l_s[NW][MT];
     __shared__ int vis_s[MT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = lane % KW, dq = lane / KW;
-    const Copy cp(it, P.HD, sm, off_s);
+    ApRing<KW, HDP, 4, ST> ring(it, P.HD, sm, bars, seq, tm_k, tm_v, box);
     __syncthreads();  // an earlier item's shared memory is no longer read
     for (int i = tid; i < MT * HDP; i += 32 * NW) {
         const int r = i / HDP, d = i % HDP, f = it.f0 + r;
@@ -604,13 +709,18 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     if (tid < MT) vis_s[tid] = it.f0 + tid < it.F ? ap_vis(it, it.f0 + tid, P.G) : 0;
     const int flast = min(it.f0 + MT, it.F) - 1;
     const int k1 = min(it.k1, ap_vis(it, flast, P.G)), vmin = ap_vis(it, it.f0, P.G);  // rows in order see more and more
-    const int first = it.k0 + warp * KW, nt = k1 > first ? (k1 - first + KT - 1) / KT : 0;  // this warp's KW keys of every KT
-    for (int t = lane / KW; t <= ST; t += 32 / KW) cp.off[(t % Copy::RING) * KW + key] = ap_offset(it, first + t * KT + key);
+    const int first = ring.first, nt = ring.tiles(k1);  // this warp's KW keys of every KT
+    ap_fence_async();
     __syncthreads();
     for (int t = 0; t < ST; t++) {
-        cp.copy_k(t, t < nt);
-        cp.copy_v(t, t < nt);
+        ring.look(t);
+        if (t < nt) {
+            ring.copy(0, t);
+            ring.copy(1, t);
+        }
     }
+    ring.look(ST);
+    bool ok = true;
     unsigned long long o[MT][DP];
     float m[MT], l[MT];
 #pragma unroll
@@ -620,19 +730,17 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 #pragma unroll
         for (int e = 0; e < DP; e++) o[r][e] = 0ull;
     }
-    for (int t = 0; t < nt; t++) {
-        long long next = 0;  // the offsets of tile t + ST + 1, a tile ahead of their use
-        if (lane < KW) next = ap_offset(it, first + (t + ST + 1) * KT + lane);
-        const unsigned char *kt = sm + (cp.k_tile(t) - ap_smem(sm)), *vt = sm + (cp.v_tile(t) - ap_smem(sm));
-        ap_wait<2 * ST - 1>();
-        __syncwarp();
-        const bool there = cp.offs(t)[key] & 1;
+    int t = 0;
+    for (; t < nt; t++) {
+        const unsigned char *kt = sm + (ring.tile(0, t) - ap_smem(sm)), *vt = sm + (ring.tile(1, t) - ap_smem(sm));
+        if (!(ok = ring.wait(0, t))) break;
+        const bool there = ring.valid(t) >> key & 1;
         unsigned long long acc[MT];
 #pragma unroll
         for (int r = 0; r < MT; r++) acc[r] = 0ull;
 #pragma unroll
         for (int c = 0; c < 8; c++) {
-            const ulonglong2 k2 = *reinterpret_cast<const ulonglong2 *>(kt + key * (HDP * 4) + (((dq * 8 + c) ^ (key & 7)) << 4));
+            const ulonglong2 k2 = *reinterpret_cast<const ulonglong2 *>(kt + dq * BLOCK + key * 128 + ((c ^ (key & 7)) << 4));
 #pragma unroll
             for (int r = 0; r < MT; r++) {
                 const ulonglong2 q2 = *reinterpret_cast<const ulonglong2 *>(&q_s[r][dq][c * 4]);
@@ -641,7 +749,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             }
         }
         __syncwarp();
-        cp.copy_k(t + ST, t + ST < nt);
+        if (t + ST < nt) ring.copy(0, t + ST);
         float s[MT];
         bool grown = false;
         const int at = first + t * KT + key;
@@ -670,15 +778,15 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             l[r] += s[r];
             if (r % DQ == dq) p_s[warp][key][r] = make_float2(s[r], s[r]);
         }
-        ap_wait<2 * ST - 1>();
         __syncwarp();
+        if (!(ok = ring.wait(1, t))) break;
 #pragma unroll
         for (int k = 0; k < KW; k++) {
                         unsigned long long v[DP];
             if constexpr (DP == 1) {
-                v[0] = *reinterpret_cast<const unsigned long long *>(vt + k * (HDP * 4) + (((lane >> 1) ^ (k & 7)) << 4) + (lane & 1) * 8);
+                v[0] = *reinterpret_cast<const unsigned long long *>(vt + (lane >> 4) * BLOCK + k * 128 + ((((lane >> 1) & 7) ^ (k & 7)) << 4) + (lane & 1) * 8);
             } else {
-                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(vt + k * (HDP * 4) + ((lane ^ (k & 7)) << 4));
+                const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(vt + (lane >> 3) * BLOCK + k * 128 + (((lane & 7) ^ (k & 7)) << 4));
                 v[0] = w.x;
                 v[DP - 1] = w.y;
             }
@@ -699,11 +807,16 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             }
         }
         __syncwarp();  // values and weights are read
-        cp.copy_v(t + ST, t + ST < nt);
-        if (lane < KW) cp.off[((t + ST + 1) % Copy::RING) * KW + lane] = next;
-        __syncwarp();
+        if (t + ST < nt) {
+            ring.copy(1, t + ST);
+            ring.look(t + ST + 1);
+        }
     }
-    ap_wait<0>();
+    seq += nt;
+    if (!ok) {  // given up (tc_err): nothing that passes for a result
+        ring.drain(t, nt);
+        l[0] = __int_as_float(0x7fc00000);
+    }
     __syncthreads();
     float *red = reinterpret_cast<float *>(sm);  // [NW][MT][HDP] floats: 32 KB at most, in the ring
 #pragma unroll
@@ -742,36 +855,39 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 // none; row tiles of a request beyond the grid's are looped).  Each launch lets
 // the next start early and waits, before it ends, for the one before it, so
 // that the join, which waits for the last, has all of them behind it.
-#define SB_AP_BODY(MT, CALL)                                                                \
-    extern __shared__ __align__(128) unsigned char ap_sm[];                                 \
-    pdl_launch_dependents();                                                                \
-    AttnItem it;                                                                            \
-    const int item = (int)blockIdx.x - P.items1;                                            \
-    it.f0 = 0;                                                                              \
-    if (item < 0) {                                                                         \
-        if (!ap_prefix_item(P, blockIdx.x, MT, it)) it.F = 0;                               \
-    } else {                                                                                \
-        int tile;                                                                           \
-        if (ap_own_item(P, item, MT, it, tile)) it.f0 = tile * MT;                          \
-        else it.F = 0;                                                                      \
-    }                                                                                       \
-    for (const int step = item < 0 ? 1 << 30 : P.tiles2 * MT; it.f0 < it.F; it.f0 += step) CALL; \
-    pdl_wait();
-#define SB_AP_MMAW(name, T, HDP, NB, CTAS)                                                                     \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, CTAS) name(const __grid_constant__ AttnParams P) { \
-        __shared__ long long off_s[4 * 8 * 16];                                                                \
-        SB_AP_BODY(8 * NB, (attn_mmaw_body<T, HDP, NB>(P, it, ap_sm, off_s)))                                  \
+#define SB_AP_KERNEL(name, CTAS, MT, SHARED, CALL)                                                                   \
+    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, CTAS)                                                  \
+        name(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap tm_k,                           \
+             const __grid_constant__ CUtensorMap tm_v, int box) {                                                      \
+        extern __shared__ __align__(1024) unsigned char ap_sm[];                                                       \
+        SHARED;                                                                                                        \
+        pdl_launch_dependents();                                                                                       \
+        AttnItem it;                                                                                                   \
+        const int item = (int)blockIdx.x - P.items1;                                                                   \
+        it.f0 = 0;                                                                                                     \
+        if (item < 0) {                                                                                                \
+            if (!ap_prefix_item(P, blockIdx.x, MT, it)) it.F = 0;                                                      \
+        } else {                                                                                                       \
+            int tile;                                                                                                  \
+            if (ap_own_item(P, item, MT, it, tile)) it.f0 = tile * MT;                                                 \
+            else it.F = 0;                                                                                             \
+        }                                                                                                              \
+        for (const int step = item < 0 ? 1 << 30 : P.tiles2 * MT; it.f0 < it.F; it.f0 += step) CALL;                   \
+        pdl_wait();                                                                                                    \
     }
-#define SB_AP_MMA(name, T, HDP)                                                                                \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, HDP == 128 ? 2 : 3) name(const __grid_constant__ AttnParams P) { \
-        __shared__ long long off_s[SB_AP_RING][64];                                                            \
-        SB_AP_BODY(64, (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))                                           \
-    }
-#define SB_AP_F32(name, HDP, MT)                                                                               \
-    extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, 3) name(const __grid_constant__ AttnParams P) { \
-        __shared__ long long off_s[4 * 8 * 16];                                                                \
-        SB_AP_BODY(MT, (attn_f32_body<HDP, MT>(P, it, ap_sm, off_s)))                                          \
-    }
+// the four warps' barriers; a warp counts its own tiles
+#define SB_AP_WARPS                                                                                                    \
+    __shared__ ApBars bars[SB_AP_THREADS / 32];                                                                        \
+    int seq = 0;                                                                                                       \
+    if ((threadIdx.x & 31) < 8) ap_bar_init(&bars[threadIdx.x >> 5].full[0][0] + (threadIdx.x & 7), 32);               \
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");                                                 \
+    __syncwarp()
+#define SB_AP_MMAW(name, T, HDP, NB, CTAS) \
+    SB_AP_KERNEL(name, CTAS, 8 * NB, SB_AP_WARPS, (attn_mmaw_body<T, HDP, NB>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
+#define SB_AP_MMA(name, T, HDP) \
+    SB_AP_KERNEL(name, (HDP == 128 ? 2 : 3), 64, __shared__ long long off_s[SB_AP_RING][64], (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))
+#define SB_AP_F32(name, HDP, MT) \
+    SB_AP_KERNEL(name, 3, MT, SB_AP_WARPS, (attn_f32_body<HDP, MT>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
 SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 3)
 SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 3)
 SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 3)

@@ -30,66 +30,16 @@
 
 #define ATC_POLY 4
 
-__device__ int tc_err;  // nonzero after a wait timed out (sb_tc_error reads and clears it)
-
 namespace atc {
 constexpr int THREADS = 512, BM = 128, KT = 128;
-constexpr unsigned long long WAIT_NS = 2000000000ull;
 template <int HDP> struct Cfg {
     static constexpr int ST = HDP == 128 ? 2 : 4, SUB = HDP / 64, TILE = KT * HDP * 2;
     static constexpr int SMEM = 1024 + (2 * ST + 2) * TILE;
 };
-SB_DEV void mbar_init(uint64_t *mb, unsigned count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(ap_smem(mb)), "r"(count) : "memory");
-}
-SB_DEV void mbar_arrive(uint64_t *mb) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ap_smem(mb)) : "memory");
-}
-SB_DEV unsigned long long now() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-SB_DEV bool mbar_try(uint64_t *mb, unsigned ph) {
-    unsigned done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done)
-                 : "r"(ap_smem(mb)), "r"(ph)
-                 : "memory");
-    return done;
-}
-// false after WAIT_NS, or (abortable) once any wait has given up
-SB_DEV bool mbar_wait(uint64_t *mb, unsigned ph, bool abortable = true) {
-    if (mbar_try(mb, ph)) return true;
-    unsigned long long t0 = 0;
-#pragma unroll 1
-    for (int spin = 0; spin < (1 << 26); spin++) {
-        if (mbar_try(mb, ph)) return true;
-        if ((spin & 1023) == 1023) {
-            if (abortable && *(volatile int *)&tc_err) return false;
-            const unsigned long long t = now();
-            if (t0 == 0) t0 = t;
-            else if (t - t0 > WAIT_NS) break;
-        }
-    }
-    atomicExch(&tc_err, 1);
-    return false;
-}
-SB_DEV void expect_tx(uint64_t *mb, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(ap_smem(mb)), "r"(bytes) : "memory");
-}
-// box {64 values, one head, rows of a page, one page}
-SB_DEV void tma_rows(unsigned dst, const CUtensorMap *tm, int d, int head, int row, int page, uint64_t *mb) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(tm), "r"(d), "r"(head), "r"(row), "r"(page), "r"(ap_smem(mb))
-        : "memory");
-}
 // the same for a converged warp, one answer for all lanes
-SB_DEV bool warp_wait(uint64_t *mb, unsigned ph, bool abortable = true) { return __all_sync(SB_FULL, mbar_wait(mb, ph, abortable)); }
+SB_DEV bool warp_wait(uint64_t *mb, unsigned ph, bool abortable = true) { return __all_sync(SB_FULL, ap_bar_wait(mb, ph, abortable)); }
 SB_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 SB_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-SB_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // 128-byte swizzled operand: rows (K-major: query rows or keys; MN-major: keys)
 // of 128 bytes, 8-row atoms 1024 bytes apart, 64-value column blocks 16 KB apart
 SB_DEV uint64_t desc(unsigned addr) {
@@ -235,17 +185,17 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
 
     if (tid == 0) {
         for (int s = 0; s < ST; s++) {
-            mbar_init(&kfull[s], 2);
-            mbar_init(&vfull[s], 2);
-            mbar_init(&kempty[s], 1);
-            mbar_init(&vempty[s], 1);
+            ap_bar_init(&kfull[s], 2);
+            ap_bar_init(&vfull[s], 2);
+            ap_bar_init(&kempty[s], 1);
+            ap_bar_init(&vempty[s], 1);
         }
         for (int x = 0; x < 2; x++) {
-            mbar_init(&sfull[x], 1);
-            mbar_init(&pfull[x], 4);
+            ap_bar_init(&sfull[x], 1);
+            ap_bar_init(&pfull[x], 4);
         }
-        mbar_init(&ofull, 1);
-        mbar_init(&qfull, 4 * nx);
+        ap_bar_init(&ofull, 1);
+        ap_bar_init(&qfull, 4 * nx);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 12) {
@@ -291,10 +241,10 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 any_tma = true;
                 if (lane == 0) {
                     if (is_k) *reinterpret_cast<uint2 *>(&valid_s[t % (2 * ST)][(warp & 1) * 2]) = make_uint2(~0u, ~0u);
-                    expect_tx(&full[s], 64 * HDP * 2);
+                    ap_expect(&full[s], 64 * HDP * 2);
                 }
                 __syncwarp();
-                if (mine) tma_rows(stage + sub * 16384 + (p0 + row) * 128, tm, sub * 64, it.kvh, in_page, page, &full[s]);
+                if (mine) ap_tma(stage + sub * 16384 + (p0 + row) * 128, tm, sub * 64, it.kvh, in_page, page, &full[s]);
                 continue;
             }
 #pragma unroll 1
@@ -314,13 +264,13 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             }
             ap_commit();
             ap_wait<0>();
-            fence_async();
+            ap_fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&full[s]);
+            if (lane == 0) ap_arrive(&full[s]);
         }
         ap_wait<0>();
         if (!ok && any_tma)  // given up: the copies that were issued still have to land
-            for (int i = t > ST ? t - ST : 0; i < t; i++) mbar_wait(&full[i % ST], (i / ST) & 1, false);
+            for (int i = t > ST ? t - ST : 0; i < t; i++) ap_bar_wait(&full[i % ST], (i / ST) & 1, false);
     } else if (warp >= 12) {
         ATC_FEWER;
         if (tid == 12 * 32) {
@@ -337,7 +287,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 }
                 commit(&sfull[x]);
             };
-            bool ok = nt > 0 && mbar_wait(&qfull, 0) && mbar_wait(&kfull[0], 0);
+            bool ok = nt > 0 && ap_bar_wait(&qfull, 0) && ap_bar_wait(&kfull[0], 0);
             if (ok) {
                 fence_after();
                 for (int x = 0; x < nx; x++) scores(x, 0);
@@ -349,10 +299,10 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 const int s1 = s + 1 == ST ? 0 : s + 1;
                 const unsigned ph1 = s1 ? ph : ph ^ 1;
                 const bool more = t + 1 < nt;
-                ok = mbar_wait(&vfull[s], ph) && (!more || mbar_wait(&kfull[s1], ph1));
+                ok = ap_bar_wait(&vfull[s], ph) && (!more || ap_bar_wait(&kfull[s1], ph1));
 #pragma unroll 1
                 for (int x = 0; x < nx && ok; x++) {
-                    ok = mbar_wait(&pfull[x], t & 1);
+                    ok = ap_bar_wait(&pfull[x], t & 1);
                     if (!ok) break;
                     fence_after();
                     const uint64_t vs = vd + s * (TILE >> 4);
@@ -390,9 +340,9 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                              "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
                              : "memory");
             }
-            fence_async();
+            ap_fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&qfull);
+            if (lane == 0) ap_arrive(&qfull);
         }
         float m = -INFINITY, l = 0.f;
         bool ok = true;
@@ -447,10 +397,10 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             wait_st();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&pfull[x]);
+            if (lane == 0) ap_arrive(&pfull[x]);
         }
         if (m == INFINITY) l = __int_as_float(0x7fc00000);  // an infinite score: NaN, as its softmax
-        ok = __all_sync(SB_FULL, mbar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
+        ok = __all_sync(SB_FULL, ap_bar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
         fence_after();
         const bool live = f < it.F && ok;
         if (live) ap_row_stats(P, it, f, m, l);
@@ -485,7 +435,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
     __syncthreads();
     if (warp == 12) {
         fence_after();
-        mbar_wait(&ofull, 0, false);
+        ap_bar_wait(&ofull, 0, false);
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }

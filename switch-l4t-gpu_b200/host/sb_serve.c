@@ -358,16 +358,27 @@ static int pages_for_attn(const sb_kv_pages *kv, struct attn_pages *p) {
     return 0;
 }
 
-/* pages as {HD, heads, positions, pages}, boxes of 64 values of one head of
- * `box` positions, 128-byte swizzle; what is past HD reads as zero */
-static int encode_pages(CUtensorMap *tm, const void *base, const sb_kv_pages *kv, int box) {
+/* Tensor maps of K and V pages, {HD, heads, positions, pages} with boxes of 128
+ * bytes of one head x `box` positions, 128-byte swizzle; what is past HD reads
+ * as zero.  Returns the box: pages, or parts of `most` positions of one (a
+ * smaller page must divide it, and hold eight positions: the swizzle's
+ * period); 0 where pages of this size, or strides that a map cannot hold, go
+ * through the kernels' own copies. */
+static int encode_pages(CUtensorMap *tk, CUtensorMap *tv, const sb_kv_pages *kv, int most) {
+    const int e = type_size(kv->type), box = kv->page % most == 0 ? most : most % kv->page == 0 && kv->page >= 8 ? kv->page : 0;
     const cuuint64_t dims[4] = {(cuuint64_t)kv->HD, (cuuint64_t)kv->NKV, (cuuint64_t)kv->page, (cuuint64_t)kv->n_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)kv->head_stride * 2, (cuuint64_t)kv->pos_stride * 2, (cuuint64_t)kv->page_stride * 2};
-    const cuuint32_t size[4] = {64, 1, (cuuint32_t)box, 1}, estr[4] = {1, 1, 1, 1};
-    return cuTensorMapEncodeTiled(tm, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, (void *)base, dims, strides, size, estr,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t strides[3] = {(cuuint64_t)kv->head_stride * e, (cuuint64_t)kv->pos_stride * e, (cuuint64_t)kv->page_stride * e};
+    const cuuint32_t size[4] = {(cuuint32_t)(128 / e), 1, (cuuint32_t)box, 1}, estr[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = e == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    for (int i = 0; box && i < 2; i++)
+        if (cuTensorMapEncodeTiled(i ? tv : tk, type, 4, i ? kv->v : kv->k, dims, strides, size, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return 0;
+    return box;
 }
+/* positions of a box: what one warp of the kernel loads at a time */
+static int attn_box(const struct attn_part *a, int type, int HD) { return a->threads == 512 ? 64 : type == SB_F32 && HD > 64 ? 8 : 16; }
 
 int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
                    int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
@@ -439,28 +450,22 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     p.tiles2 = own.tiles;
     p.items1 = (int)pre.grid;
     p.scale_log2 = scale * 1.4426950408889634f;
-    void *args[] = {&p};
-    if (pre.S && pre.threads == 512) {
-        CUtensorMap tk, tv;
-        /* whole pages (or 64-position parts of one) by TMA, in at most 32 boxes
-         * of a warp; other page sizes, and strides that a map cannot hold, by
-         * the kernel's own copies (box 0) */
-        const int pg = prefix->page;
-        int box = pg % 64 == 0 ? 64 : 64 % pg == 0 && pg >= 8 ? pg : 0;
-        if (!encode_pages(&tk, prefix->k, prefix, box ? box : 1) || !encode_pages(&tv, prefix->v, prefix, box ? box : 1)) {
-            box = 0;
-            memset(&tk, 0, sizeof tk);
-            memset(&tv, 0, sizeof tv);
-        }
-        void *tc_args[] = {&p, &tk, &tv, &box};
-        rc = sb_launch(c, pre.f, (unsigned)pre.grid, 1, pre.threads, pre.smem, (CUstream)stream, tc_args, 0);
-    } else if (pre.S) {
-        const long both = pre.f == own.f ? pre.grid + own.grid : pre.grid;
-        rc = sb_launch(c, pre.f, (unsigned)both, 1, pre.threads, pre.smem, (CUstream)stream, args, 0);
+    CUtensorMap tk, tv;
+    int box = 0;
+    memset(&tk, 0, sizeof tk);
+    memset(&tv, 0, sizeof tv);
+    void *args[] = {&p, &tk, &tv, &box};
+    if (pre.S) {
+        const int together = pre.f == own.f;
+        /* two maps cost a microsecond of the host: not for a call that is over
+         * in a few, nor for one whose two parts have pools of their own */
+        if (!together && pre.grid * (long)pre.chunk >= SB_ATTN_TMA_KEYS) box = encode_pages(&tk, &tv, prefix, attn_box(&pre, type, HD));
+        rc = sb_launch(c, pre.f, (unsigned)(pre.grid + (together ? own.grid : 0)), 1, pre.threads, pre.smem, (CUstream)stream, args, 0);
+        if (rc) return rc;
     }
-    if (rc) return rc;
     if (own.S && own.f != pre.f) { /* beside the prefix launch's last items */
-        p.items1 = 0;
+        p.items1 = box = 0;
+        if (own.grid * (long)own.chunk >= SB_ATTN_TMA_KEYS) box = encode_pages(&tk, &tv, kv, attn_box(&own, type, HD));
         rc = sb_launch(c, own.f, (unsigned)own.grid, 1, own.threads, own.smem, (CUstream)stream, args, pre.S > 0);
         if (rc) return rc;
     }
