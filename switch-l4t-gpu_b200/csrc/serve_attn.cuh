@@ -37,7 +37,7 @@ __device__ int tc_err;  // nonzero after a wait timed out
 struct AttnPages {  // strides in elements
     const void *k, *v;
     long long page_stride, pos_stride, head_stride;
-    int n_pages, page;
+    int n_pages, page, shift;  // shift: log2 of the page, -1 where it is no power of two
 };
 // parameter block, mirrored by the host (host/sb_serve.c)
 struct AttnParams {
@@ -64,14 +64,17 @@ struct AttnItem {
     int row0;        // query row of f = 0
     int vis0;        // positions that f sees: clamp(vis0 + f / G, 0, vis1)  (prefix: vis0 = vis1 = P, step 0)
     int vis1, step;
+    bool one;        // F <= G: every f is of query row 0
 };
 
 SB_DEV int ap_rows(const AttnParams &P) { return P.cu_q ? min(max(P.cu_q[P.B], 0), P.T) : P.T; }
-SB_DEV int ap_vis(const AttnItem &it, int f, int G) { return min(max(it.vis0 + it.step * (f / G), 0), it.vis1); }
+SB_DEV int ap_row(const AttnItem &it, int f, int G) { return it.one ? 0 : f / G; }
+SB_DEV int ap_vis(const AttnItem &it, int f, int G) { return min(max(it.vis0 + it.step * ap_row(it, f, G), 0), it.vis1); }
+SB_DEV int ap_page(const AttnPages &pg, int p) { return pg.shift >= 0 ? p >> pg.shift : p / pg.page; }
 
 // Item `idx` of the prefix (row tiles fastest: neighbours read the same keys)
 SB_DEV bool ap_prefix_item(const AttnParams &P, int idx, int MT, AttnItem &it) {
-    const int tile = idx % P.tiles1, rest = idx / P.tiles1;
+    const int rest = P.tiles1 > 1 ? idx / P.tiles1 : idx, tile = idx - rest * P.tiles1;
     it.kvh = rest % P.NKV;
     it.slot = rest / P.NKV;
     it.pg = P.pre;
@@ -83,16 +86,17 @@ SB_DEV bool ap_prefix_item(const AttnParams &P, int idx, int MT, AttnItem &it) {
     it.row0 = 0;
     it.vis0 = it.vis1 = P.P;
     it.step = 0;
+    it.one = it.F <= P.G;
     return it.f0 < it.F;
 }
 // Request of item `idx`, its key head and key range; row tiles are looped by the caller
 SB_DEV bool ap_own_item(const AttnParams &P, int idx, int MT, AttnItem &it, int &tile) {
-    const int s = idx % P.S2;
-    int rest = idx / P.S2;
-    tile = rest % P.tiles2;
-    rest /= P.tiles2;
-    it.kvh = rest % P.NKV;
-    const int b = rest / P.NKV;
+    int rest = P.S2 > 1 ? idx / P.S2 : idx;
+    const int s = idx - rest * P.S2;
+    const int pair = P.tiles2 > 1 ? rest / P.tiles2 : rest;
+    tile = rest - pair * P.tiles2;
+    const int b = P.NKV > 1 ? pair / P.NKV : pair;
+    it.kvh = pair - b * P.NKV;
     int q0 = b, q1 = b + 1;
     if (P.cu_q) {
         q0 = min(max(P.cu_q[b], 0), P.T);
@@ -109,12 +113,18 @@ SB_DEV bool ap_own_item(const AttnParams &P, int idx, int MT, AttnItem &it, int 
     it.vis0 = len - n + 1;
     it.vis1 = len;
     it.step = 1;
-    const int used = max(1, (len + P.chunk2 - 1) / P.chunk2);
+    it.one = it.F <= P.G;
+    const int used = P.S2 > 1 ? max(1, (len + P.chunk2 - 1) / P.chunk2) : 1;
     if (s == 0 && it.kvh == 0 && P.ws_n)
         for (int r = q0 + tile * (int)blockDim.x + (int)threadIdx.x; r < q1; r += P.tiles2 * (int)blockDim.x) P.ws_n[r] = used;
     return s < used;
 }
 
+SB_DEV float ap_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 SB_DEV unsigned ap_smem(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
 SB_DEV void ap_cp16(unsigned dst, const void *src, bool ok) {  // 16 bytes, or zeros (nothing is read)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
@@ -180,7 +190,7 @@ struct ApBars {
 // bit set (offsets are multiples of 16 bytes), 0 where it has none
 SB_DEV long long ap_offset(const AttnItem &it, int p) {
     if (p >= it.k1) return 0;
-    const int j = p / it.pg.page;
+    const int j = ap_page(it.pg, p);
     const int pg = it.table ? it.table[j] : j;
     if (pg < 0 || pg >= it.pg.n_pages) return 0;
     return (pg * it.pg.page_stride + (p - j * it.pg.page) * it.pg.pos_stride) | 1;
@@ -254,7 +264,7 @@ template <int KW, int HDP, int E, int ST> struct ApRing {
         const int p = first + t * KT + row;
         pg = -1;
         if (mine && p - row + KW <= it.k1) {
-            const int j = p / it.pg.page;
+            const int j = ap_page(it.pg, p);
             pg = it.table ? it.table[j] : j;
             in_pg = p - j * it.pg.page;
         }
@@ -303,7 +313,7 @@ template <int KW, int HDP, int E, int ST> struct ApRing {
 
 // what a finished row leaves: the output itself where the item is the only one, else its part
 SB_DEV void ap_row_stats(const AttnParams &P, const AttnItem &it, int f, float m, float l) {
-    const int row = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
+    const int qr = ap_row(it, f, P.G), row = it.row0 + qr, head = it.kvh * P.G + f - qr * P.G;
     if (P.S1 + P.S2 == 1) {
         if (P.lse) P.lse[(long long)row * P.NH + head] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
     } else {
@@ -320,12 +330,55 @@ template <> SB_DEV void ap_store2<__nv_bfloat16>(__nv_bfloat16 *p, float a, floa
 template <typename T>
 SB_DEV void ap_row_out(const AttnParams &P, const AttnItem &it, int f, int d, float a, float b, float l) {
     if (d >= P.HD) return;
-    const int row = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
+    const int qr = ap_row(it, f, P.G), row = it.row0 + qr, head = it.kvh * P.G + f - qr * P.G;
     if (P.S1 + P.S2 == 1) {
         const float w = l == 0.f ? 0.f : 1.f / l;
         ap_store2<T>(static_cast<T *>(P.out) + row * P.o_row + head * P.o_head + d, a * w, b * w);
     } else if (l != 0.f) {  // the join skips parts without weight
         ap_store2<float>(P.ws_o + (((long long)it.slot * P.T + row) * P.NH + head) * P.HD + d, a, b);
+    }
+}
+
+template <typename T> SB_DEV const T *ap_query(const AttnParams &P, const AttnItem &it, int f) {
+    const int qr = ap_row(it, f, P.G);
+    return static_cast<const T *>(P.q) + (long long)(it.row0 + qr) * P.q_row + (it.kvh * P.G + f - qr * P.G) * P.q_head;
+}
+template <typename T> SB_DEV void ap_store4(T *p, float a, float b, float c, float d) {
+    ap_store2<T>(p, a, b);
+    ap_store2<T>(p + 2, c, d);
+}
+template <> SB_DEV void ap_store4<float>(float *p, float a, float b, float c, float d) { *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d); }
+// The warps of a block join: o [warps][R][HDP], (m, l) [warps][R]; four values a thread.
+template <typename T, int HDP, int R>
+SB_DEV void ap_block_join(const AttnParams &P, const AttnItem &it, const float *o, const float (*ms)[R], const float (*ls)[R]) {
+    constexpr int NW = SB_AP_THREADS / 32;
+    for (int i = threadIdx.x; i < R * HDP / 4; i += SB_AP_THREADS) {
+        const int r = i / (HDP / 4), d = (i % (HDP / 4)) * 4, f = it.f0 + r;
+        if (f >= it.F) break;
+        if (d >= P.HD) continue;
+        float M = ms[0][r], L = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, ms[w][r]);
+        const float base = M == -INFINITY ? 0.f : M;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float e = ap_exp2(ms[w][r] - base);
+            const float4 x = *reinterpret_cast<const float4 *>(o + (w * R + r) * HDP + d);
+            L = fmaf(e, ls[w][r], L);
+            a.x = fmaf(e, x.x, a.x);
+            a.y = fmaf(e, x.y, a.y);
+            a.z = fmaf(e, x.z, a.z);
+            a.w = fmaf(e, x.w, a.w);
+        }
+        const int qr = ap_row(it, f, P.G), row = it.row0 + qr, head = it.kvh * P.G + f - qr * P.G;
+        if (d == 0) ap_row_stats(P, it, f, M, L);
+        if (P.S1 + P.S2 == 1) {
+            const float w = L == 0.f ? 0.f : 1.f / L;
+            ap_store4<T>(static_cast<T *>(P.out) + row * P.o_row + head * P.o_head + d, a.x * w, a.y * w, a.z * w, a.w * w);
+        } else if (L != 0.f) {
+            ap_store4<float>(P.ws_o + (((long long)it.slot * P.T + row) * P.NH + head) * P.HD + d, a.x, a.y, a.z, a.w);
+        }
     }
 }
 
@@ -358,11 +411,6 @@ SB_DEV void ap_ldsm_t(unsigned (&r)[4], unsigned addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
-SB_DEV float ap_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // 64-row tiles, a warp 16 rows against all keys.  HDP: head size padded to 64
 // or 128.  Shared memory: SB_AP_ST x 2 x 64 x HDP x 2 bytes, rows of 128 / 256
@@ -383,7 +431,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
     for (int h = 0; h < 2; h++) {
         const int f = fw + g + 8 * h;
         vis[h] = f < it.F ? ap_vis(it, f, P.G) : 0;
-        const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
+        const T *qp = ap_query<T>(P, it, f);
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -524,7 +572,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         const int f = it.f0 + b * 8 + g;
-        const T *qp = static_cast<const T *>(P.q) + (long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head;
+        const T *qp = ap_query<T>(P, it, f);
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -658,24 +706,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             }
         }
     __syncthreads();
-    for (int i = tid; i < 8 * NB * HDP / 2; i += 32 * NW) {
-        const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
-        if (f >= it.F) break;
-        float M = ms[0][r], L = 0.f, a = 0.f, b = 0.f;
-#pragma unroll
-        for (int w = 1; w < NW; w++) M = fmaxf(M, ms[w][r]);
-        const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            const float e = ap_exp2(ms[w][r] - base);
-            const float2 x = *reinterpret_cast<const float2 *>(ow + (w * 8 * NB + r) * HDP + d);
-            L += e * ls[w][r];
-            a += e * x.x;
-            b += e * x.y;
-        }
-        if (d == 0) ap_row_stats(P, it, f, M, L);
-        ap_row_out<T>(P, it, f, d, a, b, L);
-    }
+    ap_block_join<T, HDP, 8 * NB>(P, it, ow, ms, ls);
 }
 
 // ---------------------------------------------------------------- FP32
@@ -702,9 +733,11 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = lane % KW, dq = lane / KW;
     ApRing<KW, HDP, 4, ST> ring(it, P.HD, sm, bars, seq, tm_k, tm_v, box);
     __syncthreads();  // an earlier item's shared memory is no longer read
-    for (int i = tid; i < MT * HDP; i += 32 * NW) {
-        const int r = i / HDP, d = i % HDP, f = it.f0 + r;
-        q_s[r][d / 32][d % 32] = f < it.F && d < P.HD ? static_cast<const float *>(P.q)[(long long)(it.row0 + f / P.G) * P.q_row + (it.kvh * P.G + f % P.G) * P.q_head + d] * P.scale_log2 : 0.f;
+    for (int i = tid; i < MT * HDP / 4; i += SB_AP_THREADS) {
+        const int r = i / (HDP / 4), d = i % (HDP / 4) * 4, f = it.f0 + r;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (f < it.F && d < P.HD) v = *reinterpret_cast<const float4 *>(ap_query<float>(P, it, f) + d);
+        *reinterpret_cast<float4 *>(&q_s[r][d / 32][d % 32]) = make_float4(v.x * P.scale_log2, v.y * P.scale_log2, v.z * P.scale_log2, v.w * P.scale_log2);
     }
     if (tid < MT) vis_s[tid] = it.f0 + tid < it.F ? ap_vis(it, it.f0 + tid, P.G) : 0;
     const int flast = min(it.f0 + MT, it.F) - 1;
@@ -830,25 +863,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
         for (int e = 0; e < DP; e++) *reinterpret_cast<unsigned long long *>(red + (warp * MT + r) * HDP + lane * (2 * DP) + 2 * e) = o[r][e];
     }
     __syncthreads();
-    for (int i = tid; i < MT * HDP / 2; i += 32 * NW) {
-        const int r = i / (HDP / 2), d = (i % (HDP / 2)) * 2, f = it.f0 + r;
-        if (f >= it.F) break;
-        float M = m_s[0][r];
-#pragma unroll
-        for (int w = 1; w < NW; w++) M = fmaxf(M, m_s[w][r]);
-        const float base = M == -INFINITY ? 0.f : M;
-        float L = 0.f, a = 0.f, b = 0.f;
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            const float e = ap_exp2(m_s[w][r] - base);
-            const float2 x = *reinterpret_cast<const float2 *>(red + (w * MT + r) * HDP + d);
-            L = fmaf(e, l_s[w][r], L);
-            a = fmaf(e, x.x, a);
-            b = fmaf(e, x.y, b);
-        }
-        if (d == 0) ap_row_stats(P, it, f, M, L);
-        ap_row_out<float>(P, it, f, d, a, b, L);
-    }
+    ap_block_join<float, HDP, MT>(P, it, red, m_s, l_s);
 }
 
 // A CTA an item: the prefix items of the launch, then own ones (either may be

@@ -214,7 +214,7 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
 struct attn_pages {
     CUdeviceptr k, v;
     int64_t page_stride, pos_stride, head_stride;
-    int n_pages, page;
+    int n_pages, page, shift;
 };
 struct attn_params {
     CUdeviceptr q, out, lse, cu_q, ptable, table, kv_len, ws_o, ws_ml, ws_n;
@@ -355,6 +355,9 @@ static int pages_for_attn(const sb_kv_pages *kv, struct attn_pages *p) {
     p->head_stride = kv->head_stride;
     p->n_pages = kv->n_pages;
     p->page = kv->page;
+    p->shift = -1;
+    for (int i = 0; i < 31; i++)
+        if (kv->page == 1 << i) p->shift = i;
     return 0;
 }
 
