@@ -334,7 +334,8 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 const int r = (warp & 3) * 32 + i * RPI + lane / CH, fr = it.f0 + x * BM + r;
                 uint4 v = make_uint4(0u, 0u, 0u, 0u);
                 if (fr < it.F && c * 8 < P.HD)
-                    v = *reinterpret_cast<const uint4 *>(ap_query<T>(P, it, fr) + c * 8);
+                    v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(P.q) + (long long)(it.row0 + fr / P.G) * P.q_row +
+                                                         (it.kvh * P.G + fr % P.G) * P.q_head + c * 8);
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qst + x * TILE + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
                              "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
                              : "memory");
