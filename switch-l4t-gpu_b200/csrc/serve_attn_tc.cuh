@@ -198,6 +198,10 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         ap_bar_init(&qfull, 4 * nx);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (tid == 32 * 8 && box) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(tm_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(tm_v) : "memory");
+    }
     if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(ap_smem(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -224,15 +228,20 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         const int pieces = box ? 64 / box : 1, sub = lane / pieces, row = lane % pieces * box;
         const bool mine = box && sub < C::SUB;
         bool ok = true, any_tma = false;
-        int t = 0;
-        for (; t < nt; t++) {
-            const int s = t % ST, key = it.k0 + t * KT + p0;
-            int page = -1, in_page = 0;
-            if (mine && key + 64 <= it.k1) {
-                const int j = ap_page(it.pg, key + row);
-                page = it.table ? it.table[j] : j;
-                in_page = key + row - j * it.pg.page;
+        int t = 0, next = -1, in_next = 0;
+        auto look = [&](int t) {  // a tile ahead of its use
+            const int p = it.k0 + t * KT + p0;
+            next = -1;
+            if (mine && p + 64 <= it.k1) {
+                const int j = ap_page(it.pg, p + row);
+                next = it.table ? it.table[j] : j;
+                in_next = p + row - j * it.pg.page;
             }
+        };
+        look(0);
+        for (; t < nt; t++) {
+            const int s = t % ST, key = it.k0 + t * KT + p0, page = next, in_page = in_next;
+            look(t + 1);
             const bool by_tma = __all_sync(SB_FULL, box && (!mine || (page >= 0 && page < it.pg.n_pages)));
             if (t >= ST) ok = warp_wait(&empty[s], (unsigned)((t / ST) - 1) & 1u);
             if (!ok) break;
@@ -325,20 +334,30 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         const int x = warp >> 2, f = it.f0 + tid;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
         const float sc = fabsf(P.scale_log2);
-        {  // this warp's 32 query rows, neighbouring lanes on one row; negated for a negative scale, zeros behind the last
+        {  // this warp's 32 query rows, neighbouring lanes on one row, zeros behind the last.  A short loop: code that
+           // runs once costs six cycles an instruction to fetch
             constexpr int CH = HDP / 8, RPI = 32 / CH;
-            const int c = lane % CH;
-            const unsigned flip = P.scale_log2 < 0.f ? 0x80008000u : 0u;
-#pragma unroll
+            const int c = lane % CH, qr = f / P.G;
+            const long long at = f < it.F ? ((long long)(it.row0 + qr) * P.q_row + (it.kvh * P.G + f - qr * P.G) * P.q_head) | 1 : 0;
+            const T *col = static_cast<const T *>(P.q) + c * 8;
+            const unsigned dst = qst + x * TILE + (c >> 3) * 16384 + (warp & 3) * 4096;
+#pragma unroll 1
             for (int i = 0; i < CH; i++) {
-                const int r = (warp & 3) * 32 + i * RPI + lane / CH, fr = it.f0 + x * BM + r;
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (fr < it.F && c * 8 < P.HD)
-                    v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(P.q) + (long long)(it.row0 + fr / P.G) * P.q_row +
-                                                         (it.kvh * P.G + fr % P.G) * P.q_head + c * 8);
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(qst + x * TILE + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                             "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip)
-                             : "memory");
+                const int r = i * RPI + lane / CH;
+                const long long o = __shfl_sync(SB_FULL, at, r);
+                ap_cp16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), col + (o & ~1ll), (o & 1) && c * 8 < P.HD);
+            }
+            ap_commit();
+            ap_wait<0>();
+            __syncwarp();
+            if (P.scale_log2 < 0.f) {  // maxima are taken of the scores: a negative scale turns the queries round
+#pragma unroll 1
+                for (int i = 0; i < HDP / 2; i++) {  // this lane's row: 32 x 4 bytes of each column block
+                    const unsigned a = qst + x * TILE + (i >> 5) * 16384 + (warp & 3) * 4096 + lane * 128 + (i & 31) * 4;
+                    unsigned v;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+                    asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v ^ 0x80008000u) : "memory");
+                }
             }
             ap_fence_async();
             __syncwarp();

@@ -176,7 +176,6 @@ int sb_occupancy_of(sb_ctx *c, sb_fn_id f, int block, size_t smem);
 #define SB_ATTN_MAX_SPLITS 128     /* key ranges of the prefix, and of a request's own keys */
 #define SB_ATTN_ITEM 3             /* fixed cost of an attention item in key tiles */
 #define SB_ATTN_TMA_KEYS 32768      /* keys of all items from which their pages come by TMA */
-#define SB_ATTN_TC_ROWS 128         /* query rows of a key head from which the tcgen05 kernel takes the prefix */
 #define SB_LOGPROBS_THREADS 128     /* LP_THREADS in csrc/score_kernels.cu */
 #define SB_LOGPROBS_MAX_PARTS 128   /* parts of a row: one a thread of the join */
 

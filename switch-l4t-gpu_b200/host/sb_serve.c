@@ -235,8 +235,10 @@ struct attn_part {
 /* The kernel for `rows` query rows of a key head.  FP32: row tiles of 1, 2,
  * 4, 8 or 16, the smallest that holds them (unused rows cost FMAs).  16-bit
  * types: a tile of 8 or 16 rows (the four warps split the keys) while it holds
- * all rows, 64-row tiles up to SB_ATTN_TC_ROWS, and for a prefix behind more
- * rows the tcgen05 kernel's 256. */
+ * all rows; beyond that the prefix goes to the tcgen05 kernel's 256 rows, most
+ * of them empty at first (20 rows behind 300 keys, 32/8 heads of 128: 12.5
+ * against 15.1 us for 64-row tiles of mma.sync; 100 behind 16000: 27.6 against
+ * 49.5), and own rows, each with its own limit, to 64-row tiles. */
 static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_part *a) {
     const int wide = HD > 64, second = type == SB_BF16;
     a->threads = 128;
@@ -247,7 +249,7 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
         a->f = (sb_fn_id)(F_ATTN_F32_64_R1 + 5 * wide + i);
         a->rows = 1 << i;
         a->step = wide ? 32 : 64;
-    } else if (prefix && rows >= SB_ATTN_TC_ROWS) {
+    } else if (prefix && rows > 16) {
         a->f = (sb_fn_id)(F_ATTN_TC_F16_64 + 2 * second + wide);
         a->smem = 1024 + (wide ? 6 * 32768 : 10 * 16384);
         a->threads = 512;
@@ -264,19 +266,22 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
     }
     a->tiles = (int)CEIL_DIV(rows, a->rows);
 }
-/* Key ranges of `keys` keys for `units` independent (head, row tile) pairs.
- * An item of n tiles of keys costs about n + SB_ATTN_ITEM tile times (its
- * queries, its part to write and join), and the launch as many rounds of
- * items as the SMs need: the count with the least of that is taken.  `fill`:
- * how many items stand for one that is there (requests are shorter than the
- * longest, their last ranges empty).  `alone`: one range would need no join. */
-static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, int fill, int alone) {
+/* Key ranges of `keys` keys for `units` independent (head, row tile) pairs,
+ * the count with the least cost in tile times: an item of n tiles of keys
+ * takes about n + SB_ATTN_ITEM of them (its queries, its part to write), the
+ * launch as many rounds of items as the SMs need, and every part of `bytes` is
+ * written and read again by the join (a tile takes 0.5 us, 2 us on the
+ * tcgen05 kernel; parts move at about 4 MB / us).  `fill`: how many items
+ * stand for one that is there (requests are shorter than the longest, their
+ * last ranges empty).  `alone`: one range would need no join. */
+static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, long bytes, int fill, int alone) {
     const long cap = (long)fill * c->sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
+    const long move = a->threads == 512 ? 8L << 20 : 2L << 20;
     long best = 0, best_cost = 0;
     for (long S = 1; S <= SB_ATTN_MAX_SPLITS && S <= tiles; S++) {
-        const long n = CEIL_DIV(tiles, S), items = units * CEIL_DIV(tiles, n);
-        const long parts = CEIL_DIV(tiles, n);
-        const long cost = CEIL_DIV(items, cap) * (n + SB_ATTN_ITEM) + parts / 8 + (alone && parts > 1 ? SB_ATTN_ITEM : 0);
+        const long n = CEIL_DIV(tiles, S), parts = CEIL_DIV(tiles, n), items = units * parts;
+        const long cost = 16 * CEIL_DIV(items, cap) * (n + SB_ATTN_ITEM) + 2 * parts + 16 * parts * bytes / move +
+                          (alone && parts > 1 ? 16 * SB_ATTN_ITEM : 0);
         if (!best || cost < best_cost) {
             best = n;
             best_cost = cost;
@@ -289,16 +294,16 @@ static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, int
 }
 static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD, int max_q, int P, int max_kv,
                       struct attn_part *pre, struct attn_part *own) {
-    const long G = NH / NKV;
+    const long G = NH / NKV, bytes = (long)T * NH * HD * 8;
     memset(pre, 0, sizeof *pre);
     memset(own, 0, sizeof *own);
     if (P > 0) {
         attn_kernel(type, HD, T * G, 1, pre);
-        attn_split(c, pre, P, (long)pre->tiles * NKV, 1, max_kv == 0);
+        attn_split(c, pre, P, (long)pre->tiles * NKV, bytes, 1, max_kv == 0);
     }
     if (max_kv > 0) {
         attn_kernel(type, HD, max_q * G, 0, own);
-        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, 2, P == 0);
+        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, bytes, 2, P == 0);
     }
     if (P > 0 && max_kv > 0 && pre->f != own->f && pre->threads == 128 && pre->rows > own->rows &&
         pre->grid + own->grid <= (long)c->sms * sb_occupancy_of(c, pre->f, 128, pre->smem)) {
@@ -310,7 +315,7 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
         own->smem = pre->smem;
         own->rows = pre->rows;
         own->tiles = tiles;
-        attn_split(c, own, max_kv, (long)tiles * NKV * B, 2, 0);
+        attn_split(c, own, max_kv, (long)tiles * NKV * B, bytes, 2, 0);
     }
     SB_ARG(pre->grid + own->grid < 0x7fffffffL, "attn_prefix: too many rows for one launch");
     return 0;
@@ -461,8 +466,9 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     if (pre.S) {
         const int together = pre.f == own.f;
         /* two maps cost a microsecond of the host: not for a call that is over
-         * in a few, nor for one whose two parts have pools of their own */
-        if (!together && pre.grid * (long)pre.chunk >= SB_ATTN_TMA_KEYS) box = encode_pages(&tk, &tv, prefix, attn_box(&pre, type, HD));
+         * in a few, nor for one whose two parts have pools of their own.  The
+         * tcgen05 kernel's own copies take longer than that */
+        if (!together && (pre.threads == 512 || pre.grid * (long)pre.chunk >= SB_ATTN_TMA_KEYS)) box = encode_pages(&tk, &tv, prefix, attn_box(&pre, type, HD));
         rc = sb_launch(c, pre.f, (unsigned)(pre.grid + (together ? own.grid : 0)), 1, pre.threads, pre.smem, (CUstream)stream, args, 0);
         if (rc) return rc;
     }
