@@ -928,40 +928,53 @@ SB_AP_F32(attn_f32_128_r16, 128, 16)
 
 // ---------------------------------------------------------------- join
 // A warp a (row, head): parts of the prefix, then those of the request's own
-// keys that are in use.  Four values a lane; head sizes up to 64, 32, ... let
-// 2, 4, ... groups of lanes take parts side by side.  A part without weight
-// may not have been written and is not read.
+// keys that are in use, 32 at a time, a lane's weight each; then four values a
+// lane, where head sizes up to 64, 32, ... let 2, 4, ... groups of lanes take
+// parts side by side.  A part without weight may not have been written and
+// does not count.  Bound by latency: the row count, the row's own parts and
+// the parts' maxima and sums are read at once, then the parts themselves.
 // type: 0 f32, 1 f16, 2 bf16.
 extern "C" __global__ void __launch_bounds__(128) attn_join(const __grid_constant__ AttnParams P, int type) {
     const int lane = threadIdx.x & 31;
     const int width = P.HD > 64 ? 32 : P.HD > 32 ? 16 : P.HD > 16 ? 8 : 4, groups = 32 / width, d = (lane & (width - 1)) * 4;
+    const long long TH = (long long)P.T * P.NH;
     pdl_wait();
-    const long long rows = (long long)ap_rows(P) * P.NH, TH = (long long)P.T * P.NH;
-    for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); i < rows; i += (long long)gridDim.x * 4) {
-        const int row = (int)(i / P.NH), head = (int)(i % P.NH);
-        const int n = P.S1 + (P.S2 ? P.ws_n[row] : 0);
-        float M = -INFINITY;
-        for (int s = lane; s < n; s += 32) {
-            const float2 ml = P.ws_ml[s * TH + i];
-            if (ml.y != 0.f) M = fmaxf(M, ml.x);
-        }
-        M = warp_max(M);
-        float L = 0.f;
+    const long long rows = (long long)ap_rows(P) * P.NH;
+    for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); i < TH; i += (long long)gridDim.x * 4) {
+        const int row = TH >> 32 ? (int)(i / P.NH) : (int)((unsigned)i / (unsigned)P.NH), head = (int)(i - (long long)row * P.NH);
+        const int most = P.S1 + P.S2, own = P.S2 ? P.ws_n[row] : 0;
+        float M = -INFINITY, L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int base = 0; base < most; base += 32) {
+            float2 ml = make_float2(0.f, 0.f);
+            if (base + lane < most) ml = P.ws_ml[(base + lane) * TH + i];
+            if (i >= rows) return;  // rows behind the last request have no parts
+            const int n = min(P.S1 + own - base, 32);
+            if (n <= 0) break;
+            const bool some = lane < n && ml.y != 0.f;
+            const float top = fmaxf(M, warp_max(some ? ml.x : -INFINITY));
+            if (base && M != -INFINITY) {
+                const float f = ap_exp2(M - top);
+                L *= f;
+                acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+            }
+            M = top;
+            const float weight = some ? ap_exp2(ml.x - M) : 0.f;
+            if (some) L = fmaf(weight, ml.y, L);
 #pragma unroll 4
-        for (int s = lane / width; s < n; s += groups) {
-            const float2 ml = P.ws_ml[s * TH + i];
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (ml.y != 0.f && d < P.HD) o = *reinterpret_cast<const float4 *>(P.ws_o + (s * TH + i) * P.HD + d);
-            const float w = ml.y != 0.f ? ap_exp2(ml.x - M) : 0.f;
-            L = fmaf(w, ml.y, L);
-            acc.x = fmaf(w, o.x, acc.x);
-            acc.y = fmaf(w, o.y, acc.y);
-            acc.z = fmaf(w, o.z, acc.z);
-            acc.w = fmaf(w, o.w, acc.w);
+            for (int s = 0; s < n; s += groups) {
+                const int mine = s + lane / width;
+                const float w = __shfl_sync(SB_FULL, weight, mine);
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (w != 0.f && d < P.HD) o = *reinterpret_cast<const float4 *>(P.ws_o + ((base + mine) * TH + i) * P.HD + d);
+                acc.x = fmaf(w, o.x, acc.x);
+                acc.y = fmaf(w, o.y, acc.y);
+                acc.z = fmaf(w, o.z, acc.z);
+                acc.w = fmaf(w, o.w, acc.w);
+            }
         }
+        L = warp_sum(L);
         for (int o = width; o < 32; o <<= 1) {
-            L += __shfl_xor_sync(SB_FULL, L, o);
             acc.x += __shfl_xor_sync(SB_FULL, acc.x, o);
             acc.y += __shfl_xor_sync(SB_FULL, acc.y, o);
             acc.z += __shfl_xor_sync(SB_FULL, acc.z, o);
