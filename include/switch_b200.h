@@ -192,8 +192,9 @@ int sb_sgemm_3xtf32_multi(const float *A, const float *B, float *const *C, int n
  * Bt [N][K] row-major (an [out][in] weight matrix), no transpose pass.  Same
  * alignment rules.  No counterpart in the reference. */
 int sb_sgemm_nt_3xtf32(const float *A, const float *Bt, float *C, int M, int N, int K, void *stream);
-/* Reads and clears the tensor-core kernels' device error flag (nonzero after
- * a bounded wait gave up); synchronises the context first. */
+/* Reads and clears the device error flags of the tensor-core and attention
+ * kernels (nonzero after a bounded wait gave up); synchronises the context
+ * first. */
 int sb_tc_error(int *err);
 /* Failure-detection test hook (no counterpart in the reference): chunk >= 0
  * makes every later sb_gemm_hh launch's TMA producer stop before its K-chunk
@@ -321,8 +322,8 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * position whose page number is outside the pool is skipped, never read, and
  * so is everything past a length.  Values that some row of a tile sees must
  * be finite (a weight of 0 times an infinity is NaN).  prefix and kv may be
- * different pools; with prefix_len == 0 or max_kv == 0 the other one's
- * arguments may be NULL.  max_q (rows of a request) sizes the launch, larger
+ * different pools; the arguments of one that has no positions (prefix_len or
+ * max_kv 0) may be NULL, but one of the two pools is given.  max_q (rows of a request) sizes the launch, larger
  * requests are still right; kv_len is cut to max_kv.  A row that sees nothing
  * gives zeros and lse = -inf; rows from cu_q[B] on are left as they were.
  * lse [T][NH] (natural log of the softmax denominator) may be NULL.
@@ -341,7 +342,7 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
  * the token (larger logit, or equal and a lower id), and the top_k (0..64)
  * best ids with their log probabilities, best first, equal logits by id.
  * Any output may be NULL.  A token outside [0, V) gives logp 0 and rank -1.
- * Masked choices (-inf) have probability 0 and are not listed (id -1,
+ * temperature is at least 1e-8.  Masked choices (-inf) have probability 0 and are not listed (id -1,
  * -inf fill up); a row of them gives lse = logp = -inf and entropy 0.  A row
  * with a NaN or +inf gives NaN sums, its ids and rank mean nothing.
  * ws: sb_logprobs_ws bytes (16-byte aligned). */

@@ -11,13 +11,16 @@
 // keys meet only its own rows.
 //
 // One item runs one of these bodies; each streams K and V tiles through a
-// cp.async ring of two or three stages, positions going through the block table (an
-// offset per key, computed a tile ahead; a position without a page, or past
-// the range, is filled with zeros and masked, so nothing of it is read):
+// ring in shared memory, positions going through the block table, looked up a
+// tile ahead.  Whole pages come by TMA boxes in the first and the last two, a
+// position without a page, or past the range, is filled with zeros and masked,
+// so nothing of it is read:
 //   attn_mmaw_body f16 / bf16, mma.sync m16n8k16, up to 8 or 16 rows (the head
 //                  group of a decode step) against long own pages: memory-bound
-//   attn_mma_body  64-row tiles, a warp 16 rows
-//   attn_f32_body  FP32 on the CUDA cores: 1..16-row tiles, a thread a key
+//   attn_mma_body  64-row tiles, a warp 16 rows (own pages of requests with
+//                  more rows)
+//   attn_f32_body  FP32 on the CUDA cores: 1..16-row tiles, a lane a key
+//   attn_tc_body   the prefix for more than 16 rows (serve_attn_tc.cuh)
 // Scores, maxima, sums and outputs are FP32; the softmax weights are rounded
 // to the value type for the second tensor-core product (half a step, like
 // the values they multiply).
@@ -683,7 +686,8 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
     seq += nt;
     if (!ok) {  // given up (tc_err): nothing that passes for a result
         ring.drain(t, nt);
-        l[0][0] = l[0][1] = __int_as_float(0x7fc00000);
+#pragma unroll
+        for (int b = 0; b < NB; b++) l[b][0] = l[b][1] = __int_as_float(0x7fc00000);
     }
     float *ow = reinterpret_cast<float *>(sm);  // [NW][8 NB rows][HDP]
     __shared__ float ms[NW][8 * NB], ls[NW][8 * NB];
@@ -711,12 +715,13 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
 
 // ---------------------------------------------------------------- FP32
 // MT rows, a warp a quarter of the keys of every KT from the scores to the
-// outputs (the block meets only for the join).  Scores: a lane takes a key and 32 of its dimensions; K chunks are
-// xor-swizzled so that eight lanes reading eight keys touch all banks, query
-// values are broadcast (the DQ parts of a row 36 floats apart, on banks of
-// their own).  Outputs: a lane owns HDP / 32 dimensions of all rows, the
-// weights come as pairs from shared memory for two-wide FMAs.  Rows rescale
-// when their maximum has grown by more than 2^8, as in the other kernels.
+// outputs (the block meets only for the join).  Scores: a lane takes a key and
+// 32 of its dimensions; K chunks are xor-swizzled so that eight lanes reading
+// eight keys touch all banks, query values are broadcast (the DQ parts of a
+// row 36 floats apart, on banks of their own).  Outputs: a lane owns HDP / 32
+// dimensions of all rows, the weights come as pairs from shared memory for
+// two-wide FMAs.  Rows rescale when their maximum has grown by more than 2^8,
+// as in the other kernels.
 // Bound: HBM up to eight rows (46 of the 24 bytes per SM and cycle that HBM
 // gives at MT = 8), the shared-memory and FMA pipes beyond.  FFMA and not the
 // tensor pipe: its FP32 sums are not IEEE-rounded and drift by 1e-5 over some
@@ -815,9 +820,10 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
         if (!(ok = ring.wait(1, t))) break;
 #pragma unroll
         for (int k = 0; k < KW; k++) {
-                        unsigned long long v[DP];
+            unsigned long long v[DP];
             if constexpr (DP == 1) {
-                v[0] = *reinterpret_cast<const unsigned long long *>(vt + (lane >> 4) * BLOCK + k * 128 + ((((lane >> 1) & 7) ^ (k & 7)) << 4) + (lane & 1) * 8);
+                const int at = ((((lane >> 1) & 7) ^ (k & 7)) << 4) + (lane & 1) * 8;
+                v[0] = *reinterpret_cast<const unsigned long long *>(vt + (lane >> 4) * BLOCK + k * 128 + at);
             } else {
                 const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(vt + (lane >> 3) * BLOCK + k * 128 + (((lane & 7) ^ (k & 7)) << 4));
                 v[0] = w.x;
@@ -848,7 +854,8 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     seq += nt;
     if (!ok) {  // given up (tc_err): nothing that passes for a result
         ring.drain(t, nt);
-        l[0] = __int_as_float(0x7fc00000);
+#pragma unroll
+        for (int r = 0; r < MT; r++) l[r] = __int_as_float(0x7fc00000);
     }
     __syncthreads();
     float *red = reinterpret_cast<float *>(sm);  // [NW][MT][HDP] floats: 32 KB at most, in the ring
@@ -945,12 +952,11 @@ extern "C" __global__ void __launch_bounds__(128) attn_join(const __grid_constan
         const int most = P.S1 + P.S2, own = P.S2 ? P.ws_n[row] : 0;
         float M = -INFINITY, L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int base = 0; base < most; base += 32) {
-            float2 ml = make_float2(0.f, 0.f);
-            if (base + lane < most) ml = P.ws_ml[(base + lane) * TH + i];
-            if (i >= rows) return;  // rows behind the last request have no parts
+        float2 ml = lane < most ? P.ws_ml[lane * TH + i] : make_float2(0.f, 0.f);
+        if (i >= rows) return;  // rows behind the last request have no parts and stay as they were
+        for (int base = 0; base < P.S1 + own; base += 32) {
             const int n = min(P.S1 + own - base, 32);
-            if (n <= 0) break;
+            if (base && lane < n) ml = P.ws_ml[(base + lane) * TH + i];
             const bool some = lane < n && ml.y != 0.f;
             const float top = fmaxf(M, warp_max(some ? ml.x : -INFINITY));
             if (base && M != -INFINITY) {

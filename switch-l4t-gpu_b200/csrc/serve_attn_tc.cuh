@@ -333,7 +333,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         // ---- softmax and epilogue: a thread a row
         const int x = warp >> 2, f = it.f0 + tid;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + x * 128, o_at = tmem + lanes + 256 + x * 128;
-        const float sc = fabsf(P.scale_log2);
+        const float sc = fmaxf(fabsf(P.scale_log2), 1e-30f);  // 0 times a masked score would be NaN
         {  // this warp's 32 query rows, neighbouring lanes on one row, zeros behind the last.  A short loop: code that
            // runs once costs six cycles an instruction to fetch
             constexpr int CH = HDP / 8, RPI = 32 / CH;
@@ -421,7 +421,8 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         if (m == INFINITY) l = __int_as_float(0x7fc00000);  // an infinite score: NaN, as its softmax
         ok = __all_sync(SB_FULL, ap_bar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
         fence_after();
-        const bool live = f < it.F && ok;
+        if (!ok) l = __int_as_float(0x7fc00000);  // given up: nothing that passes for a result
+        const bool live = f < it.F;
         if (live) ap_row_stats(P, it, f, m, l);
         const int qrow = it.row0 + f / P.G, head = it.kvh * P.G + f % P.G;
         const bool whole = P.S1 + P.S2 == 1;  // the result itself, else this range's part of it

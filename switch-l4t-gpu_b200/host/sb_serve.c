@@ -26,7 +26,8 @@ int sb_kv_plan(const int *cache_len, const int *new_len, int B, int page, const 
     SB_ARG(cache_len && new_len && table && cu_q && kv_len && used, "kv_plan: null pointer");
     SB_ARG(page >= 1 && n_free >= 0 && (free_pages || n_free == 0), "kv_plan: bad page size or free list");
     SB_ARG(width >= 1 && table_stride >= width, "kv_plan: table_stride must be at least the width");
-    SB_ARG(T >= 0 && ((slots && pos && req) || T == 0), "kv_plan: bad token arrays");
+    SB_ARG(kv_len != cache_len && kv_len != new_len && cu_q != cache_len && cu_q != new_len, "kv_plan: outputs over the input lengths");
+    SB_ARG(T >= 0 && T <= 0x7ffffff0 && ((slots && pos && req) || T == 0), "kv_plan: bad token arrays");
     sb_ctx *c = sb_ctx_get();
     if (!c) return SB_ERR_STATE;
     CUdeviceptr cl = DP(cache_len), nl = DP(new_len), fp = DP(free_pages), tb = DP(table), sl = DP(slots), po = DP(pos),
@@ -137,6 +138,7 @@ int sb_rotary(const void *x, int64_t x_tok, int64_t x_head, void *y, int64_t y_t
     if (rc) return rc;
     SB_ARG(H >= 1 && ((x && y && pos) || T == 0), "rotary: null pointer");
     SB_ARG(ALIGNED(x, type_size(type)) && ALIGNED(y, type_size(type)), "rotary: misaligned rows");
+    SB_ARG(x != y || ((T <= 1 || x_tok == y_tok) && (H == 1 || x_head == y_head)), "rotary: in place needs one set of strides");
     struct rot_params p;
     memset(&p, 0, sizeof p);
     p.src[0] = DP(x);
@@ -392,12 +394,12 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
                    int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
                    int prefix_len, const sb_kv_pages *kv, const int *table, int table_stride, const int *kv_len, int max_kv,
                    float scale, void *ws, size_t ws_bytes, void *stream) {
-    const sb_kv_pages *any = prefix_len > 0 ? prefix : kv;
+    const sb_kv_pages *any = prefix_len > 0 || (max_kv <= 0 && !kv) ? prefix : kv;
     int rc = pages_args(any);
     if (!rc && prefix_len > 0 && max_kv > 0) rc = pages_args(kv);
     if (!rc) rc = attn_args(any->type, T, B, NH, any->NKV, any->HD, max_q, prefix_len, max_kv);
     if (rc) return rc;
-    SB_ARG(isfinite(scale), "attn_prefix: scale must be finite");
+    SB_ARG(isfinite(scale * 1.4426950408889634f), "attn_prefix: scale must be finite");
     SB_ARG(cu_q || (T == B && max_q == 1), "attn_prefix: without cu_q there is one row a request (T == B, max_q == 1)");
     if (T == 0 || B == 0) return 0;
     SB_ARG(q && out && ALIGNED(lse, 4), "attn_prefix: null or misaligned pointer");
@@ -413,7 +415,7 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
         SB_ARG(table && kv_len, "attn_prefix: null table or lengths");
         SB_ARG(kv->type == any->type && kv->NKV == any->NKV && kv->HD == any->HD,
                "attn_prefix: prefix and own pages must have one type, head count and head size");
-        SB_ARG(table_stride >= CEIL_DIV(max_kv, kv->page), "attn_prefix: the table is narrower than max_kv positions");
+        SB_ARG(table_stride >= CEIL_DIV((int64_t)max_kv, kv->page), "attn_prefix: the table is narrower than max_kv positions");
         if ((rc = pages_for_attn(kv, &p.suf))) return rc;
     }
     sb_ctx *c = sb_ctx_get();
@@ -541,8 +543,7 @@ int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, 
                 size_t ws_bytes, void *stream) {
     int rc = lp_args(type, R, V, top_k);
     if (rc) return rc;
-    SB_ARG(isfinite(temperature) && temperature > 0.0f && isfinite(1.4426950408889634f / temperature),
-           "logprobs: temperature must be positive");
+    SB_ARG(isfinite(temperature) && temperature >= 1e-8f, "logprobs: temperature must be at least 1e-8");
     SB_ARG(tokens || (!logp && !rank), "logprobs: logp and rank need tokens");
     SB_ARG(top_k == 0 || top_ids || top_logp, "logprobs: top_k without an output");
     if (R == 0) return 0;
@@ -584,8 +585,7 @@ int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, in
                      int64_t grad_stride, void *stream) {
     int rc = lp_args(type, R, V, 0);
     if (rc) return rc;
-    SB_ARG(isfinite(temperature) && temperature > 0.0f && isfinite(1.4426950408889634f / temperature),
-           "logprobs_grad: temperature must be positive");
+    SB_ARG(isfinite(temperature) && temperature >= 1e-8f, "logprobs_grad: temperature must be at least 1e-8");
     SB_ARG(tokens || !g_logp, "logprobs_grad: g_logp needs tokens");
     if (R == 0) return 0;
     SB_ARG(logits && grad && lse && (entropy || !g_entropy), "logprobs_grad: null pointer");

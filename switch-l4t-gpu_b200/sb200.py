@@ -393,6 +393,15 @@ def _vector(t, name, dtype, n):
         raise SbError(f"{name}: need a contiguous {dtype} tensor of at least {n} entries")
 
 
+def _ws(t):
+    """Address and bytes of a contiguous workspace, or of none."""
+    if t is None:
+        return None, 0
+    if not t.is_contiguous():
+        raise SbError("workspace: need a contiguous tensor")
+    return t.data_ptr(), t.nbytes
+
+
 def _rows3(t, name):
     """[rows, heads, head size] whose last dimension is contiguous; its shape and strides."""
     shape, stride = t.shape, t.stride()
@@ -528,9 +537,10 @@ def attn_prefix(q, out, prefix, prefix_table, prefix_len, kv, table, kv_len, sca
             _vector(prefix_table, "prefix_table", i32, -(-prefix_len // p.page))
     _vector(cu_q, "cu_q", i32, B + 1)
     _vector(lse, "lse", _tn().f32, T * NH)
+    wp, wn = _ws(ws)
     check(lib().sb_attn_prefix(q.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0], os_[1], _p(lse), T, NH, _p(cu_q), B, max_q,
                                None if prefix is None else prefix.ref, _p(prefix_table), prefix_len, None if kv is None else kv.ref,
-                               _p(table), stride, _p(kv_len), max_kv, scale, _p(ws), 0 if ws is None else ws.nbytes, _s(stream)))
+                               _p(table), stride, _p(kv_len), max_kv, scale, wp, wn, _s(stream)))
 
 
 def logprobs_ws(logits, top_k=0):
@@ -566,8 +576,9 @@ def logprobs(logits, tokens, ws, logp=None, entropy=None, lse=None, rank=None, t
     _vector(top_ids, "top_ids", n.i32, R * k)
     _vector(top_logp, "top_logp", n.f32, R * k)
     _on_device(logits, tokens, ws, logp, entropy, lse, rank, top_ids, top_logp)
+    wp, wn = _ws(ws)
     check(lib().sb_logprobs(logits.data_ptr(), stride, _type(logits), R, V, temperature, _p(tokens), _p(logp), _p(entropy), _p(lse), _p(rank),
-                            k, _p(top_ids), _p(top_logp), _p(ws), 0 if ws is None else ws.nbytes, _s(stream)))
+                            k, _p(top_ids), _p(top_logp), wp, wn, _s(stream)))
 
 
 def logprobs_grad(logits, tokens, lse, entropy, g_logp, g_entropy, grad, temperature=1.0, stream=None):

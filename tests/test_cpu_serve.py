@@ -80,7 +80,7 @@ def test_rotary_plan_yarn_ends():
 
 def test_kv_plan_refusals():
     L, p = sb200.lib(), 0x1000
-    ok = dict(B=2, page=16, n_free=4, stride=8, width=8, T=4, cl=p, nl=p, fp=p, tb=p, sl=p, po=p, rq=p, cq=p, kl=p, us=p)
+    ok = dict(B=2, page=16, n_free=4, stride=8, width=8, T=4, cl=p, nl=2 * p, fp=p, tb=3 * p, sl=4 * p, po=5 * p, rq=6 * p, cq=7 * p, kl=8 * p, us=9 * p)
 
     def call(**kw):
         a = dict(ok, **kw)
@@ -88,7 +88,7 @@ def test_kv_plan_refusals():
                             a["rq"], a["T"], a["cq"], a["kl"], a["us"], None)
     for bad in (dict(B=0), dict(B=16385), dict(page=0), dict(n_free=-1), dict(fp=None), dict(width=0), dict(stride=7), dict(T=-1),
                 dict(sl=None), dict(po=None), dict(rq=None), dict(cl=None), dict(nl=None), dict(tb=None), dict(cq=None), dict(kl=None),
-                dict(us=None)):
+                dict(us=None), dict(kl=p), dict(kl=2 * p), dict(cq=p), dict(T=2 ** 31 - 2)):
         assert call(**bad) == ERR_ARG, bad
 
 
@@ -96,13 +96,14 @@ def test_rotary_refusals():
     L, p = sb200.lib(), 0x1000
     _, r = _plan(64)
     ref = ctypes.byref(r)
-    ok = dict(x=p, y=p, type=1, T=3, H=2, HD=64, pos=p, plan=ref)
+    ok = dict(x=p, y=p, type=1, T=3, H=2, HD=64, pos=p, plan=ref, yt=128, yh=64)
 
     def call(**kw):
         a = dict(ok, **kw)
-        return L.sb_rotary(a["x"], 128, 64, a["y"], 128, 64, a["type"], a["T"], a["H"], a["HD"], a["pos"], a["plan"], 0, None)
+        return L.sb_rotary(a["x"], 128, 64, a["y"], a["yt"], a["yh"], a["type"], a["T"], a["H"], a["HD"], a["pos"], a["plan"], 0, None)
     for bad in (dict(type=3), dict(T=-1), dict(H=0), dict(HD=62), dict(HD=65), dict(x=None), dict(y=None), dict(pos=None), dict(plan=None),
-                dict(plan=ctypes.byref(sb200._RotaryPlan())), dict(x=p + 1)):
+                dict(plan=ctypes.byref(sb200._RotaryPlan())), dict(x=p + 1),
+                dict(yt=256), dict(yh=72)):  # in place with other strides
         assert call(**bad) == ERR_ARG, bad
 
     def kv(pages, **kw):
@@ -129,7 +130,9 @@ def test_attn_prefix_refusals():
                                 a["ws"], a["wsb"], None)
     for bad in (dict(pre=None), dict(kv=None), dict(pre=_pages(type=5)), dict(kv=_pages(type=0)), dict(kv=_pages(NKV=1)),
                 dict(kv=_pages(HD=32)), dict(NH=3), dict(NH=0), dict(T=-1), dict(B=-1), dict(max_q=0), dict(P=-1), dict(max_kv=-1),
-                dict(cu=None), dict(cu=None, T=2), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(out=None),
+                dict(cu=None), dict(cu=None, T=2), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(pre=None, kv=None, P=0, max_kv=0),
+                dict(kv=_pages(page=2 ** 31 - 1), stride=0),  # the table's width in 64 bits
+                dict(q=None), dict(out=None),
                 dict(q=p + 8), dict(q_row=252), dict(q_head=60), dict(lse=p + 2), dict(tb=None), dict(kl=None), dict(stride=3),
                 dict(pt=None, P=129), dict(pre=_pages(HD=136), kv=_pages(HD=136)), dict(pre=_pages(HD=12), kv=_pages(HD=12)),
                 dict(pre=_pages(k=0x10008)), dict(kv=_pages(pos_stride=132)), dict(kv=_pages(v=0x20004))):
@@ -150,7 +153,7 @@ def test_logprobs_refusals():
         return L.sb_logprobs(a["x"], a["stride"], a["type"], a["R"], a["V"], a["temp"], a["tok"], a["logp"], p, p, a["rank"], a["k"], a["ids"],
                              a["top"], p, 1 << 30, None)
     for bad in (dict(type=4), dict(R=-1), dict(V=0), dict(V=4), dict(k=-1), dict(k=65), dict(temp=0.0), dict(temp=-1.0),
-                dict(temp=float("nan")), dict(temp=1e-45), dict(tok=None), dict(ids=None, top=None), dict(x=None), dict(x=p + 2),
+                dict(temp=float("nan")), dict(temp=1e-45), dict(temp=9e-9), dict(tok=None), dict(ids=None, top=None), dict(x=None), dict(x=p + 2),
                 dict(stride=99)):
         assert call(**bad) == ERR_ARG, bad
     assert L.sb_logprobs_ws(0, 2, 100, 101, ctypes.byref(n)) == ERR_ARG and L.sb_logprobs_ws(0, 2, 100, 5, None) == ERR_ARG
@@ -159,7 +162,7 @@ def test_logprobs_refusals():
         a = dict(dict(x=p, xs=100, type=0, R=2, V=100, temp=1.0, tok=p, lse=p, ent=p, gl=p, ge=p, g=0x9000, gs=100), **kw)
         return L.sb_logprobs_grad(a["x"], a["xs"], a["type"], a["R"], a["V"], a["temp"], a["tok"], a["lse"], a["ent"], a["gl"], a["ge"], a["g"],
                                   a["gs"], None)
-    for bad in (dict(type=3), dict(V=0), dict(temp=0.0), dict(tok=None), dict(x=None), dict(lse=None), dict(ent=None), dict(g=None),
+    for bad in (dict(type=3), dict(V=0), dict(temp=0.0), dict(temp=9e-9), dict(tok=None), dict(x=None), dict(lse=None), dict(ent=None), dict(g=None),
                 dict(xs=99), dict(gs=99), dict(g=0x9001), dict(g=p, xs=100, gs=104)):
         assert grad(**bad) == ERR_ARG, bad
 
@@ -197,6 +200,8 @@ def test_binding_refuses_wrong_tensors():
         lambda: sb200.logprobs(h[0], i32, None, top_ids=torch.zeros(2, 3, dtype=torch.int32), top_logp=torch.zeros(2, 4)),
         lambda: sb200.logprobs_grad(h[0], i32, torch.zeros(2), None, None, None, h[0].float()),
     ]
+    assert sb200._ws(torch.zeros(8))[1] == 32 and sb200._ws(None) == (None, 0)
+    bad.append(lambda: sb200._ws(torch.zeros(8)[::2]))  # its bytes are not in one piece
     for i, f in enumerate(bad):
         with pytest.raises(sb200.SbError):
             f()

@@ -366,8 +366,9 @@ def test_attn_prefix_large_batch(cuda_dev, kind):
     (128, 1, 1, 64, 1, 16), (129, 2, 1, 128, 127, 7), (64, 8, 2, 80, 128, 24), (257, 1, 1, 128, 129, 1), (33, 16, 2, 64, 1300, 64),
     (40, 14, 2, 40, 700, 700), (20, 32, 2, 128, 5000, 128)])
 def test_attn_prefix_many_rows_a_key_head(cuda_dev, kind, B, NH, NKV, HD, P, page):
-    """128 query rows of a key head and more, one row tile full, over, or
-    partly filled; one key, a tile less one, a tile, one more."""
+    """More than 16 query rows of a key head (16-bit types: the tcgen05
+    kernel): one row tile full, over, or partly filled; one key, a tile less
+    one, a tile, one more; a negative scale."""
     lens = [(i * 5) % 9 for i in range(B)]
     b = Batch(kind, NH, NKV, HD, P, lens, page=page, seed=B + P)
     want = b.want()
@@ -450,6 +451,12 @@ def test_attn_prefix_only_one_side(cuda_dev, kind):
     c.check(got=(out, lse))
     sb200.attn_prefix(c.q, out, c.kv, None, 0, c.kv, None, None, c.scale, None, lse=lse, stream=stream())
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    for one in (dict(prefix=c.kv, kv=None), dict(prefix=None, kv=c.kv)):  # one of the pools says the type; a row behind the last request
+        out, lse = torch.full_like(c.q, 7.0), torch.full((2, 4), 7.0, device="cuda")
+        sb200.attn_prefix(c.q, out, prefix_table=None, prefix_len=0, table=None, kv_len=None, scale=c.scale, ws=None, cu_q=i32([0, 1]),
+                          lse=lse, stream=stream(), **one)
+        assert bool((out[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+        assert bool((out[1] == 7).all()) and bool((lse[1] == 7).all())
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
@@ -534,6 +541,97 @@ def test_attn_prefix_repeats_and_replays(cuda_dev, kind):
         want = b.want()
         b.lens, b.places = was, places
         b.check(got=(o2, l2), want=want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("NH,NKV,HD,page,P", [
+    (4, 1, 128, 16, 130),   # a row group of 4: the 8-row tiles
+    (12, 1, 64, 8, 130),    # of 12: the 16-row tiles, two pages a warp's tile
+    (1, 1, 24, 32, 0),      # a head of a fifth of a box, one row
+    (2, 1, 72, 64, 40),     # half the second box
+    (3, 1, 96, 24, 40),     # pages that only an 8-position box divides
+    (16, 1, 128, 128, 0),
+])
+def test_attn_prefix_many_own_keys(cuda_dev, kind, NH, NKV, HD, page, P):
+    """Enough keys that whole pages come as boxes; ends inside a page, pages
+    that are not there between ones that are, other rows behind the last."""
+    lens = [(i * 211) % 1100 + (i % 3 == 0) * 16 for i in range(36)]
+    b = Batch(kind, NH, NKV, HD, P, lens, page=page, seed=HD + page, pad=1)
+    b.lens = lens = [max(lens)] + lens[1:]
+    b.kv_len = i32(lens)
+    drop = [(r, j) for r in (1, 2, 5) for j in (0, 3) if j * page < lens[r]]
+    # request 0 claims as many positions as the longest, its table has pages outside the pool for all
+    b.table[0] = 10 ** 9
+    b.places[0] = tuple(x[:0] for x in b.places[0])
+    for r, j in drop:
+        keep = b.places[r][0] != int(b.table[r, j])
+        b.places[r] = tuple(x[keep] for x in b.places[r])
+        b.table[r, j] = -1
+    got = b.run()
+    b.lens = [len(p[0]) for p in b.places[:-1]]
+    b.check(got=got)
+    assert sb200.tc_error() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B,NH,NKV,HD", [(3, 4, 2, 64), (70, 8, 2, 128), (300, 2, 2, 64)])
+def test_attn_prefix_pools_of_their_own(cuda_dev, kind, B, NH, NKV, HD):
+    """Prefix and requests in pools of different page sizes and layouts."""
+    lens = [(i * 29) % 150 for i in range(B)]
+    b = Batch(kind, NH, NKV, HD, 500, lens, page=16, seed=B)
+    page, pp = 48, 11  # 500 positions in 11 pages of 48, heads outside
+    pool = torch.full((2, pp + 2, NKV, page, HD), float("nan"), dtype=b.t, device="cuda").transpose(2, 3)
+    table, i = torch.randperm(pp + 2, device="cuda")[:pp].to(torch.int32), torch.arange(500, device="cuda")
+    for x, y in zip(pool, (b.k, b.v)):
+        x[table[i // page].long(), i % page] = y[b.places[-1]]
+    kv = sb200.KvPages(pool[0], pool[1])
+    out, lse = torch.full_like(b.q, 7.0), torch.full((B, NH), 7.0, device="cuda")
+    ws = torch.full((sb200.attn_prefix_ws(b.q, kv, 500, B, max_kv=max(lens)) // 4 + 1,), float("nan"), device="cuda")
+    sb200.attn_prefix(b.q, out, kv, table, 500, b.kv, b.table, b.kv_len, b.scale, ws, max_kv=max(lens), lse=lse, stream=stream())
+    b.check(got=(out, lse))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("B", [3, 40])
+def test_attn_prefix_scale_of_zero(cuda_dev, kind, B):
+    """All keys alike: the mean of what a row sees, also where a tile's end is masked."""
+    b = Batch(kind, 8, 2, 64, 200, [(i * 7) % 40 for i in range(B)], seed=21)
+    b.scale = 0.0
+    b.check()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_attn_prefix_two_at_once(cuda_dev, kind):
+    """Two streams, then two captured graphs side by side, each call with its
+    own workspace and outputs: the bits of one alone."""
+    bs = [Batch(kind, 8, 2, 64, 900, [(i * 31) % (90 + s) for i in range(40)], seed=s) for s in (31, 32)]
+    alone = [b.run() for b in bs]
+    torch.cuda.synchronize()
+    outs = [(torch.zeros_like(o), torch.zeros_like(x)) for o, x in alone]
+    wss = [torch.empty(sb200.attn_prefix_ws(b.q, b.kv, 900, 40, max_kv=max(b.lens)), dtype=torch.uint8, device="cuda") for b in bs]
+    streams = [torch.cuda.Stream() for _ in bs]
+    graphs = []
+
+    def both():
+        for b, s, o, w in zip(bs, streams, outs, wss):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    b.run(out=o[0], lse=o[1], ws=w)
+    both()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for a, o in zip(alone, outs) for x, y in zip(a, o))
+    for b, s, o, w in zip(bs, streams, outs, wss):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=s):
+            b.run(out=o[0], lse=o[1], ws=w)
+        o[0].zero_()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for a, o in zip(alone, outs) for x, y in zip(a, o))
 
 
 def test_attn_prefix_workspace_too_small(cuda_dev):
