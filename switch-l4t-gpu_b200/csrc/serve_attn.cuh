@@ -567,7 +567,7 @@ SB_DEV unsigned ap_movmatrix(unsigned a) {
 template <typename T, int HDP, int NB>
 SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, ApBars *bars, int &seq, const CUtensorMap *tm_k,
                            const CUtensorMap *tm_v, int box) {
-    constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, ST = HDP == 128 ? 2 : 4, KT = 16 * NW;
+    constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, ST = HDP == 128 ? 1 : 2, KT = 16 * NW;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
     ApRing<16, HDP, 2, ST> ring(it, P.HD, sm, bars, seq, tm_k, tm_v, box);
     unsigned qb[NB][KS][2];  // rows f0 + 8 b + g
@@ -875,8 +875,10 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 
 // A CTA an item: the prefix items of the launch, then own ones (either may be
 // none; row tiles of a request beyond the grid's are looped).  Each launch lets
-// the next start early and waits, before it ends, for the one before it, so
-// that the join, which waits for the last, has all of them behind it.
+// the next start early and does not end before the one before it, so that the
+// join, which waits for the last, has all of them behind it.  The CTA that is
+// started last waits for that; when every CTA did, the first of the second
+// launch held their SMs until the first launch was over.
 #define SB_AP_KERNEL(name, CTAS, MT, SHARED, CALL)                                                                   \
     extern "C" __global__ void __launch_bounds__(SB_AP_THREADS, CTAS)                                                  \
         name(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap tm_k,                           \
@@ -895,7 +897,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             else it.F = 0;                                                                                             \
         }                                                                                                              \
         for (const int step = item < 0 ? 1 << 30 : P.tiles2 * MT; it.f0 < it.F; it.f0 += step) CALL;                   \
-        pdl_wait();                                                                                                    \
+        if (blockIdx.x == gridDim.x - 1) pdl_wait();                                                                   \
     }
 // the four warps' barriers; a warp counts its own tiles
 #define SB_AP_WARPS                                                                                                    \
@@ -910,14 +912,14 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     SB_AP_KERNEL(name, (HDP == 128 ? 2 : 3), 64, __shared__ long long off_s[SB_AP_RING][64], (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))
 #define SB_AP_F32(name, HDP, MT) \
     SB_AP_KERNEL(name, 3, MT, SB_AP_WARPS, (attn_f32_body<HDP, MT>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
-SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 3)
-SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 3)
-SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 3)
-SB_AP_MMAW(attn_bf16_128_r8, __nv_bfloat16, 128, 1, 3)
-SB_AP_MMAW(attn_f16_64_r16, __half, 64, 2, 3)
-SB_AP_MMAW(attn_f16_128_r16, __half, 128, 2, 2)
-SB_AP_MMAW(attn_bf16_64_r16, __nv_bfloat16, 64, 2, 3)
-SB_AP_MMAW(attn_bf16_128_r16, __nv_bfloat16, 128, 2, 2)
+SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 5)
+SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 5)
+SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 5)
+SB_AP_MMAW(attn_bf16_128_r8, __nv_bfloat16, 128, 1, 5)
+SB_AP_MMAW(attn_f16_64_r16, __half, 64, 2, 4)
+SB_AP_MMAW(attn_f16_128_r16, __half, 128, 2, 3)
+SB_AP_MMAW(attn_bf16_64_r16, __nv_bfloat16, 64, 2, 4)
+SB_AP_MMAW(attn_bf16_128_r16, __nv_bfloat16, 128, 2, 3)
 SB_AP_MMA(attn_f16_64_r64, __half, 64)
 SB_AP_MMA(attn_f16_128_r64, __half, 128)
 SB_AP_MMA(attn_bf16_64_r64, __nv_bfloat16, 64)

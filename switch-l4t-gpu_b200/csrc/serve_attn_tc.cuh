@@ -464,7 +464,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         name(const __grid_constant__ AttnParams P, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,  \
              int box) {                                                                                                                 \
         attn_tc_body<T, HDP>(P, &tm_k, &tm_v, box);                                                                                     \
-        pdl_wait();                                                                                                                     \
+        if (blockIdx.x == gridDim.x - 1) pdl_wait();                                                                                    \
     }
 ATC_KERNEL(attn_tc_f16_64, __half, 64)
 ATC_KERNEL(attn_tc_f16_128, __half, 128)

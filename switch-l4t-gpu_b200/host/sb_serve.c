@@ -244,7 +244,7 @@ struct attn_part {
 static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_part *a) {
     const int wide = HD > 64, second = type == SB_BF16;
     a->threads = 128;
-    a->smem = 65536; /* the kernels' rings: 16 KB a warp */
+    a->smem = 65536; /* the FP32 kernels' rings: 16 KB a warp */
     if (type == SB_F32) {
         int i = 0;
         while (i < 4 && (1 << i) < rows) i++;
@@ -262,7 +262,7 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
         a->f = rows <= 8 ? (sb_fn_id)(F_ATTN_F16_64_R8 + 2 * second + wide)
                          : big ? (sb_fn_id)(F_ATTN_F16_64_R64 + 2 * second + wide)
                                : (sb_fn_id)(F_ATTN_F16_64_R16 + 2 * second + wide);
-        if (big) a->smem = 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64);
+        a->smem = big ? 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64) : 32768;
         a->rows = rows <= 8 ? 8 : big ? 64 : 16;
         a->step = 64;
     }
@@ -273,11 +273,12 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
  * takes about n + SB_ATTN_ITEM of them (its queries, its part to write), the
  * launch as many rounds of items as the SMs need, and every part of `bytes` is
  * written and read again by the join (a tile takes 0.5 us, 2 us on the
- * tcgen05 kernel; parts move at about 4 MB / us).  `fill`: how many items
+ * tcgen05 kernel; parts move at about 4 MB / us).  `sms`: those that the
+ * launch has for itself.  `fill`: how many items
  * stand for one that is there (requests are shorter than the longest, their
  * last ranges empty).  `alone`: one range would need no join. */
-static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, long bytes, int fill, int alone) {
-    const long cap = (long)fill * c->sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
+static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, long bytes, long sms, int fill, int alone) {
+    const long cap = fill * sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
     const long move = a->threads == 512 ? 8L << 20 : 2L << 20;
     long best = 0, best_cost = 0;
     for (long S = 1; S <= SB_ATTN_MAX_SPLITS && S <= tiles; S++) {
@@ -299,13 +300,28 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
     const long G = NH / NKV, bytes = (long)T * NH * HD * 8;
     memset(pre, 0, sizeof *pre);
     memset(own, 0, sizeof *own);
-    if (P > 0) {
-        attn_kernel(type, HD, T * G, 1, pre);
-        attn_split(c, pre, P, (long)pre->tiles * NKV, bytes, 1, max_kv == 0);
-    }
     if (max_kv > 0) {
         attn_kernel(type, HD, max_q * G, 0, own);
-        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, bytes, 2, P == 0);
+        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, bytes, c->sms, 2, P == 0);
+    }
+    if (P > 0) {
+        attn_kernel(type, HD, T * G, 1, pre);
+        const long units = (long)pre->tiles * NKV;
+        long sms = c->sms;
+        if (max_kv > 0 && pre->threads == 512) {
+            /* The tcgen05 kernel fills an SM, so it gets the share of the SMs
+             * that it has in the work, in units of 0.2 us of one SM, and the
+             * own items run beside it on the others (a tile of either kernel's
+             * 2 and 1.2 us; half the longest length).  256 requests behind
+             * 16000 tokens, 32 / 8 heads of 128, in BF16: 103 to 110 us, all
+             * SMs to one after the other 126; 32 requests of up to 33 rows
+             * behind 4001, 14 / 2 heads of 64: 32 and 37 */
+            const long mine = units * CEIL_DIV(P, pre->step) * 10;
+            const long others = own->grid * (own->chunk / own->step + 2 * SB_ATTN_ITEM) * 3 / sb_occupancy_of(c, own->f, 128, own->smem);
+            sms = sms * mine / (mine + others);
+            if (sms < 1) sms = 1;
+        }
+        attn_split(c, pre, P, units, bytes, sms, 1, max_kv == 0);
     }
     if (P > 0 && max_kv > 0 && pre->f != own->f && pre->threads == 128 && pre->rows > own->rows &&
         pre->grid + own->grid <= (long)c->sms * sb_occupancy_of(c, pre->f, 128, pre->smem)) {
@@ -317,7 +333,7 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
         own->smem = pre->smem;
         own->rows = pre->rows;
         own->tiles = tiles;
-        attn_split(c, own, max_kv, (long)tiles * NKV * B, bytes, 2, 0);
+        attn_split(c, own, max_kv, (long)tiles * NKV * B, bytes, c->sms, 2, 0);
     }
     SB_ARG(pre->grid + own->grid < 0x7fffffffL, "attn_prefix: too many rows for one launch");
     return 0;
@@ -467,23 +483,28 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     /* Two maps cost a microsecond of the host: not for a call that is over in a
      * few, nor for a launch whose two parts have pools of their own.  The
      * tcgen05 kernel's own copies take longer than that. */
-    const int apart = own.S && own.f != pre.f;
-    if (apart) {
-        /* first, since they are bound by memory and the smaller kernel: the
-         * prefix' items then start where SMs have room (48 requests behind
-         * 1000 tokens in FP32: 38.2 us; the prefix first: 45.4, in sequence: 46.1) */
-        p.items1 = 0;
-        if (own.grid * (long)own.chunk >= SB_ATTN_TMA_KEYS) box = encode_pages(&tk, &tv, kv, attn_box(&own, type, HD));
-        rc = sb_launch(c, own.f, (unsigned)own.grid, 1, own.threads, own.smem, (CUstream)stream, args, 0);
-        if (rc) return rc;
-    }
-    if (pre.S) {
-        const long grid = pre.grid + (apart ? 0 : own.grid);
-        p.items1 = (int)pre.grid;
-        box = 0;
-        if (grid == pre.grid && (pre.threads == 512 || grid * pre.chunk >= SB_ATTN_TMA_KEYS))
-            box = encode_pages(&tk, &tv, prefix, attn_box(&pre, type, HD));
-        rc = sb_launch(c, pre.f, (unsigned)grid, 1, pre.threads, pre.smem, (CUstream)stream, args, apart);
+    /* Order.  tcgen05 items that the own items would keep waiting go first: each
+     * takes an SM, the own items those left.  Otherwise own items first, the
+     * smaller kernel: prefix items start where SMs have room (48 requests
+     * behind 1000 tokens in FP32: 38.2 us, the prefix first 45.4), and the join
+     * does not wait for a third launch in line (6 requests behind 1819, 20 / 4
+     * heads of 80, in FP16: 13.4 and 15.2) */
+    const int apart = own.S && own.f != pre.f, tc = pre.threads == 512;
+    const int prefix_first = tc && pre.grid + (own.grid < c->sms ? own.grid : c->sms) > c->sms;
+    for (int i = 0; i < 2; i++) {
+        const int of_prefix = (i == 0) == prefix_first, second = i == 1 && pre.S && apart;
+        if (of_prefix ? !pre.S : !apart) continue;
+        if (of_prefix) {
+            const long grid = pre.grid + (apart ? 0 : own.grid);
+            p.items1 = (int)pre.grid;
+            box = 0;
+            if (grid == pre.grid && (tc || grid * pre.chunk >= SB_ATTN_TMA_KEYS)) box = encode_pages(&tk, &tv, prefix, attn_box(&pre, type, HD));
+            rc = sb_launch(c, pre.f, (unsigned)grid, 1, pre.threads, pre.smem, (CUstream)stream, args, second);
+        } else {
+            p.items1 = box = 0;
+            if (own.grid * (long)own.chunk >= SB_ATTN_TMA_KEYS) box = encode_pages(&tk, &tv, kv, attn_box(&own, type, HD));
+            rc = sb_launch(c, own.f, (unsigned)own.grid, 1, own.threads, own.smem, (CUstream)stream, args, second);
+        }
         if (rc) return rc;
     }
     if (pre.S + own.S == 1) return 0;
