@@ -56,6 +56,7 @@ struct AttnParams {
     int T, B, NH, NKV, G, HD, P, max_kv, table_stride;
     int chunk1, S1, tiles1, chunk2, S2, tiles2;  // key ranges and row tiles of the items
     int items1;                                  // prefix items in this launch; own items follow them
+    int deep;                                    // 16-bit types, heads of 128: rings of two tiles instead of one
     float scale_log2;
 };
 
@@ -185,8 +186,8 @@ SB_DEV void ap_tma(unsigned dst, const CUtensorMap *tm, int d, int head, int row
 }
 // a warp's ring: K and V tiles that have landed (32 arrivals and the bytes), and which keys of a tile are there
 struct ApBars {
-    uint64_t full[2][4];
-    unsigned valid[4];
+    uint64_t full[2][2];
+    unsigned valid[2];
 };
 
 // element offset of position p in the pages (without the head) with the lowest
@@ -231,38 +232,41 @@ template <int KT, int HDP, int E> struct ApCopy {
     }
 };
 
-// The keys of one warp: KW positions of every KT, K and V tiles in a ring of ST
-// each.  The block never meets: a tile of K is asked for as soon as the warp
-// has its scores, one of V as soon as it has its outputs, so nearly 2 ST tiles
+// The keys of one warp: KW positions of every KT, K and V tiles in a ring of st
+// (1 or 2) each.  The block never meets: a tile of K is asked for as soon as the warp
+// has its scores, one of V as soon as it has its outputs, so nearly 2 st tiles
 // are always in flight.  A tile is rows of 128 bytes in column blocks, 16-byte
 // chunks xor-ed by the row's low three bits (ldmatrix, or eight lanes on eight
 // keys, touch all banks).  Whole pages come by TMA boxes, one lane a box:
 // copies by the lanes (tiles that end inside a page or miss one, other page
 // sizes, calls too small to encode a map for) cost a third of all
 // instructions of a decode tile.
-template <int KW, int HDP, int E, int ST> struct ApRing {
+template <int KW, int HDP, int E> struct ApRing {
     static constexpr int SUB = HDP * E / 128, BLOCK = KW * 128, TILE = SUB * BLOCK, KT = KW * (SB_AP_THREADS / 32);
     static constexpr int C = HDP * E / 16, STEP = 32 / C, N = KW / STEP;
     const AttnItem &it;
     const CUtensorMap *tm[2];
     ApBars *bars;
     unsigned sm;
-    int first, box, HD, seq;  // seq: tiles that went through the ring before this item
+    int st, first, box, HD, seq;  // seq: tiles that went through the ring before this item
     int pg, in_pg, row, sub;  // this lane's box of the tile looked up last
     bool mine;
-    SB_DEV ApRing(const AttnItem &item, int hd, unsigned char *ring, ApBars *b, int seq0, const CUtensorMap *k, const CUtensorMap *v, int bx)
-        : it(item), bars(b + (threadIdx.x >> 5)), box(min(bx, KW)), HD(hd), seq(seq0) {
+    SB_DEV ApRing(const AttnItem &item, int hd, int stages, unsigned char *ring, ApBars *b, int seq0, const CUtensorMap *k,
+                  const CUtensorMap *v, int bx)
+        : it(item), bars(b + (threadIdx.x >> 5)), st(stages), box(min(bx, KW)), HD(hd), seq(seq0) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = box ? KW / box : 1;
         tm[0] = k;
         tm[1] = v;
-        sm = ap_smem(ring) + warp * (2 * ST * TILE);
+        sm = ap_smem(ring) + warp * (2 * st * TILE);
         first = it.k0 + warp * KW;
         sub = lane / pieces;
         row = lane % pieces * box;
         mine = box && sub < SUB;
     }
     SB_DEV int tiles(int k1) const { return k1 > first ? (k1 - first + KT - 1) / KT : 0; }
-    SB_DEV unsigned tile(int which, int t) const { return sm + (which * ST + (seq + t) % ST) * TILE; }
+    SB_DEV int slot(int t) const { return (seq + t) & (st - 1); }
+    SB_DEV unsigned phase(int t) const { return (unsigned)((seq + t) >> (st - 1)) & 1u; }  // of st = 1 or 2
+    SB_DEV unsigned tile(int which, int t) const { return sm + (which * st + slot(t)) * TILE; }
     SB_DEV void look(int t) {  // a tile ahead of its use
         const int p = first + t * KT + row;
         pg = -1;
@@ -273,7 +277,7 @@ template <int KW, int HDP, int E, int ST> struct ApRing {
         }
     }
     SB_DEV void copy(int which, int t) {  // tile t, looked up
-        const int lane = threadIdx.x & 31, n = (seq + t) % ST;
+        const int lane = threadIdx.x & 31, n = slot(t);
         const unsigned dst = tile(which, t);
         uint64_t *bar = &bars->full[which][n];
         if (__all_sync(SB_FULL, box && (!mine || (pg >= 0 && pg < it.pg.n_pages)))) {
@@ -302,16 +306,16 @@ template <int KW, int HDP, int E, int ST> struct ApRing {
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ap_smem(bar)) : "memory");
     }
     SB_DEV bool wait(int which, int t) const {
-        return __all_sync(SB_FULL, ap_bar_wait(&bars->full[which][(seq + t) % ST], (unsigned)((seq + t) / ST) & 1u));
+        return __all_sync(SB_FULL, ap_bar_wait(&bars->full[which][slot(t)], phase(t)));
     }
     SB_DEV void drain(int t, int nt) {  // given up at tile t: what was asked for still has to land
-        for (int u = t; u < min(t + ST + 1, nt); u++) {
-            ap_bar_wait(&bars->full[0][(seq + u) % ST], (unsigned)((seq + u) / ST) & 1u, false);
-            ap_bar_wait(&bars->full[1][(seq + u) % ST], (unsigned)((seq + u) / ST) & 1u, false);
+        for (int u = t; u < min(t + st + 1, nt); u++) {
+            ap_bar_wait(&bars->full[0][slot(u)], phase(u), false);
+            ap_bar_wait(&bars->full[1][slot(u)], phase(u), false);
         }
         __syncwarp();
     }
-    SB_DEV unsigned valid(int t) const { return bars->valid[(seq + t) % ST]; }
+    SB_DEV unsigned valid(int t) const { return bars->valid[slot(t)]; }
 };
 
 // what a finished row leaves: the output itself where the item is the only one, else its part
@@ -567,9 +571,10 @@ SB_DEV unsigned ap_movmatrix(unsigned a) {
 template <typename T, int HDP, int NB>
 SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, ApBars *bars, int &seq, const CUtensorMap *tm_k,
                            const CUtensorMap *tm_v, int box) {
-    constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, ST = HDP == 128 ? 1 : 2, KT = 16 * NW;
+    constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, KT = 16 * NW;
+    const int st = HDP == 128 && !P.deep ? 1 : 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    ApRing<16, HDP, 2, ST> ring(it, P.HD, sm, bars, seq, tm_k, tm_v, box);
+    ApRing<16, HDP, 2> ring(it, P.HD, st, sm, bars, seq, tm_k, tm_v, box);
     unsigned qb[NB][KS][2];  // rows f0 + 8 b + g
     int vis[NB][2];          // of rows f0 + 8 b + 2 q4, + 1
 #pragma unroll
@@ -601,14 +606,14 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
     }
     ap_fence_async();
     __syncthreads();  // an earlier item's join has been read
-    for (int t = 0; t < ST; t++) {
+    for (int t = 0; t < st; t++) {
         ring.look(t);
         if (t < nt) {
             ring.copy(0, t);
             ring.copy(1, t);
         }
     }
-    ring.look(ST);
+    ring.look(st);
     bool ok = true;
     int t = 0;
     for (; t < nt; t++) {
@@ -629,7 +634,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             for (int b = 0; b < NB; b++) ap_mma<T>(s[b], a, qb[b][k][0], qb[b][k][1]);
         }
         __syncwarp();
-        if (t + ST < nt) ring.copy(0, t + ST);
+        if (t + st < nt) ring.copy(0, t + st);
         bool grown = false;
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -678,9 +683,9 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             for (int b = 0; b < NB; b++) ap_mma<T>(o[b][i], a, p[b][0], p[b][1]);
         }
         __syncwarp();
-        if (t + ST < nt) {
-            ring.copy(1, t + ST);
-            ring.look(t + ST + 1);
+        if (t + st < nt) {
+            ring.copy(1, t + st);
+            ring.look(t + st + 1);
         }
     }
     seq += nt;
@@ -730,13 +735,13 @@ template <int HDP, int MT>
 SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char *sm, ApBars *bars, int &seq, const CUtensorMap *tm_k,
                           const CUtensorMap *tm_v, int box) {
     constexpr int NW = SB_AP_THREADS / 32, KW = HDP == 64 ? 16 : 8, KT = KW * NW, DQ = 32 / KW, DP = HDP / 64;  // keys a warp, parts of a key, pairs of a lane
-    constexpr int ST = 2, BLOCK = KW * 128;
+    constexpr int st = 2, BLOCK = KW * 128;
     __shared__ __align__(16) float q_s[MT][DQ][36];
     __shared__ __align__(16) float2 p_s[NW][KW][MT < 2 ? 2 : MT];
     __shared__ float m_s[NW][MT], l_s[NW][MT];
     __shared__ int vis_s[MT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = lane % KW, dq = lane / KW;
-    ApRing<KW, HDP, 4, ST> ring(it, P.HD, sm, bars, seq, tm_k, tm_v, box);
+    ApRing<KW, HDP, 4> ring(it, P.HD, st, sm, bars, seq, tm_k, tm_v, box);
     __syncthreads();  // an earlier item's shared memory is no longer read
     for (int i = tid; i < MT * HDP / 4; i += SB_AP_THREADS) {
         const int r = i / (HDP / 4), d = i % (HDP / 4) * 4, f = it.f0 + r;
@@ -750,14 +755,14 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     const int first = ring.first, nt = ring.tiles(k1);  // this warp's KW keys of every KT
     ap_fence_async();
     __syncthreads();
-    for (int t = 0; t < ST; t++) {
+    for (int t = 0; t < st; t++) {
         ring.look(t);
         if (t < nt) {
             ring.copy(0, t);
             ring.copy(1, t);
         }
     }
-    ring.look(ST);
+    ring.look(st);
     bool ok = true;
     unsigned long long o[MT][DP];
     float m[MT], l[MT];
@@ -787,7 +792,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             }
         }
         __syncwarp();
-        if (t + ST < nt) ring.copy(0, t + ST);
+        if (t + st < nt) ring.copy(0, t + st);
         float s[MT];
         bool grown = false;
         const int at = first + t * KT + key;
@@ -846,9 +851,9 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             }
         }
         __syncwarp();  // values and weights are read
-        if (t + ST < nt) {
-            ring.copy(1, t + ST);
-            ring.look(t + ST + 1);
+        if (t + st < nt) {
+            ring.copy(1, t + st);
+            ring.look(t + st + 1);
         }
     }
     seq += nt;
@@ -903,7 +908,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 #define SB_AP_WARPS                                                                                                    \
     __shared__ ApBars bars[SB_AP_THREADS / 32];                                                                        \
     int seq = 0;                                                                                                       \
-    if ((threadIdx.x & 31) < 8) ap_bar_init(&bars[threadIdx.x >> 5].full[0][0] + (threadIdx.x & 7), 32);               \
+    if ((threadIdx.x & 31) < 4) ap_bar_init(&bars[threadIdx.x >> 5].full[0][0] + (threadIdx.x & 3), 32);               \
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");                                                 \
     __syncwarp()
 #define SB_AP_MMAW(name, T, HDP, NB, CTAS) \
@@ -912,10 +917,10 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     SB_AP_KERNEL(name, (HDP == 128 ? 2 : 3), 64, __shared__ long long off_s[SB_AP_RING][64], (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))
 #define SB_AP_F32(name, HDP, MT) \
     SB_AP_KERNEL(name, 3, MT, SB_AP_WARPS, (attn_f32_body<HDP, MT>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
-SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 5)
-SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 5)
-SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 5)
-SB_AP_MMAW(attn_bf16_128_r8, __nv_bfloat16, 128, 1, 5)
+SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 6)
+SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 4)
+SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 6)
+SB_AP_MMAW(attn_bf16_128_r8, __nv_bfloat16, 128, 1, 4)
 SB_AP_MMAW(attn_f16_64_r16, __half, 64, 2, 4)
 SB_AP_MMAW(attn_f16_128_r16, __half, 128, 2, 3)
 SB_AP_MMAW(attn_bf16_64_r16, __nv_bfloat16, 64, 2, 4)

@@ -138,7 +138,7 @@ typedef struct sb_ctx {
     CUmodule mod[M_COUNT];
     CUfunction fn[F_COUNT];
     int smem_set[F_COUNT]; /* dynamic smem limit already raised to this */
-    int occ[F_COUNT];      /* co-resident CTAs per SM (sb_occupancy_of) */
+    int occ[F_COUNT][2];   /* co-resident CTAs per SM (sb_occupancy_of) */
     int sms;
     CUdeviceptr tc_ws; /* split-K workspace of the tensor-core GEMM (grown on demand) */
     size_t tc_ws_bytes;
@@ -169,7 +169,8 @@ int sb_launch_coop(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned bx, unsigned sme
 int sb_launch3(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned gy, unsigned gz, unsigned bx, CUstream s, void **args);
 /* max co-resident CTAs of f per SM at this block size / dynamic smem */
 int sb_occupancy(sb_ctx *c, sb_fn_id f, int block, size_t smem);
-/* the same, at least 1, kept from the first query (a kernel with one launch shape) */
+/* the same, at least 1, kept from the first query (a kernel with one launch shape,
+ * or with two: up to 32 KB of dynamic smem and more) */
 int sb_occupancy_of(sb_ctx *c, sb_fn_id f, int block, size_t smem);
 
 /* limits of sb_serve.c's launches */

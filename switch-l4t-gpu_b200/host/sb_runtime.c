@@ -303,11 +303,12 @@ int sb_occupancy(sb_ctx *c, sb_fn_id f, int block, size_t smem) {
 }
 
 int sb_occupancy_of(sb_ctx *c, sb_fn_id f, int block, size_t smem) {
-    if (!c->occ[f]) {
+    int *occ = &c->occ[f][smem > SB_SMEM_PLAIN];
+    if (!*occ) {
         const int n = sb_occupancy(c, f, block, smem);
-        c->occ[f] = n > 0 ? n : 1;
+        *occ = n > 0 ? n : 1;
     }
-    return c->occ[f];
+    return *occ;
 }
 
 int sb_launch_coop(sb_ctx *c, sb_fn_id f, unsigned gx, unsigned bx, unsigned smem, CUstream s, void **args) {

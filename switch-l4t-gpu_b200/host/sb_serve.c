@@ -223,14 +223,23 @@ struct attn_params {
     int64_t q_row, q_head, o_row, o_head;
     struct attn_pages pre, suf;
     int T, B, NH, NKV, G, HD, P, max_kv, table_stride;
-    int chunk1, S1, tiles1, chunk2, S2, tiles2, items1;
+    int chunk1, S1, tiles1, chunk2, S2, tiles2, items1, deep;
     float scale_log2;
 };
+/* Shared memory of the kernels with a ring a warp: 8 KB (16-bit types: K and V
+ * tiles of 16 keys, one each for heads of 128, two for 64; four and six CTAs an SM)
+ * or 16 KB (FP32, and long items of heads of 128: two each, three CTAs).  256
+ * requests in BF16, 32 / 8 heads of 128, up to 40 keys: 17.7 and 22.8 us; 250:
+ * 30 and 35; 500: 49 and 49; 1000: 88 and 86; 24 / 3 heads of 96, up to 500:
+ * 18.4 and 22; 1000: 81 and 43; 2000: 158 and 83 */
+#define SB_ATTN_SHALLOW 32768u
+#define SB_ATTN_DEEP 65536u
+#define SB_ATTN_DEEP_TILES 8
 /* one of the two launches: kernel, row tiles, key ranges, items */
 struct attn_part {
     sb_fn_id f;
     unsigned smem, threads;
-    int rows, step, tiles, S, chunk;
+    int f32, wide, rows, step, tiles, S, chunk;
     long grid;
 };
 
@@ -244,7 +253,9 @@ struct attn_part {
 static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_part *a) {
     const int wide = HD > 64, second = type == SB_BF16;
     a->threads = 128;
-    a->smem = 65536; /* the FP32 kernels' rings: 16 KB a warp */
+    a->smem = SB_ATTN_DEEP;
+    a->f32 = type == SB_F32;
+    a->wide = wide;
     if (type == SB_F32) {
         int i = 0;
         while (i < 4 && (1 << i) < rows) i++;
@@ -262,7 +273,7 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
         a->f = rows <= 8 ? (sb_fn_id)(F_ATTN_F16_64_R8 + 2 * second + wide)
                          : big ? (sb_fn_id)(F_ATTN_F16_64_R64 + 2 * second + wide)
                                : (sb_fn_id)(F_ATTN_F16_64_R16 + 2 * second + wide);
-        a->smem = big ? 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64) : 32768;
+        a->smem = big ? 2 * 64 * 2 * (wide ? 2 * 128 : 3 * 64) : SB_ATTN_SHALLOW;
         a->rows = rows <= 8 ? 8 : big ? 64 : 16;
         a->step = 64;
     }
@@ -270,30 +281,35 @@ static void attn_kernel(int type, int HD, long rows, int prefix, struct attn_par
 }
 /* Key ranges of `keys` keys for `units` independent (head, row tile) pairs,
  * the count with the least cost in tile times: an item of n tiles of keys
- * takes about n + SB_ATTN_ITEM of them (its queries, its part to write), the
- * launch as many rounds of items as the SMs need, and every part of `bytes` is
- * written and read again by the join (a tile takes 0.5 us, 2 us on the
- * tcgen05 kernel; parts move at about 4 MB / us).  `sms`: those that the
- * launch has for itself.  `fill`: how many items
- * stand for one that is there (requests are shorter than the longest, their
- * last ranges empty).  `alone`: one range would need no join. */
-static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, long bytes, long sms, int fill, int alone) {
-    const long cap = fill * sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem), tiles = CEIL_DIV(keys, a->step);
-    const long move = a->threads == 512 ? 8L << 20 : 2L << 20;
-    long best = 0, best_cost = 0;
-    for (long S = 1; S <= SB_ATTN_MAX_SPLITS && S <= tiles; S++) {
-        const long n = CEIL_DIV(tiles, S), parts = CEIL_DIV(tiles, n), items = units * parts;
-        const long cost = 16 * CEIL_DIV(items, cap) * (n + SB_ATTN_ITEM) + 2 * parts + 16 * parts * bytes / move +
-                          (alone && parts > 1 ? 16 * SB_ATTN_ITEM : 0);
-        if (!best || cost < best_cost) {
-            best = n;
-            best_cost = cost;
+ * takes about n + SB_ATTN_ITEM of them (its queries, its part to write), and
+ * every part of `bytes` is written and read again by the join (a tile takes
+ * 0.5 us, 2 us on the tcgen05 kernel; parts move at about 4 MB / us).  Items
+ * of one length run in rounds on `sms` SMs; `ragged` ones (requests are shorter
+ * than the longest: half its length, and in FP32 half the items) fill in
+ * for one another, and the longest is left at the end.  `alone`: one range
+ * would need no join. */
+static void attn_split(sb_ctx *c, struct attn_part *a, int keys, long units, long bytes, long sms, int ragged, int alone) {
+    const long tiles = CEIL_DIV(keys, a->step), move = a->threads == 512 ? 8L << 20 : 2L << 20;
+    for (;;) {
+        const long cap = sms * sb_occupancy_of(c, a->f, (int)a->threads, a->smem);
+        long best = 0, best_cost = 0;
+        for (long S = 1; S <= SB_ATTN_MAX_SPLITS && S <= tiles; S++) {
+            const long n = CEIL_DIV(tiles, S), parts = CEIL_DIV(tiles, n), items = units * parts;
+            const long run = ragged && !a->f32 ? 8 * units * (tiles + (parts + 1) * SB_ATTN_ITEM) / cap + 16 * (n + SB_ATTN_ITEM)
+                                               : 16 * CEIL_DIV(items, ragged ? 2 * cap : cap) * (n + SB_ATTN_ITEM);
+            const long cost = run + 2 * parts + 16 * parts * bytes / move + (alone && parts > 1 ? 16 * SB_ATTN_ITEM : 0);
+            if (!best || cost < best_cost) {
+                best = n;
+                best_cost = cost;
+            }
+            if (items > 32 * cap) break;
         }
-        if (items > 16 * cap) break;
+        a->chunk = (int)(best * a->step);
+        a->S = (int)CEIL_DIV((long)keys, a->chunk);
+        a->grid = units * a->S;
+        if (a->smem != SB_ATTN_SHALLOW || !a->wide || best <= SB_ATTN_DEEP_TILES) return;
+        a->smem = SB_ATTN_DEEP;
     }
-    a->chunk = (int)(best * a->step);
-    a->S = (int)CEIL_DIV((long)keys, a->chunk);
-    a->grid = units * a->S;
 }
 static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD, int max_q, int P, int max_kv,
                       struct attn_part *pre, struct attn_part *own) {
@@ -302,7 +318,7 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
     memset(own, 0, sizeof *own);
     if (max_kv > 0) {
         attn_kernel(type, HD, max_q * G, 0, own);
-        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, bytes, c->sms, 2, P == 0);
+        attn_split(c, own, max_kv, (long)own->tiles * NKV * B, bytes, c->sms, 1, P == 0);
     }
     if (P > 0) {
         attn_kernel(type, HD, T * G, 1, pre);
@@ -321,7 +337,7 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
             sms = sms * mine / (mine + others);
             if (sms < 1) sms = 1;
         }
-        attn_split(c, pre, P, units, bytes, sms, 1, max_kv == 0);
+        attn_split(c, pre, P, units, bytes, sms, 0, max_kv == 0);
     }
     if (P > 0 && max_kv > 0 && pre->f != own->f && pre->threads == 128 && pre->rows > own->rows &&
         pre->grid + own->grid <= (long)c->sms * sb_occupancy_of(c, pre->f, 128, pre->smem)) {
@@ -333,8 +349,9 @@ static int attn_parts(sb_ctx *c, int type, int T, int B, int NH, int NKV, int HD
         own->smem = pre->smem;
         own->rows = pre->rows;
         own->tiles = tiles;
-        attn_split(c, own, max_kv, (long)tiles * NKV * B, bytes, c->sms, 2, 0);
+        attn_split(c, own, max_kv, (long)tiles * NKV * B, bytes, c->sms, 1, 0);
     }
+    if (pre->f == own->f) pre->smem = own->smem = pre->smem > own->smem ? pre->smem : own->smem; /* one launch */
     SB_ARG(pre->grid + own->grid < 0x7fffffffL, "attn_prefix: too many rows for one launch");
     return 0;
 }
@@ -497,11 +514,13 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
         if (of_prefix) {
             const long grid = pre.grid + (apart ? 0 : own.grid);
             p.items1 = (int)pre.grid;
+            p.deep = pre.smem == SB_ATTN_DEEP;
             box = 0;
             if (grid == pre.grid && (tc || grid * pre.chunk >= SB_ATTN_TMA_KEYS)) box = encode_pages(&tk, &tv, prefix, attn_box(&pre, type, HD));
             rc = sb_launch(c, pre.f, (unsigned)grid, 1, pre.threads, pre.smem, (CUstream)stream, args, second);
         } else {
             p.items1 = box = 0;
+            p.deep = own.smem == SB_ATTN_DEEP;
             if (own.grid * (long)own.chunk >= SB_ATTN_TMA_KEYS) box = encode_pages(&tk, &tv, kv, attn_box(&own, type, HD));
             rc = sb_launch(c, own.f, (unsigned)own.grid, 1, own.threads, own.smem, (CUstream)stream, args, second);
         }
