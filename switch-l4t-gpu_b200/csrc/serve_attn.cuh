@@ -915,8 +915,10 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     SB_AP_KERNEL(name, CTAS, 8 * NB, SB_AP_WARPS, (attn_mmaw_body<T, HDP, NB>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
 #define SB_AP_MMA(name, T, HDP) \
     SB_AP_KERNEL(name, (HDP == 128 ? 2 : 3), 64, __shared__ long long off_s[SB_AP_RING][64], (attn_mma_body<T, HDP>(P, it, ap_sm, off_s)))
+// (16 rows of heads of 128 need 250 registers: 24 rows behind 1194 keys, 16 heads on one: 27.5 us, with three CTAs and
+// 168 registers 31.8)
 #define SB_AP_F32(name, HDP, MT) \
-    SB_AP_KERNEL(name, 3, MT, SB_AP_WARPS, (attn_f32_body<HDP, MT>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
+    SB_AP_KERNEL(name, (MT * HDP == 2048 ? 2 : 3), MT, SB_AP_WARPS, (attn_f32_body<HDP, MT>(P, it, ap_sm, bars, seq, &tm_k, &tm_v, box)))
 SB_AP_MMAW(attn_f16_64_r8, __half, 64, 1, 6)
 SB_AP_MMAW(attn_f16_128_r8, __half, 128, 1, 4)
 SB_AP_MMAW(attn_bf16_64_r8, __nv_bfloat16, 64, 1, 6)
