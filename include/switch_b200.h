@@ -4,7 +4,8 @@
  * Two boundaries are provided.
  *
  * 1. Module images (the reference's own boundary).  libswitch_b200.so ships
- *    four cubins whose `extern "C" __global__` kernels keep the reference's
+ *    four cubins (beside three of its own: tc, serve and score) whose
+ *    `extern "C" __global__` kernels keep the reference's
  *    names and parameter lists, so a reference host that does
  *    cuModuleLoadData + cuModuleGetFunction + cuLaunchKernel (void** params,
  *    its hard-coded grids) works unchanged with them:
