@@ -37,7 +37,7 @@ SB_DEV void plan_scan2(int &a, int &b, int *wa, int *wb) {
     b = sb + y - b;
 }
 // pages that n positions fill; n + page - 1 < 2^32 (a 64-bit division costs 100 cycles)
-SB_DEV int plan_pages(unsigned n, unsigned page) { return (int)((n + page - 1) / page); }
+SB_DEV unsigned plan_pages(unsigned n, unsigned page) { return (n + page - 1) / page; }
 
 // dynamic shared memory: 2 (B + 1) ints
 extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
@@ -55,12 +55,14 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
     int tok = 0, add = 0, lack = 0, len = 0;
     for (int b = b0; b < b1; b++) {
         const int c = max(cache_len[b], 0), n = max(new_len[b], 0);
-        const int have = plan_pages(c, page), need = plan_pages((unsigned)c + n, page), got = max(min(need, width) - have, 0);
+        // unsigned until the width has cut it: lengths past the limit index nothing outside
+        const unsigned have = plan_pages(c, page), need = plan_pages((unsigned)c + n, page), last = min(need, (unsigned)width);
+        const int got = last > have ? (int)(last - have) : 0;
         cu[b] = n;
         first[b] = got;
         tok += n;
         add += got;
-        lack += need - have - got;
+        lack += (int)(need - have) - got;
         len = c + n;
     }
     int t0 = tok, p0 = add;
@@ -95,9 +97,9 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
     for (int b = blockIdx.x * (nthreads / 32) + (tid >> 5); b < B; b += nw) {
         const int f = first[b], n = first[b + 1] - f;
         if (n == 0) continue;
-        const int have = plan_pages(max(cache_len[b], 0), page);
+        const unsigned have = plan_pages(max(cache_len[b], 0), page);
         for (int j = lane; j < n; j += 32)
-            table[(size_t)b * table_stride + have + j] = f + j < n_free ? free_pages[f + j] : -1;
+            table[(size_t)b * table_stride + have + j] = (unsigned)(f + j) < (unsigned)n_free ? free_pages[f + j] : -1;
     }
     // tokens: four neighbours a thread
     const int total = cu[B];
@@ -114,7 +116,8 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
             b = lo;
         }
         long long slot[4];
-        int p[4], rq[4], c = -1, have = 0, j = 0, off = 0;
+        int p[4], rq[4], c = -1, off = 0;
+        unsigned have = 0, j = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             slot[i] = -1;
@@ -128,17 +131,18 @@ extern "C" __global__ void __launch_bounds__(SB_PLAN_THREADS)
             if (fresh) {
                 c = max(cache_len[b], 0);
                 have = plan_pages(c, page);
-                const int at = c + (t + i - cu[b]);
-                j = at / page;
-                off = at - j * page;
+                const unsigned at = (unsigned)c + (unsigned)(t + i - cu[b]);
+                j = at / (unsigned)page;
+                off = (int)(at - j * (unsigned)page);
             } else if (++off == page) {
                 off = 0;
                 j++;
             }
             int pg = -1;
-            if (j < width) {
+            if (j < (unsigned)width) {
+                const unsigned i_free = (unsigned)first[b] + j - have;
                 if (j < have) pg = table[(size_t)b * table_stride + j];
-                else if (first[b] + j - have < n_free) pg = free_pages[first[b] + j - have];
+                else if (i_free < (unsigned)n_free) pg = free_pages[i_free];
             }
             if (pg >= 0) slot[i] = (long long)pg * page + off;
             p[i] = c + (t + i - cu[b]);
