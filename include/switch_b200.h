@@ -307,7 +307,8 @@ int sb_rotary(const void *x, int64_t x_tok, int64_t x_head, void *y, int64_t y_t
               int HD, const int *pos, const sb_rotary_plan *r, int inverse, void *stream);
 /* One launch for a step's new tokens: q_out = q turned, k turned and v copied
  * into slot slots[t] of kv (slots of different tokens must differ; a slot
- * outside the pages, as -1, writes nothing).  Rows with pos < 0 are left. */
+ * outside the pages, as -1, writes nothing).  Rows with pos < 0 are left.
+ * q_out may be q with the same strides. */
 int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int64_t qo_tok, int64_t qo_head, const void *k,
                  int64_t k_tok, int64_t k_head, const void *v, int64_t v_tok, int64_t v_head, int T, int NH, const int *pos,
                  const int64_t *slots, const sb_rotary_plan *r, const sb_kv_pages *kv, void *stream);

@@ -176,6 +176,7 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
     const int e = type_size(kv->type);
     SB_ARG(ALIGNED(q, e) && ALIGNED(q_out, e) && ALIGNED(k, e) && ALIGNED(v, e) && ALIGNED(kv->k, e) && ALIGNED(kv->v, e),
            "rotary_kv: misaligned rows");
+    SB_ARG(q != q_out || ((T <= 1 || q_tok == qo_tok) && (NH == 1 || q_head == qo_head)), "rotary_kv: in place needs one set of strides");
     struct rot_params p;
     memset(&p, 0, sizeof p);
     p.src[0] = DP(q);

@@ -219,3 +219,12 @@ def test_fixed_point_phase_against_double():
             got = np.longdouble((pos * r.turn[i]) % 2 ** 64) / np.longdouble(2.0 ** 64)
             d = abs(float(got - want))
             assert min(d, 1 - d) < pos * 2.0 ** -52  # pow in double: half an ulp of f <= 1/6
+
+
+def test_rotary_kv_in_place_needs_one_set_of_strides():
+    L, p = sb200.lib(), 0x1000
+    _, r = _plan(64)
+    pages = _pages()
+    for tok, head in ((512, 64), (256, 128)):
+        assert L.sb_rotary_kv(p, 256, 64, p, tok, head, 2 * p, 128, 64, 3 * p, 128, 64, 2, 4, 4 * p, 5 * p, ctypes.byref(r),
+                              ctypes.byref(pages), None) == ERR_ARG

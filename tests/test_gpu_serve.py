@@ -225,6 +225,24 @@ def test_rotary_kv(cuda_dev, kind, page, HD, dim):
     assert bool((pool[left] == 5).all())  # every other place is as it was
 
 
+@pytest.mark.parametrize("kind,layout", [("f32", 0), ("bf16", 1), ("f16", 0)])
+def test_rotary_kv_in_place(cuda_dev, kind, layout):
+    """Queries turned where they are, beside keys and values of one product:
+    the bits of a call with its own output."""
+    t, T, NH, NKV, HD = DT[kind], 37, 6, 2, 64
+    g = torch.Generator("cuda").manual_seed(3)
+    qkv = torch.randn(T, NH + 2 * NKV, HD, device="cuda", generator=g).to(t)
+    before = qkv.clone()
+    q, k, v = qkv.split([NH, NKV, NKV], 1)
+    kc, vc, kc2, vc2 = (torch.zeros(4, 16, NKV, HD, dtype=t, device="cuda") for _ in range(4))
+    pos, slots = torch.arange(T, device="cuda", dtype=torch.int32) + 900, torch.randperm(64, device="cuda", generator=g)[:T]
+    plan, q_out = sb200.Rotary(32, layout=layout), torch.empty(T, NH, HD, dtype=t, device="cuda")
+    sb200.rotary_kv(q, q_out, k, v, pos, slots, plan, sb200.KvPages(kc, vc), stream=stream())
+    sb200.rotary_kv(q, q, k, v, pos, slots, plan, sb200.KvPages(kc2, vc2), stream=stream())
+    assert torch.equal(q, q_out) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+    assert torch.equal(qkv[:, NH:], before[:, NH:])
+
+
 # ---------------------------------------------------------------- attention
 class Batch:
     """Inputs of a call with sentinels and garbage wherever nothing may be
