@@ -328,8 +328,9 @@ SB_DEV void logprobs_body(const LpParams &P) {
         thr_s = -FLT_MAX;
     }
 
-    // a whole tile's loads are issued a tile ahead: twice the bytes in flight (10 us of 338 for
-    // 2048 x 151936 bf16 with the gradient).  With alternatives more CTAs per SM overlap the part behind the loop better (37 against 36 us).
+    // A whole tile's loads are issued a tile ahead: twice the bytes in flight (10 us of 338 for 2048 x 151936 bf16
+    // with the gradient; 1056 x 50257 FP32 with 5 alternatives 46 against 72 us).  16-bit types with alternatives
+    // have more CTAs per SM instead, which overlap the part behind the loop better (36 against 37 us).
     uint4 raw[LP_U], ahead[LP_U];
     bool loaded = false;
     for (int b = v0; b < v1; b += TILE, tile++) {
@@ -344,7 +345,7 @@ SB_DEV void logprobs_body(const LpParams &P) {
                 if (j < v1) raw[u] = lp_load(x, lead, P.V, j);
             }
         }
-        loaded = !TOP && b + 2 * TILE <= whole1;
+        loaded = (!TOP || sizeof(T) == 4) && b + 2 * TILE <= whole1;
         if (loaded) {
 #pragma unroll
             for (int u = 0; u < LP_U; u++) ahead[u] = ld_stream_u4(x + ((b + TILE + u * LP_THREADS + tid) * N - lead));
