@@ -19,7 +19,10 @@
 // Bound: HBM, one read and one write of the rows.  A CTA takes a few tokens,
 // computes their cosines and sines once into shared memory for all heads,
 // and streams the rows as two 16-byte vectors of a thread: values
-// [u V, u V + V) of both halves (half layout) or 2 V neighbours (pairs).
+// [u V, u V + V) of both halves of what is turned, or of the head (pairs,
+// values), so that neighbouring threads touch neighbouring vectors (16000
+// tokens, 32 heads of 128 turned as pairs, BF16: 51 us, 2 V neighbours a thread
+// 62; with a second unit's loads in flight, at a third fewer CTAs, 58).
 // VEC = 1 serves rows whose strides, sizes or addresses are not multiples of
 // 16 bytes.
 #pragma once
@@ -28,7 +31,7 @@
 #include "sb_common.cuh"
 
 #define SB_ROT_THREADS 256
-#define SB_ROT_MAX_TOK 8
+#define SB_ROT_MAX_TOK 4
 
 // parameter block, mirrored by the host (host/sb_serve.c)
 struct RotParams {
@@ -65,11 +68,12 @@ template <typename T, int V>
 SB_DEV void rotary_body(const RotParams &P) {
     __shared__ float2 cs[SB_ROT_MAX_TOK][128];
     __shared__ int pos_s[SB_ROT_MAX_TOK];
-    __shared__ long long slot_s[SB_ROT_MAX_TOK];
+    __shared__ long long at_s[SB_ROT_MAX_TOK];  // the slot's place in the pages, -1: none
     const int t0 = blockIdx.x * P.tokens_per_cta, nt = min(P.tokens_per_cta, P.T - t0), half = P.dim >> 1;
     if (threadIdx.x < nt) {
         pos_s[threadIdx.x] = P.pos[t0 + threadIdx.x];
-        slot_s[threadIdx.x] = P.slots ? P.slots[t0 + threadIdx.x] : -1;
+        const long long slot = P.slots ? P.slots[t0 + threadIdx.x] : -1;
+        at_s[threadIdx.x] = slot < 0 || slot >= P.n_slots ? -1 : slot / P.page * P.page_stride + slot % P.page * P.pos_stride;
     }
     for (int i = threadIdx.x; i < nt * half; i += SB_ROT_THREADS) {
         const int t = i / half, j = i - t * half;
@@ -85,46 +89,52 @@ SB_DEV void rotary_body(const RotParams &P) {
         const int t = i / per, r = i - t * per;
         int h = r / U;
         const int u = r - h * U, pos = pos_s[t];
-        const long long slot = slot_s[t];
+        const long long at = at_s[t];
         const int part = h < P.heads[0] ? 0 : h < P.heads[0] + P.heads[1] ? 1 : 2;
         if (part >= 1) h -= P.heads[0];
         if (part == 2) h -= P.heads[1];
-        if (pos < 0 || (part && (slot < 0 || slot >= P.n_slots))) continue;  // padding, or no place in the pages
+        if (pos < 0 || (part && at < 0)) continue;  // padding, or no place in the pages
         const T *x = static_cast<const T *>(P.src[part]) + (t0 + t) * P.st[part] + h * P.sh[part];
-        T *y = static_cast<T *>(P.dst[part]) +
-               (part ? slot / P.page * P.page_stride + slot % P.page * P.pos_stride + h * P.head_stride
-                     : (t0 + t) * P.dt + h * P.dh);
-        const bool turn = part < 2 && u < UR;
-        int ia, ib;  // the two vectors
-        if (turn && P.layout == 0) {
+        T *y = static_cast<T *>(P.dst[part]) + (part ? at + h * P.head_stride : (t0 + t) * P.dt + h * P.dh);
+        int ia, ib;  // the two vectors: neighbouring units are neighbours in both
+        bool ta, tb;
+        if (P.layout == 0 && part < 2) {
+            ta = tb = u < UR;
+            ia = ta ? u * V : P.dim + (u - UR) * V;
+            ib = ia + (ta ? half : (P.HD - P.dim) >> 1);
+        } else if (V > 1) {  // pairs inside each vector, or values
             ia = u * V;
-            ib = ia + half;
-        } else {  // pairs, or the part that is copied (u >= UR: from dim on)
-            ia = u * 2 * V;
-            ib = ia + V;
+            ib = ia + (P.HD >> 1);
+            ta = part < 2 && ia < P.dim;
+            tb = part < 2 && ib < P.dim;
+        } else {  // a pair's two values
+            ia = 2 * u;
+            ib = ia + 1;
+            ta = tb = part < 2 && ia < P.dim;
         }
         const RotVec<T, V> a = *reinterpret_cast<const RotVec<T, V> *>(x + ia), b = *reinterpret_cast<const RotVec<T, V> *>(x + ib);
         RotVec<T, V> oa = a, ob = b;
-        if (turn) {
-            if (P.layout == 0) {
+        if constexpr (V > 1) {
+            if (P.layout) {
+                auto pairs = [&](RotVec<T, V> &o, const float2 *w) {
 #pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float2 r = rot_pair(rot_f<T>(a.v[e]), rot_f<T>(b.v[e]), cs[t][u * V + e]);
-                    oa.v[e] = rot_t<T>(r.x);
-                    ob.v[e] = rot_t<T>(r.y);
-                }
-            } else {
-                T in[2 * V], out[2 * V];
+                    for (int e = 0; e < V; e += 2) {
+                        const float2 r = rot_pair(rot_f<T>(o.v[e]), rot_f<T>(o.v[e + 1]), w[e / 2]);
+                        o.v[e] = rot_t<T>(r.x);
+                        o.v[e + 1] = rot_t<T>(r.y);
+                    }
+                };
+                if (ta) pairs(oa, &cs[t][ia / 2]);
+                if (tb) pairs(ob, &cs[t][ib / 2]);
+                ta = false;
+            }
+        }
+        if (ta) {
 #pragma unroll
-                for (int e = 0; e < V; e++) { in[e] = a.v[e]; in[V + e] = b.v[e]; }
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float2 r = rot_pair(rot_f<T>(in[2 * e]), rot_f<T>(in[2 * e + 1]), cs[t][u * V + e]);
-                    out[2 * e] = rot_t<T>(r.x);
-                    out[2 * e + 1] = rot_t<T>(r.y);
-                }
-#pragma unroll
-                for (int e = 0; e < V; e++) { oa.v[e] = out[e]; ob.v[e] = out[V + e]; }
+            for (int e = 0; e < V; e++) {
+                const float2 r = rot_pair(rot_f<T>(a.v[e]), rot_f<T>(b.v[e]), cs[t][u * V + e]);
+                oa.v[e] = rot_t<T>(r.x);
+                ob.v[e] = rot_t<T>(r.y);
             }
         }
         *reinterpret_cast<RotVec<T, V> *>(y + ia) = oa;
