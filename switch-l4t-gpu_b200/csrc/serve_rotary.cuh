@@ -21,7 +21,7 @@
 // and streams the rows as two 16-byte vectors of a thread: values
 // [u V, u V + V) of both halves of what is turned, or of the head (pairs,
 // values), so that neighbouring threads touch neighbouring vectors (16000
-// tokens, 32 heads of 128 turned as pairs, BF16: 51 us, 2 V neighbours a thread
+// tokens, 32 heads of 128 turned as pairs, BF16: 49 us, 2 V neighbours a thread
 // 62; with a second unit's loads in flight, at a third fewer CTAs, 58).
 // VEC = 1 serves rows whose strides, sizes or addresses are not multiples of
 // 16 bytes.
@@ -62,6 +62,12 @@ template <> SB_DEV __nv_bfloat16 rot_t<__nv_bfloat16>(float v) { return __float2
 SB_DEV float2 rot_pair(float a, float b, float2 w) {
     return make_float2(__fmaf_rn(a, w.x, -__fmul_rn(b, w.y)), __fmaf_rn(b, w.x, __fmul_rn(a, w.y)));
 }
+// x / d as a product with ceil(2^32 / d), exact while x d < 2^32
+struct RotDiv {
+    unsigned d, m;  // m = 0: divide
+    SB_DEV RotDiv(unsigned div, bool small) : d(div), m(small && div > 1 ? 0xffffffffu / div + 1 : 0u) {}
+    SB_DEV int operator()(int x) const { return m ? (int)__umulhi((unsigned)x, m) : (int)((unsigned)x / d); }
+};
 template <typename T, int V> struct alignas(sizeof(T) * V) RotVec { T v[V]; };
 
 template <typename T, int V>
@@ -85,9 +91,10 @@ SB_DEV void rotary_body(const RotParams &P) {
     __syncthreads();
     // units of 2 V values; rows in the order query heads, key heads, value heads
     const int U = P.HD / (2 * V), UR = half / V, H = P.heads[0] + P.heads[1] + P.heads[2], per = H * U;
+    const RotDiv by_per(per, per < 32768), by_U(U, per < 32768);  // 4 per^2 < 2^32
     for (int i = blockIdx.y * SB_ROT_THREADS + threadIdx.x; i < nt * per; i += SB_ROT_THREADS * gridDim.y) {
-        const int t = i / per, r = i - t * per;
-        int h = r / U;
+        const int t = by_per(i), r = i - t * per;
+        int h = by_U(r);
         const int u = r - h * U, pos = pos_s[t];
         const long long at = at_s[t];
         const int part = h < P.heads[0] ? 0 : h < P.heads[0] + P.heads[1] ? 1 : 2;

@@ -107,7 +107,7 @@ static int rotary_launch(struct rot_params *p, const sb_rotary_plan *r, int type
     const int V = vec ? 16 / type_size(type) : 1;
     const long H = p->heads[0] + p->heads[1] + p->heads[2], units = H * (p->HD / (2 * V));
     /* tokens per CTA: up to 4 while that leaves two CTAs per SM (8: more idle at
-     * the end, 4099 tokens of 14 heads of 64 in FP32 7.1 against 6.4 us); a
+     * the end, 4099 tokens of 14 heads of 64 in FP32 6.7 against 6.0 us); a
      * single token's heads are spread over several CTAs when they exceed one pass */
     int tok = 4;
     while (tok > 1 && (CEIL_DIV(p->T, tok) < 2L * c->sms || tok * units > 8 * 256)) tok >>= 1;
