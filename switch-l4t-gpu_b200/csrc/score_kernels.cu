@@ -10,9 +10,13 @@
 // and a change of m turns (s, t) into f s, f (t + s d), f = 2^d: a thread
 // keeps (m, s, t) of its values and looks at m once per four vectors.
 // c (x - m) is one fma with the rounded product c m, the same in every term,
-// so that rounding cancels; values whose product could overflow (masks of the
-// type's lowest value, -inf) take a guarded form, chosen by the vector's
-// minimum.  Sums are FP32.
+// so that its rounding cancels: while |c m| < 2^24 it is a factor of at most
+// 2^(1/2) on s.  From 2^31 on that factor would pass FP32 (a thread that meets
+// masks of -1e10 alone, a temperature of 1e-8), so larger maxima take the
+// difference x - m first, a vector at a time (2048 x 151936 bf16, half of it
+// masks of -1e9: 150 us, of -1e4: 120; unrolled over the tile it would be 144
+// and 137).  Values whose product could overflow (masks of the type's lowest
+// value, -inf) take a guarded form, chosen by the tile's minimum.  Sums are FP32.
 //
 // Bound: HBM (one read of the logits).  For 16-bit logits the 16 exponentials
 // per SM and cycle are close behind, and issue slots too: about eight
@@ -207,7 +211,7 @@ SB_DEV uint4 lp_load(const T *x, int lead, int V, int j) {
 
 // (m, s, t) of a set of values; m in logits, s and t as at the top
 struct LpSum { float m, s, t; };
-SB_DEV bool lp_sane(float m) { return fabsf(m) < 1e30f; }  // c m does not overflow (temperature > 1e-8)
+SB_DEV bool lp_sane(float cm) { return fabsf(cm) < 16777216.f; }  // of a product c m: rounded by at most 1/2
 SB_DEV unsigned long long lp_add2(unsigned long long a, unsigned long long b) {  // two FP32 sums in one instruction
     unsigned long long r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -218,8 +222,13 @@ SB_DEV unsigned long long lp_mul2(unsigned long long a, unsigned long long b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// c (a - b), for b the maximum that sums are held against
-SB_DEV float lp_gap(float a, float b, float c) { return lp_sane(a) && lp_sane(b) ? __fmul_rn(a, c) - __fmul_rn(b, c) : (a - b) * c; }
+// c (a - b) between two maxima that sums are held against: of the rounded products where they are
+SB_DEV float lp_gap(float a, float b, float c) {
+    const float ca = __fmul_rn(a, c), cb = __fmul_rn(b, c);
+    const bool sa = lp_sane(ca), sb = lp_sane(cb);
+    if (sa && sb) return ca - cb;
+    return (a - b) * c + ((sb ? fmaf(b, c, -cb) : 0.f) - (sa ? fmaf(a, c, -ca) : 0.f));
+}
 SB_DEV void lp_raise(LpSum &a, float m, float c) {  // m >= a.m
     if (a.s != 0.f) {
         const float d = lp_max_nan(lp_gap(a.m, m, c), -200.f), f = lp_exp2(d);
@@ -264,13 +273,14 @@ SB_DEV void lp_block(LpSum &a, int &above, float c, LpShared &sh) {
 
 // ln2 (c (x - m) - l2) of a value against finished sums
 SB_DEV float lp_logp(float x, float m, float l2, float c) {
-    return ((lp_sane(x) && lp_sane(m) ? fmaf(x, c, -__fmul_rn(m, c)) : (x - m) * c) - l2) * LP_LN2;
+    const float cm = __fmul_rn(m, c);
+    return ((lp_sane(cm) ? fmaf(x, c, -cm) : (x - m) * c) - l2) * LP_LN2;
 }
 // results of a row from its joined sums; a row of masked choices has m = -inf and s = 0
 SB_DEV void lp_finish(const LpParams &P, int r, LpSum a, int above, float xt, bool given) {
     const bool none = a.m == -INFINITY && a.s == 0.f;
-    const float l2 = log2f(a.s);
-    if (P.lse) P.lse[r] = none ? -INFINITY : lp_sane(a.m) ? (__fmul_rn(a.m, P.c) + l2) * LP_LN2 : fmaf(l2, LP_LN2, a.m * P.inv_temp);
+    const float l2 = log2f(a.s), cm = __fmul_rn(a.m, P.c);
+    if (P.lse) P.lse[r] = none ? -INFINITY : lp_sane(cm) ? (cm + l2) * LP_LN2 : fmaf(l2, LP_LN2, a.m * P.inv_temp);
     if (P.entropy) P.entropy[r] = none ? 0.f : (l2 - a.t / a.s) * LP_LN2;
     if (P.logp) P.logp[r] = !given ? 0.f : none ? -INFINITY : lp_logp(xt, a.m, l2, P.c);
     if (P.rank) P.rank[r] = given ? above : -1;
@@ -354,7 +364,7 @@ SB_DEV void logprobs_body(const LpParams &P) {
         best = fmaxf(best, mx);
         if (best > a.m) lp_raise(a, best, c);
         const float mc = __fmul_rn(a.m, c);
-        const bool sane = lp_sane(a.m);
+        const bool sane = lp_sane(mc);
         if (sane) {
             const unsigned long long c2 = f2_pack(c, c), mc2 = f2_pack(-mc, -mc);
             unsigned long long s2 = 0ull, t2 = 0ull;
@@ -399,17 +409,21 @@ SB_DEV void logprobs_body(const LpParams &P) {
                 for (int e = 0; e < N; e++) sum += v[e];
             }
             if (sum != sum) a.s = sum;
-        } else {  // maxima that c would overflow
-#pragma unroll
-            for (int u = 0; u < LP_U; u++) {
-                if (b + u * LP_THREADS + tid >= v1) continue;
+        } else {  // a large maximum: differences first
 #pragma unroll 1
+            for (int u = 0; u < LP_U; u++) {  // a vector at a time, the tile turned round
+                float v[N];
+                Vec::values(raw[0], v);
+#pragma unroll
                 for (int e = 0; e < N; e++) {
-                    const float y = lp_at<T>(raw[u], e);
-                    const float d = lp_max_nan((y - a.m) * c, -200.f), w = lp_exp2(d);
+                    const float d = lp_max_nan((v[e] - a.m) * c, -200.f), w = lp_exp2(d);
                     a.s += w;
                     a.t = fmaf(w, d, a.t);
                 }
+                const uint4 first = raw[0];
+#pragma unroll
+                for (int i = 0; i + 1 < LP_U; i++) raw[i] = raw[i + 1];
+                raw[LP_U - 1] = first;
             }
         }
         if (count) {
@@ -631,7 +645,7 @@ SB_DEV void logprobs_grad_body(const LpGradParams &P) {
     const int jt = given ? (tok + lead) / N : -1;
     const float lse = P.lse[r], H = P.g_entropy ? P.entropy[r] : 0.f;
     const float gl = given && P.g_logp ? P.g_logp[r] * P.inv_temp : 0.f, ge = P.g_entropy ? P.g_entropy[r] * P.inv_temp : 0.f;
-    const bool none = lse == -INFINITY, sane = lp_sane(lse);
+    const bool none = lse == -INFINITY, sane = fabsf(lse) < 1e30f;  // c times a value of its size does not overflow
     constexpr float L2E = 1.4426950408889634f, L2E_LO = 1.925963033500e-08f;
     const float hi = sane ? lse * L2E : 0.f, lo = sane ? fmaf(lse, L2E, -hi) + lse * L2E_LO : 0.f;
     // dx = -p (a0 + a1 log2 p) with log2 p = d - lo, d = c x - hi: 2^-lo goes into the factors

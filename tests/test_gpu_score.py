@@ -155,6 +155,50 @@ def test_logprobs_lowest_value_masks(cuda_dev, kind, R):
     assert bool(((grad.double() - want).abs() <= torch.finfo(t).eps / 2 * want.abs() + 2.0 ** -19).all())
 
 
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("R", [1, 700])
+@pytest.mark.parametrize("mask,temperature,offset", [
+    (-1e9, 1.0, 0.0), (-1e10, 1.0, 0.0), (-3e15, 0.7, 0.0), (-9e29, 1.0, 0.0), (-9e29, 1e-8, 0.0), (-1e4, 1e-8, 0.0),
+    (-6e4, 1e-8, 20.0), (-6e4, 3e-5, 20.0), (-6e4, 1e-6, -20.0), (-1e30, 1.0, 7e5), (-1e30, 1.0, 7.5e5), (0.0, 1.0, 3e10)])
+def test_logprobs_large_products(cuda_dev, kind, R, mask, temperature, offset):
+    """Maxima whose product with 1 / temperature has no bits left for the
+    choices (masks of -1e10 that fill a thread's share of the row, tiny
+    temperatures, offsets): as exact as without them."""
+    V, k, t = 9001, 5, DT[kind]
+    if max(abs(mask), abs(offset)) > torch.finfo(t).max:
+        pytest.skip("not a value of this type")
+    g = torch.Generator("cuda").manual_seed(V)
+    # steps of a type's last place around the offset, apart by some units of the temperature
+    step = max(abs(offset) * torch.finfo(t).eps, 2 * temperature)
+    x = (offset + step * torch.randint(-6, 1, (R, V), device="cuda", generator=g)).to(t)
+    x[0, : V // 2] = mask
+    x[-1, V // 3: V // 3 * 2] = mask
+    if R > 1:
+        x[1] = mask  # every choice
+        x[2, ::2] = mask
+    tok = torch.randint(0, V, (R,), device="cuda", generator=g).to(torch.int32)
+    got = run(x, tok, k, temperature)
+    top = x.amax(-1).double()  # differences to it, as a quotient of 1e30 holds no ln V in 64 bits either
+    y = (x.double() - top[:, None]) / temperature
+    want = reference(y, tok, k, 1.0) | {n: w for n, w in reference(x, tok, k, 1.0).items() if n in ("rank", "top_ids")}
+    low = want["lse"].clone()
+    want["lse"] += top / temperature
+    base = (V / 256 + 16) * 2.0 ** -24 + 2.0 ** -21
+    spread = -y.gather(1, tok.long()[:, None])[:, 0]
+    seen = torch.where(low[:, None] - y < 700, -y, torch.zeros_like(y)).amax(-1)
+    lim = dict(lse=base + 2.0 ** -22 * want["lse"].abs(), logp=2 * base + 2.0 ** -21 * (spread + math.log(V)),
+               entropy=(2 * base + 2.0 ** -21 * (seen + 1)) * (1 + math.log(V)),
+               top_logp=(torch.full_like(low, 2 * base + 2.0 ** -21 * (math.log(V) + 1)))[:, None] + 2.0 ** -21 * want["top_logp"].abs())
+    for n, b in lim.items():
+        err = (got[n].double() - want[n]).abs()
+        # finite values whose quotient passes FP32 are -inf there
+        big = want[n].abs() > 3.4e38
+        assert bool((err <= b)[~big].all()), (n, float((err / b)[~big].max()))
+        assert bool((got[n][big].abs() > 3.4e38).all()), n
+    for n in ("rank", "top_ids"):
+        assert torch.equal(got[n].long(), want[n]), n
+
+
 def test_logprobs_nan_and_inf(cuda_dev):
     """A NaN or +inf makes its own row's sums NaN, no other row's."""
     x = torch.randn(6, 3001, device="cuda")
