@@ -655,6 +655,8 @@ SB_DEV void logprobs_grad_body(const LpGradParams &P) {
         const float g = lp_exp2(d) * fmaf(b1, d, b0);
         return none ? 0.f : id == tok ? g + gl : g;
     };
+    // values above this need no such limit: |b1 d| stays below 1e37 (a power of two of 0 times an infinity is NaN)
+    const float least = fmaxf(-1e30f, (hi - 1e37f / fmaxf(fabsf(b1), 1.f)) / P.c);
     const unsigned long long c2 = f2_pack(P.c, P.c), hi2 = f2_pack(-hi, -hi), b12 = f2_pack(b1, b1), b02 = f2_pack(b0, b0);
     for (int b = v0; b < v1; b += TILE) {
         uint4 raw[LP_U];
@@ -662,7 +664,7 @@ SB_DEV void logprobs_grad_body(const LpGradParams &P) {
         if (whole) {
 #pragma unroll
             for (int u = 0; u < LP_U; u++) raw[u] = *reinterpret_cast<const uint4 *>(x + ((b + u * LP_THREADS + tid) * N - lead));
-            if (Vec::min(raw) > -1e30f) {
+            if (Vec::min(raw) > least) {
 #pragma unroll
                 for (int u = 0; u < LP_U; u++) {
                     const int j = b + u * LP_THREADS + tid;

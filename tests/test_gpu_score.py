@@ -311,6 +311,45 @@ def test_logprobs_gradient_parts(cuda_dev):
     assert bool(((both - a - b).abs() <= 2.0 ** -19 * (a.abs() + b.abs()) + 1e-9).all())
 
 
+def gradient_bound(x, gl, ge, temperature, want, tok):
+    """As in test_logprobs_gradient, with the choices' spread instead of their
+    size: c (x - m) is rounded relative to itself and the product of the
+    maximum is the same in every term."""
+    y, V = x.double() / temperature, x.shape[1]
+    p = torch.softmax(y, -1)
+    seen = p > 0
+    top = y.amax(-1)
+    spread = torch.where(seen, top[:, None] - y, torch.zeros_like(y)).amax(-1)
+    rel = (V / 256 + 16) * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -21 * (spread + math.log(V) + 1)
+    size = p * (gl.double().abs()[:, None] + ge.double().abs()[:, None] * (2 * math.log(V) + 2 * spread[:, None] + 2)) / temperature
+    hot = torch.zeros_like(p).scatter_(1, tok.long()[:, None], gl.double().abs()[:, None] / temperature)
+    least = {torch.float16: 2.0 ** -25, torch.float32: 1e-37, torch.bfloat16: 1e-37}[x.dtype]
+    return rel[:, None] * size + 2.0 ** -23 * hot + torch.finfo(x.dtype).eps / 2 * want.abs() + least
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("mask,temperature,weight", [(-9e29, 1e-4, 4.0), (-1e22, 1e-8, 1.0), (-9e29, 1.0, 1e10), (-1e4, 1.0, 1.0), (-9e29, 1e-8, 1e-3)])
+def test_logprobs_gradient_large_finite_masks(cuda_dev, kind, mask, temperature, weight):
+    """Masks far below the choices, between the type's lowest value and
+    ordinary logits: their probability is 0, and so is their gradient, also
+    where the entropy's weight times the exponent passes FP32."""
+    R, V, t = 3, 20001, DT[kind]
+    g = torch.Generator("cuda").manual_seed(3)
+    x = (torch.randn(R, V, device="cuda", generator=g) * 2 * temperature).to(t)
+    x[0, : V // 2] = mask
+    x[1, V // 3:] = mask
+    x[2, ::2] = mask
+    tok = torch.tensor([V - 1, 5, 7], dtype=torch.int32, device="cuda")
+    gl, ge = torch.tensor([1.0, -0.5, 0.25], device="cuda"), torch.tensor([weight, -weight, weight], device="cuda")
+    f = run(x, tok, 0, temperature)
+    want, grad = gradient(x, tok, gl, ge, temperature), torch.full_like(x, 7)
+    sb200.logprobs_grad(x, tok, f["lse"], f["entropy"], gl, ge, grad, temperature=temperature, stream=stream())
+    assert not bool(torch.isnan(grad).any())
+    assert bool((grad[x == x.new_tensor(mask)] == 0).all())
+    bound = gradient_bound(x, gl, ge, temperature, want, tok)
+    assert bool(((grad.double() - want).abs() <= bound).all()), float(((grad.double() - want).abs() / bound).max())
+
+
 def test_logprobs_repeats_and_replays(cuda_dev):
     x = torch.randn(5, 60001, device="cuda").half()
     tok = torch.arange(5, dtype=torch.int32, device="cuda")
