@@ -357,6 +357,9 @@ int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, 
  * with lse and entropy from sb_logprobs at the same temperature.  g_logp or
  * g_entropy may be NULL (0); entropy may be NULL without g_entropy.  A row
  * without a token takes no g_logp, a row of masked choices gives zeros.
+ * Rows whose |lse| is 256 and more (16-bit types 1024), where a rounded lse
+ * holds too little of p, are read once more for their maximum and sum, by one
+ * CTA each; an lse that does not agree with these logits is taken as given.
  * grad has the logits' type and may be the logits (same strides). */
 int sb_logprobs_grad(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
                      const float *lse, const float *entropy, const float *g_logp, const float *g_entropy, void *grad,

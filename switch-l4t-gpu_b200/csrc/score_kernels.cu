@@ -45,6 +45,8 @@
 #define LP_CELLS 32    // cells of a thread
 #define LP_KMAX 64
 #define LP_LN2 0.6931471805599453f
+#define LP_L2E 1.4426950408889634f
+#define LP_L2E_LO 1.925963033500e-08f  // log2 e less its FP32 value
 
 // parameter block, mirrored by the host (host/sb_serve.c)
 struct LpParams {
@@ -276,11 +278,16 @@ SB_DEV float lp_logp(float x, float m, float l2, float c) {
     const float cm = __fmul_rn(m, c);
     return ((lp_sane(cm) ? fmaf(x, c, -cm) : (x - m) * c) - l2) * LP_LN2;
 }
-// results of a row from its joined sums; a row of masked choices has m = -inf and s = 0
+// a row of masked choices has m = -inf and s = 0
+SB_DEV float lp_lse(LpSum a, float l2, float c, float inv_temp) {
+    const float cm = __fmul_rn(a.m, c);
+    return a.m == -INFINITY && a.s == 0.f ? -INFINITY : lp_sane(cm) ? (cm + l2) * LP_LN2 : fmaf(l2, LP_LN2, a.m * inv_temp);
+}
+// results of a row from its joined sums
 SB_DEV void lp_finish(const LpParams &P, int r, LpSum a, int above, float xt, bool given) {
     const bool none = a.m == -INFINITY && a.s == 0.f;
-    const float l2 = log2f(a.s), cm = __fmul_rn(a.m, P.c);
-    if (P.lse) P.lse[r] = none ? -INFINITY : lp_sane(cm) ? (cm + l2) * LP_LN2 : fmaf(l2, LP_LN2, a.m * P.inv_temp);
+    const float l2 = log2f(a.s);
+    if (P.lse) P.lse[r] = lp_lse(a, l2, P.c, P.inv_temp);
     if (P.entropy) P.entropy[r] = none ? 0.f : (l2 - a.t / a.s) * LP_LN2;
     if (P.logp) P.logp[r] = !given ? 0.f : none ? -INFINITY : lp_logp(xt, a.m, l2, P.c);
     if (P.rank) P.rank[r] = given ? above : -1;
@@ -618,7 +625,15 @@ extern "C" __global__ void __launch_bounds__(LP_THREADS) logprobs_join(const __g
 // ---------------------------------------------------------------- gradient
 // d logits[v] = (g_logp (1[v = tok] - p_v) - g_entropy p_v (ln p_v + H)) / temperature,
 // p_v = e^(x_v - lse).  Bound: HBM, one read and one write.  lse log2(e) is
-// held as two floats: its rounding alone would be 1e-6 of every p.
+// held as two floats: its rounding alone would be 1e-6 of every p.  What lse
+// lost when it was rounded to FP32 is half a step, |lse| 2^-24 of every p.
+// Below LP_FAR that is at most 2^-17 (16-bit types 2^-15); a row beyond (a
+// common offset of the logits, a tiny temperature, nothing but the type's
+// lowest value, -inf) is the work of one CTA, which takes its maximum and sum
+// again as the forward pass does, before anything of it is written (grad may
+// be the logits): 2048 x 151936 bf16 offset by 1e4 357 us instead of 205, 300 x
+// 50257 FP32 67 instead of 22, one row of 151936 109 instead of 3.5.  An lse
+// that is not the row's own is used as given.
 struct LpGradParams {
     const void *x;
     void *dx;
@@ -628,6 +643,106 @@ struct LpGradParams {
     const int *tok;
     const float *lse, *entropy, *g_logp, *g_entropy;
 };
+template <typename T> constexpr float LP_FAR = sizeof(T) == 4 ? 256.f : 1024.f;
+// dx = -p (a0 + a1 log2 p) / temperature with log2 p = d - lo: 2^-lo goes into the factors
+struct LpFactors { float lo, gl, b0, b1; };
+SB_DEV LpFactors lp_factors(const LpGradParams &P, int r, bool given, float lo) {
+    const float gl = given && P.g_logp ? P.g_logp[r] * P.inv_temp : 0.f, ge = P.g_entropy ? P.g_entropy[r] * P.inv_temp : 0.f;
+    const float a1 = ge * LP_LN2, a0 = gl + ge * (P.g_entropy ? P.entropy[r] : 0.f), f = lp_exp2(-lo);
+    return {lo, gl, -(a0 - a1 * lo) * f, -a1 * f};
+}
+// one value at d, any range
+SB_DEV float lp_grad1(float d, const LpFactors &F, bool token) {
+    d = lp_max_nan(d, -200.f);
+    const float g = lp_exp2(d) * fmaf(F.b1, d, F.b0);
+    return token ? g + F.gl : g;
+}
+// vector j of a row, and its gradient
+template <typename T> SB_DEV uint4 lp_load_again(const T *x, int lead, int V, int j) {  // not as constant memory
+    const int e0 = j * LpVec<T>::N - lead;
+    return e0 >= 0 && e0 + LpVec<T>::N <= V ? *reinterpret_cast<const uint4 *>(x + e0) : lp_load(x, lead, V, j);
+}
+template <typename T> SB_DEV void lp_store(T *dx, bool same, int lead, int V, int j, const float (&v)[LpVec<T>::N]) {
+    constexpr int N = LpVec<T>::N;
+    const int e0 = j * N - lead;
+    if (same && e0 >= 0 && e0 + N <= V) *reinterpret_cast<uint4 *>(dx + e0) = LpVec<T>::packed(v);
+    else
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (e0 + e >= 0 && e0 + e < V) dx[e0 + e] = lp_to<T>(v[e]);
+}
+// A row whose lse is far from 0, by one CTA.  Not inlined: its code and registers are not those of the kernel below.
+template <typename T>
+__device__ __noinline__ void logprobs_grad_far(const LpGradParams &P, int r) {
+    using Vec = LpVec<T>;
+    constexpr int N = Vec::N, STEP = LP_THREADS * LP_U;
+    __shared__ LpShared sum_s;
+    const T *x = static_cast<const T *>(P.x) + r * P.stride;
+    T *dx = static_cast<T *>(P.dx) + r * P.dstride;
+    const int lead = (int)(((uintptr_t)x & 15) / sizeof(T)), nv = (int)(((long long)lead + P.V + N - 1) / N);
+    const bool same = (((uintptr_t)x ^ (uintptr_t)dx) & 15) == 0;
+    const float c = P.c, lse = P.lse[r];
+    uint4 raw[LP_U];
+    LpSum a = {-INFINITY, 0.f, 0.f};
+    for (int b = threadIdx.x; b < nv; b += STEP) {
+#pragma unroll
+        for (int u = 0; u < LP_U; u++) {
+            raw[u] = make_uint4(Vec::NEG_INF, Vec::NEG_INF, Vec::NEG_INF, Vec::NEG_INF);
+            if (b + u * LP_THREADS < nv) raw[u] = lp_load_again(x, lead, P.V, b + u * LP_THREADS);
+        }
+        const float mx = Vec::max(raw);
+        if (mx > a.m) lp_raise(a, mx, c);
+        if (a.m == -INFINITY) continue;
+        const float mc = __fmul_rn(a.m, c);
+        const bool sane = lp_sane(mc);
+        const float off = sane ? 0.f : a.m, base = sane ? -mc : 0.f;
+#pragma unroll
+        for (int u = 0; u < LP_U; u++) {
+            float v[N];
+            Vec::values(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < N; e++) a.s += lp_exp2(fmaf(v[e] - off, c, base));
+        }
+        a.t = 0.f;
+    }
+    int count = 0;
+    lp_block(a, count, c, sum_s);
+    // p = 2^(d - lo), d = (x k - off) c1 - hi
+    const float l2 = log2f(a.s), own = lp_lse(a, l2, c, P.inv_temp);
+    float k = 1.f, off = 0.f, c1 = c, hi = 0.f, lo = 0.f;
+    bool none = lse == -INFINITY;
+    if (own == lse || fabsf(own - lse) <= fabsf(lse) * 4.76837158e-7f) {  // 2^-21: both are rounded, on either side
+        none = a.m == -INFINITY;
+        const float cm = __fmul_rn(a.m, c);
+        if (lp_sane(cm)) hi = cm;
+        else off = a.m;
+        lo = none ? 0.f : l2;
+    } else if (fabsf(lse) < 1e30f) {  // of more than this row
+        hi = lse * LP_L2E;
+        lo = fmaf(lse, LP_L2E, -hi) + lse * LP_L2E_LO;
+    } else {
+        k = P.inv_temp;
+        off = lse;
+        c1 = LP_L2E;
+    }
+    const int tok = P.tok ? P.tok[r] : -1;
+    const LpFactors F = lp_factors(P, r, tok >= 0 && tok < P.V, lo);
+    for (int b = threadIdx.x; b < nv; b += STEP) {
+#pragma unroll
+        for (int u = 0; u < LP_U; u++)
+            if (b + u * LP_THREADS < nv) raw[u] = lp_load_again(x, lead, P.V, b + u * LP_THREADS);
+#pragma unroll
+        for (int u = 0; u < LP_U; u++) {
+            const int j = b + u * LP_THREADS;
+            if (j >= nv) break;
+            float v[N];
+            Vec::values(raw[u], v);
+#pragma unroll
+            for (int e = 0; e < N; e++) v[e] = none ? 0.f : lp_grad1(fmaf(fmaf(v[e], k, -off), c1, -hi), F, j * N - lead + e == tok);
+            lp_store(dx, same, lead, P.V, j, v);
+        }
+    }
+}
 template <typename T>
 SB_DEV void logprobs_grad_body(const LpGradParams &P) {
     using Vec = LpVec<T>;
@@ -643,24 +758,20 @@ SB_DEV void logprobs_grad_body(const LpGradParams &P) {
     const int tok = P.tok ? P.tok[r] : -1;
     const bool given = tok >= 0 && tok < P.V;
     const int jt = given ? (tok + lead) / N : -1;
-    const float lse = P.lse[r], H = P.g_entropy ? P.entropy[r] : 0.f;
-    const float gl = given && P.g_logp ? P.g_logp[r] * P.inv_temp : 0.f, ge = P.g_entropy ? P.g_entropy[r] * P.inv_temp : 0.f;
-    const bool none = lse == -INFINITY, sane = fabsf(lse) < 1e30f;  // c times a value of its size does not overflow
-    constexpr float L2E = 1.4426950408889634f, L2E_LO = 1.925963033500e-08f;
-    const float hi = sane ? lse * L2E : 0.f, lo = sane ? fmaf(lse, L2E, -hi) + lse * L2E_LO : 0.f;
-    // dx = -p (a0 + a1 log2 p) with log2 p = d - lo, d = c x - hi: 2^-lo goes into the factors
-    const float a1 = ge * LP_LN2, a0 = gl + ge * H, f = lp_exp2(-lo), b1 = -a1 * f, b0 = -(a0 - a1 * lo) * f;
-    auto grad = [&](float v, int id) {  // one value, any range
-        const float d = lp_max_nan(sane ? fmaf(v, P.c, -hi) : (v * P.inv_temp - lse) * L2E, -200.f);
-        const float g = lp_exp2(d) * fmaf(b1, d, b0);
-        return none ? 0.f : id == tok ? g + gl : g;
-    };
+    const float lse = P.lse[r];
+    if (fabsf(lse) >= LP_FAR<T>) {  // not a NaN: that makes a row of them
+        if (part == 0) logprobs_grad_far<T>(P, r);
+        return;
+    }
+    const float hi = lse * LP_L2E;
+    const LpFactors F = lp_factors(P, r, given, fmaf(lse, LP_L2E, -hi) + lse * LP_L2E_LO);
+    auto grad = [&](float v, int id) { return lp_grad1(fmaf(v, P.c, -hi), F, id == tok); };
     // values above this need no such limit: |b1 d| stays below 1e37 (a power of two of 0 times an infinity is NaN)
-    const float least = fmaxf(-1e30f, (hi - 1e37f / fmaxf(fabsf(b1), 1.f)) / P.c);
-    const unsigned long long c2 = f2_pack(P.c, P.c), hi2 = f2_pack(-hi, -hi), b12 = f2_pack(b1, b1), b02 = f2_pack(b0, b0);
+    const float least = fmaxf(-1e30f, (hi - 1e37f / fmaxf(fabsf(F.b1), 1.f)) / P.c);
+    const unsigned long long c2 = f2_pack(P.c, P.c), hi2 = f2_pack(-hi, -hi), b12 = f2_pack(F.b1, F.b1), b02 = f2_pack(F.b0, F.b0);
     for (int b = v0; b < v1; b += TILE) {
         uint4 raw[LP_U];
-        const bool whole = same && sane && b >= whole0 && b + TILE <= whole1;
+        const bool whole = same && b >= whole0 && b + TILE <= whole1;
         if (whole) {
 #pragma unroll
             for (int u = 0; u < LP_U; u++) raw[u] = *reinterpret_cast<const uint4 *>(x + ((b + u * LP_THREADS + tid) * N - lead));

@@ -324,7 +324,9 @@ def gradient_bound(x, gl, ge, temperature, want, tok):
     size = p * (gl.double().abs()[:, None] + ge.double().abs()[:, None] * (2 * math.log(V) + 2 * spread[:, None] + 2)) / temperature
     hot = torch.zeros_like(p).scatter_(1, tok.long()[:, None], gl.double().abs()[:, None] / temperature)
     least = {torch.float16: 2.0 ** -25, torch.float32: 1e-37, torch.bfloat16: 1e-37}[x.dtype]
-    return rel[:, None] * size + 2.0 ** -23 * hot + torch.finfo(x.dtype).eps / 2 * want.abs() + least
+    # a power of two below 2^-126 is flushed to 0: there the whole value is missing, p times the same factor
+    flushed = 2.0 ** -126 * (gl.double().abs() + ge.double().abs() * (2 * math.log(V) + 2 * spread + 2)) / temperature
+    return rel[:, None] * size + flushed[:, None] + 2.0 ** -23 * hot + torch.finfo(x.dtype).eps / 2 * want.abs() + least
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
@@ -348,6 +350,77 @@ def test_logprobs_gradient_large_finite_masks(cuda_dev, kind, mask, temperature,
     assert bool((grad[x == x.new_tensor(mask)] == 0).all())
     bound = gradient_bound(x, gl, ge, temperature, want, tok)
     assert bool(((grad.double() - want).abs() <= bound).all()), float(((grad.double() - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("R,V", [(2, 20001), (700, 3001)])
+@pytest.mark.parametrize("offset,temperature", [(1e4, 1.0), (-1e4, 1.0), (0.0, 1e-3), (3e4, 0.5), (300.0, 1.0)])
+def test_logprobs_gradient_offset(cuda_dev, R, V, offset, temperature):
+    """A common offset of a row, or a temperature that makes one, changes no
+    probability: the gradient is as exact as without, and what the token and
+    the choices get adds up to nothing.  (Logits in steps of 2^-9, so that the
+    offset is exact.)"""
+    g = torch.Generator("cuda").manual_seed(V)
+    x = torch.round(torch.randn(R, V, device="cuda", generator=g) * 2 * 512) / 512
+    x = x + offset
+    tok = torch.randint(0, V, (R,), device="cuda", generator=g).to(torch.int32)
+    gl, ge = (torch.randn(R, device="cuda", generator=g) for _ in range(2))
+    f = run(x, tok, 0, temperature)
+    for a, b in ((gl, ge), (gl, None), (None, ge)):
+        zero = torch.zeros_like(gl)
+        want = gradient(x, tok, zero if a is None else a, zero if b is None else b, temperature)
+        bound = gradient_bound(x, zero if a is None else a, zero if b is None else b, temperature, want, tok)
+        grad = torch.full_like(x, 7)
+        sb200.logprobs_grad(x, tok, f["lse"], f["entropy"], a, b, grad, temperature=temperature, stream=stream())
+        assert bool(((grad.double() - want).abs() <= bound).all()), float(((grad.double() - want).abs() / bound).max())
+        assert bool((grad.double().sum(-1).abs() <= bound.sum(-1)).all())
+        z = x.clone()
+        sb200.logprobs_grad(z, tok, f["lse"], f["entropy"], a, b, z, temperature=temperature, stream=stream())
+        assert torch.equal(z, grad)  # in place
+
+
+@pytest.mark.parametrize("kind", list(DT))
+@pytest.mark.parametrize("R,temperature", [(1, 1.0), (700, 1.0), (3, 0.5)])
+def test_logprobs_gradient_equal_lowest_values(cuda_dev, kind, R, temperature):
+    """A row of the type's lowest value (every choice masked that way): n equal
+    choices of probability 1 / n, as the forward call has them."""
+    V, t = 3001, DT[kind]
+    x = torch.full((R, V), torch.finfo(t).min, dtype=t, device="cuda")
+    tok = torch.full((R,), 2000, dtype=torch.int32, device="cuda")
+    g = torch.Generator("cuda").manual_seed(R)
+    gl, ge = (torch.randn(R, device="cuda", generator=g) for _ in range(2))
+    for _ in range(2):
+        f = run(x, tok, 0, temperature)
+        p = (x > -math.inf).double()
+        p /= p.sum(-1, keepdim=True)
+        H = -torch.log(p.amax(-1, keepdim=True))  # = - ln p of every choice: the entropy's gradient is 0
+        want = torch.where(p > 0, -gl.double()[:, None] * p, torch.zeros_like(p))
+        want.scatter_add_(1, tok.long()[:, None], gl.double()[:, None])
+        want /= temperature
+        grad = torch.full_like(x, 7)
+        sb200.logprobs_grad(x, tok, f["lse"], f["entropy"], gl, ge, grad, temperature=temperature, stream=stream())
+        # p to (n / 256 + 16) half steps and 2^-20; the entropy's terms, of size ln n p, cancel to as much
+        bound = 2.0 ** -17 * p * (gl.double().abs()[:, None] + ge.double().abs()[:, None] * (2 * H + 2)) / temperature
+        bound += 2.0 ** -23 * want.abs() + torch.finfo(t).eps / 2 * want.abs() + (2.0 ** -25 if t == torch.float16 else 1e-37)
+        assert bool(((grad.double() - want).abs() <= bound).all()), float(((grad.double() - want).abs() / bound).max())
+        x[:, : V // 2] = -math.inf
+
+
+def test_logprobs_gradient_takes_the_given_lse(cuda_dev):
+    """The softmax may go over more than these logits (a vocabulary cut over
+    several calls): an lse that is not the row's own is taken as it is."""
+    g = torch.Generator("cuda").manual_seed(11)
+    x = torch.round(torch.randn(4, 30000, device="cuda", generator=g) * 512) / 512 + 5000.0
+    tok, one = torch.tensor([3, 17, -1, 9], dtype=torch.int32, device="cuda"), torch.ones(4, device="cuda")
+    f = run(x, tok)
+    half = x[:, :15000].contiguous()
+    grad = torch.empty_like(half)
+    sb200.logprobs_grad(half, tok, f["lse"], None, one, None, grad, stream=stream())
+    p = torch.exp(half.double() - f["lse"].double()[:, None])
+    want = -p
+    want[torch.tensor([0, 1, 3]), torch.tensor([3, 17, 9])] += 1
+    want[2] = 0
+    # c x - lse log2(e): a half step of FP32 of 7213 is 2^-12
+    assert bool(((grad.double() - want).abs() <= 2.0 ** -12 * p + 2.0 ** -23 * want.abs()).all())
 
 
 def test_logprobs_repeats_and_replays(cuda_dev):
