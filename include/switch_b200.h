@@ -317,7 +317,8 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * all of them, and each request's own positions.  q, out [T][NH][HD] (HD % 8
  * == 0, <= 128; 16-byte aligned rows) of the pages' type; NH / NKV query
  * heads share a key head.  Rows cu_q[b] .. cu_q[b + 1] belong to request b
- * (cu_q nondecreasing from 0; NULL: row b is request b); row i of n sees all
+ * (cu_q nondecreasing from 0; rows from T on are not there, and change nothing
+ * for the others; NULL: row b is request b); row i of n sees all
  * prefix_len positions of the prefix and the first kv_len[b] - n + i + 1 of
  * the request's own (its new tokens are in the pages already).  prefix_table
  * and table rows hold page numbers (prefix_table NULL: 0, 1, 2, ...); a

@@ -101,18 +101,20 @@ SB_DEV bool ap_own_item(const AttnParams &P, int idx, int MT, AttnItem &it, int 
     tile = rest - pair * P.tiles2;
     const int b = P.NKV > 1 ? pair / P.NKV : pair;
     it.kvh = pair - b * P.NKV;
-    int q0 = b, q1 = b + 1;
+    int q0 = b, q1 = b + 1, n = 1;  // rows that are there, and all of the request's: their limits go by these
     if (P.cu_q) {
         q0 = min(max(P.cu_q[b], 0), P.T);
-        q1 = min(max(P.cu_q[b + 1], q0), P.T);
+        q1 = max(P.cu_q[b + 1], q0);
+        n = q1 - q0;
+        q1 = min(q1, P.T);
     }
-    const int len = min(max(P.kv_len[b], 0), P.max_kv), n = q1 - q0;
+    const int len = min(max(P.kv_len[b], 0), P.max_kv);
     it.slot = P.S1 + s;
     it.pg = P.suf;
     it.table = P.table + (long long)b * P.table_stride;
     it.k0 = s * P.chunk2;
     it.k1 = min(it.k0 + P.chunk2, len);
-    it.F = n * P.G;
+    it.F = (q1 - q0) * P.G;
     it.row0 = q0;
     it.vis0 = len - n + 1;
     it.vis1 = len;

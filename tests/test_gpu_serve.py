@@ -372,6 +372,24 @@ def test_attn_prefix_many_rows(cuda_dev, kind, NH, NKV, HD, P, lens, rows, page,
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("NH,NKV,HD,P,lens,rows,T", [
+    (14, 2, 64, 40, [20, 9, 30], [3, 4, 2], 6),      # the second request's last row and the third's are not there
+    (4, 2, 128, 0, [70, 60, 90], [30, 40, 20], 50),  # row tiles of 64
+    (4, 2, 64, 300, [200, 90], [150, 60], 140),      # a prefix of 256-row tiles
+    (4, 2, 64, 0, [5, 2, 9], [4, 6, 2], 8)])         # more rows than positions
+def test_attn_prefix_rows_past_the_last(cuda_dev, kind, NH, NKV, HD, P, lens, rows, T):
+    """Fewer rows than the requests have together (as the page plan lists
+    fewer tokens than there are): those that are there see what they would
+    see among all of them."""
+    b = Batch(kind, NH, NKV, HD, P, lens, rows=rows, seed=41)
+    wo, wl, size = b.want()
+    b.q, b.T = b.q[:T].contiguous(), T
+    out, lse = b.run()
+    b.rows = [T]
+    b.check(got=(out, lse), want=(wo[:T], wl[:T], size[:T]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attn_prefix_large_batch(cuda_dev, kind):
     """Many row tiles on one key head, a long prefix cut into ranges, ragged
     own lengths."""
