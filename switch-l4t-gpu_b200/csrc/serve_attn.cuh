@@ -960,7 +960,7 @@ extern "C" __global__ void __launch_bounds__(128) attn_join(const __grid_constan
     const long long rows = (long long)ap_rows(P) * P.NH;
     for (long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5); i < TH; i += (long long)gridDim.x * 4) {
         const int row = TH >> 32 ? (int)(i / P.NH) : (int)((unsigned)i / (unsigned)P.NH), head = (int)(i - (long long)row * P.NH);
-        const int most = P.S1 + P.S2, own = P.S2 ? P.ws_n[row] : 0;
+        const int most = P.S1 + P.S2, own = P.S2 ? min(max(P.ws_n[row], 0), P.S2) : 0;  // a row of no request has no count
         float M = -INFINITY, L = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         float2 ml = lane < most ? P.ws_ml[lane * TH + i] : make_float2(0.f, 0.f);

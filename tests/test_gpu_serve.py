@@ -390,6 +390,22 @@ def test_attn_prefix_rows_past_the_last(cuda_dev, kind, NH, NKV, HD, P, lens, ro
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_rows_of_no_request(cuda_dev, kind):
+    """Row offsets that do not start at 0: the rows before the first request
+    mean nothing, but no part outside the workspace is read for them, and the
+    others are right."""
+    b = Batch(kind, 14, 2, 64, 1000, [40, 300, 170], rows=[2, 1, 3], seed=43)
+    wo, wl, size = b.want()
+    b.run()
+    ws = torch.full((sb200.attn_prefix_ws(b.q, b.kv, 1000, 2, max_q=3, max_kv=300) // 4 + 4,), float("nan"), device="cuda")
+    out, lse = torch.full_like(b.q, 7.0), torch.full((b.T, 14), 7.0, device="cuda")
+    sb200.attn_prefix(b.q, out, b.kv, b.ptable, 1000, b.kv, b.table[1:], b.kv_len[1:], b.scale, ws, cu_q=b.cu[1:], max_q=3, max_kv=300,
+                      lse=lse, stream=stream())
+    b.rows = [4]
+    b.check(got=(out[2:], lse[2:]), want=(wo[2:], wl[2:], size[2:]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attn_prefix_large_batch(cuda_dev, kind):
     """Many row tiles on one key head, a long prefix cut into ranges, ragged
     own lengths."""
