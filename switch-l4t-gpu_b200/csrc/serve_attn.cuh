@@ -242,7 +242,9 @@ template <int KT, int HDP, int E> struct ApCopy {
 // keys, touch all banks).  Whole pages come by TMA boxes, one lane a box:
 // copies by the lanes (tiles that end inside a page or miss one, other page
 // sizes, calls too small to encode a map for) cost a third of all
-// instructions of a decode tile.
+// instructions of a decode tile.  Where a box may follow into the place of a
+// tile that the lanes copied, that tile has a gap: its reader orders the two by
+// a proxy fence before it gives the place up.
 template <int KW, int HDP, int E> struct ApRing {
     static constexpr int SUB = HDP * E / 128, BLOCK = KW * 128, TILE = SUB * BLOCK, KT = KW * (SB_AP_THREADS / 32);
     static constexpr int C = HDP * E / 16, STEP = 32 / C, N = KW / STEP;
@@ -623,7 +625,8 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
         const int key = first + t * KT + g;
         if (!(ok = ring.wait(0, t))) break;
         const unsigned valid = ring.valid(t);
-        const bool there0 = valid >> g & 1, there1 = valid >> (g + 8) & 1;
+        const bool there0 = valid >> g & 1, there1 = valid >> (g + 8) & 1, gaps = valid != ~0u;
+        if (gaps) ap_fence_async();
         float s[NB][4];
 #pragma unroll
         for (int b = 0; b < NB; b++) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
@@ -676,6 +679,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             p[b][1] = ap_movmatrix(ap_pack<T>(s[b][2], s[b][3]));
         }
         if (!(ok = ring.wait(1, t))) break;
+        if (gaps) ap_fence_async();
 #pragma unroll
         for (int i = 0; i < KS; i++) {
             const int mid = lane >> 3, r = (mid >> 1) * 8 + (lane & 7), c = 2 * i + (mid & 1);
@@ -779,7 +783,9 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     for (; t < nt; t++) {
         const unsigned char *kt = sm + (ring.tile(0, t) - ap_smem(sm)), *vt = sm + (ring.tile(1, t) - ap_smem(sm));
         if (!(ok = ring.wait(0, t))) break;
-        const bool there = ring.valid(t) >> key & 1;
+        const unsigned valid = ring.valid(t);
+        const bool there = valid >> key & 1, gaps = valid != ~0u;
+        if (gaps) ap_fence_async();
         unsigned long long acc[MT];
 #pragma unroll
         for (int r = 0; r < MT; r++) acc[r] = 0ull;
@@ -825,6 +831,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
         }
         __syncwarp();
         if (!(ok = ring.wait(1, t))) break;
+        if (gaps) ap_fence_async();
 #pragma unroll
         for (int k = 0; k < KW; k++) {
             unsigned long long v[DP];

@@ -487,6 +487,31 @@ def _missing_pages(b):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("NH,NKV,HD,rows,page", [(4, 2, 64, 1, 16), (8, 2, 128, 1, 32), (12, 2, 64, 2, 8), (4, 2, 128, 6, 64)])
+def test_attn_prefix_missing_pages_among_many(cuda_dev, kind, NH, NKV, HD, rows, page):
+    """Enough keys that whole pages come by boxes, with pages missing all
+    along: tiles that are copied otherwise and boxes take the same places in
+    turn."""
+    B = 40
+    b = Batch(kind, NH, NKV, HD, 700, [1000 + 13 * i for i in range(B)], rows=[rows] * B, page=page, seed=47)
+    gone = torch.rand(b.table.shape, generator=torch.Generator().manual_seed(5)) < 0.2
+    lens = list(b.lens)
+    for r in range(B):
+        j = torch.arange(lens[r], device="cuda") // page
+        gone[r, int(j[-rows]):] = False  # the rows' own positions, so that their limits cut what is there
+        keep = ~gone[r].cuda()[j]
+        b.places[r] = tuple(x[keep] for x in b.places[r])
+        b.table[r][gone[r].cuda()] = -1
+    first = torch.arange(b.ptable.numel(), device="cuda")
+    b.ptable[first % 4 == 1] = -1
+    at = torch.arange(700, device="cuda")
+    b.places[-1] = tuple(x[at // page % 4 != 1] for x in b.places[-1])
+    got = b.run()
+    b.lens, b.P = [len(p[0]) for p in b.places[:-1]], len(b.places[-1][0])
+    b.check(got=got, want=b.want())
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attn_prefix_only_one_side(cuda_dev, kind):
     """No own positions at all (max_kv 0), or no prefix: the other side's
     arguments may be absent; nothing on both sides gives zeros."""
