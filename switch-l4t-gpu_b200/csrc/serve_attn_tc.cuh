@@ -394,11 +394,21 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             const float mx = max_nan(max_nan(mx4[0], mx4[1]), max_nan(mx4[2], mx4[3])) * sc;
             if (t == 0) m = mx;
             // the weights are taken against the maximum so far, beside the search for the new one; where that has
-            // grown too far (or a NaN turns up) they are taken again
+            // grown too far (or a NaN turns up) they are taken again.  sc s - m is one fma with a rounded m: from 2^24 on
+            // that is off by 1/2 and more, as the FP32 scores are, and from 2^31 on it passes FP32 as a power of two.
+            // There the scores are rounded first, as m was
             unsigned long long l2;
+            float by = sc;
             for (;;) {
-                l2 = weights<T>(r, sc, m == -INFINITY ? 0.f : m, s_at);
-                if (!__any_sync(SB_FULL, mx > m + 8.f || (mx != mx && m == m))) break;
+                l2 = weights<T>(r, by, m == -INFINITY ? 0.f : m, s_at);
+                if (!__any_sync(SB_FULL, mx > m + 8.f || (fabsf(mx) >= 16777216.f && by != 1.f) || (mx != mx && m == m))) break;
+                if (by != 1.f && __any_sync(SB_FULL, fabsf(mx) >= 16777216.f)) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) r[c][i] = __float_as_uint(__fmul_rn(__uint_as_float(r[c][i]), sc));
+                    by = 1.f;
+                }
                 const float to = max_nan(m, mx), a = m == to ? 1.f : ap_exp2(m - to);
                 m = to;
                 l *= a;

@@ -461,6 +461,34 @@ def test_attn_prefix_peaked_scores(cuda_dev, kind):
     assert bool(((lse.double() - wl).abs() <= 130 * 2.0 ** -24 * 1536 * b.scale + 2.0 ** -21 * wl.abs()).all())
 
 
+@pytest.mark.parametrize("kind,size", [("bf16", 1e6), ("bf16", 3e3), ("f16", 1e4), ("f32", 1e6), ("f32", 1e10)])
+@pytest.mark.parametrize("B,NH,NKV,HD,P,scale", [
+    (40, 8, 2, 64, 600, 0.125), (3, 4, 2, 64, 300, 0.125), (60, 8, 2, 128, 0, 0.09), (5, 100, 2, 128, 300, 0.09), (40, 8, 2, 64, 600, -0.125),
+    (40, 8, 2, 128, 300, math.log(2.0))])
+def test_attn_prefix_far_scores(cuda_dev, kind, size, B, NH, NKV, HD, P, scale):
+    """Scores from 2^24 to far past 2^31: FP32 holds them to 2^-19 of what
+    their products add up to (HD + 2 terms, truncated), so a row whose best
+    score leads by 30 and twice that much is its value; lse is that score."""
+    b = Batch(kind, NH, NKV, HD, P, [(i * 37) % 90 + 2 for i in range(B)], seed=3, peak=size)
+    b.scale = scale
+    out, lse = b.run()
+    assert bool(torch.isfinite(out.float()).all()) and bool(torch.isfinite(lse).all())
+    G, clear = NH // NKV, 0
+    for r in range(B):
+        k, v = (torch.cat([x[b.places[-1]], x[b.places[r]]]).double().transpose(0, 1) for x in (b.k, b.v))
+        q = b.q[r].double().view(NKV, G, HD)
+        s = torch.einsum("hgd,hkd->hgk", q, k) * scale
+        off = 2.0 ** -19 * abs(scale) * torch.einsum("hgd,hkd->hgk", q.abs(), k.abs()).amax(-1)
+        two = torch.topk(s, 2, -1)
+        ok = two.values[..., 0] - two.values[..., 1] > 30 + 2 * off
+        want = torch.gather(v[:, None].expand(-1, G, -1, -1), 2, two.indices[..., :1, None].expand(-1, -1, 1, HD))[:, :, 0]
+        got = out[r].double().view(NKV, G, HD)
+        assert bool(((got - want).abs()[ok] <= 2.0 ** -20 * want.abs()[ok]).all())  # the weight 1, and its own division
+        assert bool(((lse[r].double().view(NKV, G) - two.values[..., 0]).abs()[ok] <= off[ok] + 2.0 ** -22 * two.values[..., 0].abs()[ok]).all())
+        clear += int(ok.sum())
+    assert clear > 0.9 * B * NH
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_attn_prefix_missing_pages(cuda_dev, kind):
     """A page number outside the pool: its positions are skipped, as if they
