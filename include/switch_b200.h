@@ -330,7 +330,9 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * requests are still right; kv_len is cut to max_kv.  A row that sees nothing
  * gives zeros and lse = -inf; rows from cu_q[B] on are left as they were.
  * lse [T][NH] (natural log of the softmax denominator) may be NULL.
- * ws: sb_attn_prefix_ws bytes for the same sizes (32-byte aligned).  FP32
+ * ws: sb_attn_prefix_ws bytes for the same sizes (32-byte aligned); fewer
+ * rows or shorter lengths may need more, as they are cut into more ranges, so
+ * one workspace for several sizes has the largest answer among them.  FP32
  * runs on CUDA cores in FP32 throughout; 16-bit types use the tensor cores
  * with FP32 scores, sums and outputs and 16-bit softmax weights. */
 int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes);
@@ -348,7 +350,8 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
  * temperature is at least 1e-8.  Masked choices (-inf) have probability 0 and are not listed (id -1,
  * -inf fill up); a row of them gives lse = logp = -inf and entropy 0.  A row
  * with a NaN or +inf gives NaN sums, its ids and rank mean nothing.
- * ws: sb_logprobs_ws bytes (16-byte aligned). */
+ * ws: sb_logprobs_ws bytes (16-byte aligned), enough for any smaller R, V and
+ * top_k too. */
 int sb_logprobs_ws(int type, int R, int V, int top_k, size_t *bytes);
 int sb_logprobs(const void *logits, int64_t row_stride, int type, int R, int V, float temperature, const int *tokens,
                 float *logp, float *entropy, float *lse, int *rank, int top_k, int *top_ids, float *top_logp, void *ws,

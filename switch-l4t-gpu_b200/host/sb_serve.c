@@ -576,7 +576,11 @@ int sb_logprobs_ws(int type, int R, int V, int top_k, size_t *bytes) {
     if (R == 0) return 0;
     sb_ctx *c = sb_ctx_get();
     if (!c) return SB_ERR_STATE;
-    *bytes = lp_ws_bytes(R, lp_parts(c, R, V, type, 8), top_k);
+    /* fewer rows are cut into more parts, so the most is needed by some number below R */
+    for (int r = R < 4 * c->sms ? R : 4 * c->sms; r > 0; r--) {
+        const size_t need = lp_ws_bytes(r, lp_parts(c, r, V, type, 8), top_k);
+        if (need > *bytes) *bytes = need;
+    }
     return 0;
 }
 

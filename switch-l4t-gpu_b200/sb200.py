@@ -502,7 +502,8 @@ def rotary_kv(q, q_out, k, v, pos, slots, plan, kv, stream=None):
 
 def attn_prefix_ws(q, kv, prefix_len, B, max_q=1, max_kv=0):
     """Workspace bytes of attn_prefix for these sizes (kv: the prefix' or the
-    requests' pages)."""
+    requests' pages).  Smaller sizes may need more: a workspace for several
+    has the largest answer among them."""
     n = ctypes.c_size_t()
     check(lib().sb_attn_prefix_ws(_type(q), q.shape[0], B, q.shape[1], kv.NKV, kv.HD, max_q, prefix_len, max_kv, ctypes.byref(n)))
     return n.value
@@ -544,7 +545,8 @@ def attn_prefix(q, out, prefix, prefix_table, prefix_len, kv, table, kv_len, sca
 
 
 def logprobs_ws(logits, top_k=0):
-    """Workspace bytes of logprobs for these logits [R, V]."""
+    """Workspace bytes of logprobs for logits of up to [R, V] and up to top_k
+    alternatives."""
     n = ctypes.c_size_t()
     check(lib().sb_logprobs_ws(_type(logits), logits.shape[0], logits.shape[1], top_k, ctypes.byref(n)))
     return n.value

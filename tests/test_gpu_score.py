@@ -228,6 +228,24 @@ def test_logprobs_some_outputs(cuda_dev):
         sb200.logprobs(x, None, ws, logp=lse)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_logprobs_workspace_for_smaller_batches(cuda_dev, kind):
+    """One workspace, asked for at the largest sizes, for every smaller batch,
+    vocabulary and number of alternatives (fewer rows are cut into more
+    parts)."""
+    g = torch.Generator("cuda").manual_seed(2)
+    x = torch.randn(1300, 20001, device="cuda", generator=g).to(DT[kind])
+    tok = torch.randint(0, 3000, (1300,), device="cuda", generator=g).to(torch.int32)
+    ws = torch.full((sb200.logprobs_ws(x, 20),), 0xFF, dtype=torch.uint8, device="cuda")
+    for R, V, k in ((1300, 20001, 20), (592, 20001, 20), (591, 20001, 20), (300, 20001, 20), (149, 20001, 20), (7, 20001, 20), (1, 20001, 20),
+                    (40, 3000, 20), (591, 9000, 5), (3, 20001, 1)):
+        assert sb200.logprobs_ws(x[:R, :V], k) <= ws.numel()
+        want = run(x[:R, :V], tok[:R], k)
+        got = {n: torch.zeros_like(v) for n, v in want.items()}
+        sb200.logprobs(x[:R, :V], tok[:R], ws, stream=stream(), **got)
+        assert all(torch.equal(got[n], want[n]) for n in got), (R, V, k)
+
+
 def gradient(x, tok, gl, ge, temperature):
     y = x.double() / temperature
     logs = torch.log_softmax(y, -1)

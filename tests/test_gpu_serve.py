@@ -748,6 +748,18 @@ def test_attn_prefix_workspace_too_small(cuda_dev):
             sb200.attn_prefix(b.q, torch.empty_like(b.q), b.kv, b.ptable, 1000, b.kv, b.table, b.kv_len, b.scale, ws, max_kv=50)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_attn_prefix_one_workspace_for_several_sizes(cuda_dev, kind):
+    """The largest answer among the sizes that run serves them all, in any
+    order."""
+    sizes = [(70, 900, 200), (64, 900, 200), (8, 900, 200), (1, 900, 1500), (40, 0, 1500), (64, 900, 30), (3, 40, 3)]
+    bs = [Batch(kind, 16, 4, 128, P, [(i * 31) % S + 1 for i in range(B)], seed=B) for B, P, S in sizes]
+    most = max(sb200.attn_prefix_ws(b.q, b.kv, b.P, len(b.lens), max_kv=max(b.lens)) for b in bs)
+    ws = torch.full((most,), 0xFF, dtype=torch.uint8, device="cuda")
+    for b in bs + bs[::-1]:
+        b.check(got=b.run(ws=ws))
+
+
 def test_attn_prefix_reads_an_engine_cache(cuda_dev, qwen_weights):
     """A prompt that an engine has prefilled, as the shared prefix of a batch:
     the same attention as the single-sequence kernel on the same cache."""
