@@ -335,6 +335,15 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * one workspace for several sizes has the largest answer among them.  FP32
  * runs on CUDA cores in FP32 throughout; 16-bit types use the tensor cores
  * with FP32 scores, sums and outputs and 16-bit softmax weights. */
+/* Failure-detection test hook: tile >= 0 makes every later sb_attn_prefix
+ * call's loaders of keys stop before that tile of each key range (tiles of
+ * 64 keys, 128 of a prefix on tcgen05, 32 of heads past 64 in FP32; not the
+ * 64-row kernel, which waits on no barrier), so that the bounded wait for it
+ * runs out (~2 s), what was asked for drains, and the call returns with NaN
+ * rows and the error flag set (sb_tc_error).  Later calls are not affected by
+ * the flag, except replays of the captured call that gave up, until it is
+ * read.  -1 turns the hook off. */
+int sb_attn_set_test_skip(int tile);
 int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes);
 int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
                    int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,

@@ -35,7 +35,8 @@
 #define SB_AP_ST(HDP) ((HDP) == 128 ? 2 : 3)
 #define SB_AP_RING 4  // offsets of the tiles in flight
 
-__device__ int tc_err;  // nonzero after a wait timed out
+__device__ int tc_err;        // nonzero after a wait timed out
+__device__ unsigned tc_call;  // the last call in which one did: its other waits need not run out too
 
 struct AttnPages {  // strides in elements
     const void *k, *v;
@@ -58,6 +59,8 @@ struct AttnParams {
     int items1;                                  // prefix items in this launch; own items follow them
     int deep;                                    // 16-bit types, heads of 128: rings of two tiles instead of one
     float scale_log2;
+    unsigned call;   // this call's number, not 0
+    int test_skip;   // test hook: 0, or 1 + the tile of every item before which the loaders of keys stop
 };
 
 struct AttnItem {
@@ -139,7 +142,8 @@ SB_DEV void ap_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> SB_DEV void ap_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ---- barriers.  Every wait is bounded: after two seconds it sets tc_err
-// (sb_tc_error reads and clears it) and the caller stops.
+// (sb_tc_error reads and clears it) and tc_call, and the caller stops.  The
+// call's results are NaN where that happened; another call's are not touched.
 SB_DEV void ap_bar_init(uint64_t *b, unsigned count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(ap_smem(b)), "r"(count) : "memory");
 }
@@ -160,8 +164,8 @@ SB_DEV unsigned long long ap_now() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-// false after WAIT_NS, or (abortable) once any wait has given up
-SB_DEV bool ap_bar_wait(uint64_t *b, unsigned ph, bool abortable = true) {
+// false after WAIT_NS, or once a wait of this call has given up (call 0: only after WAIT_NS)
+SB_DEV bool ap_bar_wait(uint64_t *b, unsigned ph, unsigned call) {
     constexpr unsigned long long WAIT_NS = 2000000000ull;
     if (ap_bar_try(b, ph)) return true;
     unsigned long long t0 = 0;
@@ -169,13 +173,17 @@ SB_DEV bool ap_bar_wait(uint64_t *b, unsigned ph, bool abortable = true) {
     for (int spin = 0; spin < (1 << 26); spin++) {
         if (ap_bar_try(b, ph)) return true;
         if ((spin & 1023) == 1023) {
-            if (abortable && *(volatile int *)&tc_err) return false;
+            if (call && *(volatile unsigned *)&tc_call == call) return false;
             const unsigned long long t = ap_now();
             if (t0 == 0) t0 = t;
             else if (t - t0 > WAIT_NS) break;
         }
     }
     atomicExch(&tc_err, 1);
+    if (call) {
+        atomicExch(&tc_call, call);
+        __threadfence();
+    }
     return false;
 }
 SB_DEV void ap_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -248,16 +256,17 @@ template <int KT, int HDP, int E> struct ApCopy {
 template <int KW, int HDP, int E> struct ApRing {
     static constexpr int SUB = HDP * E / 128, BLOCK = KW * 128, TILE = SUB * BLOCK, KT = KW * (SB_AP_THREADS / 32);
     static constexpr int C = HDP * E / 16, STEP = 32 / C, N = KW / STEP;
+    const AttnParams &P;
     const AttnItem &it;
     const CUtensorMap *tm[2];
     ApBars *bars;
     unsigned sm;
-    int st, first, box, HD, seq;  // seq: tiles that went through the ring before this item
+    int st, first, box, HD, seq;  // seq: tiles that went through the ring before this item, -1 after giving up
     int pg, in_pg, row, sub;  // this lane's box of the tile looked up last
     bool mine;
-    SB_DEV ApRing(const AttnItem &item, int hd, int stages, unsigned char *ring, ApBars *b, int seq0, const CUtensorMap *k,
+    SB_DEV ApRing(const AttnParams &prm, const AttnItem &item, int stages, unsigned char *ring, ApBars *b, int seq0, const CUtensorMap *k,
                   const CUtensorMap *v, int bx)
-        : it(item), bars(b + (threadIdx.x >> 5)), st(stages), box(min(bx, KW)), HD(hd), seq(seq0) {
+        : P(prm), it(item), bars(b + (threadIdx.x >> 5)), st(stages), box(min(bx, KW)), HD(prm.HD), seq(seq0) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pieces = box ? KW / box : 1;
         tm[0] = k;
         tm[1] = v;
@@ -267,7 +276,7 @@ template <int KW, int HDP, int E> struct ApRing {
         row = lane % pieces * box;
         mine = box && sub < SUB;
     }
-    SB_DEV int tiles(int k1) const { return k1 > first ? (k1 - first + KT - 1) / KT : 0; }
+    SB_DEV int tiles(int k1) const { return k1 > first && seq >= 0 ? (k1 - first + KT - 1) / KT : 0; }
     SB_DEV int slot(int t) const { return (seq + t) & (st - 1); }
     SB_DEV unsigned phase(int t) const { return (unsigned)((seq + t) >> (st - 1)) & 1u; }  // of st = 1 or 2
     SB_DEV unsigned tile(int which, int t) const { return sm + (which * st + slot(t)) * TILE; }
@@ -281,6 +290,7 @@ template <int KW, int HDP, int E> struct ApRing {
         }
     }
     SB_DEV void copy(int which, int t) {  // tile t, looked up
+        if (which == 0 && t + 1 == P.test_skip) return;
         const int lane = threadIdx.x & 31, n = slot(t);
         const unsigned dst = tile(which, t);
         uint64_t *bar = &bars->full[which][n];
@@ -310,13 +320,11 @@ template <int KW, int HDP, int E> struct ApRing {
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(ap_smem(bar)) : "memory");
     }
     SB_DEV bool wait(int which, int t) const {
-        return __all_sync(SB_FULL, ap_bar_wait(&bars->full[which][slot(t)], phase(t)));
+        return __all_sync(SB_FULL, ap_bar_wait(&bars->full[which][slot(t)], phase(t), P.call));
     }
-    SB_DEV void drain(int t, int nt) {  // given up at tile t: what was asked for still has to land
-        for (int u = t; u < min(t + st + 1, nt); u++) {
-            ap_bar_wait(&bars->full[0][slot(u)], phase(u), false);
-            ap_bar_wait(&bars->full[1][slot(u)], phase(u), false);
-        }
+    SB_DEV void drain(int t, int nt, int at_v) {  // given up at tile t, its K or V: what was asked for still has to land
+        for (int u = t + at_v; u < min(t + st + at_v, nt); u++) ap_bar_wait(&bars->full[0][slot(u)], phase(u), 0);
+        for (int u = t; u < min(t + st, nt); u++) ap_bar_wait(&bars->full[1][slot(u)], phase(u), 0);
         __syncwarp();
     }
     SB_DEV unsigned valid(int t) const { return bars->valid[slot(t)]; }
@@ -578,7 +586,7 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
     constexpr int NW = SB_AP_THREADS / 32, KS = HDP / 16, KT = 16 * NW;
     const int st = HDP == 128 && !P.deep ? 1 : 2;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q4 = lane & 3;
-    ApRing<16, HDP, 2> ring(it, P.HD, st, sm, bars, seq, tm_k, tm_v, box);
+    ApRing<16, HDP, 2> ring(P, it, st, sm, bars, seq, tm_k, tm_v, box);
     unsigned qb[NB][KS][2];  // rows f0 + 8 b + g
     int vis[NB][2];          // of rows f0 + 8 b + 2 q4, + 1
 #pragma unroll
@@ -618,8 +626,8 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
         }
     }
     ring.look(st);
-    bool ok = true;
-    int t = 0;
+    bool ok = seq >= 0;
+    int t = 0, at_v = 0;
     for (; t < nt; t++) {
         const unsigned kt = ring.tile(0, t), vt = ring.tile(1, t);
         const int key = first + t * KT + g;
@@ -678,7 +686,10 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             p[b][0] = ap_movmatrix(ap_pack<T>(s[b][0], s[b][1]));
             p[b][1] = ap_movmatrix(ap_pack<T>(s[b][2], s[b][3]));
         }
-        if (!(ok = ring.wait(1, t))) break;
+        if (!(ok = ring.wait(1, t))) {
+            at_v = 1;
+            break;
+        }
         if (gaps) ap_fence_async();
 #pragma unroll
         for (int i = 0; i < KS; i++) {
@@ -694,9 +705,10 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
             ring.look(t + st + 1);
         }
     }
-    seq += nt;
-    if (!ok) {  // given up (tc_err): nothing that passes for a result
-        ring.drain(t, nt);
+    if (ok) seq += nt;
+    if (!ok) {  // given up (tc_err), here or in an item before: nothing that passes for a result
+        ring.drain(t, nt, at_v);
+        seq = -1;
 #pragma unroll
         for (int b = 0; b < NB; b++) l[b][0] = l[b][1] = __int_as_float(0x7fc00000);
     }
@@ -747,7 +759,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
     __shared__ float m_s[NW][MT], l_s[NW][MT];
     __shared__ int vis_s[MT];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = lane % KW, dq = lane / KW;
-    ApRing<KW, HDP, 4> ring(it, P.HD, st, sm, bars, seq, tm_k, tm_v, box);
+    ApRing<KW, HDP, 4> ring(P, it, st, sm, bars, seq, tm_k, tm_v, box);
     __syncthreads();  // an earlier item's shared memory is no longer read
     for (int i = tid; i < MT * HDP / 4; i += SB_AP_THREADS) {
         const int r = i / (HDP / 4), d = i % (HDP / 4) * 4, f = it.f0 + r;
@@ -769,7 +781,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
         }
     }
     ring.look(st);
-    bool ok = true;
+    bool ok = seq >= 0;
     unsigned long long o[MT][DP];
     float m[MT], l[MT];
 #pragma unroll
@@ -779,7 +791,7 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
 #pragma unroll
         for (int e = 0; e < DP; e++) o[r][e] = 0ull;
     }
-    int t = 0;
+    int t = 0, at_v = 0;
     for (; t < nt; t++) {
         const unsigned char *kt = sm + (ring.tile(0, t) - ap_smem(sm)), *vt = sm + (ring.tile(1, t) - ap_smem(sm));
         if (!(ok = ring.wait(0, t))) break;
@@ -830,7 +842,10 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             if (r % DQ == dq) p_s[warp][key][r] = make_float2(s[r], s[r]);
         }
         __syncwarp();
-        if (!(ok = ring.wait(1, t))) break;
+        if (!(ok = ring.wait(1, t))) {
+            at_v = 1;
+            break;
+        }
         if (gaps) ap_fence_async();
 #pragma unroll
         for (int k = 0; k < KW; k++) {
@@ -865,9 +880,10 @@ SB_DEV void attn_f32_body(const AttnParams &P, const AttnItem &it, unsigned char
             ring.look(t + st + 1);
         }
     }
-    seq += nt;
-    if (!ok) {  // given up (tc_err): nothing that passes for a result
-        ring.drain(t, nt);
+    if (ok) seq += nt;
+    if (!ok) {  // given up (tc_err), here or in an item before: nothing that passes for a result
+        ring.drain(t, nt, at_v);
+        seq = -1;
 #pragma unroll
         for (int r = 0; r < MT; r++) l[r] = __int_as_float(0x7fc00000);
     }

@@ -37,7 +37,7 @@ template <int HDP> struct Cfg {
     static constexpr int SMEM = 1024 + (2 * ST + 2) * TILE;
 };
 // the same for a converged warp, one answer for all lanes
-SB_DEV bool warp_wait(uint64_t *mb, unsigned ph, bool abortable = true) { return __all_sync(SB_FULL, ap_bar_wait(mb, ph, abortable)); }
+SB_DEV bool warp_wait(uint64_t *mb, unsigned ph, unsigned call) { return __all_sync(SB_FULL, ap_bar_wait(mb, ph, call)); }
 SB_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 SB_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // 128-byte swizzled operand: rows (K-major: query rows or keys; MN-major: keys)
@@ -243,7 +243,8 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             const int s = t % ST, key = it.k0 + t * KT + p0, page = next, in_page = in_next;
             look(t + 1);
             const bool by_tma = __all_sync(SB_FULL, box && (!mine || (page >= 0 && page < it.pg.n_pages)));
-            if (t >= ST) ok = warp_wait(&empty[s], (unsigned)((t / ST) - 1) & 1u);
+            if (t >= ST) ok = warp_wait(&empty[s], (unsigned)((t / ST) - 1) & 1u, P.call);
+            if (is_k && t + 1 == P.test_skip) ok = false;
             if (!ok) break;
             const unsigned stage = (is_k ? kst : vst) + s * TILE;
             if (by_tma) {
@@ -279,7 +280,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         }
         ap_wait<0>();
         if (!ok && any_tma)  // given up: the copies that were issued still have to land
-            for (int i = t > ST ? t - ST : 0; i < t; i++) ap_bar_wait(&full[i % ST], (i / ST) & 1, false);
+            for (int i = t > ST ? t - ST : 0; i < t; i++) ap_bar_wait(&full[i % ST], (i / ST) & 1, 0);
     } else if (warp >= 12) {
         ATC_FEWER;
         if (tid == 12 * 32) {
@@ -296,7 +297,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 }
                 commit(&sfull[x]);
             };
-            bool ok = nt > 0 && ap_bar_wait(&qfull, 0) && ap_bar_wait(&kfull[0], 0);
+            bool ok = nt > 0 && ap_bar_wait(&qfull, 0, P.call) && ap_bar_wait(&kfull[0], 0, P.call);
             if (ok) {
                 fence_after();
                 for (int x = 0; x < nx; x++) scores(x, 0);
@@ -308,10 +309,10 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
                 const int s1 = s + 1 == ST ? 0 : s + 1;
                 const unsigned ph1 = s1 ? ph : ph ^ 1;
                 const bool more = t + 1 < nt;
-                ok = ap_bar_wait(&vfull[s], ph) && (!more || ap_bar_wait(&kfull[s1], ph1));
+                ok = ap_bar_wait(&vfull[s], ph, P.call) && (!more || ap_bar_wait(&kfull[s1], ph1, P.call));
 #pragma unroll 1
                 for (int x = 0; x < nx && ok; x++) {
-                    ok = ap_bar_wait(&pfull[x], t & 1);
+                    ok = ap_bar_wait(&pfull[x], t & 1, P.call);
                     if (!ok) break;
                     fence_after();
                     const uint64_t vs = vd + s * (TILE >> 4);
@@ -366,7 +367,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int t = 0; t < nt && ok; t++) {
-            ok = warp_wait(&sfull[x], t & 1);
+            ok = warp_wait(&sfull[x], t & 1, P.call);
             if (!ok) break;
             fence_after();
             const uint4 valid = *reinterpret_cast<const uint4 *>(valid_s[t % (2 * ST)]);
@@ -429,7 +430,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
             if (lane == 0) ap_arrive(&pfull[x]);
         }
         if (m == INFINITY) l = __int_as_float(0x7fc00000);  // an infinite score: NaN, as its softmax
-        ok = __all_sync(SB_FULL, ap_bar_wait(&ofull, 0, false) && ok && !*(volatile int *)&tc_err);
+        ok = __all_sync(SB_FULL, ap_bar_wait(&ofull, 0, 0) && ok && *(volatile unsigned *)&tc_call != P.call);
         fence_after();
         if (!ok) l = __int_as_float(0x7fc00000);  // given up: nothing that passes for a result
         const bool live = f < it.F;
@@ -465,7 +466,7 @@ SB_DEV void attn_tc_body(const AttnParams &P, const CUtensorMap *tm_k, const CUt
     __syncthreads();
     if (warp == 12) {
         fence_after();
-        ap_bar_wait(&ofull, 0, false);
+        ap_bar_wait(&ofull, 0, 0);
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }

@@ -541,6 +541,10 @@ int sb_tc_error(int *err) {
         if (e) {
             *err = e;
             SB_CK(cuMemsetD32(p, 0, 1));
+            if (mods[i] == M_SERVE) {
+                SB_CK(cuModuleGetGlobal(&p, &bytes, c->mod[M_SERVE], "tc_call"));
+                SB_CK(cuMemsetD32(p, 0, 1));
+            }
         }
     }
     return 0;

@@ -227,7 +227,17 @@ struct attn_params {
     int T, B, NH, NKV, G, HD, P, max_kv, table_stride;
     int chunk1, S1, tiles1, chunk2, S2, tiles2, items1, deep;
     float scale_log2;
+    unsigned call;
+    int test_skip;
 };
+/* a number for every call (a kernel that gives up stops its own call only), and the test hook */
+static unsigned attn_calls;
+static int attn_test_skip;
+int sb_attn_set_test_skip(int tile) {
+    SB_ARG(tile >= -1 && tile < 1 << 30, "tile must be >= -1");
+    __atomic_store_n(&attn_test_skip, tile + 1, __ATOMIC_RELAXED);
+    return 0;
+}
 /* Shared memory of the kernels with a ring a warp: 8 KB (16-bit types: K and V
  * tiles of 16 keys, one each for heads of 128, two for 64; four and six CTAs an SM)
  * or 16 KB (FP32, and long items of heads of 128: two each, three CTAs).  256
@@ -494,6 +504,9 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
     p.S2 = own.S;
     p.tiles2 = own.tiles;
     p.scale_log2 = scale * 1.4426950408889634f;
+    do p.call = __atomic_add_fetch(&attn_calls, 1, __ATOMIC_RELAXED);
+    while (p.call == 0);
+    p.test_skip = __atomic_load_n(&attn_test_skip, __ATOMIC_RELAXED);
     CUtensorMap tk, tv;
     int box = 0;
     memset(&tk, 0, sizeof tk);

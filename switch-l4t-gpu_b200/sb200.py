@@ -129,6 +129,7 @@ def lib():
     _sig(L.sb_rotary_plan_init, I, P, I, I, D, I, D, I)
     _sig(L.sb_rotary, I, P, L64, L64, P, L64, L64, I, I, I, I, P, P, I, P)
     _sig(L.sb_rotary_kv, I, P, L64, L64, P, L64, L64, P, L64, L64, P, L64, L64, I, I, P, P, P, P, P)
+    _sig(L.sb_attn_set_test_skip, I, I)
     _sig(L.sb_attn_prefix_ws, I, I, I, I, I, I, I, I, I, I, ctypes.POINTER(SZ))
     _sig(L.sb_attn_prefix, I, P, L64, L64, P, L64, L64, P, I, I, P, I, I, P, P, I, P, P, I, P, I, F, P, SZ, P)
     _sig(L.sb_logprobs_ws, I, I, I, I, I, ctypes.POINTER(SZ))

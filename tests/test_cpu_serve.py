@@ -228,3 +228,9 @@ def test_rotary_kv_in_place_needs_one_set_of_strides():
     for tok, head in ((512, 64), (256, 128)):
         assert L.sb_rotary_kv(p, 256, 64, p, tok, head, 2 * p, 128, 64, 3 * p, 128, 64, 2, 4, 4 * p, 5 * p, ctypes.byref(r),
                               ctypes.byref(pages), None) == ERR_ARG
+
+
+def test_attn_test_skip_refusals():
+    L = sb200.lib()
+    assert L.sb_attn_set_test_skip(-2) == ERR_ARG and L.sb_attn_set_test_skip(1 << 30) == ERR_ARG
+    assert L.sb_attn_set_test_skip(3) == 0 and L.sb_attn_set_test_skip(-1) == 0

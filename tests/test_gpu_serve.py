@@ -2,6 +2,7 @@
 plain implementations in 64 bits, at the sizes, masks, strides and tables
 where they can go wrong."""
 import math
+import time
 
 import numpy as np
 import pytest
@@ -758,6 +759,52 @@ def test_attn_prefix_one_workspace_for_several_sizes(cuda_dev, kind):
     ws = torch.full((most,), 0xFF, dtype=torch.uint8, device="cuda")
     for b in bs + bs[::-1]:
         b.check(got=b.run(ws=ws))
+
+
+@pytest.mark.parametrize("kind,NH,NKV,HD,B,P,S,page,skip", [
+    ("f32", 4, 2, 64, 60, 0, 900, 16, 1),       # decode rows, boxes
+    ("f32", 8, 1, 128, 5, 0, 90, 24, 0),        # the lanes' copies
+    ("f16", 8, 2, 64, 60, 0, 900, 16, 1),
+    ("bf16", 8, 2, 128, 60, 0, 900, 32, 1),
+    ("f16", 12, 1, 64, 60, 0, 900, 16, 1),      # 16 rows
+    ("bf16", 8, 2, 128, 40, 16000, 0, 64, 1),   # the prefix on tcgen05, boxes
+    ("f16", 8, 2, 64, 40, 16000, 0, 24, 0)])    # and the loaders' copies
+def test_attn_prefix_wait_timeout_recovers(cuda_dev, kind, NH, NKV, HD, B, P, S, page, skip):
+    """Failure detection without a GPU fault: the test hook makes the loaders
+    of keys stop before a tile, the bounded wait for it runs out, what was
+    asked for drains, and the rows are NaN.  The next call with the hook off
+    is right before the flag is read, and the flag is there once."""
+    b = Batch(kind, NH, NKV, HD, P, [S] * B, page=page, seed=51)
+    assert sb200.tc_error() == 0
+    sb200.check(sb200.lib().sb_attn_set_test_skip(skip))
+    try:
+        t0 = time.time()
+        out, lse = b.run(own=S > 0)
+        torch.cuda.synchronize()
+        assert time.time() - t0 < 30
+    finally:
+        sb200.check(sb200.lib().sb_attn_set_test_skip(-1))
+    assert bool(torch.isnan(out.float()).all()) and bool(torch.isnan(lse).all())
+    b.check(got=b.run(own=S > 0))
+    assert sb200.tc_error() != 0
+    assert sb200.tc_error() == 0
+    b.check(got=b.run(own=S > 0))
+
+
+def test_attn_prefix_wait_timeout_with_rows_left(cuda_dev):
+    """More rows than the launch was sized for: a CTA that gave up at its
+    first rows takes the others up no more, and all are NaN."""
+    b = Batch("f16", 14, 2, 64, 0, [900] * 20, rows=[4] * 20, seed=52)
+    sb200.check(sb200.lib().sb_attn_set_test_skip(1))
+    try:
+        out, lse = b.run(max_q=1)
+        torch.cuda.synchronize()
+    finally:
+        sb200.check(sb200.lib().sb_attn_set_test_skip(-1))
+    assert sb200.tc_error() != 0
+    assert bool(torch.isnan(out.float()).all()) and bool(torch.isnan(lse).all())
+    b.check(got=b.run(max_q=1))
+    assert sb200.tc_error() == 0
 
 
 def test_attn_prefix_reads_an_engine_cache(cuda_dev, qwen_weights):
