@@ -3,6 +3,8 @@ probabilities) where no GPU is needed: refusals of bad arguments, the layout of
 the structs that the binding mirrors, and the rotary frequencies."""
 import ctypes
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -234,3 +236,25 @@ def test_attn_test_skip_refusals():
     L = sb200.lib()
     assert L.sb_attn_set_test_skip(-2) == ERR_ARG and L.sb_attn_set_test_skip(1 << 30) == ERR_ARG
     assert L.sb_attn_set_test_skip(3) == 0 and L.sb_attn_set_test_skip(-1) == 0
+
+
+def test_kv_plan_indexes_nothing_outside(tmp_path):
+    """The kernel's own source on the host, under the address sanitizer:
+    hostile lengths (sums past 2^31, pages of 2^31 - 1) stay inside the
+    tables, and ordinary ones give the plan."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    text = open(os.path.join(here, "..", "switch-l4t-gpu_b200", "csrc", "serve_plan.cuh")).read()
+    for was, now in (('#include "sb_common.cuh"\n', ""), ("extern __shared__ int plan_sm[];", "int *plan_sm = shared_ints;")):
+        assert text.count(was) == 1
+        text = text.replace(was, now)
+    source, binary = tmp_path / "plan.inc", tmp_path / "plan"
+    source.write_text(text)
+    build = ["g++", "-std=c++17", "-O1", "-g", "-fwrapv", "-w", f'-DPLAN_SOURCE="{source}"', os.path.join(here, "plan_emulation.cpp"), "-o", str(binary)]
+    probe = tmp_path / "probe.cpp"
+    probe.write_text("int main() { return 0; }\n")
+    if subprocess.run(["g++", "-fsanitize=address", str(probe), "-o", str(tmp_path / "probe")], capture_output=True).returncode:
+        pytest.skip("no address sanitizer")
+    subprocess.run(build + ["-fsanitize=address"], check=True)
+    env = dict(os.environ, ASAN_OPTIONS="detect_stack_use_after_return=0:detect_leaks=0")
+    run = subprocess.run([str(binary), "3000"], capture_output=True, text=True, env=env, timeout=120)
+    assert run.returncode == 0 and run.stdout == "3000 cases\n", (run.stdout + run.stderr)[-3000:]
