@@ -285,7 +285,10 @@ int sb_kv_plan(const int *cache_len, const int *new_len, int B, int page, const 
  * turn once and less by factor, blends between, and multiplies cosine and
  * sine by 0.1 ln factor + 1; BANDS keeps pairs of 4 turns and more, divides
  * those of 1 turn and less, blends by turns between.  The plan is plain host
- * memory (copied into each launch), exact for any position below 2^31. */
+ * memory (copied into each launch).  Its frequencies are good to 2^-62: at any
+ * position below 2^31 the angle is off by 2^-25 of a half turn, in FP32 (the
+ * rounding of the angle itself).  Where few turns are trained (orig_ctx below
+ * 2 pi), YARN's published ramp keeps pair 0. */
 #define SB_ROTARY_MAX_DIM 256
 #define SB_ROPE_HALF 0
 #define SB_ROPE_PAIRS 1

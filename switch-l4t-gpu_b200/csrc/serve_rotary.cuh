@@ -10,10 +10,11 @@
 // The angle at a far position needs more bits than FP32 has (pos 10^6 x f 1
 // leaves 0.06 rad of error), and tables cost reads and a length limit.  So a
 // frequency is held as a 64-bit fixed-point fraction of a turn, F = f / 2 pi
-// x 2^64: pos * F modulo 2^64 is the fraction of the last turn, exact up to
-// pos x 2^-65 turns, from one integer multiply.  Its top 32 bits as a signed
-// fraction give the angle within +-pi to 2^-25 of a half turn, and
-// sincospif takes it from there.  All frequencies are a kernel parameter
+// x 2^64: pos * F modulo 2^64 is the fraction of the last turn from one integer
+// multiply, off by pos times what F is off (the host's powl: 2^-62 of f / 2 pi,
+// and half a unit of 2^-64).  Its top 32 bits as a signed fraction, rounded to
+// FP32, give the angle within +-pi to 2^-25 of a half turn, and sincospif takes
+// it from there.  All frequencies are a kernel parameter
 // (1 KB): no table in memory.
 //
 // Bound: HBM, one read and one write of the rows.  A CTA takes a few tokens,

@@ -54,8 +54,11 @@ int sb_rotary_plan_init(sb_rotary_plan *r, int dim, int layout, double theta, in
     SB_ARG(scaling < SB_ROPE_YARN || orig_ctx >= 1, "rotary_plan_init: this scaling needs the trained context");
     SB_ARG(scaling != SB_ROPE_NTK || dim > 2, "rotary_plan_init: this scaling needs dim > 2");
     const double pi2 = 6.283185307179586476925286766559;
+    /* frequencies in long double (64-bit mantissa): a double's half unit is 2^-25 turns at a position of 2^31 */
+    const long double pi2l = 6.283185307179586476925286766559L;
+    long double base = theta;
     double lo = 0, hi = 0;
-    if (scaling == SB_ROPE_NTK) theta *= pow(factor, dim / (dim - 2.0));
+    if (scaling == SB_ROPE_NTK) base *= powl(factor, dim / (dim - 2.0L));
     if (scaling == SB_ROPE_YARN) { /* pairs that turn 32 times and once over the trained context */
         lo = floor(dim * log(orig_ctx / (32.0 * pi2)) / (2.0 * log(theta)));
         hi = ceil(dim * log(orig_ctx / pi2) / (2.0 * log(theta)));
@@ -68,20 +71,19 @@ int sb_rotary_plan_init(sb_rotary_plan *r, int dim, int layout, double theta, in
     r->mscale = 1.0f;
     if (scaling == SB_ROPE_YARN) r->mscale = (float)(0.1 * log(factor) + 1.0);
     for (int i = 0; i < dim / 2; i++) {
-        double f = pow(theta, -2.0 * i / dim);
+        long double f = powl(base, -2.0L * i / dim);
         if (scaling == SB_ROPE_LINEAR) f /= factor;
         if (scaling == SB_ROPE_YARN) {
-            double ramp = (i - lo) / (hi > lo ? hi - lo : 0.001);
+            long double ramp = (i - lo) / (hi > lo ? hi - lo : 0.001L);
             ramp = ramp < 0 ? 0 : ramp > 1 ? 1 : ramp;
-            f = f / factor * ramp + f * (1.0 - ramp);
+            f = f / factor * ramp + f * (1 - ramp);
         }
         if (scaling == SB_ROPE_BANDS) { /* turns over the trained context: 1 and fewer stretched, 4 and more kept */
-            double s = (orig_ctx * f / pi2 - 1.0) / 3.0;
+            long double s = (orig_ctx * f / pi2l - 1) / 3;
             s = s < 0 ? 0 : s > 1 ? 1 : s;
-            f = f / factor * (1.0 - s) + f * s;
+            f = f / factor * (1 - s) + f * s;
         }
-        /* the fraction of a turn per position in units of 2^-64, from a long double (64-bit mantissa) */
-        r->turn[i] = (uint64_t)(f / (long double)6.283185307179586476925286766559L * 18446744073709551616.0L + 0.5L);
+        r->turn[i] = (uint64_t)(f / pi2l * 18446744073709551616.0L + 0.5L); /* turns per position in units of 2^-64 */
     }
     return 0;
 }

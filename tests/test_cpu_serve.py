@@ -2,6 +2,7 @@
 probabilities) where no GPU is needed: refusals of bad arguments, the layout of
 the structs that the binding mirrors, and the rotary frequencies."""
 import ctypes
+import decimal
 import math
 import os
 import subprocess
@@ -258,3 +259,32 @@ def test_kv_plan_indexes_nothing_outside(tmp_path):
     env = dict(os.environ, ASAN_OPTIONS="detect_stack_use_after_return=0:detect_leaks=0")
     run = subprocess.run([str(binary), "3000"], capture_output=True, text=True, env=env, timeout=120)
     assert run.returncode == 0 and run.stdout == "3000 cases\n", (run.stdout + run.stderr)[-3000:]
+
+
+@pytest.mark.parametrize("dim,theta,factor,orig", [(64, 1e6, 8.0, 4096), (128, 1e4, 3.7, 2048), (80, 500000.0, 32.0, 8192), (6, 1.5, 2.0, 100)])
+def test_rotary_plan_frequencies_in_long_double(dim, theta, factor, orig):
+    """Against 50 digits: powl, a product or quotient or four of a blend, each
+    within 2^-64 relative, and the fraction's own half unit."""
+    D, pi = decimal.Decimal, decimal.Decimal("3.14159265358979323846264338327950288419716939937510")
+    with decimal.localcontext() as ctx:
+        ctx.prec = 50
+        th, k = D(theta), D(factor)
+        for scaling in range(5):
+            rc, r = _plan(dim, theta=theta, scaling=scaling, factor=factor, orig=orig)
+            assert rc == 0
+            lo = max(math.floor(dim * math.log(orig / (64 * math.pi)) / (2 * math.log(theta))), 0)
+            hi = min(math.ceil(dim * math.log(orig / (2 * math.pi)) / (2 * math.log(theta))), dim - 1)
+            for i in range(dim // 2):
+                base = th * k ** (D(dim) / D(dim - 2)) if scaling == 2 else th
+                f = base ** (D(-2 * i) / D(dim))
+                if scaling == 1:
+                    f /= k
+                if scaling == 3:
+                    ramp = min(max(D(i - lo) / (D(hi - lo) if hi > lo else D("0.001")), D(0)), D(1))
+                    f = f / k * ramp + f * (1 - ramp)
+                if scaling == 4:
+                    s = min(max((orig * f / (2 * pi) - 1) / 3, D(0)), D(1))
+                    f = f / k * (1 - s) + f * s
+                turns = f / (2 * pi) * D(2) ** 64
+                # the blends: s is off by up to 4 relative units of a number of turns up to 4, and multiplies f
+                assert abs(D(int(r.turn[i])) - turns) <= turns * D(2) ** (-62 if scaling != 4 else -60) + D("0.51"), (scaling, i)
