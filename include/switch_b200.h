@@ -304,7 +304,8 @@ typedef struct sb_rotary_plan {
 } sb_rotary_plan;
 int sb_rotary_plan_init(sb_rotary_plan *r, int dim, int layout, double theta, int scaling, double factor, int orig_ctx);
 /* y = x [T][H][HD] turned by pos[t] (strides in elements; y may be x with
- * the same strides); inverse != 0 turns back, the gradient of the rotation.
+ * the same strides); inverse != 0 turns back: the gradient of the rotation,
+ * YARN's factor in it.
  * Rows with pos < 0 are left as they were. */
 int sb_rotary(const void *x, int64_t x_tok, int64_t x_head, void *y, int64_t y_tok, int64_t y_head, int type, int T, int H,
               int HD, const int *pos, const sb_rotary_plan *r, int inverse, void *stream);
@@ -329,15 +330,23 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * so is everything past a length.  Values that some row of a tile sees must
  * be finite (a weight of 0 times an infinity is NaN).  prefix and kv may be
  * different pools; the arguments of one that has no positions (prefix_len or
- * max_kv 0) may be NULL, but one of the two pools is given.  max_q (rows of a request) sizes the launch, larger
- * requests are still right; kv_len is cut to max_kv.  A row that sees nothing
+ * max_kv 0) may be NULL, but one of the two pools is given.  max_q (rows of a
+ * request) sizes the launch, larger requests are still right; kv_len is cut to
+ * max_kv.  A row that sees nothing
  * gives zeros and lse = -inf; rows from cu_q[B] on are left as they were.
  * lse [T][NH] (natural log of the softmax denominator) may be NULL.
  * ws: sb_attn_prefix_ws bytes for the same sizes (32-byte aligned); fewer
  * rows or shorter lengths may need more, as they are cut into more ranges, so
  * one workspace for several sizes has the largest answer among them.  FP32
  * runs on CUDA cores in FP32 throughout; 16-bit types use the tensor cores
- * with FP32 scores, sums and outputs and 16-bit softmax weights. */
+ * with FP32 scores, sums and outputs and softmax weights of the values' type
+ * (of normal values, FP16 outputs are off from 64 bits by 2.9e-4 and BF16 by
+ * 2.3e-3 relative; rounding the outputs alone is 2.1e-4 and 1.7e-3). */
+int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes);
+int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
+                   int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
+                   int prefix_len, const sb_kv_pages *kv, const int *table, int table_stride, const int *kv_len, int max_kv,
+                   float scale, void *ws, size_t ws_bytes, void *stream);
 /* Failure-detection test hook: tile >= 0 makes every later sb_attn_prefix
  * call's loaders of keys stop before that tile of each key range (tiles of
  * 64 keys, 128 of a prefix on tcgen05, 32 of heads past 64 in FP32; not the
@@ -347,11 +356,6 @@ int sb_rotary_kv(const void *q, int64_t q_tok, int64_t q_head, void *q_out, int6
  * the flag, except replays of the captured call that gave up, until it is
  * read.  -1 turns the hook off. */
 int sb_attn_set_test_skip(int tile);
-int sb_attn_prefix_ws(int type, int T, int B, int NH, int NKV, int HD, int max_q, int prefix_len, int max_kv, size_t *bytes);
-int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float *lse, int T,
-                   int NH, const int *cu_q, int B, int max_q, const sb_kv_pages *prefix, const int *prefix_table,
-                   int prefix_len, const sb_kv_pages *kv, const int *table, int table_stride, const int *kv_len, int max_kv,
-                   float scale, void *ws, size_t ws_bytes, void *stream);
 
 /* Log probabilities from logits [R][V] (any row stride and alignment) in one
  * pass, x = logits / temperature: lse[r] = ln sum e^x, entropy[r] of the
@@ -359,8 +363,8 @@ int sb_attn_prefix(const void *q, int64_t q_row, int64_t q_head, void *out, int6
  * the token (larger logit, or equal and a lower id), and the top_k (0..64)
  * best ids with their log probabilities, best first, equal logits by id.
  * Any output may be NULL.  A token outside [0, V) gives logp 0 and rank -1.
- * temperature is at least 1e-8.  Masked choices (-inf) have probability 0 and are not listed (id -1,
- * -inf fill up); a row of them gives lse = logp = -inf and entropy 0.  A row
+ * temperature is at least 1e-8.  Masked choices (-inf) have probability 0 and
+ * are not listed (id -1, -inf fill up); a row of them gives lse = logp = -inf and entropy 0.  A row
  * with a NaN or +inf gives NaN sums, its ids and rank mean nothing.
  * ws: sb_logprobs_ws bytes (16-byte aligned), enough for any smaller R, V and
  * top_k too. */

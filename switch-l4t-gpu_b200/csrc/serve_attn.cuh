@@ -459,7 +459,7 @@ SB_DEV void attn_mma_body(const AttnParams &P, const AttnItem &it, unsigned char
                 qa[k][h + 2 * e] = f < it.F && d < P.HD ? *reinterpret_cast<const unsigned *>(qp + d) : 0u;
             }
     }
-    // keys that some row of the tile sees end here; a tile of keys below every row's limit needs no mask
+    // keys that some row of the tile sees end here
     const int flast = min(it.f0 + 64, it.F) - 1;
     const int k1 = min(it.k1, ap_vis(it, flast, P.G));
     const int nt = k1 > it.k0 ? (k1 - it.k0 + KT - 1) / KT : 0;
@@ -745,8 +745,11 @@ SB_DEV void attn_mmaw_body(const AttnParams &P, const AttnItem &it, unsigned cha
 // dimensions of all rows, the weights come as pairs from shared memory for
 // two-wide FMAs.  Rows rescale when their maximum has grown by more than 2^8,
 // as in the other kernels.
-// Bound: HBM up to eight rows (46 of the 24 bytes per SM and cycle that HBM
-// gives at MT = 8), the shared-memory and FMA pipes beyond.  FFMA and not the
+// Bound: HBM up to eight rows, the shared-memory and FMA pipes beyond.  HBM
+// gives an SM 23 bytes a cycle (6.55 TB/s, 148 SMs, 1.9 GHz); at MT rows of 64
+// the FMA pipe takes MT cycles a key (128 MT products, 128 a cycle) of 512
+// bytes, 64 bytes a cycle at 8 rows and 32 at 16, where the reads of queries
+// and weights from shared memory take as long again.  FFMA and not the
 // tensor pipe: its FP32 sums are not IEEE-rounded and drift by 1e-5 over some
 // thousand keys.
 template <int HDP, int MT>

@@ -373,6 +373,16 @@ def test_attn_prefix_many_rows(cuda_dev, kind, NH, NKV, HD, P, lens, rows, page,
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("NH,NKV,HD,P,lens,rows,page", [
+    (8, 2, 64, 0, [400, 130, 1], [300, 129, 1], 16),
+    (4, 1, 128, 200, [513, 0, 77], [513, 0, 60], 24),
+    (14, 2, 64, 333, [257, 700], [256, 255], 64)])
+def test_attn_prefix_rows_of_a_prompt(cuda_dev, kind, NH, NKV, HD, P, lens, rows, page):
+    """A prompt's own rows: hundreds a request, each with its own limit."""
+    Batch(kind, NH, NKV, HD, P, lens, rows=rows, page=page, seed=53).check()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("NH,NKV,HD,P,lens,rows,T", [
     (14, 2, 64, 40, [20, 9, 30], [3, 4, 2], 6),      # the second request's last row and the third's are not there
     (4, 2, 128, 0, [70, 60, 90], [30, 40, 20], 50),  # row tiles of 64
